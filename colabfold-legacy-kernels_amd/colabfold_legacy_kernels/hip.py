@@ -13,6 +13,13 @@ stream, with the FFI binding's buffer order, attributes, result shapes and error
   layer_norm          VoltaLayerNorm      (cuda/volta_ops.cu:86-94)
   gated_dual_proj     VoltaGdp            (volta_ops.cu:258-269)
 
+and, without a counterpart in the reference, the RMS norm and the 8-bit serving path beside them:
+
+  rms_norm, rms_norm_bwd      RMS norm with the residual's addition, and its gradients
+  rms_norm_q8                 the same norm with 8-bit rows as its result
+  quantize_rows, dequantize_rows  8-bit rows of a matrix (or of its relu or swish gate), and back
+  q8_projection               8-bit rows times 8-bit weights, scales, bias and residual
+
 Results are allocated here with torch (as XLA preallocates them) unless passed in, which is how a
 caller aliases an output to its residual / input. The fused ops take fp16 or bf16 activations
 (all of a call's activations and results one type; weights, biases and keep fp16); results come
@@ -27,8 +34,8 @@ import torch
 
 from . import library_path
 
-CLK_S32, CLK_U8, CLK_F16, CLK_F32, CLK_BF16 = 4, 6, 10, 11, 16
-_DTYPES = {torch.int32: CLK_S32, torch.uint8: CLK_U8, torch.float16: CLK_F16,
+CLK_S8, CLK_S32, CLK_U8, CLK_F16, CLK_F32, CLK_BF16 = 2, 4, 6, 10, 11, 16
+_DTYPES = {torch.int8: CLK_S8, torch.int32: CLK_S32, torch.uint8: CLK_U8, torch.float16: CLK_F16,
            torch.float32: CLK_F32, torch.bfloat16: CLK_BF16}
 INVALID_ARGUMENT, INTERNAL = 3, 13
 
@@ -74,6 +81,13 @@ _SIGNATURES = {
     "clk_gated_dual_proj": [ctypes.c_void_p, ctypes.c_int32] + [_P] * 7 + [ctypes.c_int64],
     "clk_opm_update": [ctypes.c_void_p] + [_P] * 6 + [ctypes.c_float, ctypes.c_int32],
     "clk_opm_outer": [ctypes.c_void_p] + [_P] * 4,
+    "clk_rms_norm": [ctypes.c_void_p] + [_P] * 6 + [ctypes.c_float, ctypes.c_int32, ctypes.c_int32],
+    "clk_rms_norm_q8": [ctypes.c_void_p] + [_P] * 6 + [ctypes.c_float, ctypes.c_int32],
+    "clk_rms_norm_bwd": [ctypes.c_void_p] + [_P] * 7 +
+                        [ctypes.c_int32, ctypes.c_void_p, ctypes.c_size_t],
+    "clk_quantize_rows": [ctypes.c_void_p] + [_P] * 3 + [ctypes.c_int64],
+    "clk_dequantize_rows": [ctypes.c_void_p] + [_P] * 3,
+    "clk_q8_projection": [ctypes.c_void_p] + [_P] * 7 + [ctypes.c_int32, ctypes.c_int32],
 }
 
 
@@ -93,6 +107,8 @@ def lib():
         handle.clk_attention_bwd_plan.argtypes = [ctypes.c_int32] + [ctypes.c_int64] * 5 + \
             [ctypes.POINTER(ctypes.c_int64), ctypes.c_int32]
         handle.clk_attention_bwd_plan.restype = ctypes.c_int
+        handle.clk_rms_norm_bwd_workspace_size.argtypes = [_P]
+        handle.clk_rms_norm_bwd_workspace_size.restype = ctypes.c_size_t
         handle.clk_attention_bwd_noalloc_scratch_size.argtypes = []
         handle.clk_attention_bwd_noalloc_scratch_size.restype = ctypes.c_size_t
         _lib = handle
@@ -366,4 +382,122 @@ def opm_outer(left, right, wT, out=None):
     out = torch.empty((b, d, f), dtype=torch.float16, device=left.device) if out is None else out
     bufs, hold = _frame(left, right, wT, out)
     _check(lib().clk_opm_outer(_stream(left), *bufs))
+    return out
+
+
+# ---- RMS norm and 8-bit rows (no counterpart in the reference) --------------------------------
+
+def _call(name, tensors, *attrs):
+    """One entry point on the current stream of the tensors' GPU, whichever GPU is the current one. An
+    absent optional buffer is given as any tensor of its type."""
+    dev = tensors[0].device
+    for t in tensors:
+        if t.device != dev or not t.is_cuda:
+            raise InvalidArgument(INVALID_ARGUMENT, "%s: all tensors must be on one GPU, got %s and %s"
+                                  % (name[4:], dev, t.device))
+    bufs, hold = _frame(*tensors)
+    fn = getattr(lib(), name)
+    if dev.index == torch._C._cuda_getDevice():
+        _check(fn(_stream(tensors[0]), *bufs, *attrs))
+    else:
+        with torch.cuda.device(dev):
+            _check(fn(_stream(tensors[0]), *bufs, *attrs))
+
+
+def _matrix(name, t):
+    if t.dim() != 2:
+        raise InvalidArgument(INVALID_ARGUMENT, "%s: expected a matrix, got shape %s" % (name, tuple(t.shape)))
+    return t.shape
+
+
+def padded_k(k):
+    """The columns of 8-bit rows of k values: k rounded up to a multiple of 64."""
+    return (k + 63) // 64 * 64
+
+
+def rms_norm(x, scale, residual=None, eps=1e-5, want_rstd=False, out=None, sum_out=None, rstd=None):
+    """(out, sum, rstd): out [M,C] = s / sqrt(mean(s^2) + eps) * scale with s = x, or s = x + residual
+    rounded to x's type, which is the returned sum (None without a residual); rstd [M] F32 for the
+    backward, None without want_rstd. x, residual F16 or BF16, scale [C] F32. sum_out may be x or
+    residual itself, out may be x."""
+    m, _ = _matrix("rms_norm", x)
+    out = torch.empty_like(x) if out is None else out
+    if residual is not None and sum_out is None:
+        sum_out = torch.empty_like(x)
+    want_rstd = want_rstd or rstd is not None
+    if want_rstd and rstd is None:
+        rstd = torch.empty(m, dtype=torch.float32, device=x.device)
+    has_residual = residual is not None
+    _call("clk_rms_norm", (x, residual if has_residual else x, scale, sum_out if has_residual else x, out,
+                           rstd if want_rstd else scale), float(eps), int(has_residual), int(want_rstd))
+    return out, (sum_out if has_residual else None), rstd
+
+
+def rms_norm_q8(x, scale, residual=None, eps=1e-5, q=None, q_scale=None, sum_out=None):
+    """(q, q_scale, sum): rms_norm with its result as 8-bit rows, q [M,Kp] S8 (Kp = padded_k(C), zeros
+    past C) and q_scale [M] F32; sum as in rms_norm."""
+    m, c = _matrix("rms_norm_q8", x)
+    if q is None:
+        q = torch.empty((m, padded_k(c)), dtype=torch.int8, device=x.device)
+    if q_scale is None:
+        q_scale = torch.empty(m, dtype=torch.float32, device=x.device)
+    has_residual = residual is not None
+    if has_residual and sum_out is None:
+        sum_out = torch.empty_like(x)
+    _call("clk_rms_norm_q8", (x, residual if has_residual else x, scale, sum_out if has_residual else x, q, q_scale),
+          float(eps), int(has_residual))
+    return q, q_scale, (sum_out if has_residual else None)
+
+
+def rms_norm_bwd_workspace(s):
+    bufs, hold = _frame(s)
+    return int(lib().clk_rms_norm_bwd_workspace_size(*bufs))
+
+
+def rms_norm_bwd(s, scale, rstd, dout, dsum=None, workspace=None, grads=None):
+    """(ds, dscale): the gradients of rms_norm from its s (x, or the returned sum) and rstd; dsum is the
+    gradient that reaches sum itself. ds [M,C] is the gradient of x and of residual alike, dscale [C]
+    F32; written into `grads` = (ds, dscale) when given."""
+    ds, dscale = grads if grads is not None else (torch.empty_like(s), torch.empty_like(scale))
+    if workspace is None:
+        workspace = torch.empty(max(rms_norm_bwd_workspace(s), 1), dtype=torch.uint8, device=s.device)
+    elif workspace.device != s.device or not workspace.is_contiguous():
+        raise InvalidArgument(INVALID_ARGUMENT, "rms_norm_bwd: workspace must be contiguous, on the tensors' GPU")
+    _call("clk_rms_norm_bwd", (s, scale, rstd, dout, s if dsum is None else dsum, ds, dscale),
+          int(dsum is not None), ctypes.c_void_p(workspace.data_ptr()), workspace.numel() * workspace.element_size())
+    return ds, dscale
+
+
+def quantize_rows(x, activation=0, q=None, q_scale=None):
+    """(q, q_scale): the 8-bit rows of h [M,K], q [M,Kp] S8 (Kp = padded_k(K), zeros past K) and q_scale
+    [M] F32. activation 0: h = x; 1: h = relu(x); 2: h = swish(x[:, :K]) * x[:, K:] with x [M,2K]. x F16,
+    BF16 or F32."""
+    m, k = _matrix("quantize_rows", x)
+    k = k // 2 if activation == 2 else k
+    if q is None:
+        q = torch.empty((m, padded_k(k)), dtype=torch.int8, device=x.device)
+    if q_scale is None:
+        q_scale = torch.empty(m, dtype=torch.float32, device=x.device)
+    _call("clk_quantize_rows", (x, q, q_scale), int(activation))
+    return q, q_scale
+
+
+def dequantize_rows(q, q_scale, k=None, dtype=torch.float16, out=None):
+    """out [M,k]: what the 8-bit rows stand for; k defaults to all of q's columns."""
+    m, kp = _matrix("dequantize_rows", q)
+    if out is None:
+        out = torch.empty((m, kp if k is None else k), dtype=dtype, device=q.device)
+    _call("clk_dequantize_rows", (q, q_scale, out))
+    return out
+
+
+def q8_projection(q, q_scale, wq, w_scale, b=None, residual=None, dtype=torch.float16, out=None):
+    """out [M,N] = (q @ w^T) * q_scale[m] * w_scale[n] [+ b[n]] [+ residual]: 8-bit rows times 8-bit
+    weights, wq laid out by layouts.q8_blocked; b [N] F32; residual and out of `dtype`, F16 or BF16. out
+    may be residual itself."""
+    m, _ = _matrix("q8_projection", q)
+    if out is None:
+        out = torch.empty((m, w_scale.shape[0]), dtype=dtype, device=q.device)
+    _call("clk_q8_projection", (q, q_scale, wq, w_scale, w_scale if b is None else b, out if residual is None else residual,
+                                out), int(b is not None), int(residual is not None))
     return out

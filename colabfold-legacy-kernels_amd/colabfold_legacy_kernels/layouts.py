@@ -12,6 +12,11 @@ call. The target layouts are fixed by the reference's FFI comments and kernels:
   transition          w1 [C, H] -> w1T [H, C]; w2 [H, C] -> w2T [H/64][C][64] with
                       w2T[j][c][i] = w2[64 j + i][c]             (volta_fused_ffi.h:216-217)
 
+and the layout of the 8-bit projection's weights, which has no counterpart there:
+
+  q8_projection       q [N, Kp] (8-bit rows of w^T, Kp a multiple of 64) ->
+                      wq [ceil(N/64), Kp/64, 4, 4, 16, 16]
+
 Each function takes and returns torch tensors (any device) or numpy arrays, and returns a
 contiguous result of the input's dtype.
 """
@@ -75,3 +80,34 @@ def w2_unblocked(w2T):
     if hasattr(w2T, "permute"):
         return w2T.permute(0, 2, 1).reshape(j * i, c).contiguous()
     return _contig(w2T.transpose(0, 2, 1).reshape(j * i, c))
+
+
+Q8_BLOCK = 64  # channels and inputs of a block of the 8-bit weights
+
+
+def q8_blocked(q):
+    """q [N, Kp] -> wq [ceil(N/64), Kp/64, 4, 4, 16, 16] (q8_projection): blocks of 64 channels by 64
+    inputs, wq[., ., b, c, 4 g + i, j] = q[channel 16 g + 4 b + i, input 16 c + j] of the block, zeros
+    for channels past N."""
+    if q.ndim != 2 or q.shape[1] % Q8_BLOCK:
+        raise ValueError("expected q [N, Kp] with Kp a multiple of 64, got shape %s" % (tuple(q.shape),))
+    n, kp = q.shape
+    blocks = -(-n // Q8_BLOCK)
+    if hasattr(q, "new_zeros"):
+        p = q.new_zeros((blocks * Q8_BLOCK, kp))
+        p[:n] = q
+        return p.view(blocks, 4, 4, 4, kp // 64, 4, 16).permute(0, 4, 2, 5, 1, 3, 6).reshape(
+            blocks, kp // 64, 4, 4, 16, 16).contiguous()
+    import numpy as np
+    p = np.zeros((blocks * Q8_BLOCK, kp), q.dtype)
+    p[:n] = q
+    return np.ascontiguousarray(p.reshape(blocks, 4, 4, 4, kp // 64, 4, 16).transpose(
+        0, 4, 2, 5, 1, 3, 6).reshape(blocks, kp // 64, 4, 4, 16, 16))
+
+
+def q8_unblocked(wq, n):
+    """The inverse of q8_blocked: wq -> q [n, Kp]."""
+    blocks, kbs = wq.shape[:2]
+    p = wq.reshape(blocks, kbs, 4, 4, 4, 4, 16)
+    p = p.permute(0, 4, 2, 5, 1, 3, 6) if hasattr(p, "permute") else p.transpose(0, 4, 2, 5, 1, 3, 6)
+    return _contig(p.reshape(blocks * Q8_BLOCK, kbs * Q8_BLOCK)[:n])

@@ -18,9 +18,14 @@ provides on top of `hip` (the C ABI binding):
                    the row count (tests/test_fused.py:96-229 calls them so)
   fused_available  whether a fused target takes a width and dtype (tests/test_fused.py:223-229:
                    other widths and dtypes decline to the caller's own path)
+  rms_norm         RMS norm with the residual's addition, differentiable in the input, the residual
+                   and the scale
+  rms_norm_q8, quantize_rows, dequantize_rows, q8_weights, q8_projection, q8_transition
+                   the 8-bit serving path: norms and activations as 8-bit rows, weights quantised
+                   once, projections and an MLP in 8-bit products (no counterpart in the reference)
 
-Everything runs on the GPU through the built library; there is no CPU path. The fused wrappers
-are forward only (the reference's callers take their gradients from jnp references). They take
+Everything runs on the GPU through the built library; there is no CPU path. The fused and the
+8-bit wrappers are forward only (the reference's callers take their gradients from jnp references). They take
 fp16 or bf16 activations, with weights and biases cast to fp16 for the kernels.
 """
 import torch
@@ -204,3 +209,112 @@ def transition(x, scale, offset, w1, b1, w2, b2, keep=None, add_input=False, eps
                          keep=_keep_rows(keep), eps=eps, add_input=add_input,
                          out=x2 if add_input else None)
     return out.reshape(lead + (out.shape[-1],))
+
+
+# ---- RMS norm and the 8-bit path (no counterpart in the reference) ----------------------------
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, scale, residual, eps):
+        out, total, rstd = hip.rms_norm(x, scale, residual, eps, want_rstd=True)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x if residual is None else total, scale, rstd)
+        return out if residual is None else (out, total)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, dsum=None):
+        s, scale, rstd = ctx.saved_tensors
+        dsum = None if dsum is None else dsum.to(s.dtype).contiguous()
+        if dout is None:  # only the sum was used
+            ds, dscale = dsum, torch.zeros_like(scale)
+        else:
+            ds, dscale = hip.rms_norm_bwd(s, scale, rstd, dout.to(s.dtype).contiguous(), dsum)
+        need = ctx.needs_input_grad
+        return ds if need[0] else None, dscale if need[1] else None, ds if need[2] else None, None
+
+
+def rms_norm(x, scale, residual=None, eps=1e-5):
+    """y [..., c] = s / sqrt(mean(s^2) + eps) * scale with s = x, or (y, s) with s = x + residual
+    rounded to x's type: the residual stream, which the next block adds to. x and residual fp16 or
+    bf16, one shape; scale [c]. Differentiable in x, residual and scale (once).
+
+    A call that needs gradients is refused while a HIP graph is being captured: torch may order such a
+    backward against the streams of an eager pass over the same leaves, which a capture cannot
+    hold. Capture hip.rms_norm and hip.rms_norm_bwd instead, which take their buffers."""
+    if residual is not None and residual.shape != x.shape:
+        raise hip.InvalidArgument(hip.INVALID_ARGUMENT, "rms_norm: residual must be like x, got %s and %s"
+                                  % (tuple(residual.shape), tuple(x.shape)))
+    if torch.is_grad_enabled() and x.is_cuda and torch.cuda.is_current_stream_capturing() and any(
+            t is not None and t.requires_grad for t in (x, scale, residual)):
+        raise hip.InvalidArgument(hip.INVALID_ARGUMENT, "rms_norm: a differentiated call cannot be captured into a "
+                                  "graph; capture hip.rms_norm and hip.rms_norm_bwd")
+    x2, lead = _rows(x)
+    r2 = None if residual is None else _rows(residual)[0]
+    res = _RmsNorm.apply(x2, scale.float().contiguous(), r2, float(eps))
+    if residual is None:
+        return res.reshape(lead + (x.shape[-1],))
+    return tuple(t.reshape(lead + (x.shape[-1],)) for t in res)
+
+
+def _q8_lead(q, q_scale, lead):
+    return q.reshape(lead + (q.shape[-1],)), q_scale.reshape(lead)
+
+
+def rms_norm_q8(x, scale, residual=None, eps=1e-5):
+    """(q, q_scale, s): rms_norm with its result as 8-bit rows, q [..., hip.padded_k(c)] int8 and
+    q_scale [...] fp32; s as in rms_norm, None without a residual."""
+    x2, lead = _rows(x)
+    r2 = None if residual is None else _rows(residual)[0]
+    q, q_scale, total = hip.rms_norm_q8(x2, scale.float().contiguous(), r2, eps)
+    return _q8_lead(q, q_scale, lead) + (None if total is None else total.reshape(x.shape),)
+
+
+_ACTIVATIONS = {None: 0, "relu": 1, "swish_gate": 2}
+
+
+def quantize_rows(x, activation=None):
+    """(q, q_scale): the 8-bit rows of x [..., k] (fp16, bf16 or fp32), of relu(x) ("relu"), or of
+    swish(x[..., :k]) * x[..., k:] ("swish_gate", x [..., 2k])."""
+    if activation not in _ACTIVATIONS:
+        raise hip.InvalidArgument(hip.INVALID_ARGUMENT, "quantize_rows: activation is None, 'relu' or 'swish_gate', got %r"
+                                  % (activation,))
+    x2, lead = _rows(x)
+    return _q8_lead(*hip.quantize_rows(x2, _ACTIVATIONS[activation]), lead)
+
+
+def dequantize_rows(q, q_scale, k=None, dtype=torch.float16):
+    """What 8-bit rows stand for: [..., k] of `dtype` (k: all of q's columns)."""
+    q2, lead = _rows(q)
+    out = hip.dequantize_rows(q2, q_scale.reshape(-1).contiguous(), k, dtype)
+    return out.reshape(lead + (out.shape[-1],))
+
+
+def q8_weights(w):
+    """(wq, w_scale) of w [k, n]: each output channel quantised with a scale of its own and laid out for
+    q8_projection, once, when a program loads its weights."""
+    q, w_scale = hip.quantize_rows(layouts.linear_T(w))
+    return layouts.q8_blocked(q), w_scale
+
+
+def q8_projection(q, q_scale, weights, b=None, residual=None, dtype=torch.float16):
+    """out [..., n] = x@w (+ b) (+ residual) for the 8-bit rows q, q_scale of x and weights =
+    q8_weights(w); in residual's type, or `dtype` without one."""
+    wq, w_scale = weights
+    q2, lead = _rows(q)
+    r2 = None if residual is None else _rows(residual)[0]
+    out = hip.q8_projection(q2, q_scale.reshape(-1).contiguous(), wq, w_scale, None if b is None else b.float().contiguous(),
+                            r2, dtype if r2 is None else r2.dtype)
+    return out.reshape(lead + (out.shape[-1],))
+
+
+def q8_transition(x, scale, w1, b1, w2, b2, residual=None, activation="relu", add_input=False, eps=1e-5):
+    """out [..., c] = h@w2 + b2 (+ s), h the activation ("relu", or "swish_gate" over w1's two halves) of
+    RMS(s)@w1 + b1, s = x or x + residual: the transition with an RMS norm and 8-bit products. w1, w2 =
+    q8_weights of [c, hidden] (or [c, 2 hidden]) and [hidden, c]; b1, b2 may be None. With a residual
+    (out, s)."""
+    q, q_scale, total = rms_norm_q8(x, scale, residual, eps)
+    s = x if total is None else total
+    h = q8_projection(q, q_scale, w1, b1, dtype=x.dtype)
+    out = q8_projection(*quantize_rows(h, activation), w2, b2, residual=s if add_input else None, dtype=x.dtype)
+    return out if residual is None else (out, s)

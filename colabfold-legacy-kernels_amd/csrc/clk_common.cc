@@ -15,6 +15,7 @@ int g_stage_count = 0;
 
 const char* type_name(int t) {
     switch (t) {
+    case CLK_S8: return "S8";
     case CLK_S32: return "S32";
     case CLK_U8: return "U8";
     case CLK_F16: return "F16";

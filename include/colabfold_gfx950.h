@@ -26,7 +26,7 @@ extern "C" {
 
 typedef struct ihipStream_t* clk_stream; /* a hipStream_t; NULL is the null stream */
 
-enum clk_dtype { CLK_S32 = 4, CLK_U8 = 6, CLK_F16 = 10, CLK_F32 = 11, CLK_BF16 = 16 };
+enum clk_dtype { CLK_S8 = 2, CLK_S32 = 4, CLK_U8 = 6, CLK_F16 = 10, CLK_F32 = 11, CLK_BF16 = 16 };
 
 enum clk_status { CLK_OK = 0, CLK_INVALID_ARGUMENT = 3, CLK_INTERNAL = 13 };
 
@@ -210,6 +210,67 @@ int clk_opm_update(clk_stream stream, const clk_buffer* lhs, const clk_buffer* t
  * 16, D a multiple of 4 (D/4 at most 65535), F in {16,32,64,128}. */
 int clk_opm_outer(clk_stream stream, const clk_buffer* left, const clk_buffer* right,
                   const clk_buffer* wT, const clk_buffer* out);
+
+/* ---- RMS norm and 8-bit rows (no counterpart in the reference) ------------------------- */
+
+/* Activations (x, residual, sum, s, dout, dsum, ds, and out where it is 16-bit) are F16 or BF16, all of
+ * a call's one type. An absent optional buffer is any buffer of its type, unread and unwritten.
+ *
+ * 8-bit rows are a pair: q [R,Kp] S8 and scale [R] F32, with Kp = K rounded up to a multiple of 64 and
+ * the columns past K zero; column k of row r stands for q[r,k] * scale[r]. A row is quantised by its
+ * largest magnitude a: q = 127 t / a to the nearest integer (ties to even) and scale = a / 127, so q lies
+ * in -127..127. A row whose a is under 2^-119 (its scale would leave fp32's normal range) is all
+ * zeros with scale 0; a row that holds an infinity or NaN is all zeros with scale NaN. */
+
+/* out [M,C] = s / sqrt(mean(s^2) + eps) * scale over the last axis, with s = x, or with has_residual
+ * s = x + residual rounded to the activation type, which is also written to sum [M,C] (the residual
+ * stream). scale [C] F32; rstd [M] F32 receives 1 / sqrt(mean(s^2) + eps) with want_rstd, for the
+ * backward. C at least 1. sum may alias x or residual, and out either of them,
+ * but not sum. */
+int clk_rms_norm(clk_stream stream, const clk_buffer* x, const clk_buffer* residual,
+                 const clk_buffer* scale, const clk_buffer* sum, const clk_buffer* out,
+                 const clk_buffer* rstd, float eps, int32_t has_residual, int32_t want_rstd);
+
+/* The same norm with its result as 8-bit rows: q [M,Kp] S8, q_scale [M] F32. The rounding to 8 bits is
+ * the only one: s * scale is quantised from fp32, and q_scale carries 1 / sqrt(mean(s^2) + eps). */
+int clk_rms_norm_q8(clk_stream stream, const clk_buffer* x, const clk_buffer* residual,
+                    const clk_buffer* scale, const clk_buffer* sum, const clk_buffer* q,
+                    const clk_buffer* q_scale, float eps, int32_t has_residual);
+
+/* Gradients of clk_rms_norm: s [M,C] (x, or the forward's sum), scale [C], rstd [M], dout [M,C] and, with
+ * has_dsum, the gradient of sum, dsum [M,C] -> ds [M,C] = rstd (g - xh mean(g xh)) + dsum with xh =
+ * s rstd and g = dout scale (the gradient of x and of residual alike), dscale [C] F32 = the sum over the
+ * M rows of dout xh (zeros for M = 0). ds may alias dout or dsum. workspace: device scratch of at least
+ * clk_rms_norm_bwd_workspace_size() bytes, 256-byte aligned, not shared by two calls in flight.
+ * Bit-identical from run to run (no atomics). */
+int clk_rms_norm_bwd(clk_stream stream, const clk_buffer* s, const clk_buffer* scale,
+                     const clk_buffer* rstd, const clk_buffer* dout, const clk_buffer* dsum,
+                     const clk_buffer* ds, const clk_buffer* dscale, int32_t has_dsum,
+                     void* workspace, size_t workspace_bytes);
+
+/* Bytes of workspace clk_rms_norm_bwd needs for s [M,C] (0 on a shape that it would reject). */
+size_t clk_rms_norm_bwd_workspace_size(const clk_buffer* s);
+
+/* 8-bit rows q [M,Kp], q_scale [M] of h [M,K]: activation 0: h = x [M,K]; 1: h = relu(x); 2: h =
+ * swish(x[:, :K]) x[:, K:] with x [M,2K], swish(g) = g / (1 + exp(-g)). x F16, BF16 or F32; h is held in
+ * fp32. The same entry point quantises activations by token and weights wT [N,K] by output channel. */
+int clk_quantize_rows(clk_stream stream, const clk_buffer* x, const clk_buffer* q,
+                      const clk_buffer* q_scale, int64_t activation);
+
+/* out [M,K] (F16, BF16 or F32) = what the 8-bit rows q [M,Kp], q_scale [M] stand for. */
+int clk_dequantize_rows(clk_stream stream, const clk_buffer* q, const clk_buffer* q_scale,
+                        const clk_buffer* out);
+
+/* out [M,N] = (q w^T) * q_scale[m] * w_scale[n] [+ b[n]] [+ residual[m,n]], the products of 8-bit
+ * integers summed exactly in 32 bits. q [M,Kp] S8, q_scale [M] F32: 8-bit rows; wq S8
+ * [ceil(N/64), Kp/64, 4, 4, 16, 16]: the rows of 8-bit weights [N,Kp] in blocks of 64 channels by 64
+ * inputs, entry [., ., b, c, 4 g + i, j] being channel 16 g + 4 b + i, input 16 c + j of its block, zeros
+ * for channels past N; w_scale [N], b [N] F32; residual, out [M,N] F16 or BF16, one type. Kp at most
+ * 131008. out may alias residual. */
+int clk_q8_projection(clk_stream stream, const clk_buffer* q, const clk_buffer* q_scale,
+                      const clk_buffer* wq, const clk_buffer* w_scale, const clk_buffer* b,
+                      const clk_buffer* residual, const clk_buffer* out, int32_t has_b,
+                      int32_t has_residual);
 
 #ifdef __cplusplus
 }

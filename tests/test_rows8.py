@@ -1,0 +1,235 @@
+"""The RMS norm and the 8-bit path on the CPU: the float64 oracle against independent statements, the
+weights' layout element by element, and every refusal of the entry points, none of which touches a
+device. No kernel is launched here."""
+import numpy as np
+import pytest
+import torch
+
+from colabfold_legacy_kernels import hip as H
+from colabfold_legacy_kernels import layouts, torch_ops
+from oracle import rows8 as orr
+from test_capi import F16, F32, S32, buf, lib  # noqa: F401
+
+S8, BF16 = 2, 16
+
+
+# ---- the oracle ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind,dtype", [("f16", torch.float16), ("bf16", torch.bfloat16)])
+def test_round16_is_torchs(kind, dtype):
+    rng = np.random.default_rng(0)
+    v = (rng.standard_normal(4000) * 2.0 ** rng.integers(-30, 20, 4000)).astype(np.float32)
+    v[:4] = [0.0, 1e-7, 65519.0, 65520.0]
+    want = torch.from_numpy(v).to(dtype).double().numpy()
+    assert np.array_equal(orr.round16(v, kind), want)
+
+
+@pytest.mark.parametrize("with_dsum", [False, True])
+def test_gradients_against_differences(with_dsum):
+    """d/ds and d/dw of sum(y dy) + sum(s dsum) by central differences of the forward: with steps of 1e-5
+    their error is about 1e-10 from the third derivative and 1e-16 / 1e-5 from the subtraction."""
+    rng = np.random.default_rng(1)
+    s, w, dy, dsum = (rng.standard_normal(n) for n in ((3, 7), 7, (3, 7), (3, 7)))
+    eps, h = 1e-3, 1e-5
+
+    def loss(s, w):
+        return (orr.rms_norm(s, w, eps)[0] * dy).sum() + ((s * dsum).sum() if with_dsum else 0.0)
+
+    ds, dw = orr.rms_norm_bwd(s, w, dy, dsum if with_dsum else None, eps)
+    for i in range(3):
+        for j in range(7):
+            d = np.zeros((3, 7))
+            d[i, j] = h
+            assert abs((loss(s + d, w) - loss(s - d, w)) / (2 * h) - ds[i, j]) < 1e-8
+    for j in range(7):
+        d = np.zeros(7)
+        d[j] = h
+        assert abs((loss(s, w + d) - loss(s, w - d)) / (2 * h) - dw[j]) < 1e-8
+
+
+def test_quotients_and_project():
+    t = np.array([[1.0, -2.0, 0.5], [0.0, 0.0, 0.0], [1.0, np.inf, 0.0], [np.nan, 1.0, 2.0], [1e-37, 0.0, -1e-38]])
+    q, scale = orr.quotients(t)
+    assert np.allclose(q[0], [63.5, -127.0, 31.75]) and scale[0] == 2.0 / 127
+    assert (q[1:] == 0).all() and scale[1] == 0 and np.isnan(scale[2]) and np.isnan(scale[3]) and scale[4] == 0
+    rng = np.random.default_rng(2)
+    a, b = rng.integers(-127, 128, (3, 5)), rng.integers(-127, 128, (4, 5))
+    out, _ = orr.project(a, [1, 2, 3], b, [1, 1, 2, 1], [0.5] * 4, np.ones((3, 4)))
+    for i in range(3):
+        for j in range(4):
+            s = sum(int(a[i, k]) * int(b[j, k]) for k in range(5))
+            assert out[i, j] == s * [1, 2, 3][i] * [1, 1, 2, 1][j] + 1.5
+
+
+# ---- layouts ------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("lib_", ("numpy", "torch"))
+@pytest.mark.parametrize("n,kp", [(1, 64), (64, 128), (130, 192)])
+def test_q8_blocked(lib_, n, kp):
+    q = np.random.default_rng(n).integers(-127, 128, (n, kp)).astype(np.int8)
+    arg = torch.from_numpy(q) if lib_ == "torch" else q
+    wq = layouts.q8_blocked(arg)
+    assert tuple(wq.shape) == (-(-n // 64), kp // 64, 4, 4, 16, 16)
+    for ch in range(0, wq.shape[0] * 64):
+        for k in (0, 15, 16, kp - 1, (7 * ch) % kp):
+            r, i = ch % 64, k % 64
+            got = int(wq[ch // 64, k // 64, (r // 4) % 4, i // 16, 4 * (r // 16) + r % 4, i % 16])
+            assert got == (int(q[ch, k]) if ch < n else 0)
+    assert np.array_equal(np.asarray(layouts.q8_unblocked(wq, n)), q)
+
+
+def test_q8_blocked_refuses_other_widths():
+    with pytest.raises(ValueError, match="multiple of 64"):
+        layouts.q8_blocked(torch.zeros((4, 65), dtype=torch.int8))
+
+
+# ---- refusals of the C entry points ----------------------------------------------------------
+
+def refs(args):
+    return [a[0] for a in args]
+
+
+def norm_args(m=6, c=40, act=F16, **other):
+    d = dict(x=buf(act, m, c), residual=buf(act, m, c, data=0x200000), scale=buf(F32, c), sum=buf(act, m, c, data=0x300000),
+             out=buf(act, m, c, data=0x400000), rstd=buf(F32, m))
+    d.update(other)
+    return refs(d.values())
+
+
+@pytest.mark.parametrize("other,eps,message", [
+    (dict(x=buf(F16, 6)), 1e-5, r"x must be \[M,C\]"),
+    (dict(x=buf(F32, 6, 40)), 1e-5, "must be F16, got F32"),
+    (dict(residual=buf(BF16, 6, 40)), 1e-5, "must be F16, got BF16"),
+    (dict(residual=buf(F16, 6, 41)), 1e-5, "residual and sum must be like x"),
+    (dict(sum=buf(F16, 5, 40)), 1e-5, "residual and sum must be like x"),
+    (dict(scale=buf(F32, 41)), 1e-5, r"scale must be \[C\]"),
+    (dict(out=buf(F16, 6, 39)), 1e-5, "out must be like x"),
+    (dict(out=buf(F16, 6, 40, data=0x300000)), 1e-5, "must not be the same buffer"),
+    (dict(rstd=buf(F32, 7)), 1e-5, r"rstd must be \[M\]"),
+    (dict(), -1.0, "eps must not be negative"),
+    (dict(), float("nan"), "eps must not be negative"),
+])
+def test_rms_norm_refusals(lib, other, eps, message):
+    import re
+    st = lib.clk_rms_norm(None, *norm_args(**other), eps, 1, 1)
+    assert st == 3 and re.search(message, lib.clk_last_error().decode()), lib.clk_last_error()
+
+
+def test_rms_norm_empty(lib):
+    assert lib.clk_rms_norm(None, *norm_args(m=0), 1e-5, 1, 1) == 0
+    assert lib.clk_rms_norm(None, *norm_args(c=0), 1e-5, 1, 1) == 3
+    assert "C must be at least 1" in lib.clk_last_error().decode()
+
+
+def test_rms_norm_q8_refusals(lib):
+    a = dict(x=buf(F16, 6, 40), residual=buf(F16, 1), scale=buf(F32, 40), sum=buf(F16, 1), q=buf(S8, 6, 64), qs=buf(F32, 6))
+    for other, message in ((dict(q=buf(S8, 6, 40)), "q must be [M,Kp]"), (dict(q=buf(F16, 6, 64)), "must be S8"),
+                           (dict(qs=buf(F32, 5)), "q_scale must be [M]"),
+                           (dict(q=buf(S8, 6, 64, data=0x100008)), "16-byte aligned")):
+        assert lib.clk_rms_norm_q8(None, *refs({**a, **other}.values()), 1e-5, 0) == 3
+        assert message in lib.clk_last_error().decode()
+
+
+def test_rms_norm_bwd_refusals(lib):
+    m, c = 6, 40
+    a = dict(s=buf(F16, m, c), scale=buf(F32, c), rstd=buf(F32, m), dout=buf(F16, m, c), dsum=buf(F16, m, c),
+             ds=buf(F16, m, c), dscale=buf(F32, c))
+    need = lib.clk_rms_norm_bwd_workspace_size(a["s"][0])
+    assert need >= 4 * c and need % 256 == 0
+    for other, message in ((dict(scale=buf(F32, c + 1)), "scale and dscale must be [C]"),
+                           (dict(dscale=buf(F32, c - 1)), "scale and dscale must be [C]"),
+                           (dict(rstd=buf(F32, m + 1)), "rstd must be [M]"),
+                           (dict(dout=buf(F16, m, c + 1)), "must be like s"), (dict(dsum=buf(F16, 1)), "must be like s"),
+                           (dict(ds=buf(BF16, m, c)), "must be F16")):
+        assert lib.clk_rms_norm_bwd(None, *refs({**a, **other}.values()), 1, 0x100000, need) == 3
+        assert message in lib.clk_last_error().decode()
+    for ws, size, message in ((0x100000, need - 1, "workspace of"), (None, need, "workspace of"),
+                              (0x100010, need, "256-byte aligned")):
+        assert lib.clk_rms_norm_bwd(None, *refs(a.values()), 1, ws, size) == 3
+        assert message in lib.clk_last_error().decode()
+    assert lib.clk_rms_norm_bwd_workspace_size(buf(F16, 0, c)[0]) == 0
+    assert lib.clk_rms_norm_bwd_workspace_size(None) == 0
+
+
+def test_quantize_rows_refusals(lib):
+    for x, q, s, act, message in (
+            (buf(F16, 6, 40), buf(S8, 6, 64), buf(F32, 6), 3, "activation is 0 (none)"),
+            (buf(F16, 6, 40), buf(S8, 6, 64), buf(F32, 6), -1, "activation is 0 (none)"),
+            (buf(S32, 6, 40), buf(S8, 6, 64), buf(F32, 6), 0, "must be F16, got S32"),
+            (buf(F16, 6, 41), buf(S8, 6, 64), buf(F32, 6), 2, "must be [M,2K]"),
+            (buf(F16, 6, 40), buf(S8, 6, 40), buf(F32, 6), 0, "q must be [M,Kp]"),
+            (buf(F16, 6, 160), buf(S8, 6, 192), buf(F32, 6), 2, "q must be [M,Kp]"),
+            (buf(F16, 6, 40), buf(S8, 6, 64), buf(F32, 7), 0, "q_scale must be [M]"),
+            (buf(F16, 6, 0), buf(S8, 6, 0), buf(F32, 6), 0, "C must be at least 1"),
+            (buf(F16, 6), buf(S8, 6, 64), buf(F32, 6), 0, "must be [M,C]"),
+            (buf(F16, 6, 40), buf(S8, 6, 64, data=0x100004), buf(F32, 6), 0, "16-byte aligned")):
+        assert lib.clk_quantize_rows(None, x[0], q[0], s[0], act) == 3
+        assert message in lib.clk_last_error().decode(), message
+    assert lib.clk_quantize_rows(None, buf(F16, 0, 40)[0], buf(S8, 0, 64)[0], buf(F32, 0)[0], 0) == 0
+
+
+def test_dequantize_rows_refusals(lib):
+    for q, s, out, message in ((buf(S8, 6, 64), buf(F32, 6), buf(F16, 6, 65), "q must be [M,Kp]"),
+                               (buf(S8, 6, 64), buf(F32, 5), buf(F16, 6, 64), "q_scale must be [M]"),
+                               (buf(S8, 6, 64), buf(F32, 6), buf(S32, 6, 64), "must be F16, got S32"),
+                               (buf(F16, 6, 64), buf(F32, 6), buf(F16, 6, 64), "must be S8")):
+        assert lib.clk_dequantize_rows(None, q[0], s[0], out[0]) == 3
+        assert message in lib.clk_last_error().decode()
+
+
+def test_q8_projection_refusals(lib):
+    m, kp, n = 6, 128, 100
+    a = dict(q=buf(S8, m, kp), qs=buf(F32, m), wq=buf(S8, 2, 2, 4, 4, 16, 16), ws=buf(F32, n), b=buf(F32, n),
+             residual=buf(F16, m, n), out=buf(F16, m, n))
+    for other, message in ((dict(q=buf(S8, m, 96)), "Kp must be a multiple of 64"),
+                           (dict(q=buf(S8, m, 131072)), "from 64 to 131008"),
+                           (dict(q=buf(S8, m, 0)), "Kp must be a multiple of 64"),
+                           (dict(q=buf(S8, m + 1, kp)), "q must be [M,Kp] and out [M,N]"),
+                           (dict(q=buf(F16, m, kp)), "must be S8"),
+                           (dict(qs=buf(F32, m - 1)), "q_scale must be [M]"),
+                           (dict(wq=buf(S8, 1, 2, 4, 4, 16, 16)), "wq must be"),
+                           (dict(wq=buf(S8, 2, 1, 4, 4, 16, 16)), "wq must be"),
+                           (dict(wq=buf(S8, n, kp)), "wq must be"),
+                           (dict(ws=buf(F32, n + 1)), "w_scale and b must be [N]"),
+                           (dict(b=buf(F32, 1)), "w_scale and b must be [N]"),
+                           (dict(b=buf(F16, n)), "must be F32"),
+                           (dict(residual=buf(F16, 1)), "residual must be like out"),
+                           (dict(residual=buf(BF16, m, n)), "must be F16, got BF16"),
+                           (dict(out=buf(F32, m, n)), "must be F16"),
+                           (dict(wq=buf(S8, 2, 2, 4, 4, 16, 16, data=0x100008)), "16-byte aligned")):
+        st = lib.clk_q8_projection(None, *refs({**a, **other}.values()), 1, 1)
+        assert st == 3 and message in lib.clk_last_error().decode(), (message, lib.clk_last_error())
+    empty = dict(a, q=buf(S8, 0, kp), qs=buf(F32, 0), residual=buf(F16, 0, n), out=buf(F16, 0, n))
+    assert lib.clk_q8_projection(None, *refs(empty.values()), 1, 1) == 0
+    none = dict(a, wq=buf(S8, 0, 2, 4, 4, 16, 16), ws=buf(F32, 0), b=buf(F32, 0), residual=buf(F16, m, 0), out=buf(F16, m, 0))
+    assert lib.clk_q8_projection(None, *refs(none.values()), 1, 1) == 0
+
+
+# ---- refusals of the Python entry points -------------------------------------------------------
+
+def test_cpu_tensors_are_refused():
+    x, w = torch.zeros((4, 64), dtype=torch.float16), torch.ones(64)
+    q, s = torch.zeros((4, 64), dtype=torch.int8), torch.ones(4)
+    wq, ws = layouts.q8_blocked(torch.zeros((8, 64), dtype=torch.int8)), torch.ones(8)
+    for call in (lambda: H.rms_norm(x, w), lambda: H.rms_norm_q8(x, w), lambda: H.quantize_rows(x),
+                 lambda: H.dequantize_rows(q, s), lambda: H.q8_projection(q, s, wq, ws),
+                 lambda: H.rms_norm_bwd(x, w, s, x), lambda: torch_ops.rms_norm(x, w),
+                 lambda: torch_ops.q8_projection(q, s, (wq, ws))):
+        with pytest.raises(H.InvalidArgument, match="must be on one GPU"):
+            call()
+
+
+def test_shapes_are_refused():
+    x = torch.zeros((2, 4, 64), dtype=torch.float16)
+    for call in (lambda: H.rms_norm(x, x), lambda: H.rms_norm_q8(x, x), lambda: H.quantize_rows(x),
+                 lambda: H.dequantize_rows(x, x), lambda: H.q8_projection(x, x, x, x)):
+        with pytest.raises(H.InvalidArgument, match="expected a matrix"):
+            call()
+    with pytest.raises(H.InvalidArgument, match="residual must be like x"):
+        torch_ops.rms_norm(x, torch.ones(64), x[:1])
+    with pytest.raises(H.InvalidArgument, match="activation is None"):
+        torch_ops.quantize_rows(x, "gelu")
+
+
+def test_padded_k():
+    assert [H.padded_k(k) for k in (1, 63, 64, 65, 128, 8191)] == [64, 64, 64, 128, 128, 8192]
