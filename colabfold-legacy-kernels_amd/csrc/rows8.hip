@@ -13,6 +13,7 @@
 #include "clk_common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace clk {
 
@@ -64,12 +65,127 @@ __device__ __forceinline__ float inv_rms(float ss, float inv_c, float eps) { ret
 constexpr float kBig = 0x1p40f, kDown = 0x1p-90f;
 __device__ __forceinline__ bool is_big(uint32_t bits) { return bits >= __builtin_bit_cast(uint32_t, kBig) && bits < kInfBits; }
 
-// Sum and maximum over the threads of a block, in every thread; `slot` alternates between calls that no
-// barrier separates otherwise.
+// v of the lane that DPP control CTRL names
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+struct Sum {
+    __device__ __forceinline__ uint32_t operator()(uint32_t a, uint32_t b) const {
+        return __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b));
+    }
+};
+struct Max {
+    __device__ __forceinline__ uint32_t operator()(uint32_t a, uint32_t b) const { return max(a, b); }
+};
+
+// op over each aligned group of W lanes (8 to 64), in every lane of it: by DPP within 16 lanes (pairs, quads,
+// mirrored halves), then by swaps of 16- and 32-lane rows. Both lanes of a step take the same two
+// values, so all lanes end with the same bits.
+template <int W, typename Op>
+__device__ __forceinline__ uint32_t lanes_all(uint32_t v, Op op) {
+    v = op(v, dpp<0xB1>(v));   // quad_perm [1,0,3,2]
+    v = op(v, dpp<0x4E>(v));   // quad_perm [2,3,0,1]
+    v = op(v, dpp<0x141>(v));  // row_half_mirror
+    if constexpr (W >= 16) v = op(v, dpp<0x140>(v));  // row_mirror
+    if constexpr (W >= 32) {
+        const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = op(s[0], s[1]);
+    }
+    if constexpr (W >= 64) {
+        const auto s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = op(s[0], s[1]);
+    }
+    return v;
+}
+template <int W>
+__device__ __forceinline__ float lanes_sum(float v) {
+    return __builtin_bit_cast(float, lanes_all<W>(__builtin_bit_cast(uint32_t, v), Sum()));
+}
+template <int W>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) { return lanes_all<W>(v, Max()); }
+
+// A row's sum and maxima over its TPR threads: its lane group, or (TPR > 64) the block's waves through LDS. `slots`
+// is one of two sets that alternate, so that one barrier a call is enough: a wave that writes a set again
+// has passed the barrier of the call between, which every reader of the set reached after its reads.
+struct Stats {
+    float sum;
+    uint32_t max0, max1;
+};
+template <int TPR>
+struct RowShare {
+    Stats slots[2][TPR > kWave ? TPR / kWave : 1];
+};
+template <int TPR>
+__device__ __forceinline__ Stats row_all(Stats s, RowShare<TPR>& share, int& turn) {
+    constexpr int W = TPR < kWave ? TPR : kWave;
+    s.sum = lanes_sum<W>(s.sum);
+    s.max0 = lanes_max<W>(s.max0);
+    s.max1 = lanes_max<W>(s.max1);
+    if constexpr (TPR > kWave) {
+        Stats* slot = share.slots[turn];
+        turn ^= 1;
+        if ((threadIdx.x & (kWave - 1)) == 0) slot[threadIdx.x / kWave] = s;
+        __syncthreads();
+        s = slot[0];
+#pragma unroll
+        for (int i = 1; i < TPR / kWave; ++i) {
+            s.sum += slot[i].sum;
+            s.max0 = max(s.max0, slot[i].max0);
+            s.max1 = max(s.max1, slot[i].max1);
+        }
+    }
+    return s;
+}
+
+// Rows are split in chunks of 8 values. Widths and addresses are any, so a chunk is loaded and stored by one
+// 16-byte access of 2-byte alignment (the hardware takes any; aligned rows lose nothing), and the one
+// chunk that the width cuts value by value.
+__device__ __forceinline__ half8 load8(const half_t* row, int col, int C) {
+    if (col + 8 <= C) return *reinterpret_cast<const half8u*>(row + col);
+    half8 v = {};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (col + e < C) v[e] = row[col + e];
+    return v;
+}
+__device__ __forceinline__ void store8(half_t* row, int col, int C, half8 v) {
+    if (col + 8 <= C) {
+        *reinterpret_cast<half8u*>(row + col) = v;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (col + e < C) row[col + e] = v[e];
+    }
+}
+__device__ __forceinline__ float8v load8f(const float* row, int col, int C) {
+    if (col + 8 <= C) return *reinterpret_cast<const float8u*>(row + col);
+    float8v v = {};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (col + e < C) v[e] = row[col + e];
+    return v;
+}
+__device__ __forceinline__ void store8f(float* row, int col, int C, float8v v) {
+    if (col + 8 <= C) {
+        *reinterpret_cast<float8u*>(row + col) = v;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (col + e < C) row[col + e] = v[e];
+    }
+}
+__device__ __forceinline__ uint2v quant8(const float (&t)[8], float inv) {
+    int q[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[e] = quant(t[e], inv);
+    return uint2v{pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7])};
+}
+
+// Sum and maximum over the 256 threads of a block, for the kernels that take a row of any length.
 template <int THREADS>
 __device__ __forceinline__ float block_sum(float v, float* slot) {
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) v += __shfl_xor(v, o);
+    v = lanes_sum<kWave>(v);
     if ((threadIdx.x & (kWave - 1)) == 0) slot[threadIdx.x / kWave] = v;
     __syncthreads();
     float s = 0.f;
@@ -80,8 +196,7 @@ __device__ __forceinline__ float block_sum(float v, float* slot) {
 }
 template <int THREADS>
 __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* slot) {
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
+    v = lanes_max<kWave>(v);
     if ((threadIdx.x & (kWave - 1)) == 0) slot[threadIdx.x / kWave] = v;
     __syncthreads();
     uint32_t s = 0;
@@ -172,6 +287,84 @@ __global__ __launch_bounds__(256) void rms_norm_any_kernel(RmsArgs a) {
     }
 }
 
+// Rows of up to 8 TPR NCH values, held in registers: TPR threads a row, NCH chunks each, one pass over memory.
+constexpr int block_of(int tpr) { return tpr < 256 ? 256 : tpr; }
+
+template <bool BF, int TPR, int NCH, bool RES, bool Q8>
+__global__ __launch_bounds__(block_of(TPR)) void rms_norm_kernel(RmsArgs a) {
+    constexpr int ROWS = block_of(TPR) / TPR;
+    __shared__ RowShare<TPR> share;
+    const int part = threadIdx.x % TPR, sub = threadIdx.x / TPR, C = (int)a.C, Kp = (int)a.Kp;
+    int turn = 0;
+    float8v w[NCH];
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) w[j] = load8f(a.w, 8 * (part + TPR * j), C);
+    for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.M; r0 += (int64_t)gridDim.x * ROWS) {
+        const int64_t row = r0 + sub;
+        const bool in = ROWS == 1 || row < a.M;
+        const int len = in ? C : 0;  // a row past M is read as one of no values
+        const half_t* xr = a.x + row * C;
+        half8 v[NCH], res[NCH];
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) v[j] = load8(xr, 8 * (part + TPR * j), len);
+        if constexpr (RES) {
+#pragma unroll
+            for (int j = 0; j < NCH; ++j) res[j] = load8(a.residual + row * C, 8 * (part + TPR * j), len);
+#pragma unroll
+            for (int j = 0; j < NCH; ++j) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[j][e] = act_cvt<BF>(act_get<BF>(v[j], e) + act_get<BF>(res[j], e));
+                store8(a.sum + row * C, 8 * (part + TPR * j), len, v[j]);
+            }
+        }
+        Stats s{0.f, 0, 0};
+        const auto collect = [&](float d) __attribute__((always_inline)) {
+            s = Stats{0.f, 0, 0};
+#pragma unroll
+            for (int j = 0; j < NCH; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float f = act_get<BF>(v[j], e) * d;
+                    s.sum += f * f;
+                    if constexpr (BF) s.max0 = max(s.max0, abs_bits(f));
+                    if constexpr (Q8) s.max1 = max(s.max1, abs_bits(f * w[j][e]));
+                }
+            s = row_all<TPR>(s, share, turn);
+        };
+        collect(1.f);
+        float d = 1.f;
+        if constexpr (BF) {
+            if (is_big(s.max0)) {
+                d = kDown;
+                collect(d);
+            }
+        }
+        const float r = inv_rms(s.sum, a.inv_c, d == 1.f ? a.eps : 0.f);
+        if constexpr (Q8) {
+            float inv, scale;
+            row_scale(s.max1, r, inv, scale);
+            if (part == 0 && in) a.stat[row] = scale;
+#pragma unroll
+            for (int j = 0; j < NCH; ++j) {
+                const int col = 8 * (part + TPR * j);
+                float t[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) t[e] = act_get<BF>(v[j], e) * d * w[j][e];
+                if (in && col < Kp) *reinterpret_cast<uint2v*>(a.q + row * Kp + col) = quant8(t, inv);
+            }
+        } else {
+            if (part == 0 && in && a.stat != nullptr) a.stat[row] = r * d;
+#pragma unroll
+            for (int j = 0; j < NCH; ++j) {
+                half8 o;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] = act_cvt<BF>(act_get<BF>(v[j], e) * d * r * w[j][e]);
+                store8(a.out + row * C, 8 * (part + TPR * j), len, o);
+            }
+        }
+    }
+}
+
 // ---- its gradients ------------------------------------------------------------------------
 
 struct RmsBwdArgs {
@@ -213,30 +406,128 @@ __global__ __launch_bounds__(256) void rms_norm_bwd_any_kernel(RmsBwdArgs a) {
     }
 }
 
-// dw[c] = the sum of the P partial rows, in their order within each of 8 interleaved groups
+// Rows of up to 8 TPR NCH values in registers, a block's share of dw in registers too, until its rows are done.
+template <bool BF, int TPR, int NCH, bool DSUM>
+__global__ __launch_bounds__(block_of(TPR)) void rms_norm_bwd_kernel(RmsBwdArgs a) {
+    constexpr int ROWS = block_of(TPR) / TPR;
+    __shared__ RowShare<TPR> share;
+    __shared__ float8v groups[ROWS > 1 ? (ROWS - 1) * TPR * NCH : 1];
+    const int part = threadIdx.x % TPR, sub = threadIdx.x / TPR, C = (int)a.C;
+    int turn = 0;
+    float8v w[NCH], dw[NCH];
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) {
+        w[j] = load8f(a.w, 8 * (part + TPR * j), C);
+        dw[j] = float8v{};
+    }
+    for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.M; r0 += (int64_t)a.P * ROWS) {
+        const int64_t row = r0 + sub;
+        const int len = ROWS == 1 || row < a.M ? C : 0;
+        const float r = len > 0 ? a.rstd[row] : 0.f;
+        half8 s[NCH], dy[NCH], dz[NCH];
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            s[j] = load8(a.s + row * C, 8 * (part + TPR * j), len);
+            dy[j] = load8(a.dout + row * C, 8 * (part + TPR * j), len);
+            if constexpr (DSUM) dz[j] = load8(a.dsum + row * C, 8 * (part + TPR * j), len);
+        }
+        Stats t{0.f, 0, 0};
+#pragma unroll
+        for (int j = 0; j < NCH; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float g = act_get<BF>(dy[j], e), xh = act_get<BF>(s[j], e) * r;
+                t.sum += g * w[j][e] * xh;
+                dw[j][e] += g * xh;
+            }
+        const float dot = row_all<TPR>(t, share, turn).sum * a.inv_c;
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            half8 o;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float xh = act_get<BF>(s[j], e) * r;
+                float d = r * (act_get<BF>(dy[j], e) * w[j][e] - xh * dot);
+                if constexpr (DSUM) d += act_get<BF>(dz[j], e);
+                o[e] = act_cvt<BF>(d);
+            }
+            store8(a.ds + row * C, 8 * (part + TPR * j), len, o);
+        }
+    }
+    if constexpr (ROWS > 1) {  // the block's row groups, in order
+#pragma unroll
+        for (int j = 0; j < NCH; ++j)
+            if (sub > 0) groups[((sub - 1) * NCH + j) * TPR + part] = dw[j];
+        __syncthreads();
+        if (sub > 0) return;
+#pragma unroll
+        for (int j = 0; j < NCH; ++j)
+            for (int i = 0; i < ROWS - 1; ++i) dw[j] += groups[(i * NCH + j) * TPR + part];
+    }
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) {
+        const int col = 8 * (part + TPR * j);
+        if (col < a.ldp) *reinterpret_cast<float8v*>(a.partial + (int64_t)blockIdx.x * a.ldp + col) = dw[j];
+    }
+}
+
+// dw[c] = the sum of the P partial rows: 16 interleaved groups of them, each in order, then the groups
 __global__ __launch_bounds__(256) void rms_norm_dw_kernel(RmsBwdArgs a) {
-    __shared__ float sums[8][32];
-    const int col = threadIdx.x & 31, grp = threadIdx.x >> 5;
-    const int64_t c = (int64_t)blockIdx.x * 32 + col;
+    __shared__ float sums[16][16];
+    const int col = threadIdx.x & 15, grp = threadIdx.x >> 4;
+    const int64_t c = (int64_t)blockIdx.x * 16 + col;
     float v = 0.f;
     if (c < a.C) {
-        for (int p = grp; p < a.P; p += 8) v += a.partial[(int64_t)p * a.ldp + c];
+        const float* p = a.partial + c;
+        int i = grp;
+        for (; i + 7 * 16 < a.P; i += 8 * 16) {
+            float u[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) u[k] = p[(int64_t)(i + 16 * k) * a.ldp];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v += u[k];
+        }
+        for (; i < a.P; i += 16) v += p[(int64_t)i * a.ldp];
     }
     sums[grp][col] = v;
     __syncthreads();
     if (grp == 0 && c < a.C) {
         float t = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) t += sums[i][col];
+        for (int i = 0; i < 16; ++i) t += sums[i][col];
         a.dw[c] = t;
     }
 }
 
+// Threads a row and 8-value chunks a thread for rows of Kp values (0: the kernels for rows of any length).
+struct Route {
+    int tpr, nch;
+};
+Route route_of(int64_t Kp) {
+    if (Kp <= 64) return {8, 1};
+    if (Kp <= 128) return {16, 1};
+    if (Kp <= 256) return {32, 1};
+    if (Kp <= 512) return {64, 1};
+    if (Kp <= 1024) return {64, 2};
+    if (Kp <= 2048) return {256, 1};
+    if (Kp <= 4096) return {256, 2};
+    if (Kp <= 6144) return {256, 3};
+    if (Kp <= 8192) return {512, 2};
+    if (Kp <= 16384) return {1024, 2};
+    return {0, 0};
+}
+#define CLK_ROUTES(X_) X_(8, 1) X_(16, 1) X_(32, 1) X_(64, 1) X_(64, 2) X_(256, 1) X_(256, 2) X_(256, 3) X_(512, 2) X_(1024, 2)
+
+int64_t padded64(int64_t k) { return (k + 63) / 64 * 64; }
+
 // The workgroups of the backward's first kernel: a rule on the shape alone, so that results do not
-// depend on the device.
+// depend on the device. One round of what 256 CUs hold, but where rows are few, about 8 steps each: a
+// workgroup costs its row of partial sums, written and read.
 int bwd_parts(int64_t M, int64_t C) {
-    (void)C;
-    return (int)std::min<int64_t>(M, 512);
+    const Route rt = route_of(padded64(C));
+    const int rows = rt.tpr > 0 ? block_of(rt.tpr) / rt.tpr : 1, threads = rt.tpr > 0 ? block_of(rt.tpr) : 256;
+    const int64_t steps = (M + rows - 1) / rows, most = 256 * 1024 / threads;
+    return (int)std::min(steps, std::min<int64_t>(most, std::max<int64_t>(256, steps / 8)));
 }
 int64_t bwd_ldp(int64_t C) { return (C + 63) / 64 * 64; }
 
@@ -290,6 +581,60 @@ __global__ __launch_bounds__(256) void quantize_any_kernel(QuantArgs a) {
     }
 }
 
+// 8 values of h from column col of a row
+template <int T, int ACT>
+__device__ __forceinline__ void hidden8(const void* x, int64_t row, int col, int K, int len, float (&h)[8]) {
+    const int64_t at = row * (ACT == kActSwish ? 2 * (int64_t)K : K);
+    if constexpr (T == kF32) {
+        const float* p = static_cast<const float*>(x) + at;
+        const float8v g = load8f(p, col, len);
+        float8v u;
+        if constexpr (ACT == kActSwish) u = load8f(p + K, col, len);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = ACT == kActSwish ? g[e] * sigmoid_fast(g[e]) * u[e] : ACT == kActRelu ? relu(g[e]) : g[e];
+    } else {
+        constexpr bool BF = T == kBf16;
+        const half_t* p = static_cast<const half_t*>(x) + at;
+        const half8 g = load8(p, col, len);
+        half8 u;
+        if constexpr (ACT == kActSwish) u = load8(p + K, col, len);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float f = act_get<BF>(g, e);
+            h[e] = ACT == kActSwish ? f * sigmoid_fast(f) * act_get<BF>(u, e) : ACT == kActRelu ? relu(f) : f;
+        }
+    }
+}
+
+template <int T, int ACT, int TPR, int NCH>
+__global__ __launch_bounds__(block_of(TPR)) void quantize_kernel(QuantArgs a) {
+    constexpr int ROWS = block_of(TPR) / TPR;
+    __shared__ RowShare<TPR> share;
+    const int part = threadIdx.x % TPR, sub = threadIdx.x / TPR, K = (int)a.K, Kp = (int)a.Kp;
+    int turn = 0;
+    for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.M; r0 += (int64_t)gridDim.x * ROWS) {
+        const int64_t row = r0 + sub;
+        const bool in = ROWS == 1 || row < a.M;
+        float h[NCH][8];
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) hidden8<T, ACT>(a.x, row, 8 * (part + TPR * j), K, in ? K : 0, h[j]);
+        Stats s{0.f, 0, 0};
+#pragma unroll
+        for (int j = 0; j < NCH; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s.max0 = max(s.max0, abs_bits(h[j][e]));
+        s = row_all<TPR>(s, share, turn);
+        float inv, scale;
+        row_scale(s.max0, 1.f, inv, scale);
+        if (part == 0 && in) a.scale[row] = scale;
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            const int col = 8 * (part + TPR * j);
+            if (in && col < Kp) *reinterpret_cast<uint2v*>(a.q + row * Kp + col) = quant8(h[j], inv);
+        }
+    }
+}
+
 struct DequantArgs {
     const int8_t* q;
     const float* scale;
@@ -297,26 +642,31 @@ struct DequantArgs {
     int64_t M, K, Kp;
 };
 
+// 2^shift threads a row, 8 values each at a time
 template <int T>
-__global__ __launch_bounds__(256) void dequantize_any_kernel(DequantArgs a) {
-    for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
+__global__ __launch_bounds__(256) void dequantize_kernel(DequantArgs a, int shift) {
+    const int part = threadIdx.x & ((1 << shift) - 1), rows = 256 >> shift;
+    for (int64_t row = (int64_t)blockIdx.x * rows + (threadIdx.x >> shift); row < a.M; row += (int64_t)gridDim.x * rows) {
         const float sc = a.scale[row];
-        for (int64_t k = threadIdx.x; k < a.K; k += 256) {
-            const float v = (float)a.q[row * a.Kp + k] * sc;
+        for (int64_t c = 8 * part; c < a.K; c += 8 << shift) {
+            const uint2v q = *reinterpret_cast<const uint2v*>(a.q + row * a.Kp + c);
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)(q[e >> 2] >> 8 * (e & 3)) * sc;
+            const int left = (int)min<int64_t>(a.K - c, 8);
             if constexpr (T == kF32) {
-                static_cast<float*>(a.out)[row * a.K + k] = v;
+                store8f(static_cast<float*>(a.out) + row * a.K + c, 0, left, float8v{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]});
             } else {
-                static_cast<half_t*>(a.out)[row * a.K + k] = act_cvt<T == kBf16>(v);
+                half8 h;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) h[e] = act_cvt<T == kBf16>(v[e]);
+                store8(static_cast<half_t*>(a.out) + row * a.K + c, 0, left, h);
             }
         }
     }
 }
 
 // ---- host ---------------------------------------------------------------------------------
-
-int64_t padded64(int64_t k) { return (k + 63) / 64 * 64; }
-
-bool is_act(int t) { return t == CLK_F16 || t == CLK_BF16; }
 
 // M [rows] and C of an activation; the checks shared by the norm's entry points
 int check_rows(const char* what, const clk_buffer* x) {
@@ -328,7 +678,13 @@ int check_rows(const char* what, const clk_buffer* x) {
 
 bool is_matrix(const clk_buffer* b, int64_t r, int64_t c) { return b->rank == 2 && b->dims[0] == r && b->dims[1] == c; }
 
-unsigned row_blocks(int64_t M) { return (unsigned)std::min<int64_t>(M, 1 << 20); }
+unsigned any_blocks(int64_t M) { return (unsigned)std::min<int64_t>(M, 1 << 20); }
+
+// Workgroups for M rows of tpr threads each
+unsigned row_blocks(int64_t M, int tpr) {
+    const int rows = block_of(tpr) / tpr;
+    return (unsigned)std::min<int64_t>((M + rows - 1) / rows, 1 << 20);
+}
 
 int rms_forward(const char* what, clk_stream stream, const clk_buffer* x, const clk_buffer* residual,
                 const clk_buffer* scale, const clk_buffer* sum, const clk_buffer* out, const clk_buffer* stat,
@@ -358,12 +714,26 @@ int rms_forward(const char* what, clk_stream stream, const clk_buffer* x, const 
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const bool bf = act == CLK_BF16;
     stage_mark(s, 0);
-#define CLK_RMS(BF_, RES_, Q8_)                                                                      \
-    if (bf == BF_ && (has_residual != 0) == RES_ && q8 == Q8_)                                       \
-        hipLaunchKernelGGL((rms_norm_any_kernel<BF_, RES_, Q8_>), dim3(row_blocks(M)), dim3(256), 0, s, a);
-    CLK_RMS(false, false, false) CLK_RMS(false, false, true) CLK_RMS(false, true, false) CLK_RMS(false, true, true)
-    CLK_RMS(true, false, false) CLK_RMS(true, false, true) CLK_RMS(true, true, false) CLK_RMS(true, true, true)
-#undef CLK_RMS
+    const Route rt = route_of(Kp);
+#define CLK_RMS_RT(TPR_, NCH_)                                                                                        \
+    if (rt.tpr == TPR_ && rt.nch == NCH_) {                                                                           \
+        if (has_residual) hipLaunchKernelGGL((rms_norm_kernel<BF, TPR_, NCH_, true, Q8>), grid, block, 0, s, a);      \
+        else hipLaunchKernelGGL((rms_norm_kernel<BF, TPR_, NCH_, false, Q8>), grid, block, 0, s, a);                  \
+    }
+    const auto launch = [&](auto bf_, auto q8_) {
+        constexpr bool BF = decltype(bf_)::value, Q8 = decltype(q8_)::value;
+        if (rt.tpr == 0) {
+            const dim3 grid(any_blocks(M)), block(256);
+            if (has_residual) hipLaunchKernelGGL((rms_norm_any_kernel<BF, true, Q8>), grid, block, 0, s, a);
+            else hipLaunchKernelGGL((rms_norm_any_kernel<BF, false, Q8>), grid, block, 0, s, a);
+            return;
+        }
+        const dim3 grid(row_blocks(M, rt.tpr)), block(block_of(rt.tpr));
+        CLK_ROUTES(CLK_RMS_RT)
+    };
+    if (bf) q8 ? launch(std::true_type(), std::true_type()) : launch(std::true_type(), std::false_type());
+    else q8 ? launch(std::false_type(), std::true_type()) : launch(std::false_type(), std::false_type());
+#undef CLK_RMS_RT
     stage_mark(s, 1);
     return launch_status(what);
 }
@@ -421,10 +791,22 @@ extern "C" int clk_rms_norm_bwd(clk_stream stream, const clk_buffer* s, const cl
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     stage_mark(st, 0);
     if (M > 0) {
-        if (act == CLK_BF16) hipLaunchKernelGGL(rms_norm_bwd_any_kernel<true>, dim3(a.P), dim3(256), 0, st, a);
-        else hipLaunchKernelGGL(rms_norm_bwd_any_kernel<false>, dim3(a.P), dim3(256), 0, st, a);
+        const Route rt = route_of(padded64(C));
+#define CLK_BWD_RT(TPR_, NCH_)                                                                                        \
+    if (rt.tpr == TPR_ && rt.nch == NCH_) {                                                                           \
+        if (has_dsum) hipLaunchKernelGGL((rms_norm_bwd_kernel<BF, TPR_, NCH_, true>), grid, block, 0, st, a);         \
+        else hipLaunchKernelGGL((rms_norm_bwd_kernel<BF, TPR_, NCH_, false>), grid, block, 0, st, a);                 \
     }
-    hipLaunchKernelGGL(rms_norm_dw_kernel, dim3((unsigned)((C + 31) / 32)), dim3(256), 0, st, a);
+        const auto launch = [&](auto bf_) {
+            constexpr bool BF = decltype(bf_)::value;
+            const dim3 grid(a.P), block(rt.tpr == 0 ? 256 : block_of(rt.tpr));
+            if (rt.tpr == 0) hipLaunchKernelGGL(rms_norm_bwd_any_kernel<BF>, grid, block, 0, st, a);
+            CLK_ROUTES(CLK_BWD_RT)
+        };
+        act == CLK_BF16 ? launch(std::true_type()) : launch(std::false_type());
+#undef CLK_BWD_RT
+    }
+    hipLaunchKernelGGL(rms_norm_dw_kernel, dim3((unsigned)((C + 15) / 16)), dim3(256), 0, st, a);
     stage_mark(st, 1);
     return launch_status("rms_norm_bwd");
 }
@@ -448,13 +830,25 @@ extern "C" int clk_quantize_rows(clk_stream stream, const clk_buffer* x, const c
     if (!aligned16(q->data)) return invalid("quantize_rows: q must be 16-byte aligned");
     QuantArgs a{x->data, static_cast<int8_t*>(q->data), static_cast<float*>(q_scale->data), M, K, Kp};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    const int t = xt == CLK_F32 ? kF32 : xt == CLK_BF16 ? kBf16 : kF16;
     stage_mark(s, 0);
-#define CLK_QR(T_, A_) \
-    if (t == T_ && activation == A_) hipLaunchKernelGGL((quantize_any_kernel<T_, A_>), dim3(row_blocks(M)), dim3(256), 0, s, a);
-    CLK_QR(kF16, 0) CLK_QR(kF16, 1) CLK_QR(kF16, 2) CLK_QR(kBf16, 0) CLK_QR(kBf16, 1) CLK_QR(kBf16, 2)
-    CLK_QR(kF32, 0) CLK_QR(kF32, 1) CLK_QR(kF32, 2)
-#undef CLK_QR
+    const Route rt = route_of(Kp);
+#define CLK_QR_RT(TPR_, NCH_) \
+    if (rt.tpr == TPR_ && rt.nch == NCH_) hipLaunchKernelGGL((quantize_kernel<T, A, TPR_, NCH_>), grid, block, 0, s, a);
+    const auto launch = [&](auto t_, auto a_) {
+        constexpr int T = decltype(t_)::value, A = decltype(a_)::value;
+        const dim3 grid(rt.tpr == 0 ? any_blocks(M) : row_blocks(M, rt.tpr)), block(rt.tpr == 0 ? 256 : block_of(rt.tpr));
+        if (rt.tpr == 0) hipLaunchKernelGGL((quantize_any_kernel<T, A>), grid, block, 0, s, a);
+        CLK_ROUTES(CLK_QR_RT)
+    };
+    const auto by_act = [&](auto t_) {
+        if (activation == kActNone) launch(t_, std::integral_constant<int, kActNone>());
+        else if (activation == kActRelu) launch(t_, std::integral_constant<int, kActRelu>());
+        else launch(t_, std::integral_constant<int, kActSwish>());
+    };
+    if (xt == CLK_F32) by_act(std::integral_constant<int, kF32>());
+    else if (xt == CLK_BF16) by_act(std::integral_constant<int, kBf16>());
+    else by_act(std::integral_constant<int, kF16>());
+#undef CLK_QR_RT
     stage_mark(s, 1);
     return launch_status("quantize_rows");
 }
@@ -474,9 +868,12 @@ extern "C" int clk_dequantize_rows(clk_stream stream, const clk_buffer* q, const
     DequantArgs a{static_cast<const int8_t*>(q->data), static_cast<const float*>(q_scale->data), out->data, M, K, Kp};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     stage_mark(s, 0);
-    if (ot == CLK_F32) hipLaunchKernelGGL(dequantize_any_kernel<kF32>, dim3(row_blocks(M)), dim3(256), 0, s, a);
-    else if (ot == CLK_BF16) hipLaunchKernelGGL(dequantize_any_kernel<kBf16>, dim3(row_blocks(M)), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL(dequantize_any_kernel<kF16>, dim3(row_blocks(M)), dim3(256), 0, s, a);
+    int shift = 3;
+    while (shift < 8 && (8 << shift) < K) ++shift;
+    const dim3 grid(row_blocks(M, 1 << shift)), block(256);
+    if (ot == CLK_F32) hipLaunchKernelGGL(dequantize_kernel<kF32>, grid, block, 0, s, a, shift);
+    else if (ot == CLK_BF16) hipLaunchKernelGGL(dequantize_kernel<kBf16>, grid, block, 0, s, a, shift);
+    else hipLaunchKernelGGL(dequantize_kernel<kF16>, grid, block, 0, s, a, shift);
     stage_mark(s, 1);
     return launch_status("dequantize_rows");
 }
