@@ -51,6 +51,10 @@ __device__ __forceinline__ int4v load16(Rsrc r, uint32_t off) {
     return __builtin_bit_cast(int4v, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
 }
 
+// A sum with its scales and bias (0: none), in one order of roundings for every kernel, so that a row's
+// results do not depend on how many rows a call has
+__device__ __forceinline__ float scaled(int sum, float sx, float sw, float b) { return __builtin_fmaf((float)sum * sx, sw, b); }
+
 // Four consecutive channels n .. n + 3 of row m, of which those below N exist
 template <bool BF>
 __device__ __forceinline__ void store4(const GemmArgs& a, int m, int n, int4v acc) {
@@ -60,11 +64,7 @@ __device__ __forceinline__ void store4(const GemmArgs& a, int m, int n, int4v ac
     if (n + 4 <= a.N) {
         float v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = (float)acc[i] * sx * a.ws[n + i];
-        if (a.b != nullptr) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] += a.b[n + i];
-        }
+        for (int i = 0; i < 4; ++i) v[i] = scaled(acc[i], sx, a.ws[n + i], a.b != nullptr ? a.b[n + i] : 0.f);
         if (a.residual != nullptr) {
             const half4 h = *reinterpret_cast<const half4u*>(a.residual + at);
             const half8 r = half8{h[0], h[1], h[2], h[3], 0, 0, 0, 0};
@@ -76,8 +76,7 @@ __device__ __forceinline__ void store4(const GemmArgs& a, int m, int n, int4v ac
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (n + i >= a.N) break;
-            float v = (float)acc[i] * sx * a.ws[n + i];
-            if (a.b != nullptr) v += a.b[n + i];
+            float v = scaled(acc[i], sx, a.ws[n + i], a.b != nullptr ? a.b[n + i] : 0.f);
             if (a.residual != nullptr) v += act_get<BF>(half8{a.residual[at + i]}, 0);
             a.out[at + i] = act_cvt<BF>(v);
         }
@@ -126,6 +125,134 @@ __global__ __launch_bounds__(256) void q8_gemm_kernel(GemmArgs a) {
     }
 }
 
+// Large products. A workgroup computes BM = 16 MF WM rows by BN = 64 NB WN channels; wave (wm, wn) of WM x WN
+// has MF operands of 16 rows and NB weight blocks of 64 channels. Both operands go through LDS, 128 inputs
+// (two MFMA steps) a stage, two stages: the loads of the next stage are in flight while one is computed.
+//   weights  by 1024-byte direct-to-LDS loads, in memory order: an operand read is 64 lanes' consecutive 16
+//            bytes
+//   rows     eight rows of 128 bytes a load, position p of row r holding its 16-byte chunk p ^ (r / 2 % 8): a
+//            16-lane group reads one chunk of 16 rows from 16 different bank quadruples
+template <bool BF, int MF, int NB, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void q8_tile_kernel(GemmArgs a) {
+    constexpr int WAVES = WM * WN, BM = 16 * MF * WM, NBLK = NB * WN;
+    constexpr int XS = BM * 128, WS = NBLK * 8192;
+    __shared__ __attribute__((aligned(1024))) char lds[2 * (XS + WS)];
+    const int item = xcd_item(blockIdx.x, gridDim.x);
+    // groups of four row tiles, in a group row tiles fastest: what an XCD runs at a time is a patch of the
+    // result, whose operands its L2 holds
+    const int per = 4 * a.ntiles, grp = item / per, in = item - grp * per;
+    const int gm = min(4, a.mtiles - 4 * grp), nt = in / gm, mt = 4 * grp + in - nt * gm;
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int r16 = lane & 15, g = lane >> 4, wm = wave % WM, wn = wave / WM;
+    const int m0 = BM * mt, rows = min(BM, a.M - m0), Kp = a.Kp, kbs = Kp / 64;
+    const int nb0 = NBLK * nt, nblks = min(NBLK, (a.N + 63) / 64 - nb0);
+    const auto rx = rsrc_of(a.q + (int64_t)m0 * Kp, (uint32_t)(rows * Kp));
+    const auto rw = rsrc_of(a.wq + (int64_t)nb0 * 64 * Kp, (uint32_t)(nblks * 64 * Kp));
+
+    constexpr int XL = BM / 8 / WAVES, WL = NBLK * 8 / WAVES;  // loads a wave a stage
+    uint32_t xoff[XL], woff[WL];
+#pragma unroll
+    for (int i = 0; i < XL; ++i) {
+        const int r = 8 * (XL * wave + i) + (lane >> 3);
+        xoff[i] = (uint32_t)(r * Kp + 16 * ((lane & 7) ^ ((r >> 1) & 7)));
+    }
+#pragma unroll
+    for (int i = 0; i < WL; ++i) {
+        const int u = WL * wave + i;  // block u / 8, its step u / 4 % 2, operand u % 4
+        woff[i] = (uint32_t)((u >> 3) * 64 * Kp + (u & 7) * 1024 + 16 * lane);
+    }
+    const auto fetch = [&](int st, int buf) __attribute__((always_inline)) {
+        char* base = lds + buf * (XS + WS);
+#pragma unroll
+        for (int i = 0; i < XL; ++i) dma_lds<16>(rx, base + 1024 * (XL * wave + i), xoff[i] + 128u * st);
+#pragma unroll
+        for (int i = 0; i < WL; ++i) dma_lds<16>(rw, base + XS + 1024 * (WL * wave + i), woff[i] + 8192u * st);
+    };
+    int4v acc[NB][4][MF];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int mf = 0; mf < MF; ++mf) acc[nb][b][mf] = int4v{0, 0, 0, 0};
+
+    const int xrow = 16 * MF * wm + r16;  // operand mf of this lane: row xrow + 16 mf
+    const auto step = [&](int kb, int buf) __attribute__((always_inline)) {
+        const char* X = lds + buf * (XS + WS);
+        const char* W = X + XS;
+        int4v x[MF], w[NB][4];
+#pragma unroll
+        for (int mf = 0; mf < MF; ++mf) {
+            x[mf] = *reinterpret_cast<const int4v*>(X + (xrow + 16 * mf) * 128 + 16 * ((4 * kb + g) ^ ((r16 >> 1) & 7)));
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                w[nb][b] = *reinterpret_cast<const int4v*>(W + (((wn * NB + nb) * 2 + kb) * 4 + b) * 1024 + 16 * lane);
+            }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int mf = 0; mf < MF; ++mf) acc[nb][b][mf] = mfma_i8(w[nb][b], x[mf], acc[nb][b][mf]);
+    };
+    const int stages = (kbs + 1) / 2;
+    fetch(0, 0);
+    for (int st = 0; st < stages; ++st) {
+        // this stage's loads have landed, and every wave is done with the other buffer
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        if (st + 1 < stages) fetch(st + 1, (st + 1) & 1);
+        step(0, st & 1);
+        if (2 * st + 1 < kbs) step(1, st & 1);
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        const int n = 64 * (nb0 + wn * NB + nb) + 16 * g;
+        float sw[16], bv[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            sw[i] = n + i < a.N ? a.ws[n + i] : 0.f;
+            bv[i] = a.b != nullptr && n + i < a.N ? a.b[n + i] : 0.f;
+        }
+#pragma unroll
+        for (int mf = 0; mf < MF; ++mf) {
+            const int m = m0 + xrow + 16 * mf;
+            if (m >= a.M) continue;
+            const float sx = a.qs[m];
+            const int64_t at = (int64_t)m * a.N + n;
+            float v[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = scaled(acc[nb][i >> 2][mf][i & 3], sx, sw[i], bv[i]);
+            if (n + 16 <= a.N) {
+                if (a.residual != nullptr) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const half8 r = *reinterpret_cast<const half8u*>(a.residual + at + 8 * h);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[8 * h + i] += act_get<BF>(r, i);
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    half8 o;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) o[i] = act_cvt<BF>(v[8 * h + i]);
+                    *reinterpret_cast<half8u*>(a.out + at + 8 * h) = o;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    if (n + i >= a.N) break;
+                    if (a.residual != nullptr) v[i] += act_get<BF>(half8{a.residual[at + i]}, 0);
+                    a.out[at + i] = act_cvt<BF>(v[i]);
+                }
+            }
+        }
+    }
+}
+
 // |sum| <= 128^2 Kp has to stay below 2^31
 constexpr int64_t kMaxKp = 131008;
 
@@ -168,6 +295,15 @@ extern "C" int clk_q8_projection(clk_stream stream, const clk_buffer* q, const c
                (int)M, (int)N, (int)Kp, (int)mt, (int)nt, fast_div(mt)};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     stage_mark(s, 0);
+    if (M >= 256 && N >= 256) {
+        a.mtiles = (int)((M + 255) / 256);
+        a.ntiles = (int)((N + 255) / 256);
+        const dim3 grid((unsigned)(a.mtiles * a.ntiles)), block(512);
+        if (act == CLK_BF16) hipLaunchKernelGGL((q8_tile_kernel<true, 4, 2, 4, 2>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((q8_tile_kernel<false, 4, 2, 4, 2>), grid, block, 0, s, a);
+        stage_mark(s, 1);
+        return launch_status("q8_projection");
+    }
     if (act == CLK_BF16) hipLaunchKernelGGL(q8_gemm_kernel<true>, dim3((unsigned)(mt * nt)), dim3(256), 0, s, a);
     else hipLaunchKernelGGL(q8_gemm_kernel<false>, dim3((unsigned)(mt * nt)), dim3(256), 0, s, a);
     stage_mark(s, 1);
