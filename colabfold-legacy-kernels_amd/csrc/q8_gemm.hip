@@ -177,36 +177,57 @@ __global__ __launch_bounds__(64 * WM * WN) void q8_tile_kernel(GemmArgs a) {
             for (int mf = 0; mf < MF; ++mf) acc[nb][b][mf] = int4v{0, 0, 0, 0};
 
     const int xrow = 16 * MF * wm + r16;  // operand mf of this lane: row xrow + 16 mf
-    const auto step = [&](int kb, int buf) __attribute__((always_inline)) {
+    struct Operands {
+        int4v x[MF], w[NB][4];
+    };
+    const auto read = [&](int kb, int buf, Operands& o) __attribute__((always_inline)) {
         const char* X = lds + buf * (XS + WS);
         const char* W = X + XS;
-        int4v x[MF], w[NB][4];
 #pragma unroll
         for (int mf = 0; mf < MF; ++mf) {
-            x[mf] = *reinterpret_cast<const int4v*>(X + (xrow + 16 * mf) * 128 + 16 * ((4 * kb + g) ^ ((r16 >> 1) & 7)));
+            o.x[mf] = *reinterpret_cast<const int4v*>(X + (xrow + 16 * mf) * 128 + 16 * ((4 * kb + g) ^ ((r16 >> 1) & 7)));
         }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
-                w[nb][b] = *reinterpret_cast<const int4v*>(W + (((wn * NB + nb) * 2 + kb) * 4 + b) * 1024 + 16 * lane);
+                o.w[nb][b] = *reinterpret_cast<const int4v*>(W + (((wn * NB + nb) * 2 + kb) * 4 + b) * 1024 + 16 * lane);
             }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const auto multiply = [&](const Operands& o) __attribute__((always_inline)) {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int b = 0; b < 4; ++b)
 #pragma unroll
-                for (int mf = 0; mf < MF; ++mf) acc[nb][b][mf] = mfma_i8(w[nb][b], x[mf], acc[nb][b][mf]);
+                for (int mf = 0; mf < MF; ++mf) acc[nb][b][mf] = mfma_i8(o.w[nb][b], o.x[mf], acc[nb][b][mf]);
+        __builtin_amdgcn_sched_barrier(0);
     };
+    // The operands of a step are read while the step before it is multiplied, and the barrier stands between the
+    // two steps of a stage: past it every wave holds its second step's operands, so the stage's buffer takes
+    // the loads of the stage after next, and the next stage's loads have landed.
     const int stages = (kbs + 1) / 2;
+    Operands even, odd;
     fetch(0, 0);
-    for (int st = 0; st < stages; ++st) {
-        // this stage's loads have landed, and every wave is done with the other buffer
+    if (stages > 1) {
+        fetch(1, 1);
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(XL + WL) : "memory");
+    } else {
         asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        if (st + 1 < stages) fetch(st + 1, (st + 1) & 1);
-        step(0, st & 1);
-        if (2 * st + 1 < kbs) step(1, st & 1);
     }
+    read(0, 0, even);
+    for (int st = 0; st + 1 < stages; ++st) {
+        read(1, st & 1, odd);
+        multiply(even);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (st + 2 < stages) fetch(st + 2, st & 1);
+        read(0, (st + 1) & 1, even);
+        multiply(odd);
+    }
+    if (kbs % 2 == 0) read(1, (stages - 1) & 1, odd);
+    multiply(even);
+    if (kbs % 2 == 0) multiply(odd);
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
         const int n = 64 * (nb0 + wn * NB + nb) + 16 * g;
