@@ -39,7 +39,6 @@ struct GemmArgs {
     half_t* out;
     int M, N, Kp;
     int mtiles, ntiles;
-    FastDiv mdiv;
 };
 
 template <typename P>
@@ -55,227 +54,328 @@ __device__ __forceinline__ int4v load16(Rsrc r, uint32_t off) {
 // results do not depend on how many rows a call has
 __device__ __forceinline__ float scaled(int sum, float sx, float sw, float b) { return __builtin_fmaf((float)sum * sx, sw, b); }
 
-// Four consecutive channels n .. n + 3 of row m, of which those below N exist
-template <bool BF>
-__device__ __forceinline__ void store4(const GemmArgs& a, int m, int n, int4v acc) {
+// RL consecutive channels n .. of row m, of which those below N exist: their scales and biases, and the results
+template <int RL>
+struct Channels {
+    float sw[RL], b[RL];
+    __device__ __forceinline__ Channels(const GemmArgs& a, int n) {
+#pragma unroll
+        for (int i = 0; i < RL; ++i) {
+            sw[i] = n + i < a.N ? a.ws[n + i] : 0.f;
+            b[i] = a.b != nullptr && n + i < a.N ? a.b[n + i] : 0.f;
+        }
+    }
+};
+template <int W>
+struct Vec16;
+template <>
+struct Vec16<4> {
+    typedef half4 type;
+    typedef half4u unaligned;
+};
+template <>
+struct Vec16<8> {
+    typedef half8 type;
+    typedef half8u unaligned;
+};
+template <bool BF, int RL>
+__device__ __forceinline__ void store_run(const GemmArgs& a, int m, int n, const Channels<RL>& ch, const int (&sum)[RL]) {
+    constexpr int W = RL < 8 ? RL : 8;  // channels an access
     if (m >= a.M || n >= a.N) return;
     const float sx = a.qs[m];
     const int64_t at = (int64_t)m * a.N + n;
-    if (n + 4 <= a.N) {
-        float v[4];
+    float v[RL];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = scaled(acc[i], sx, a.ws[n + i], a.b != nullptr ? a.b[n + i] : 0.f);
+    for (int i = 0; i < RL; ++i) v[i] = scaled(sum[i], sx, ch.sw[i], ch.b[i]);
+    if (n + RL <= a.N) {
         if (a.residual != nullptr) {
-            const half4 h = *reinterpret_cast<const half4u*>(a.residual + at);
-            const half8 r = half8{h[0], h[1], h[2], h[3], 0, 0, 0, 0};
+            typename Vec16<W>::type r[RL / W];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] += act_get<BF>(r, i);
+            for (int h = 0; h < RL / W; ++h) r[h] = *reinterpret_cast<const typename Vec16<W>::unaligned*>(a.residual + at + W * h);
+#pragma unroll
+            for (int i = 0; i < RL; ++i) v[i] += act_get<BF>(half8{r[i / W][i % W]}, 0);
         }
-        *reinterpret_cast<half4u*>(a.out + at) = half4{act_cvt<BF>(v[0]), act_cvt<BF>(v[1]), act_cvt<BF>(v[2]), act_cvt<BF>(v[3])};
+#pragma unroll
+        for (int h = 0; h < RL / W; ++h) {
+            typename Vec16<W>::type o;
+#pragma unroll
+            for (int i = 0; i < W; ++i) o[i] = act_cvt<BF>(v[W * h + i]);
+            *reinterpret_cast<typename Vec16<W>::unaligned*>(a.out + at + W * h) = o;
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < RL; ++i) {
             if (n + i >= a.N) break;
-            float v = scaled(acc[i], sx, a.ws[n + i], a.b != nullptr ? a.b[n + i] : 0.f);
-            if (a.residual != nullptr) v += act_get<BF>(half8{a.residual[at + i]}, 0);
-            a.out[at + i] = act_cvt<BF>(v);
+            if (a.residual != nullptr) v[i] += act_get<BF>(half8{a.residual[at + i]}, 0);
+            a.out[at + i] = act_cvt<BF>(v[i]);
         }
     }
 }
 
-// A workgroup computes 64 rows by 64 channels; its four waves split k and join their sums through LDS.
-// Operands go from memory straight to registers.
+// Up to four rows: a product is the reading of its weights. A workgroup computes one operand of 16 channels; its
+// four waves split k in runs of steps and join their sums through LDS. Operands go from memory straight to
+// registers, four steps ahead, so a wave has 4 to 8 KB in flight; the rows' 16-byte pieces come in operand
+// order, which is slow for 16 rows (see below) but costs little where most lanes have none. [1, 4096] x
+// [4096, 4096]: 4.6 us (16.8 MB: 3.6 TB/s from the far cache), 0.3 us less than the kernel below; with five
+// and more rows that one is as fast or faster (7 rows, 8192 to 2048: 5.2 against 6.1 us).
+constexpr int kFewRows = 4;
+
 template <bool BF>
-__global__ __launch_bounds__(256) void q8_gemm_kernel(GemmArgs a) {
-    __shared__ __attribute__((aligned(16))) int4v part[4][16][kWave];
-    const int item = xcd_item(blockIdx.x, gridDim.x);
-    const int nt = fdiv(item, a.mdiv), mt = item - nt * a.mtiles;
+__global__ __launch_bounds__(256) void q8_rows_kernel(GemmArgs a) {
+    constexpr int KW = 4, U = 4;
+    __shared__ __attribute__((aligned(16))) int4v part[KW][kWave];
+    const int o = xcd_item(blockIdx.x, gridDim.x);  // operand o % 4 of block o / 4
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int r16 = lane & 15, g = lane >> 4;
-    const int m0 = 64 * mt, rows = min(64, a.M - m0), kbs = a.Kp / 64;
-    const auto rw = rsrc_of(a.wq + (int64_t)nt * 64 * a.Kp, (uint32_t)(64 * a.Kp));
-    const auto rx = rsrc_of(a.q + (int64_t)m0 * a.Kp, (uint32_t)(rows * a.Kp));
-    int4v acc[4][4];
+    const int r16 = lane & 15, g = lane >> 4, kbs = a.Kp / 64;
+    const auto rw = rsrc_of(a.wq + (int64_t)(o / 4) * 64 * a.Kp, (uint32_t)(64 * a.Kp));
+    const auto rx = rsrc_of(a.q, (uint32_t)(a.M * a.Kp));
+    const int run = (kbs + KW - 1) / KW, begin = min(kbs, run * wave), end = min(kbs, begin + run);
+    int4v acc{0, 0, 0, 0}, x[U], w[U];
+    // (a step past the run's end reads past the buffers' range: zeros, no traffic)
+    const auto load = [&](int kb, int4v& xs, int4v& ws) __attribute__((always_inline)) {
+        const uint32_t past = kb < end ? 0u : 0x80000000u;
+        ws = load16(rw, past + (uint32_t)(4096 * kb + 1024 * (o % 4) + 16 * lane));
+        xs = load16(rx, past + (uint32_t)(r16 * a.Kp + 64 * kb + 16 * g));
+    };
 #pragma unroll
-    for (int b = 0; b < 4; ++b)
+    for (int i = 0; i < U; ++i) load(begin + i, x[i], w[i]);
+    for (int kb = begin; kb < end; kb += U) {
 #pragma unroll
-        for (int mb = 0; mb < 4; ++mb) acc[b][mb] = int4v{0, 0, 0, 0};
-    for (int kb = wave; kb < kbs; kb += 4) {
-        int4v w[4], x[4];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) w[b] = load16(rw, (uint32_t)(4096 * kb + 1024 * b + 16 * lane));
-#pragma unroll
-        for (int mb = 0; mb < 4; ++mb) x[mb] = load16(rx, (uint32_t)((16 * mb + r16) * a.Kp + 64 * kb + 16 * g));
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int mb = 0; mb < 4; ++mb) acc[b][mb] = mfma_i8(w[b], x[mb], acc[b][mb]);
+        for (int i = 0; i < U; ++i) {
+            acc = mfma_i8(w[i], x[i], acc);
+            load(kb + U + i, x[i], w[i]);
+        }
     }
-#pragma unroll
-    for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int mb = 0; mb < 4; ++mb) part[wave][4 * b + mb][lane] = acc[b][mb];
+    part[wave][lane] = acc;
     __syncthreads();
+    if (wave > 0) return;
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {  // wave w finishes rows 16 w .. + 15
-        int4v s = part[0][4 * b + wave][lane];
-#pragma unroll
-        for (int v = 1; v < 4; ++v) s += part[v][4 * b + wave][lane];
-        store4<BF>(a, m0 + 16 * wave + r16, 64 * nt + 16 * g + 4 * b, s);
-    }
+    for (int v = 1; v < KW; ++v) acc += part[v][lane];
+    const int n = 64 * (o / 4) + 16 * g + 4 * (o % 4);
+    store_run<BF, 4>(a, r16, n, Channels<4>(a, n), {acc[0], acc[1], acc[2], acc[3]});
 }
 
-// Large products. A workgroup computes BM = 16 MF WM rows by BN = 64 NB WN channels; wave (wm, wn) of WM x WN
-// has MF operands of 16 rows and NB weight blocks of 64 channels. Both operands go through LDS, 128 inputs
-// (two MFMA steps) a stage, two stages: the loads of the next stage are in flight while one is computed.
+// A workgroup computes 16 MF WM rows by 16 NU WN channels. Its waves are KS groups of WM x WN; wave (wm, wn) of a
+// group has MF operands of 16 rows and NU of 16 channels, and the groups take every KS-th step of 64 inputs
+// (one MFMA step) and join their sums through LDS. Both operands go through LDS, a step at a time, in a
+// ring of RING buffers a group: a buffer is filled again as soon as every wave of the group holds its
+// operands in registers, so the loads of RING - 1 steps are in flight while one is computed.
 //   weights  by 1024-byte direct-to-LDS loads, in memory order: an operand read is 64 lanes' consecutive 16
 //            bytes
-//   rows     eight rows of 128 bytes a load, position p of row r holding its 16-byte chunk p ^ (r / 2 % 8): a
-//            16-lane group reads one chunk of 16 rows from 16 different bank quadruples
-template <bool BF, int MF, int NB, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void q8_tile_kernel(GemmArgs a) {
-    constexpr int WAVES = WM * WN, BM = 16 * MF * WM, NBLK = NB * WN;
-    constexpr int XS = BM * 128, WS = NBLK * 8192;
-    __shared__ __attribute__((aligned(1024))) char lds[2 * (XS + WS)];
+//   rows     16 rows of 64 bytes a load, position p of row r holding its 16-byte chunk p ^ (r / 4 % 4): a
+//            16-lane group reads one chunk of 16 rows from 16 different bank quadruples. (Loaded straight in
+//            operand order, 16 bytes of 16 rows after each other, the same kilobyte takes three times as long:
+//            16 bytes a clock and CU against 44.)
+template <bool BF, int MF, int NU, int WM, int WN, int KS, int RING>
+__global__ __launch_bounds__(64 * WM * WN * KS) void q8_tile_kernel(GemmArgs a) {
+    constexpr int G = WM * WN, XT = MF * WM, WT = NU * WN, STEP = 1024 * (XT + WT), BM = 16 * XT;
+    constexpr int XL = XT / G, WL = WT / G, L = XL + WL;  // loads a wave a step
+    static_assert(XL * G == XT && WL * G == WT && RING >= 3 && (RING - 1) * L < 64 && KS * RING * STEP <= 160 * 1024);
+    __shared__ __attribute__((aligned(1024))) char lds[KS * RING * STEP];
     const int item = xcd_item(blockIdx.x, gridDim.x);
     // groups of four row tiles, in a group row tiles fastest: what an XCD runs at a time is a patch of the
     // result, whose operands its L2 holds
-    const int per = 4 * a.ntiles, grp = item / per, in = item - grp * per;
-    const int gm = min(4, a.mtiles - 4 * grp), nt = in / gm, mt = 4 * grp + in - nt * gm;
+    const int per = 4 * a.ntiles, grp4 = item / per, in = item - grp4 * per;
+    const int gm = min(4, a.mtiles - 4 * grp4), nt = in / gm, mt = 4 * grp4 + in - nt * gm;
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int r16 = lane & 15, g = lane >> 4, wm = wave % WM, wn = wave / WM;
+    const int r16 = lane & 15, g = lane >> 4, grp = wave / G, wg = wave % G, wm = wg % WM, wn = wg / WM;
     const int m0 = BM * mt, rows = min(BM, a.M - m0), Kp = a.Kp, kbs = Kp / 64;
-    const int nb0 = NBLK * nt, nblks = min(NBLK, (a.N + 63) / 64 - nb0);
+    const int o0 = WT * nt, nb0 = o0 / 4;  // the tile's first operand of channels, and its block
+    const int nblks = min((o0 % 4 + WT + 3) / 4, (a.N + 63) / 64 - nb0);
     const auto rx = rsrc_of(a.q + (int64_t)m0 * Kp, (uint32_t)(rows * Kp));
     const auto rw = rsrc_of(a.wq + (int64_t)nb0 * 64 * Kp, (uint32_t)(nblks * 64 * Kp));
+    char* ring = lds + grp * RING * STEP;
 
-    constexpr int XL = BM / 8 / WAVES, WL = NBLK * 8 / WAVES;  // loads a wave a stage
     uint32_t xoff[XL], woff[WL];
 #pragma unroll
     for (int i = 0; i < XL; ++i) {
-        const int r = 8 * (XL * wave + i) + (lane >> 3);
-        xoff[i] = (uint32_t)(r * Kp + 16 * ((lane & 7) ^ ((r >> 1) & 7)));
+        const int r = 16 * (XL * wg + i) + (lane >> 2);
+        xoff[i] = (uint32_t)(r * Kp + 16 * ((lane & 3) ^ ((r >> 2) & 3)));
     }
 #pragma unroll
     for (int i = 0; i < WL; ++i) {
-        const int u = WL * wave + i;  // block u / 8, its step u / 4 % 2, operand u % 4
-        woff[i] = (uint32_t)((u >> 3) * 64 * Kp + (u & 7) * 1024 + 16 * lane);
+        const int o = o0 % 4 + WL * wg + i;
+        woff[i] = (uint32_t)((o >> 2) * 64 * Kp + (o & 3) * 1024 + 16 * lane);
     }
-    const auto fetch = [&](int st, int buf) __attribute__((always_inline)) {
-        char* base = lds + buf * (XS + WS);
-#pragma unroll
-        for (int i = 0; i < XL; ++i) dma_lds<16>(rx, base + 1024 * (XL * wave + i), xoff[i] + 128u * st);
-#pragma unroll
-        for (int i = 0; i < WL; ++i) dma_lds<16>(rw, base + XS + 1024 * (WL * wave + i), woff[i] + 8192u * st);
+    // load i of the group's step t (past the last one it reads past the buffers' range: zeros, no traffic)
+    const auto fetch = [&](int i, int t, char* base) __attribute__((always_inline)) {
+        const int s = KS * t + grp;
+        if (i < XL) dma_lds<16>(rx, base + 1024 * (XL * wg + i), xoff[i] + (s < kbs ? 64u * s : 0x80000000u));
+        else dma_lds<16>(rw, base + 1024 * (XT + WL * wg + i - XL), woff[i - XL] + (s < kbs ? 4096u * s : 0x80000000u));
     };
-    int4v acc[NB][4][MF];
+    int4v acc[NU][MF];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+    for (int u = 0; u < NU; ++u)
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int mf = 0; mf < MF; ++mf) acc[nb][b][mf] = int4v{0, 0, 0, 0};
+        for (int mf = 0; mf < MF; ++mf) acc[u][mf] = int4v{0, 0, 0, 0};
 
-    const int xrow = 16 * MF * wm + r16;  // operand mf of this lane: row xrow + 16 mf
     struct Operands {
-        int4v x[MF], w[NB][4];
+        int4v x[MF], w[NU];
     };
-    const auto read = [&](int kb, int buf, Operands& o) __attribute__((always_inline)) {
-        const char* X = lds + buf * (XS + WS);
-        const char* W = X + XS;
+    constexpr int R = MF + NU;  // operand reads of a step
+    const int xat = (16 * MF * wm + r16) * 64 + 16 * (g ^ ((r16 >> 2) & 3)), wat = 1024 * (XT + NU * wn) + 16 * lane;
+    const auto read = [&](int i, const char* base, Operands& o) __attribute__((always_inline)) {
+        if (i < MF) o.x[i] = *reinterpret_cast<const int4v*>(base + xat + 1024 * i);
+        else o.w[i - MF] = *reinterpret_cast<const int4v*>(base + wat + 1024 * (i - MF));
+    };
+    // Step t, with its operands in `cur` or on their way there: past the wait (and, in a group of several
+    // waves, the barrier) they are in the registers, so their buffer takes the loads of step t + RING, and
+    // step t + 1 has landed (newer than it are the loads of RING - 2 steps). Its operands are read while step
+    // t is multiplied. Reads and loads are issued one by one between the products, which wait for neither:
+    // in a burst they hold up the wave at a full queue. Steps go in pairs; one past the last adds zeros.
+    int buf = 0;  // byte offset of step t's buffer
+    const auto turn = [&](int t, const Operands& cur, Operands& next) __attribute__((always_inline)) {
+        if constexpr (G > 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((RING - 2) * L) : "memory");
+        else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((RING - 2) * L) : "memory");
+        char* free = ring + buf;
+        buf = buf == (RING - 1) * STEP ? 0 : buf + STEP;
+        const char* ready = ring + buf;
+        constexpr int P = NU * MF;  // products of a step
+        if constexpr (P < R) {
 #pragma unroll
-        for (int mf = 0; mf < MF; ++mf) {
-            o.x[mf] = *reinterpret_cast<const int4v*>(X + (xrow + 16 * mf) * 128 + 16 * ((4 * kb + g) ^ ((r16 >> 1) & 7)));
+            for (int i = 0; i < R; ++i) read(i, ready, next);
+#pragma unroll
+            for (int i = 0; i < L; ++i) fetch(i, t + RING, free);
         }
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+        for (int n = 0; n < P; ++n) {
+            const int u = n / MF, mf = n % MF;
+            acc[u][mf] = mfma_i8(cur.w[u], cur.x[mf], acc[u][mf]);
+            if constexpr (P >= R) {
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                o.w[nb][b] = *reinterpret_cast<const int4v*>(W + (((wn * NB + nb) * 2 + kb) * 4 + b) * 1024 + 16 * lane);
+                for (int i = 0; i < R; ++i)
+                    if (n == i * (P * 3 / 4 / R > 0 ? P * 3 / 4 / R : 1)) read(i, ready, next);
+#pragma unroll
+                for (int i = 0; i < L; ++i)
+                    if (n == (2 * i + 1) * P / (2 * L)) fetch(i, t + RING, free);
+                __builtin_amdgcn_sched_barrier(0);
             }
-        __builtin_amdgcn_sched_barrier(0);
+        }
     };
-    const auto multiply = [&](const Operands& o) __attribute__((always_inline)) {
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-#pragma unroll
-                for (int mf = 0; mf < MF; ++mf) acc[nb][b][mf] = mfma_i8(o.w[nb][b], o.x[mf], acc[nb][b][mf]);
-        __builtin_amdgcn_sched_barrier(0);
-    };
-    // The operands of a step are read while the step before it is multiplied, and the barrier stands between the
-    // two steps of a stage: past it every wave holds its second step's operands, so the stage's buffer takes
-    // the loads of the stage after next, and the next stage's loads have landed.
-    const int stages = (kbs + 1) / 2;
     Operands even, odd;
-    fetch(0, 0);
-    if (stages > 1) {
-        fetch(1, 1);
-        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(XL + WL) : "memory");
-    } else {
-        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+    for (int t = 0; t < RING; ++t)
+#pragma unroll
+        for (int i = 0; i < L; ++i) fetch(i, t, ring + t * STEP);
+    if constexpr (G > 1) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((RING - 1) * L) : "memory");
+    else asm volatile("s_waitcnt vmcnt(%0)" ::"n"((RING - 1) * L) : "memory");
+#pragma unroll
+    for (int i = 0; i < R; ++i) read(i, ring, even);
+    const int steps = (kbs + KS - 1) / KS;
+    for (int t = 0; t < steps; t += 2) {
+        turn(t, even, odd);
+        turn(t + 1, odd, even);
     }
-    read(0, 0, even);
-    for (int st = 0; st + 1 < stages; ++st) {
-        read(1, st & 1, odd);
-        multiply(even);
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (st + 2 < stages) fetch(st + 2, st & 1);
-        read(0, (st + 1) & 1, even);
-        multiply(odd);
-    }
-    if (kbs % 2 == 0) read(1, (stages - 1) & 1, odd);
-    multiply(even);
-    if (kbs % 2 == 0) multiply(odd);
+    // no load may write LDS past the workgroup's end, nor over the sums below
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+
+    if constexpr (KS == 1) {
+        constexpr int NE = NU < 4 ? NU : 4;  // operands of a run: 4 NE channels
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        const int n = 64 * (nb0 + wn * NB + nb) + 16 * g;
-        float sw[16], bv[16];
+        for (int u = 0; u < NU; u += NE) {
+            const int o = o0 + NU * wn + u, n = 64 * (o / 4) + 16 * g + 4 * (o % 4);
+            const Channels<4 * NE> ch(a, n);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            sw[i] = n + i < a.N ? a.ws[n + i] : 0.f;
-            bv[i] = a.b != nullptr && n + i < a.N ? a.b[n + i] : 0.f;
-        }
+            for (int mf = 0; mf < MF; ++mf) {
+                int sum[4 * NE];
 #pragma unroll
-        for (int mf = 0; mf < MF; ++mf) {
-            const int m = m0 + xrow + 16 * mf;
-            if (m >= a.M) continue;
-            const float sx = a.qs[m];
-            const int64_t at = (int64_t)m * a.N + n;
-            float v[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = scaled(acc[nb][i >> 2][mf][i & 3], sx, sw[i], bv[i]);
-            if (n + 16 <= a.N) {
-                if (a.residual != nullptr) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const half8 r = *reinterpret_cast<const half8u*>(a.residual + at + 8 * h);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) v[8 * h + i] += act_get<BF>(r, i);
-                    }
-                }
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    half8 o;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) o[i] = act_cvt<BF>(v[8 * h + i]);
-                    *reinterpret_cast<half8u*>(a.out + at + 8 * h) = o;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    if (n + i >= a.N) break;
-                    if (a.residual != nullptr) v[i] += act_get<BF>(half8{a.residual[at + i]}, 0);
-                    a.out[at + i] = act_cvt<BF>(v[i]);
-                }
+                for (int i = 0; i < 4 * NE; ++i) sum[i] = acc[u + i / 4][mf][i % 4];
+                store_run<BF, 4 * NE>(a, m0 + 16 * (MF * wm + mf) + r16, n, ch, sum);
             }
+        }
+    } else {
+        // wave wg of group j finishes runs j, j + KS, ... of its place in the tile
+        constexpr int NE = MF * NU >= 4 * KS && NU % 4 == 0 ? 4 : 1, RUNS = MF * NU / NE;
+        static_assert(KS * G * MF * NU <= KS * RING * (XT + WT));
+        int4v* part = reinterpret_cast<int4v*>(lds);
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int mf = 0; mf < MF; ++mf) part[((grp * G + wg) * NU * MF + u * MF + mf) * kWave + lane] = acc[u][mf];
+        __syncthreads();
+        for (int f = grp; f < RUNS; f += KS) {
+            const int u = f / MF * NE, mf = f % MF;
+            int sum[4 * NE];
+#pragma unroll
+            for (int e = 0; e < NE; ++e) {
+                int4v s = part[(wg * NU * MF + (u + e) * MF + mf) * kWave + lane];
+#pragma unroll
+                for (int j = 1; j < KS; ++j) s += part[((j * G + wg) * NU * MF + (u + e) * MF + mf) * kWave + lane];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[4 * e + i] = s[i];
+            }
+            const int o = o0 + NU * wn + u, n = 64 * (o / 4) + 16 * g + 4 * (o % 4);
+            store_run<BF, 4 * NE>(a, m0 + 16 * (MF * wm + mf) + r16, n, Channels<4 * NE>(a, n), sum);
         }
     }
 }
 
 // |sum| <= 128^2 Kp has to stay below 2^31
 constexpr int64_t kMaxKp = 131008;
+
+// The tiles for more than 64 rows, by estimated time: a round of 256 tiles, one for each CU, costs a fixed part
+// (loads that wait for the first operands, the results) and one for k. Measured in us, for 1024 inputs, from
+// 8192 x k x 8192 at k = 1024 and 8192 (v0 to v3 of the sizes below: 88, 81, 94, 162 us and 413, 464, 579,
+// 831 us): large tiles read less for each product, small ones fill the card where there are few.
+struct Tile {
+    int rows, channels;
+    double fixed, per1024;
+};
+constexpr Tile kTiles[] = {{256, 256, 10.5, 11.6}, {128, 256, 3.4, 6.83}, {128, 128, 1.55, 4.33}, {64, 64, 1.04, 1.5}};
+
+int best_tile(int64_t M, int64_t N, int64_t Kp) {
+    int best = 0;
+    double least = 0;
+    for (int i = 0; i < 4; ++i) {
+        const Tile& t = kTiles[i];
+        const int64_t tiles = (M + t.rows - 1) / t.rows * ((N + t.channels - 1) / t.channels);
+        const double us = (double)((tiles + 255) / 256) * (t.fixed + t.per1024 * (double)Kp / 1024);
+        if (i == 0 || us < least) {
+            best = i;
+            least = us;
+        }
+    }
+    return best;
+}
+
+template <bool BF>
+void launch(hipStream_t s, GemmArgs& a) {
+    const int operands = (a.N + 63) / 64 * 4;
+    if (a.M <= kFewRows) {
+        hipLaunchKernelGGL(q8_rows_kernel<BF>, dim3((unsigned)operands), dim3(256), 0, s, a);
+        return;
+    }
+#define CLK_TILE(MF_, NU_, WM_, WN_, KS_, RING_)                                                                 \
+    {                                                                                                            \
+        a.mtiles = (a.M + 16 * MF_ * WM_ - 1) / (16 * MF_ * WM_);                                                \
+        a.ntiles = (operands + NU_ * WN_ - 1) / (NU_ * WN_);                                                     \
+        hipLaunchKernelGGL((q8_tile_kernel<BF, MF_, NU_, WM_, WN_, KS_, RING_>),                                 \
+                           dim3((unsigned)a.mtiles * (unsigned)a.ntiles), dim3(64 * WM_ * WN_ * KS_), 0, s, a);  \
+        return;                                                                                                  \
+    }
+    // Up to 64 rows every wave works for itself (no barriers), eight of them splitting k. One operand of
+    // channels a workgroup while that gives 256 workgroups at most, for every CU one, then two, which
+    // halves the reading of the rows: 32 rows, 8192 to 8192: 15.7 and 13.0 us; 4096 to 4096: 5.9 and 6.6.
+    if (a.M <= 16) CLK_TILE(1, 1, 1, 1, 4, 8)
+    if (operands <= 256) {
+        if (a.M <= 32) CLK_TILE(2, 1, 1, 1, 8, 5)
+        if (a.M <= 48) CLK_TILE(3, 1, 1, 1, 8, 4)
+        if (a.M <= 64) CLK_TILE(4, 1, 1, 1, 8, 4)
+    } else {
+        if (a.M <= 32) CLK_TILE(2, 2, 1, 1, 8, 4)
+        if (a.M <= 48) CLK_TILE(3, 2, 1, 1, 8, 3)
+        if (a.M <= 64) CLK_TILE(4, 2, 1, 1, 8, 3)
+    }
+    switch (best_tile(a.M, a.N, a.Kp)) {
+    case 0: CLK_TILE(4, 8, 4, 2, 1, 4)
+    case 1: CLK_TILE(4, 8, 2, 2, 1, 3)
+    case 2: CLK_TILE(4, 4, 2, 2, 1, 5)
+    default: CLK_TILE(2, 4, 2, 1, 2, 4)
+    }
+#undef CLK_TILE
+}
 
 }  // namespace
 
@@ -306,27 +406,16 @@ extern "C" int clk_q8_projection(clk_stream stream, const clk_buffer* q, const c
     if (elements(w_scale) != N || (has_b && elements(b) != N)) return invalid("q8_projection: w_scale and b must be [N]");
     if (has_residual && !same_shape(residual, out)) return invalid("q8_projection: residual must be like out");
     if (M == 0 || N == 0) return ok();
-    const int64_t mt = (M + 63) / 64;
-    if (M > INT32_MAX || N > INT32_MAX - 64 || mt * nt > INT32_MAX / 256) return invalid("q8_projection: too large");
+    if (M > INT32_MAX - 256 || N > INT32_MAX - 256 || (M + 63) / 64 * nt > INT32_MAX / 512) return invalid("q8_projection: too large");
     if (!aligned16(q->data) || !aligned16(wq->data)) return invalid("q8_projection: q and wq must be 16-byte aligned");
     GemmArgs a{static_cast<const int8_t*>(q->data), static_cast<const float*>(q_scale->data),
                static_cast<const int8_t*>(wq->data), static_cast<const float*>(w_scale->data),
                has_b ? static_cast<const float*>(b->data) : nullptr,
                has_residual ? static_cast<const half_t*>(residual->data) : nullptr, static_cast<half_t*>(out->data),
-               (int)M, (int)N, (int)Kp, (int)mt, (int)nt, fast_div(mt)};
+               (int)M, (int)N, (int)Kp, 0, 0};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     stage_mark(s, 0);
-    if (M >= 256 && N >= 256) {
-        a.mtiles = (int)((M + 255) / 256);
-        a.ntiles = (int)((N + 255) / 256);
-        const dim3 grid((unsigned)(a.mtiles * a.ntiles)), block(512);
-        if (act == CLK_BF16) hipLaunchKernelGGL((q8_tile_kernel<true, 4, 2, 4, 2>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((q8_tile_kernel<false, 4, 2, 4, 2>), grid, block, 0, s, a);
-        stage_mark(s, 1);
-        return launch_status("q8_projection");
-    }
-    if (act == CLK_BF16) hipLaunchKernelGGL(q8_gemm_kernel<true>, dim3((unsigned)(mt * nt)), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL(q8_gemm_kernel<false>, dim3((unsigned)(mt * nt)), dim3(256), 0, s, a);
+    act == CLK_BF16 ? launch<true>(s, a) : launch<false>(s, a);
     stage_mark(s, 1);
     return launch_status("q8_projection");
 }
