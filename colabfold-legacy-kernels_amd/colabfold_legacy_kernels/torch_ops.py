@@ -245,16 +245,28 @@ def rms_norm(x, scale, residual=None, eps=1e-5):
     if residual is not None and residual.shape != x.shape:
         raise hip.InvalidArgument(hip.INVALID_ARGUMENT, "rms_norm: residual must be like x, got %s and %s"
                                   % (tuple(residual.shape), tuple(x.shape)))
-    if torch.is_grad_enabled() and x.is_cuda and torch.cuda.is_current_stream_capturing() and any(
-            t is not None and t.requires_grad for t in (x, scale, residual)):
+    differentiated = torch.is_grad_enabled() and (x.requires_grad or scale.requires_grad or (
+        residual is not None and residual.requires_grad))
+    if differentiated and x.is_cuda and torch.cuda.is_current_stream_capturing():
         raise hip.InvalidArgument(hip.INVALID_ARGUMENT, "rms_norm: a differentiated call cannot be captured into a "
                                   "graph; capture hip.rms_norm and hip.rms_norm_bwd")
-    x2, lead = _rows(x)
-    r2 = None if residual is None else _rows(residual)[0]
-    res = _RmsNorm.apply(x2, scale.float().contiguous(), r2, float(eps))
-    if residual is None:
-        return res.reshape(lead + (x.shape[-1],))
-    return tuple(t.reshape(lead + (x.shape[-1],)) for t in res)
+    shape = x.shape
+    x2 = _matrix(x)
+    r2 = None if residual is None else _matrix(residual)
+    w = scale.float().contiguous()
+    if differentiated:
+        res = _RmsNorm.apply(x2, w, r2, float(eps))
+    else:
+        res = hip.rms_norm(x2, w, r2, eps)
+        res = res[0] if residual is None else res[:2]
+    if len(shape) == 2:
+        return res
+    return res.reshape(shape) if residual is None else tuple(t.reshape(shape) for t in res)
+
+
+def _matrix(x):
+    """x [..., C] as [M, C], contiguous; x itself where it is that"""
+    return x.contiguous() if x.dim() == 2 else _rows(x)[0]
 
 
 def _q8_lead(q, q_scale, lead):

@@ -13,6 +13,7 @@
 #include "clk_common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace clk {
 
@@ -105,9 +106,10 @@ __device__ __forceinline__ void store_run(const GemmArgs& a, int m, int n, const
     } else {
 #pragma unroll
         for (int i = 0; i < RL; ++i) {
-            if (n + i >= a.N) break;
-            if (a.residual != nullptr) v[i] += act_get<BF>(half8{a.residual[at + i]}, 0);
-            a.out[at + i] = act_cvt<BF>(v[i]);
+            if (n + i < a.N) {
+                if (a.residual != nullptr) v[i] += act_get<BF>(half8{a.residual[at + i]}, 0);
+                a.out[at + i] = act_cvt<BF>(v[i]);
+            }
         }
     }
 }
@@ -312,6 +314,138 @@ __global__ __launch_bounds__(64 * WM * WN * KS) void q8_tile_kernel(GemmArgs a) 
     }
 }
 
+// Many rows, short k: the product is the reading of rows and the writing of results, so a wave keeps its weights
+// (NU operands of channels, KB steps) in registers and streams rows past them. A workgroup's four waves
+// are WM x WN over rows and channels, 16 or 32 rows a wave and tile; tiles come through LDS, two
+// ahead; scales and biases wait in LDS, the next tile's row scales and residual in registers. Results go
+// out as 16-byte buffer stores, whose range drops what lies past M and N, so that every tile issues the
+// same number of memory accesses and a tile's wait can count them. A weight operand's rows are picked so that
+// a store's four lanes of a row write 64 consecutive bytes. Without a residual the stores are nontemporal:
+// 65536 x 256 x 1024 takes 36 us with and 55 us without that; with a residual, read through the same caches,
+// it is as often slower (147456 x 128 x 512: 68.5 and 62.7 us).
+template <bool BF, int KB, int NU, int MF, int WN, bool RES>
+__global__ __launch_bounds__(256) void q8_stream_kernel(GemmArgs a) {
+    constexpr int BR = 16 * MF, WM = 4 / WN, XT = MF * WM * KB, XL = (XT + 3) / 4, RING = 3, SLOT = 4096 * XL;
+    constexpr int CW = 16 * NU, H = NU / 2;  // channels a wave; 16-byte pieces of a lane's results a row
+    constexpr uint32_t kDrop = 0x80000000u;
+    __shared__ __attribute__((aligned(1024))) char lds[RING * SLOT];
+    __shared__ __attribute__((aligned(16))) float params[2][CW * WN];
+    const int item = xcd_item(blockIdx.x, gridDim.x), nt = item % a.ntiles, first = item / a.ntiles;
+    const int stride = gridDim.x / a.ntiles, Kp = a.Kp, kbs = Kp / 64;
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int r16 = lane & 15, g = lane >> 4, wm = wave / WN, wn = wave % WN;
+    const int c0 = CW * WN * nt, n0 = c0 + CW * wn;  // the workgroup's and the wave's first channel
+    for (int i = threadIdx.x; i < CW * WN; i += 256) {
+        params[0][i] = c0 + i < a.N ? a.ws[c0 + i] : 0.f;
+        params[1][i] = a.b != nullptr && c0 + i < a.N ? a.b[c0 + i] : 0.f;
+    }
+    const int blocks = (a.N + 63) / 64;
+    int4v w[KB][NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+        const int blk = n0 / 64 + u / 4;
+        const auto rw = rsrc_of(a.wq + (int64_t)min(blk, blocks - 1) * 64 * Kp, (uint32_t)(64 * Kp));
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            // row r16 of operand u % 4 is channel c of the block, which the layout has as row 4 (c / 16) + c % 4 of
+            // operand c / 4 % 4
+            const int c = 32 * (u % 4 / 2) + 8 * (r16 / 4) + 4 * (u % 2) + r16 % 4;
+            w[kb][u] = load16(rw, kb < kbs && blk < blocks ? (uint32_t)(4096 * kb + 1024 * (c / 4 % 4) + 256 * g + 16 * (4 * (c / 16) + c % 4)) : kDrop);
+        }
+    }
+    // load j of a tile: operand j / KB of rows, step j % KB
+    const auto fetch = [&](int mt, char* slot) __attribute__((always_inline)) {
+        const int m0 = BR * WM * mt, rows = max(0, min(BR * WM, a.M - m0));
+        const auto rx = rsrc_of(a.q + (int64_t)(rows > 0 ? m0 : 0) * Kp, (uint32_t)(rows * Kp));
+#pragma unroll
+        for (int i = 0; i < XL; ++i) {
+            const int j = 4 * i + wave, kb = j % KB, r = 16 * (j / KB) + (lane >> 2);
+            dma_lds<16>(rx, slot + 1024 * j, j < XT && kb < kbs ? (uint32_t)(r * Kp + 64 * kb + 16 * ((lane & 3) ^ ((r >> 2) & 3))) : kDrop);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");  // what is counted as newer stays newer
+    };
+    struct Rows {
+        float qs[MF];
+        half8 res[MF][RES ? H : 1];
+    };
+    const auto rows_of = [&](int mt, Rows& o) __attribute__((always_inline)) {
+        const int m0 = BR * (WM * mt + wm), rows = max(0, min(BR, a.M - m0)), base = rows > 0 ? m0 : 0;
+        const auto rs = rsrc_of(a.qs + base, (uint32_t)(rows * 4));
+        const auto rr = rsrc_of(RES ? a.residual + (int64_t)base * a.N : a.out, RES ? (uint32_t)rows * (uint32_t)a.N * 2u : 0u);
+#pragma unroll
+        for (int mf = 0; mf < MF; ++mf) {
+            const int r = 16 * mf + r16;
+            o.qs[mf] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, (uint32_t)(4 * r), 0, 0));
+            if constexpr (RES) {
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    const int n = n0 + 64 * (h / 2) + 32 * (h % 2) + 8 * g;
+                    o.res[mf][h] = __builtin_bit_cast(half8, load16(rr, n < a.N ? ((uint32_t)r * (uint32_t)a.N + (uint32_t)n) * 2u : kDrop));
+                }
+            }
+        }
+    };
+    const auto tile = [&](int mt, const char* slot, const Rows& now) __attribute__((always_inline)) {
+        const int m0 = BR * (WM * mt + wm), rows = max(0, min(BR, a.M - m0));
+        const auto ro = rsrc_of(a.out + (int64_t)(rows > 0 ? m0 : 0) * a.N, (uint32_t)rows * (uint32_t)a.N * 2u);
+        int4v acc[NU][MF];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            int4v x[MF];
+#pragma unroll
+            for (int mf = 0; mf < MF; ++mf) {
+                x[mf] = *reinterpret_cast<const int4v*>(slot + 1024 * ((MF * wm + mf) * KB + kb) + r16 * 64 + 16 * (g ^ ((r16 >> 2) & 3)));
+            }
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+                for (int mf = 0; mf < MF; ++mf) acc[u][mf] = mfma_i8(w[kb][u], x[mf], kb == 0 ? int4v{0, 0, 0, 0} : acc[u][mf]);
+        }
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            const int c = CW * wn + 64 * (h / 2) + 32 * (h % 2) + 8 * g;
+            const float8v sw = *reinterpret_cast<const float8v*>(&params[0][c]), bv = *reinterpret_cast<const float8v*>(&params[1][c]);
+            const int n = c0 + c;
+#pragma unroll
+            for (int mf = 0; mf < MF; ++mf) {
+                half8 o;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float v = scaled(acc[2 * h + i / 4][mf][i % 4], now.qs[mf], sw[i], bv[i]);
+                    if constexpr (RES) v += act_get<BF>(now.res[mf][h], i);
+                    o[i] = act_cvt<BF>(v);
+                }
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uint4v, o), ro,
+                                                       n < a.N ? ((uint32_t)(16 * mf + r16) * (uint32_t)a.N + (uint32_t)n) * 2u : kDrop, 0, RES ? 0 : 2);
+            }
+        }
+    };
+    const int tiles = (a.M + BR * WM - 1) / (BR * WM);
+    // newer than a tile's loads at its wait: one tile's loads, and two tiles' row scales, residual and stores
+    constexpr int kNewer = XL + 2 * (MF + (RES ? MF * H : 0) + MF * H);
+    static_assert(kNewer < 64);
+    Rows ra, rb;
+    int at = 0;
+    fetch(first, lds);
+    fetch(first + stride, lds + SLOT);
+    rows_of(first, ra);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const auto turn = [&](int mt, const Rows& now, Rows& next) __attribute__((always_inline)) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kNewer) : "memory");
+        const int free = at == 0 ? (RING - 1) * SLOT : at - SLOT;
+        fetch(mt + 2 * stride, lds + free);
+        rows_of(mt + stride, next);
+        tile(mt, lds + at, now);
+        at = at == (RING - 1) * SLOT ? 0 : at + SLOT;
+    };
+    for (int mt = first; mt < tiles; mt += 2 * stride) {
+        turn(mt, ra, rb);
+        turn(mt + stride, rb, ra);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may write LDS past the workgroup's end
+}
+
 // |sum| <= 128^2 Kp has to stay below 2^31
 constexpr int64_t kMaxKp = 131008;
 
@@ -338,6 +472,30 @@ int best_tile(int64_t M, int64_t N, int64_t Kp) {
         }
     }
     return best;
+}
+
+// Whether the kernel for many rows and short k takes a call. From 2048 rows on it was the faster one for all of
+// 27 shapes with k of 64 to 512 (147456 x 128 x 512: 41.9 against 74.8 us, 65536 x 512 x 2048: 82 against
+// 141, 4096 x 64 x 64: 3.6 against 4.2); at 1024 rows and below it loses as often as it wins. 16-byte stores need
+// aligned rows of results.
+bool streams(const GemmArgs& a) {
+    return a.M >= 2048 && a.M <= 1 << 30 && a.Kp <= 512 && a.N % 8 == 0 && a.N <= 1 << 20 && aligned16(a.out) &&
+           aligned16(a.residual);
+}
+
+template <bool BF, int KB, int NU, int MF, bool RES>
+void launch_stream(hipStream_t s, GemmArgs& a, int workgroups) {
+    const auto go = [&](auto wn_) {
+        constexpr int WN = decltype(wn_)::value;
+        a.ntiles = (a.N + 16 * NU * WN - 1) / (16 * NU * WN);
+        const int rows = 16 * MF * (4 / WN), mtiles = (a.M + rows - 1) / rows;
+        const int most = std::max(1, workgroups / a.ntiles);
+        hipLaunchKernelGGL((q8_stream_kernel<BF, KB, NU, MF, WN, RES>), dim3((unsigned)(std::min(mtiles, most) * a.ntiles)),
+                           dim3(256), 0, s, a);
+    };
+    if (a.N <= 16 * NU) go(std::integral_constant<int, 1>());
+    else if (a.N <= 32 * NU) go(std::integral_constant<int, 2>());
+    else go(std::integral_constant<int, 4>());
 }
 
 template <bool BF>
@@ -367,6 +525,26 @@ void launch(hipStream_t s, GemmArgs& a) {
         if (a.M <= 32) CLK_TILE(2, 2, 1, 1, 8, 4)
         if (a.M <= 48) CLK_TILE(3, 2, 1, 1, 8, 3)
         if (a.M <= 64) CLK_TILE(4, 2, 1, 1, 8, 3)
+    }
+    if (streams(a)) {
+        // Operands a wave and workgroups, measured at 147456 and 65536 rows: with few channels, or none but
+        // the results to move, small waves and more of them; with a residual at many channels, large ones
+        // (147456 x 128 x 512 with a residual: 63 us with 8 channel operands a wave and 512 workgroups, 69 to 71
+        // us with 4; without one 39 us with 4, 45 with 8).
+        const int kbs = a.Kp / 64;
+        const bool res = a.residual != nullptr;
+        if (kbs == 1) {
+            if (a.N <= 256) res ? launch_stream<BF, 1, 4, 1, true>(s, a, 768) : launch_stream<BF, 1, 4, 1, false>(s, a, 768);
+            else res ? launch_stream<BF, 1, 8, 2, true>(s, a, 512) : launch_stream<BF, 1, 4, 2, false>(s, a, 1024);
+        } else if (kbs == 2) {
+            if (a.N <= 256) res ? launch_stream<BF, 2, 4, 1, true>(s, a, 768) : launch_stream<BF, 2, 4, 1, false>(s, a, 768);
+            else res ? launch_stream<BF, 2, 8, 1, true>(s, a, 512) : launch_stream<BF, 2, 4, 2, false>(s, a, 1024);
+        } else if (kbs <= 4) {
+            res ? launch_stream<BF, 4, 4, 1, true>(s, a, 512) : launch_stream<BF, 4, 4, 1, false>(s, a, 512);
+        } else {
+            res ? launch_stream<BF, 8, 4, 1, true>(s, a, 512) : launch_stream<BF, 8, 4, 1, false>(s, a, 512);
+        }
+        return;
     }
     switch (best_tile(a.M, a.N, a.Kp)) {
     case 0: CLK_TILE(4, 8, 4, 2, 1, 4)

@@ -81,6 +81,26 @@ def test_large(hip, m, k, n):
         check(call(hip, t, kind), t, kind)
 
 
+@pytest.mark.parametrize("k", [1, 64, 100, 128, 192, 256, 300, 512, 513])
+@pytest.mark.parametrize("m,n", [(2047, 64), (2048, 8), (2049, 72), (2100, 256), (2500, 264), (3001, 520), (5003, 128),
+                                 (20011, 40), (2300, 1032)])
+def test_many_rows_short_k(hip, m, n, k):
+    """Where rows stream past weights in registers: every depth, ends inside tiles, channels past a block."""
+    for kind, b, residual in (("f16", True, True), ("bf16", True, False), ("f16", False, False)):
+        t = operands(m, k, n, kind, b, residual)
+        out, ok = guarded((m, n), DT[kind], 7.0)
+        check(call(hip, t, kind, out=out), t, kind)
+        assert ok()
+    t = operands(m, k, n, "bf16", True, True)
+    want = call(hip, t, "bf16")
+    res = t["residual"].clone()
+    assert torch.equal(call(hip, dict(t, residual=res), "bf16", out=res), want)
+    assert torch.equal(call(hip, dict(t, residual=shifted(t["residual"])), "bf16"), want)
+    assert torch.equal(call(hip, t, "bf16", out=shifted(want)), want)
+    rows = dict(t, q=t["q"][7:60].contiguous(), qs=t["qs"][7:60].contiguous(), residual=t["residual"][7:60].contiguous())
+    assert torch.equal(call(hip, rows, "bf16"), want[7:60])  # a row's result is the same in a batch of any size
+
+
 @pytest.mark.parametrize("m", [1, 20, 70, 300, 600])
 def test_sums_are_exact(hip, m):
     """The longest rows of the largest integers: the sums reach 131008 * 128 * 128, just under 2^31, and one
