@@ -314,6 +314,24 @@ __global__ __launch_bounds__(64 * WM * WN * KS) void q8_tile_kernel(GemmArgs a) 
     }
 }
 
+// A buffer descriptor as its four words, and a direct-to-LDS load of 16 bytes a lane that the compiler does not
+// know as one: with the builtin it waits for every such load in flight before the next LDS read of the
+// kernel below. The load has no result, and whoever reads its bytes waits for it by vmcnt. (A write of m0
+// needs one wait state before such a load.)
+template <typename P>
+__device__ __forceinline__ uint4v words_of(const P* p, uint32_t bytes) {
+    const uint64_t at = reinterpret_cast<uint64_t>(p);
+    return uint4v{(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, bytes, 0x00020000u};
+}
+__device__ __forceinline__ void dma_lds_untracked(uint4v rsrc, void* dst, uint32_t off) {
+#ifdef __HIP_DEVICE_COMPILE__
+    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)dst;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc) : "memory");
+#else
+    (void)rsrc, (void)dst, (void)off;
+#endif
+}
+
 // Many rows, short k: the product is the reading of rows and the writing of results, so a wave keeps its weights
 // (NU operands of channels, KB steps) in registers and streams rows past them. A workgroup's four waves
 // are WM x WN over rows and channels, 16 or 32 rows a wave and tile; tiles come through LDS, two
@@ -328,16 +346,16 @@ __global__ __launch_bounds__(256) void q8_stream_kernel(GemmArgs a) {
     constexpr int BR = 16 * MF, WM = 4 / WN, XT = MF * WM * KB, XL = (XT + 3) / 4, RING = 3, SLOT = 4096 * XL;
     constexpr int CW = 16 * NU, H = NU / 2;  // channels a wave; 16-byte pieces of a lane's results a row
     constexpr uint32_t kDrop = 0x80000000u;
-    __shared__ __attribute__((aligned(1024))) char lds[RING * SLOT];
-    __shared__ __attribute__((aligned(16))) float params[2][CW * WN];
+    __shared__ __attribute__((aligned(1024))) char lds[RING * SLOT + 8 * CW * WN];  // the ring; scales, biases
+    float* params = reinterpret_cast<float*>(lds + RING * SLOT);
     const int item = xcd_item(blockIdx.x, gridDim.x), nt = item % a.ntiles, first = item / a.ntiles;
     const int stride = gridDim.x / a.ntiles, Kp = a.Kp, kbs = Kp / 64;
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int r16 = lane & 15, g = lane >> 4, wm = wave / WN, wn = wave % WN;
     const int c0 = CW * WN * nt, n0 = c0 + CW * wn;  // the workgroup's and the wave's first channel
     for (int i = threadIdx.x; i < CW * WN; i += 256) {
-        params[0][i] = c0 + i < a.N ? a.ws[c0 + i] : 0.f;
-        params[1][i] = a.b != nullptr && c0 + i < a.N ? a.b[c0 + i] : 0.f;
+        params[i] = c0 + i < a.N ? a.ws[c0 + i] : 0.f;
+        params[CW * WN + i] = a.b != nullptr && c0 + i < a.N ? a.b[c0 + i] : 0.f;
     }
     const int blocks = (a.N + 63) / 64;
     int4v w[KB][NU];
@@ -353,14 +371,18 @@ __global__ __launch_bounds__(256) void q8_stream_kernel(GemmArgs a) {
             w[kb][u] = load16(rw, kb < kbs && blk < blocks ? (uint32_t)(4096 * kb + 1024 * (c / 4 % 4) + 256 * g + 16 * (4 * (c / 16) + c % 4)) : kDrop);
         }
     }
+    // 0 .. most, kept on the scalar unit (a median would go to the vector unit, and with it a buffer's range)
+    const auto clamp = [](int v, int most) __attribute__((always_inline)) {
+        return __builtin_amdgcn_readfirstlane(max(0, min(most, v)));
+    };
     // load j of a tile: operand j / KB of rows, step j % KB
     const auto fetch = [&](int mt, char* slot) __attribute__((always_inline)) {
-        const int m0 = BR * WM * mt, rows = max(0, min(BR * WM, a.M - m0));
-        const auto rx = rsrc_of(a.q + (int64_t)(rows > 0 ? m0 : 0) * Kp, (uint32_t)(rows * Kp));
+        const int m0 = BR * WM * mt, rows = clamp(a.M - m0, BR * WM);
+        const auto rx = words_of(a.q + (int64_t)(rows > 0 ? m0 : 0) * Kp, (uint32_t)(rows * Kp));
 #pragma unroll
         for (int i = 0; i < XL; ++i) {
             const int j = 4 * i + wave, kb = j % KB, r = 16 * (j / KB) + (lane >> 2);
-            dma_lds<16>(rx, slot + 1024 * j, j < XT && kb < kbs ? (uint32_t)(r * Kp + 64 * kb + 16 * ((lane & 3) ^ ((r >> 2) & 3))) : kDrop);
+            dma_lds_untracked(rx, slot + 1024 * j, j < XT && kb < kbs ? (uint32_t)(r * Kp + 64 * kb + 16 * ((lane & 3) ^ ((r >> 2) & 3))) : kDrop);
         }
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("" ::: "memory");  // what is counted as newer stays newer
@@ -370,7 +392,7 @@ __global__ __launch_bounds__(256) void q8_stream_kernel(GemmArgs a) {
         half8 res[MF][RES ? H : 1];
     };
     const auto rows_of = [&](int mt, Rows& o) __attribute__((always_inline)) {
-        const int m0 = BR * (WM * mt + wm), rows = max(0, min(BR, a.M - m0)), base = rows > 0 ? m0 : 0;
+        const int m0 = BR * (WM * mt + wm), rows = clamp(a.M - m0, BR), base = rows > 0 ? m0 : 0;
         const auto rs = rsrc_of(a.qs + base, (uint32_t)(rows * 4));
         const auto rr = rsrc_of(RES ? a.residual + (int64_t)base * a.N : a.out, RES ? (uint32_t)rows * (uint32_t)a.N * 2u : 0u);
 #pragma unroll
@@ -387,7 +409,7 @@ __global__ __launch_bounds__(256) void q8_stream_kernel(GemmArgs a) {
         }
     };
     const auto tile = [&](int mt, const char* slot, const Rows& now) __attribute__((always_inline)) {
-        const int m0 = BR * (WM * mt + wm), rows = max(0, min(BR, a.M - m0));
+        const int m0 = BR * (WM * mt + wm), rows = clamp(a.M - m0, BR);
         const auto ro = rsrc_of(a.out + (int64_t)(rows > 0 ? m0 : 0) * a.N, (uint32_t)rows * (uint32_t)a.N * 2u);
         int4v acc[NU][MF];
 #pragma unroll
@@ -405,7 +427,7 @@ __global__ __launch_bounds__(256) void q8_stream_kernel(GemmArgs a) {
 #pragma unroll
         for (int h = 0; h < H; ++h) {
             const int c = CW * wn + 64 * (h / 2) + 32 * (h % 2) + 8 * g;
-            const float8v sw = *reinterpret_cast<const float8v*>(&params[0][c]), bv = *reinterpret_cast<const float8v*>(&params[1][c]);
+            const float8v sw = *reinterpret_cast<const float8v*>(params + c), bv = *reinterpret_cast<const float8v*>(params + CW * WN + c);
             const int n = c0 + c;
 #pragma unroll
             for (int mf = 0; mf < MF; ++mf) {
