@@ -79,7 +79,9 @@ struct Vec16<8> {
     typedef half8 type;
     typedef half8u unaligned;
 };
-template <bool BF, int RL>
+// (NT: nontemporal stores, for the large tiles' results: 8192 x 8192 x 8192 with a residual takes 424 us with and
+// 445 us without them, 8192 x 1024 x 8192 94 and 111 us.)
+template <bool BF, int RL, bool NT>
 __device__ __forceinline__ void store_run(const GemmArgs& a, int m, int n, const Channels<RL>& ch, const int (&sum)[RL]) {
     constexpr int W = RL < 8 ? RL : 8;  // channels an access
     if (m >= a.M || n >= a.N) return;
@@ -101,7 +103,9 @@ __device__ __forceinline__ void store_run(const GemmArgs& a, int m, int n, const
             typename Vec16<W>::type o;
 #pragma unroll
             for (int i = 0; i < W; ++i) o[i] = act_cvt<BF>(v[W * h + i]);
-            *reinterpret_cast<typename Vec16<W>::unaligned*>(a.out + at + W * h) = o;
+            typename Vec16<W>::unaligned* to = reinterpret_cast<typename Vec16<W>::unaligned*>(a.out + at + W * h);
+            if constexpr (NT) __builtin_nontemporal_store(o, to);
+            else *to = o;
         }
     } else {
 #pragma unroll
@@ -154,7 +158,7 @@ __global__ __launch_bounds__(256) void q8_rows_kernel(GemmArgs a) {
 #pragma unroll
     for (int v = 1; v < KW; ++v) acc += part[v][lane];
     const int n = 64 * (o / 4) + 16 * g + 4 * (o % 4);
-    store_run<BF, 4>(a, r16, n, Channels<4>(a, n), {acc[0], acc[1], acc[2], acc[3]});
+    store_run<BF, 4, false>(a, r16, n, Channels<4>(a, n), {acc[0], acc[1], acc[2], acc[3]});
 }
 
 // A workgroup computes 16 MF WM rows by 16 NU WN channels. Its waves are KS groups of WM x WN; wave (wm, wn) of a
@@ -283,7 +287,7 @@ __global__ __launch_bounds__(64 * WM * WN * KS) void q8_tile_kernel(GemmArgs a) 
                 int sum[4 * NE];
 #pragma unroll
                 for (int i = 0; i < 4 * NE; ++i) sum[i] = acc[u + i / 4][mf][i % 4];
-                store_run<BF, 4 * NE>(a, m0 + 16 * (MF * wm + mf) + r16, n, ch, sum);
+                store_run<BF, 4 * NE, true>(a, m0 + 16 * (MF * wm + mf) + r16, n, ch, sum);
             }
         }
     } else {
@@ -309,7 +313,7 @@ __global__ __launch_bounds__(64 * WM * WN * KS) void q8_tile_kernel(GemmArgs a) 
                 for (int i = 0; i < 4; ++i) sum[4 * e + i] = s[i];
             }
             const int o = o0 + NU * wn + u, n = 64 * (o / 4) + 16 * g + 4 * (o % 4);
-            store_run<BF, 4 * NE>(a, m0 + 16 * (MF * wm + mf) + r16, n, Channels<4 * NE>(a, n), sum);
+            store_run<BF, 4 * NE, false>(a, m0 + 16 * (MF * wm + mf) + r16, n, Channels<4 * NE>(a, n), sum);
         }
     }
 }
@@ -472,14 +476,15 @@ __global__ __launch_bounds__(256) void q8_stream_kernel(GemmArgs a) {
 constexpr int64_t kMaxKp = 131008;
 
 // The tiles for more than 64 rows, by estimated time: a round of 256 tiles, one for each CU, costs a fixed part
-// (loads that wait for the first operands, the results) and one for k. Measured in us, for 1024 inputs, from
-// 8192 x k x 8192 at k = 1024 and 8192 (v0 to v3 of the sizes below: 88, 81, 94, 162 us and 413, 464, 579,
-// 831 us): large tiles read less for each product, small ones fill the card where there are few.
+// (loads that wait for the first operands, the results) and one for k. Both measured, in us and in us for
+// 1024 inputs, from 8192 x k x 8192 at k = 1024 and 8192: 86 and 420 us with the first of the sizes below, 79 and
+// 455, 103 and 557, 181 and 842 with the others. Large tiles read less for each product, small ones fill
+// the card where there are few.
 struct Tile {
     int rows, channels;
     double fixed, per1024;
 };
-constexpr Tile kTiles[] = {{256, 256, 10.5, 11.6}, {128, 256, 3.4, 6.83}, {128, 128, 1.55, 4.33}, {64, 64, 1.04, 1.5}};
+constexpr Tile kTiles[] = {{256, 256, 9.4, 11.9}, {128, 256, 3.2, 6.7}, {128, 128, 2.4, 4.05}, {64, 64, 1.35, 1.48}};
 
 int best_tile(int64_t M, int64_t N, int64_t Kp) {
     int best = 0;
@@ -571,7 +576,7 @@ void launch(hipStream_t s, GemmArgs& a) {
     switch (best_tile(a.M, a.N, a.Kp)) {
     case 0: CLK_TILE(4, 8, 4, 2, 1, 4)
     case 1: CLK_TILE(4, 8, 2, 2, 1, 3)
-    case 2: CLK_TILE(4, 4, 2, 2, 1, 5)
+    case 2: CLK_TILE(2, 4, 4, 2, 1, 4)
     default: CLK_TILE(2, 4, 2, 1, 2, 4)
     }
 #undef CLK_TILE
