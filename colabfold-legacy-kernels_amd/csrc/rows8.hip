@@ -138,15 +138,34 @@ __device__ __forceinline__ Stats row_all(Stats s, RowShare<TPR>& share, int& tur
     return s;
 }
 
-// Rows are split in chunks of 8 values. Widths and addresses are any, so a chunk is loaded and stored by one
-// 16-byte access of 2-byte alignment (the hardware takes any; aligned rows lose nothing), and the one
-// chunk that the width cuts value by value.
+// Rows are split in chunks of 8 values. Widths and addresses are any, so a chunk is one 16-byte access of 2-byte
+// alignment: the hardware takes any, and only rows on odd multiples of 2 bytes lose by it (norm of [8192, 8191] in
+// bf16 with the residual 124 us, of [8192, 8190] 99, of [8192, 8192] 96). Accesses by pairs or single values,
+// which need no alignment, were slower.
+//
+// A chunk that the width cuts, and one past it, is loaded from the row's last 8 values and shifted down in its
+// registers, so that every lane's loads are issued without a branch before any is waited for (a branch
+// of its own for the cut chunk made its wave, and at the barrier the row, wait for it: gradients of [8192,
+// 8190] 177 us against 108). Rows of less than 8 values are read one by one.
 __device__ __forceinline__ half8 load8(const half_t* row, int col, int C) {
-    if (col + 8 <= C) return *reinterpret_cast<const half8u*>(row + col);
+    if (C >= 8) return *reinterpret_cast<const half8u*>(row + min(col, C - 8));
     half8 v = {};
 #pragma unroll
     for (int e = 0; e < 8; ++e)
         if (col + e < C) v[e] = row[col + e];
+    return v;
+}
+// what load8 gave as the values col .. col + 7, zeros past C
+__device__ __forceinline__ half8 cut8(half8 v, int col, int C) {
+    const int over = col + 8 - C;  // values past the end
+    if (C >= 8 && over > 0) {
+        typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+        u64x2 w = __builtin_bit_cast(u64x2, v);
+        if (over & 4) w = u64x2{w[1], 0};
+        const int bits = 16 * (over & 3);
+        if (bits > 0) w = u64x2{w[0] >> bits | w[1] << (64 - bits), w[1] >> bits};
+        v = over >= 8 ? half8{} : __builtin_bit_cast(half8, w);
+    }
     return v;
 }
 __device__ __forceinline__ void store8(half_t* row, int col, int C, half8 v) {
@@ -302,20 +321,25 @@ __global__ __launch_bounds__(block_of(TPR)) void rms_norm_kernel(RmsArgs a) {
     for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.M; r0 += (int64_t)gridDim.x * ROWS) {
         const int64_t row = r0 + sub;
         const bool in = ROWS == 1 || row < a.M;
-        const int len = in ? C : 0;  // a row past M is read as one of no values
-        const half_t* xr = a.x + row * C;
+        const int64_t from = ROWS == 1 ? row : min(row, a.M - 1);  // a row past M reads the last one and stores nothing
+        const int len = in ? C : 0;
         half8 v[NCH], res[NCH];
 #pragma unroll
-        for (int j = 0; j < NCH; ++j) v[j] = load8(xr, 8 * (part + TPR * j), len);
+        for (int j = 0; j < NCH; ++j) v[j] = load8(a.x + from * C, 8 * (part + TPR * j), C);
         if constexpr (RES) {
 #pragma unroll
-            for (int j = 0; j < NCH; ++j) res[j] = load8(a.residual + row * C, 8 * (part + TPR * j), len);
+            for (int j = 0; j < NCH; ++j) res[j] = load8(a.residual + from * C, 8 * (part + TPR * j), C);
 #pragma unroll
             for (int j = 0; j < NCH; ++j) {
+                v[j] = cut8(v[j], 8 * (part + TPR * j), C);
+                res[j] = cut8(res[j], 8 * (part + TPR * j), C);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[j][e] = act_cvt<BF>(act_get<BF>(v[j], e) + act_get<BF>(res[j], e));
                 store8(a.sum + row * C, 8 * (part + TPR * j), len, v[j]);
             }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NCH; ++j) v[j] = cut8(v[j], 8 * (part + TPR * j), C);
         }
         Stats s{0.f, 0, 0};
         const auto collect = [&](float d) __attribute__((always_inline)) {
@@ -381,13 +405,11 @@ struct RmsBwdArgs {
     float inv_c;
 };
 
-// Workgroup p takes rows p, p + P, ...; its share of dw goes to row p of the workspace, where each thread
-// adds to columns of its own.
+// Rows of any length: a block a row for ds; dw by columns in a kernel of its own, which reads s and dout again.
 template <bool BF>
 __global__ __launch_bounds__(256) void rms_norm_bwd_any_kernel(RmsBwdArgs a) {
     __shared__ float slot[4];
-    float* part = a.partial + (int64_t)blockIdx.x * a.ldp;
-    for (int64_t row = blockIdx.x; row < a.M; row += a.P) {
+    for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
         const float r = a.rstd[row];
         const half_t* sr = a.s + row * a.C;
         const half_t* dr = a.dout + row * a.C;
@@ -401,9 +423,23 @@ __global__ __launch_bounds__(256) void rms_norm_bwd_any_kernel(RmsBwdArgs a) {
             float d = r * (dy * a.w[c] - xh * dot);
             if (a.dsum != nullptr) d += get16<BF>(a.dsum + row * a.C + c);
             a.ds[row * a.C + c] = act_cvt<BF>(d);
-            part[c] = (row == blockIdx.x ? 0.f : part[c]) + dy * xh;
         }
     }
+}
+// 2048 columns a block, 8 a thread; rows blockIdx.y, + P, ...
+template <bool BF>
+__global__ __launch_bounds__(256) void rms_norm_dw_any_kernel(RmsBwdArgs a) {
+    const int64_t col = 8 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
+    if (col >= a.C) return;
+    float8v dw = {};
+    for (int64_t row = blockIdx.y; row < a.M; row += a.P) {
+        const float r = a.rstd[row];
+        const half8 s = cut8(load8(a.s + row * a.C, (int)col, (int)a.C), (int)col, (int)a.C);
+        const half8 dy = cut8(load8(a.dout + row * a.C, (int)col, (int)a.C), (int)col, (int)a.C);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dw[e] += act_get<BF>(dy, e) * (act_get<BF>(s, e) * r);
+    }
+    *reinterpret_cast<float8v*>(a.partial + (int64_t)blockIdx.y * a.ldp + col) = dw;
 }
 
 // Rows of up to 8 TPR NCH values in registers, a block's share of dw in registers too, until its rows are done.
@@ -422,14 +458,23 @@ __global__ __launch_bounds__(block_of(TPR)) void rms_norm_bwd_kernel(RmsBwdArgs 
     }
     for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.M; r0 += (int64_t)a.P * ROWS) {
         const int64_t row = r0 + sub;
-        const int len = ROWS == 1 || row < a.M ? C : 0;
-        const float r = len > 0 ? a.rstd[row] : 0.f;
+        const bool in = ROWS == 1 || row < a.M;
+        const int64_t from = ROWS == 1 ? row : min(row, a.M - 1);  // a row past M reads the last one and counts as zeros
+        const int len = in ? C : 0;
+        const float r = a.rstd[from];
         half8 s[NCH], dy[NCH], dz[NCH];
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
-            s[j] = load8(a.s + row * C, 8 * (part + TPR * j), len);
-            dy[j] = load8(a.dout + row * C, 8 * (part + TPR * j), len);
-            if constexpr (DSUM) dz[j] = load8(a.dsum + row * C, 8 * (part + TPR * j), len);
+            s[j] = load8(a.s + from * C, 8 * (part + TPR * j), C);
+            dy[j] = load8(a.dout + from * C, 8 * (part + TPR * j), C);
+            if constexpr (DSUM) dz[j] = load8(a.dsum + from * C, 8 * (part + TPR * j), C);
+        }
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            s[j] = cut8(s[j], 8 * (part + TPR * j), C);
+            dy[j] = cut8(dy[j], 8 * (part + TPR * j), C);
+            if constexpr (DSUM) dz[j] = cut8(dz[j], 8 * (part + TPR * j), C);
+            if (!in) s[j] = dy[j] = half8{};
         }
         Stats t{0.f, 0, 0};
 #pragma unroll
@@ -513,19 +558,29 @@ Route route_of(int64_t Kp) {
     if (Kp <= 4096) return {256, 2};
     if (Kp <= 6144) return {256, 3};
     if (Kp <= 8192) return {512, 2};
+    if (Kp <= 12288) return {512, 3};
     if (Kp <= 16384) return {1024, 2};
+    if (Kp <= 32768) return {1024, 4};
     return {0, 0};
 }
-#define CLK_ROUTES(X_) X_(8, 1) X_(16, 1) X_(32, 1) X_(64, 1) X_(64, 2) X_(256, 1) X_(256, 2) X_(256, 3) X_(512, 2) X_(1024, 2)
+#define CLK_ROUTES(X_) X_(8, 1) X_(16, 1) X_(32, 1) X_(64, 1) X_(64, 2) X_(256, 1) X_(256, 2) X_(256, 3) X_(512, 2) X_(512, 3) X_(1024, 2) X_(1024, 4)
 
 int64_t padded64(int64_t k) { return (k + 63) / 64 * 64; }
+
+// The gradients hold twice the registers: for [4096, 12000] 512 threads with 3 chunks take 100 us, 1024 with 2 88 us.
+Route bwd_route(int64_t C) {
+    const Route rt = route_of(padded64(C));
+    if (rt.nch == 4) return {0, 0};
+    return rt.nch == 3 && rt.tpr == 512 ? Route{1024, 2} : rt;
+}
 
 // The workgroups of the backward's first kernel: a rule on the shape alone, so that results do not
 // depend on the device. One round of what 256 CUs hold, but where rows are few, about 8 steps each: a
 // workgroup costs its row of partial sums, written and read.
 int bwd_parts(int64_t M, int64_t C) {
-    const Route rt = route_of(padded64(C));
-    const int rows = rt.tpr > 0 ? block_of(rt.tpr) / rt.tpr : 1, threads = rt.tpr > 0 ? block_of(rt.tpr) : 256;
+    const Route rt = bwd_route(C);
+    if (rt.tpr == 0) return (int)std::min<int64_t>(M, 64);
+    const int rows = block_of(rt.tpr) / rt.tpr, threads = block_of(rt.tpr);
     const int64_t steps = (M + rows - 1) / rows, most = 256 * 1024 / threads;
     return (int)std::min(steps, std::min<int64_t>(most, std::max<int64_t>(256, steps / 8)));
 }
@@ -581,48 +636,63 @@ __global__ __launch_bounds__(256) void quantize_any_kernel(QuantArgs a) {
     }
 }
 
-// 8 values of h from column col of a row
-template <int T, int ACT>
-__device__ __forceinline__ void hidden8(const void* x, int64_t row, int col, int K, int len, float (&h)[8]) {
-    const int64_t at = row * (ACT == kActSwish ? 2 * (int64_t)K : K);
+// 8 values from column col of a row of h: read, and made of what was read
+template <int T>
+struct Raw8 {
+    half8 v;
+};
+template <>
+struct Raw8<kF32> {
+    float8v v;
+};
+template <int T>
+__device__ __forceinline__ void read8(const void* x, int64_t at, int col, int K, Raw8<T>& r) {
+    if constexpr (T == kF32) r.v = load8f(static_cast<const float*>(x) + at, col, K);
+    else r.v = load8(static_cast<const half_t*>(x) + at, col, K);
+}
+template <int T>
+__device__ __forceinline__ void floats8(const Raw8<T>& r, int col, int K, float (&f)[8]) {
     if constexpr (T == kF32) {
-        const float* p = static_cast<const float*>(x) + at;
-        const float8v g = load8f(p, col, len);
-        float8v u;
-        if constexpr (ACT == kActSwish) u = load8f(p + K, col, len);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] = ACT == kActSwish ? g[e] * sigmoid_fast(g[e]) * u[e] : ACT == kActRelu ? relu(g[e]) : g[e];
+        for (int e = 0; e < 8; ++e) f[e] = r.v[e];
     } else {
-        constexpr bool BF = T == kBf16;
-        const half_t* p = static_cast<const half_t*>(x) + at;
-        const half8 g = load8(p, col, len);
-        half8 u;
-        if constexpr (ACT == kActSwish) u = load8(p + K, col, len);
+        const half8 v = cut8(r.v, col, K);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float f = act_get<BF>(g, e);
-            h[e] = ACT == kActSwish ? f * sigmoid_fast(f) * act_get<BF>(u, e) : ACT == kActRelu ? relu(f) : f;
-        }
+        for (int e = 0; e < 8; ++e) f[e] = act_get<T == kBf16>(v, e);
     }
 }
 
 template <int T, int ACT, int TPR, int NCH>
 __global__ __launch_bounds__(block_of(TPR)) void quantize_kernel(QuantArgs a) {
     constexpr int ROWS = block_of(TPR) / TPR;
+    constexpr bool GATE = ACT == kActSwish;
     __shared__ RowShare<TPR> share;
     const int part = threadIdx.x % TPR, sub = threadIdx.x / TPR, K = (int)a.K, Kp = (int)a.Kp;
     int turn = 0;
     for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.M; r0 += (int64_t)gridDim.x * ROWS) {
         const int64_t row = r0 + sub;
         const bool in = ROWS == 1 || row < a.M;
-        float h[NCH][8];
+        const int64_t at = (ROWS == 1 ? row : min(row, a.M - 1)) * (GATE ? 2 * (int64_t)K : K);  // past M: the last row, unused
+        Raw8<T> raw[NCH], up[GATE ? NCH : 1];
 #pragma unroll
-        for (int j = 0; j < NCH; ++j) hidden8<T, ACT>(a.x, row, 8 * (part + TPR * j), K, in ? K : 0, h[j]);
+        for (int j = 0; j < NCH; ++j) {
+            read8(a.x, at, 8 * (part + TPR * j), K, raw[j]);
+            if constexpr (GATE) read8(a.x, at + K, 8 * (part + TPR * j), K, up[j]);
+        }
+        float h[NCH][8];
         Stats s{0.f, 0, 0};
 #pragma unroll
-        for (int j = 0; j < NCH; ++j)
+        for (int j = 0; j < NCH; ++j) {
+            float u[8];
+            floats8(raw[j], 8 * (part + TPR * j), K, h[j]);
+            if constexpr (GATE) floats8(up[j], 8 * (part + TPR * j), K, u);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s.max0 = max(s.max0, abs_bits(h[j][e]));
+            for (int e = 0; e < 8; ++e) {
+                if constexpr (GATE) h[j][e] = h[j][e] * sigmoid_fast(h[j][e]) * u[e];
+                if constexpr (ACT == kActRelu) h[j][e] = relu(h[j][e]);
+                s.max0 = max(s.max0, abs_bits(h[j][e]));
+            }
+        }
         s = row_all<TPR>(s, share, turn);
         float inv, scale;
         row_scale(s.max0, 1.f, inv, scale);
@@ -791,16 +861,21 @@ extern "C" int clk_rms_norm_bwd(clk_stream stream, const clk_buffer* s, const cl
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     stage_mark(st, 0);
     if (M > 0) {
-        const Route rt = route_of(padded64(C));
+        const Route rt = bwd_route(C);
 #define CLK_BWD_RT(TPR_, NCH_)                                                                                        \
-    if (rt.tpr == TPR_ && rt.nch == NCH_) {                                                                           \
-        if (has_dsum) hipLaunchKernelGGL((rms_norm_bwd_kernel<BF, TPR_, NCH_, true>), grid, block, 0, st, a);         \
-        else hipLaunchKernelGGL((rms_norm_bwd_kernel<BF, TPR_, NCH_, false>), grid, block, 0, st, a);                 \
+    if (rt.tpr == TPR_ && rt.nch == NCH_ && NCH_ < 4) {                                                               \
+        if (has_dsum) hipLaunchKernelGGL((rms_norm_bwd_kernel<BF, TPR_, NCH_ < 4 ? NCH_ : 1, true>), grid, block, 0, st, a);         \
+        else hipLaunchKernelGGL((rms_norm_bwd_kernel<BF, TPR_, NCH_ < 4 ? NCH_ : 1, false>), grid, block, 0, st, a);                 \
     }
         const auto launch = [&](auto bf_) {
             constexpr bool BF = decltype(bf_)::value;
-            const dim3 grid(a.P), block(rt.tpr == 0 ? 256 : block_of(rt.tpr));
-            if (rt.tpr == 0) hipLaunchKernelGGL(rms_norm_bwd_any_kernel<BF>, grid, block, 0, st, a);
+            if (rt.tpr == 0) {
+                // dw first: ds may overwrite dout
+                hipLaunchKernelGGL(rms_norm_dw_any_kernel<BF>, dim3((unsigned)((C + 2047) / 2048), a.P), dim3(256), 0, st, a);
+                hipLaunchKernelGGL(rms_norm_bwd_any_kernel<BF>, dim3(any_blocks(M)), dim3(256), 0, st, a);
+                return;
+            }
+            const dim3 grid(a.P), block(block_of(rt.tpr));
             CLK_ROUTES(CLK_BWD_RT)
         };
         act == CLK_BF16 ? launch(std::true_type()) : launch(std::false_type());
