@@ -611,7 +611,10 @@ extern "C" int clk_q8_projection(clk_stream stream, const clk_buffer* q, const c
     if (elements(w_scale) != N || (has_b && elements(b) != N)) return invalid("q8_projection: w_scale and b must be [N]");
     if (has_residual && !same_shape(residual, out)) return invalid("q8_projection: residual must be like out");
     if (M == 0 || N == 0) return ok();
-    if (M > INT32_MAX - 256 || N > INT32_MAX - 256 || (M + 63) / 64 * nt > INT32_MAX / 512) return invalid("q8_projection: too large");
+    // a launch holds 2^32 threads: 256 for each 64 x 64 tile, or 512 for each 16 channels of up to 64 rows
+    if (M > INT32_MAX - 256 || (M <= 64 ? nt >= 1 << 21 : nt >= 1 << 24 || (M + 63) / 64 * nt >= 1 << 24)) {
+        return invalid("q8_projection: too large");
+    }
     if (!aligned16(q->data) || !aligned16(wq->data)) return invalid("q8_projection: q and wq must be 16-byte aligned");
     GemmArgs a{static_cast<const int8_t*>(q->data), static_cast<const float*>(q_scale->data),
                static_cast<const int8_t*>(wq->data), static_cast<const float*>(w_scale->data),

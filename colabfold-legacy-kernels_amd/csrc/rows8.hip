@@ -859,7 +859,8 @@ extern "C" int clk_rms_norm_bwd(clk_stream stream, const clk_buffer* s, const cl
                  static_cast<const float*>(rstd->data), static_cast<half_t*>(ds->data), static_cast<float*>(workspace),
                  static_cast<float*>(dscale->data), M, C, bwd_ldp(C), M > 0 ? bwd_parts(M, C) : 0, 1.f / (float)C};
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    stage_mark(st, 0);
+    int stage = 0;
+    stage_mark(st, stage);
     if (M > 0) {
         const Route rt = bwd_route(C);
 #define CLK_BWD_RT(TPR_, NCH_)                                                                                        \
@@ -872,6 +873,7 @@ extern "C" int clk_rms_norm_bwd(clk_stream stream, const clk_buffer* s, const cl
             if (rt.tpr == 0) {
                 // dw first: ds may overwrite dout
                 hipLaunchKernelGGL(rms_norm_dw_any_kernel<BF>, dim3((unsigned)((C + 2047) / 2048), a.P), dim3(256), 0, st, a);
+                stage_mark(st, ++stage);
                 hipLaunchKernelGGL(rms_norm_bwd_any_kernel<BF>, dim3(any_blocks(M)), dim3(256), 0, st, a);
                 return;
             }
@@ -879,10 +881,11 @@ extern "C" int clk_rms_norm_bwd(clk_stream stream, const clk_buffer* s, const cl
             CLK_ROUTES(CLK_BWD_RT)
         };
         act == CLK_BF16 ? launch(std::true_type()) : launch(std::false_type());
+        stage_mark(st, ++stage);
 #undef CLK_BWD_RT
     }
     hipLaunchKernelGGL(rms_norm_dw_kernel, dim3((unsigned)((C + 15) / 16)), dim3(256), 0, st, a);
-    stage_mark(st, 1);
+    stage_mark(st, ++stage);
     return launch_status("rms_norm_bwd");
 }
 

@@ -230,6 +230,27 @@ def test_rms_norm_autograd(hip, kind):
     assert torch.equal(x.grad.view(40, 200), 2 * hip.rms_norm_bwd(s2, w.detach(), rstd, dy)[0])
 
 
+def test_rms_norm_autograd_corners(hip):
+    """No rows, one value, an expanded gradient, a gradient of another type, a scale of its own shape, a
+    second derivative."""
+    w = torch.ones(96, device="cuda", requires_grad=True)
+    x = torch.empty((0, 96), dtype=torch.float16, device="cuda", requires_grad=True)
+    gx, gw = torch.autograd.grad(torch_ops.rms_norm(x, w), (x, w), torch.empty_like(x))
+    assert gx.shape == x.shape and (gw == 0).all()
+    x, _, w = inputs(5, 64, "bf16", False)
+    x, w = x.view(1, 5, 64).requires_grad_(), w.view(1, 64).requires_grad_()
+    y = torch_ops.rms_norm(x, w)
+    g1 = torch.autograd.grad(y.sum(), (x, w), retain_graph=True)  # a gradient without strides
+    g2 = torch.autograd.grad(y, (x, w), torch.ones_like(y))
+    assert torch.equal(g1[0], g2[0]) and torch.equal(g1[1], g2[1]) and g1[1].shape == w.shape
+    with pytest.raises(RuntimeError):
+        g = torch.autograd.grad(torch_ops.rms_norm(x, w).float().square().sum(), x, create_graph=True)[0]
+        g.sum().backward()
+    one = torch.full((1, 1), -3.0, dtype=torch.float16, device="cuda", requires_grad=True)
+    y = torch_ops.rms_norm(one, torch.ones(1, device="cuda"), eps=0.0)
+    assert y.item() == -1 and torch.autograd.grad(y, one)[0].abs().item() < 1e-3
+
+
 def test_rms_norm_gradient_against_differences(hip):
     """The GPU's gradients against central differences of the float64 forward on the same values. The
     gradient carries a rounding to bf16 (2^-8 of itself), the differences an error far below that."""

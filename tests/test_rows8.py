@@ -199,6 +199,11 @@ def test_q8_projection_refusals(lib):
                            (dict(wq=buf(S8, 2, 2, 4, 4, 16, 16, data=0x100008)), "16-byte aligned")):
         st = lib.clk_q8_projection(None, *refs({**a, **other}.values()), 1, 1)
         assert st == 3 and message in lib.clk_last_error().decode(), (message, lib.clk_last_error())
+    for rows, n2 in ((1, 1 << 28), (1 << 21, 1 << 16), (1 << 31, n)):  # more than a launch holds
+        big = dict(a, q=buf(S8, rows, kp), qs=buf(F32, rows), wq=buf(S8, -(-n2 // 64), 2, 4, 4, 16, 16), ws=buf(F32, n2),
+                   b=buf(F32, n2), residual=buf(F16, rows, n2), out=buf(F16, rows, n2))
+        assert lib.clk_q8_projection(None, *refs(big.values()), 1, 1) == 3
+        assert "too large" in lib.clk_last_error().decode()
     empty = dict(a, q=buf(S8, 0, kp), qs=buf(F32, 0), residual=buf(F16, 0, n), out=buf(F16, 0, n))
     assert lib.clk_q8_projection(None, *refs(empty.values()), 1, 1) == 0
     none = dict(a, wq=buf(S8, 0, 2, 4, 4, 16, 16), ws=buf(F32, 0), b=buf(F32, 0), residual=buf(F16, m, 0), out=buf(F16, m, 0))
