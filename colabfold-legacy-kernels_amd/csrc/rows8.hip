@@ -59,11 +59,14 @@ __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
 // 1 / sqrt(ss / C + eps) from a row's sum of squares
 __device__ __forceinline__ float inv_rms(float ss, float inv_c, float eps) { return 1.f / sqrtf(ss * inv_c + eps); }
 
-// A bf16 row with values past kBig has sums of squares, or products with w, past fp32's range: it is
-// taken with its values scaled by kDown (a power of two, so every product stays what it was), where eps
-// is nothing.
-constexpr float kBig = 0x1p40f, kDown = 0x1p-90f;
-__device__ __forceinline__ bool is_big(uint32_t bits) { return bits >= __builtin_bit_cast(uint32_t, kBig) && bits < kInfBits; }
+// A bf16 row with values past 2^40 has sums of squares, or products with w, past fp32's range; one of
+// values below 2^-40 has them below it, which counts where eps is next to nothing. Such a row is taken
+// with its values times a power of two (so every product stays what it was) and eps times its square.
+__device__ __forceinline__ float row_shift(uint32_t bits, float eps) {
+    if (bits >= kInfBits) return 1.f;
+    const float a = __builtin_bit_cast(float, bits);
+    return a >= 0x1p40f ? 0x1p-90f : a < 0x1p-40f && eps < 0x1p-100f ? 0x1p90f : 1.f;
+}
 
 // v of the lane that DPP control CTRL names
 template <int CTRL>
@@ -274,9 +277,8 @@ __global__ __launch_bounds__(256) void rms_norm_any_kernel(RmsArgs a) {
         const half_t* vr = RES ? sr : xr;  // each thread reads back only what it wrote
         ss = block_sum<256>(ss, fslot);
         m = block_max<256>(m, uslot);
-        float d = 1.f;
-        if (BF && is_big(m)) {
-            d = kDown;
+        const float d = BF ? row_shift(m, a.eps) : 1.f;
+        if (d != 1.f) {
             ss = 0.f;
             mt = 0;
             for (int64_t c = threadIdx.x; c < a.C; c += 256) {
@@ -286,7 +288,7 @@ __global__ __launch_bounds__(256) void rms_norm_any_kernel(RmsArgs a) {
             }
             ss = block_sum<256>(ss, fslot);
         }
-        const float r = inv_rms(ss, a.inv_c, d == 1.f ? a.eps : 0.f);
+        const float r = inv_rms(ss, a.inv_c, a.eps * d * d);
         if constexpr (Q8) {
             mt = block_max<256>(max(mt, m >= kInfBits ? m : 0u), uslot);
             float inv, scale;
@@ -358,12 +360,10 @@ __global__ __launch_bounds__(block_of(TPR)) void rms_norm_kernel(RmsArgs a) {
         collect(1.f);
         float d = 1.f;
         if constexpr (BF) {
-            if (is_big(s.max0)) {
-                d = kDown;
-                collect(d);
-            }
+            d = row_shift(s.max0, a.eps);
+            if (d != 1.f) collect(d);
         }
-        const float r = inv_rms(s.sum, a.inv_c, d == 1.f ? a.eps : 0.f);
+        const float r = inv_rms(s.sum, a.inv_c, a.eps * d * d);
         if constexpr (Q8) {
             float inv, scale;
             row_scale(s.max1, r, inv, scale);
@@ -584,6 +584,8 @@ int bwd_parts(int64_t M, int64_t C) {
     const int64_t steps = (M + rows - 1) / rows, most = 256 * 1024 / threads;
     return (int)std::min(steps, std::min<int64_t>(most, std::max<int64_t>(256, steps / 8)));
 }
+// 16 threads a column, and a launch takes fewer than 2^32 threads
+constexpr int64_t kMostBwd = 1 << 27;
 int64_t bwd_ldp(int64_t C) { return (C + 63) / 64 * 64; }
 
 // ---- rows to 8 bits and back --------------------------------------------------------------
@@ -828,7 +830,7 @@ extern "C" int clk_rms_norm_q8(clk_stream stream, const clk_buffer* x, const clk
 
 extern "C" size_t clk_rms_norm_bwd_workspace_size(const clk_buffer* s) {
     if (s == nullptr || s->rank != 2 || s->dims == nullptr || s->dims[0] < 1 || s->dims[1] < 1 ||
-        s->dims[0] > INT32_MAX || s->dims[1] > INT32_MAX / 2) {
+        s->dims[0] > INT32_MAX || s->dims[1] > kMostBwd) {
         return 0;
     }
     return (size_t)bwd_parts(s->dims[0], s->dims[1]) * bwd_ldp(s->dims[1]) * 4;
@@ -843,6 +845,7 @@ extern "C" int clk_rms_norm_bwd(clk_stream stream, const clk_buffer* s, const cl
     const int types[] = {act, CLK_F32, CLK_F32, act, act, act, CLK_F32};
     if (int st = check_types("rms_norm_bwd", bufs, types, 7)) return st;
     if (int st = check_rows("rms_norm_bwd", s)) return st;
+    if (s->dims[1] > kMostBwd) return invalid("rms_norm_bwd: too large");
     const int64_t M = s->dims[0], C = s->dims[1];
     if (elements(scale) != C || elements(dscale) != C) return invalid("rms_norm_bwd: scale and dscale must be [C]");
     if (elements(rstd) != M) return invalid("rms_norm_bwd: rstd must be [M]");

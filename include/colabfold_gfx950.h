@@ -240,7 +240,7 @@ int clk_rms_norm_q8(clk_stream stream, const clk_buffer* x, const clk_buffer* re
 /* Gradients of clk_rms_norm: s [M,C] (x, or the forward's sum), scale [C], rstd [M], dout [M,C] and, with
  * has_dsum, the gradient of sum, dsum [M,C] -> ds [M,C] = rstd (g - xh mean(g xh)) + dsum with xh =
  * s rstd and g = dout scale (the gradient of x and of residual alike), dscale [C] F32 = the sum over the
- * M rows of dout xh (zeros for M = 0). ds may alias dout or dsum. workspace: device scratch of at least
+ * M rows of dout xh (zeros for M = 0). C at most 2^27. ds may alias dout or dsum. workspace: device scratch of at least
  * clk_rms_norm_bwd_workspace_size() bytes, 256-byte aligned, not shared by two calls in flight.
  * Bit-identical from run to run (no atomics). */
 int clk_rms_norm_bwd(clk_stream stream, const clk_buffer* s, const clk_buffer* scale,

@@ -151,6 +151,17 @@ def test_rms_norm_bwd_refusals(lib):
     assert lib.clk_rms_norm_bwd_workspace_size(None) == 0
 
 
+def test_rms_norm_bwd_of_the_longest_rows(lib):
+    """Rows past 2^27 values would need more threads than a launch takes."""
+    for m, c in ((1, 2 ** 27), (1, 2 ** 27 + 1), (5, 2 ** 29)):
+        s = buf(F16, m, c)
+        need = lib.clk_rms_norm_bwd_workspace_size(s[0])
+        assert (need == 0) == (c > 2 ** 27)
+        if c > 2 ** 27:
+            st = lib.clk_rms_norm_bwd(None, *refs([s, buf(F32, c), buf(F32, m), s, s, s, buf(F32, c)]), 0, 0x100000, 2 ** 40)
+            assert st == 3 and "rms_norm_bwd: too large" in lib.clk_last_error().decode()
+
+
 def test_quantize_rows_refusals(lib):
     for x, q, s, act, message in (
             (buf(F16, 6, 40), buf(S8, 6, 64), buf(F32, 6), 3, "activation is 0 (none)"),

@@ -180,6 +180,20 @@ def test_eps_zero_and_large(hip):
     check_norm(y, rstd, host(x), w, 100.0, "f16")
 
 
+@pytest.mark.parametrize("std,eps", [(2.0 ** -85, 0.0), (2.0 ** -126, 0.0), (2.0 ** -55, 2.0 ** -110),
+                                     (2.0 ** -85, 2.0 ** -140), (2.0 ** -45, 1e-5), (2.0 ** 45, 2.0 ** 92)])
+@pytest.mark.parametrize("c", [128, 1000, 40000])
+def test_squares_out_of_range(hip, c, std, eps):
+    """bf16 rows whose squares leave fp32's range below (eps next to nothing) or above, eps of their size too."""
+    x, _, w = inputs(5, c, "bf16", False)
+    x = (x.double() * std).to(torch.bfloat16)
+    y, _, rstd = hip.rms_norm(x, w, None, eps, want_rstd=True)
+    check_norm(y, rstd if std > 2.0 ** -120 else None, host(x), w, eps, "bf16")
+    q, qs, _ = hip.rms_norm_q8(x, w, None, eps)
+    t, r = host(x) * host(w), orr.rms_norm(host(x), host(w), eps)[1]
+    check_q8(q, qs, t * 2.0 ** 120 if std < 1 else t, r * (2.0 ** -120 if std < 1 else 1.0), slack=E)
+
+
 @pytest.mark.parametrize("c", [128, 1000, 9000, 40000])
 def test_in_place(hip, c):
     """sum over x or over residual, out over x: the same bits as into buffers of their own."""
