@@ -308,7 +308,9 @@ __global__ __launch_bounds__(256) void rms_norm_any_kernel(RmsArgs a) {
     }
 }
 
-// Rows of up to 8 TPR NCH values, held in registers: TPR threads a row, NCH chunks each, one pass over memory.
+// Rows of up to 8 TPR NCH values, held in registers: TPR threads a row, NCH chunks each, one pass over memory,
+// which bounds it. [16384, 8192] bf16 with the residual: 176 us (1.07 GB, 6.1 TB/s); [147456, 128] fp16: 13.8 us
+// (5.5 TB/s); 8-bit rows of [4099, 5120] bf16 with the residual: 27 us (5.4 TB/s).
 constexpr int block_of(int tpr) { return tpr < 256 ? 256 : tpr; }
 
 template <bool BF, int TPR, int NCH, bool RES, bool Q8>
@@ -442,7 +444,8 @@ __global__ __launch_bounds__(256) void rms_norm_dw_any_kernel(RmsBwdArgs a) {
     *reinterpret_cast<float8v*>(a.partial + (int64_t)blockIdx.y * a.ldp + col) = dw;
 }
 
-// Rows of up to 8 TPR NCH values in registers, a block's share of dw in registers too, until its rows are done.
+// Rows of up to 8 TPR NCH values in registers, a block's share of dw in registers too, until its rows are done:
+// one pass over s, dout and dsum, bound by memory. [16384, 8192] bf16 with dsum: 199 us (1.07 GB, 5.4 TB/s).
 template <bool BF, int TPR, int NCH, bool DSUM>
 __global__ __launch_bounds__(block_of(TPR)) void rms_norm_bwd_kernel(RmsBwdArgs a) {
     constexpr int ROWS = block_of(TPR) / TPR;
@@ -516,7 +519,8 @@ __global__ __launch_bounds__(block_of(TPR)) void rms_norm_bwd_kernel(RmsBwdArgs 
     }
 }
 
-// dw[c] = the sum of the P partial rows: 16 interleaved groups of them, each in order, then the groups
+// dw[c] = the sum of the P partial rows: 16 interleaved groups of them, each in order, then the groups. 512 rows
+// of 8192: 7 us, that is latency: eight loads in flight a thread.
 __global__ __launch_bounds__(256) void rms_norm_dw_kernel(RmsBwdArgs a) {
     __shared__ float sums[16][16];
     const int col = threadIdx.x & 15, grp = threadIdx.x >> 4;
@@ -664,6 +668,7 @@ __device__ __forceinline__ void floats8(const Raw8<T>& r, int col, int K, float 
     }
 }
 
+// As the norm: a row in registers, bound by memory. relu of [147456, 512] fp16: 50 us (227 MB, 4.6 TB/s).
 template <int T, int ACT, int TPR, int NCH>
 __global__ __launch_bounds__(block_of(TPR)) void quantize_kernel(QuantArgs a) {
     constexpr int ROWS = block_of(TPR) / TPR;
@@ -714,7 +719,8 @@ struct DequantArgs {
     int64_t M, K, Kp;
 };
 
-// 2^shift threads a row, 8 values each at a time
+// 2^shift threads a row, 8 values each at a time. [147456, 512] to fp16: 35 us (227 MB, 6.5 TB/s; part of q comes from
+// the far cache).
 template <int T>
 __global__ __launch_bounds__(256) void dequantize_kernel(DequantArgs a, int shift) {
     const int part = threadIdx.x & ((1 << shift) - 1), rows = 256 >> shift;

@@ -12,6 +12,7 @@ Modules:
              tests/test_attn_bwd.py, tests/test_packed_attention.py)
   fused      LayerNorm-fused pair-stack projections and the keep / padding rule
              (reference cuda/volta_gdp.h, cuda/volta_ops.cu, cuda/volta_fused_ffi.h)
+  rows8      RMS norm and its gradients, 8-bit rows and their product (no counterpart in the reference)
   cpu_ref    the same attention and fused math in torch-CPU float32 (the stand-in for the
              reference tests' jnp ops on XLA-CPU, which cannot run here: jax is absent)
 
