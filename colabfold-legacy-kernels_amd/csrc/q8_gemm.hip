@@ -74,6 +74,22 @@ struct Channels {
         }
     }
 };
+// a and b: two pieces of row lane % 16. Then a is a piece of row lane % 8, b one of row lane % 8 + 8: the first of the
+// pieces in lanes with lane % 16 < 8, the second in the others, so that a store of each fills eight rows' lines. (Writing
+// 151 MB by nontemporal stores of half lines takes 41 us, of whole lines 26.)
+__device__ __forceinline__ void rows_of_eight(half8& a, half8& b) {
+    constexpr int kTurn8 = 0x128;  // each 16 lanes rotated by 8
+    const uint4v x = __builtin_bit_cast(uint4v, a), y = __builtin_bit_cast(uint4v, b);
+    uint4v u, v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        u[i] = (uint32_t)__builtin_amdgcn_update_dpp((int)x[i], (int)y[i], kTurn8, 0xf, 0xc, false);
+        v[i] = (uint32_t)__builtin_amdgcn_update_dpp((int)y[i], (int)x[i], kTurn8, 0xf, 0x3, false);
+    }
+    a = __builtin_bit_cast(half8, u);
+    b = __builtin_bit_cast(half8, v);
+}
+
 template <int W>
 struct Vec16;
 template <>
@@ -86,42 +102,72 @@ struct Vec16<8> {
     typedef half8 type;
     typedef half8u unaligned;
 };
-// (NT: nontemporal stores, for the large tiles' results: 8192 x 8192 x 8192 with a residual takes 424 us with and
-// 445 us without them, 8192 x 1024 x 8192 94 and 111 us.)
-template <bool BF, int RL, bool NT>
-__device__ __forceinline__ void store_run(const GemmArgs& a, int m, int n, const Channels<RL>& ch, const int (&sum)[RL]) {
+__device__ __forceinline__ int64_t at_of(const GemmArgs& a, int m, int n) { return (int64_t)m * a.N + n; }
+// The results of row m, all of whose RL channels exist: with the residual, rounded
+template <bool BF, int RL>
+__device__ __forceinline__ void finish_run(const GemmArgs& a, int m, int n, const Channels<RL>& ch, const int (&sum)[RL],
+                                           typename Vec16<(RL < 8 ? RL : 8)>::type (&o)[RL < 8 ? 1 : RL / 8]) {
     constexpr int W = RL < 8 ? RL : 8;  // channels an access
-    if (m >= a.M || n >= a.N) return;
     const float sx = a.qs[m];
-    const int64_t at = (int64_t)m * a.N + n;
+    const int64_t at = at_of(a, m, n);
     float v[RL];
 #pragma unroll
     for (int i = 0; i < RL; ++i) v[i] = scaled(sum[i], sx, ch.sw[i], ch.b[i]);
-    if (n + RL <= a.N) {
-        if (a.residual != nullptr) {
-            typename Vec16<W>::type r[RL / W];
+    if (a.residual != nullptr) {
+        typename Vec16<W>::type r[RL / W];
 #pragma unroll
-            for (int h = 0; h < RL / W; ++h) r[h] = *reinterpret_cast<const typename Vec16<W>::unaligned*>(a.residual + at + W * h);
+        for (int h = 0; h < RL / W; ++h) r[h] = *reinterpret_cast<const typename Vec16<W>::unaligned*>(a.residual + at + W * h);
 #pragma unroll
-            for (int i = 0; i < RL; ++i) v[i] += act_get<BF>(half8{r[i / W][i % W]}, 0);
+        for (int i = 0; i < RL; ++i) v[i] += act_get<BF>(half8{r[i / W][i % W]}, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < RL; ++i) o[i / W][i % W] = act_cvt<BF>(v[i]);
+}
+// the channels n .. below N of row m, one by one
+template <bool BF, int RL>
+__device__ __forceinline__ void store_few(const GemmArgs& a, int m, int n, const Channels<RL>& ch, const int (&sum)[RL]) {
+    const float sx = a.qs[m];
+    const int64_t at = at_of(a, m, n);
+#pragma unroll
+    for (int i = 0; i < RL; ++i) {
+        if (n + i < a.N) {
+            float v = scaled(sum[i], sx, ch.sw[i], ch.b[i]);
+            if (a.residual != nullptr) v += act_get<BF>(half8{a.residual[at + i]}, 0);
+            a.out[at + i] = act_cvt<BF>(v);
         }
+    }
+}
+template <bool BF, int RL>
+__device__ __forceinline__ void store_run(const GemmArgs& a, int m, int n, const Channels<RL>& ch, const int (&sum)[RL]) {
+    constexpr int W = RL < 8 ? RL : 8;
+    if (m >= a.M || n >= a.N) return;
+    if (n + RL > a.N) {
+        store_few<BF>(a, m, n, ch, sum);
+        return;
+    }
+    typename Vec16<W>::type o[RL / W];
+    finish_run<BF>(a, m, n, ch, sum, o);
 #pragma unroll
-        for (int h = 0; h < RL / W; ++h) {
-            typename Vec16<W>::type o;
+    for (int h = 0; h < RL / W; ++h) *reinterpret_cast<typename Vec16<W>::unaligned*>(a.out + at_of(a, m, n) + W * h) = o[h];
+}
+// The same for a wave's 16 rows m0 + r16 and 64 channels n64 .. (16 g .. a lane), with nontemporal stores of whole
+// lines: 20000 x 1024 x 1024 with a residual takes 37 us, 38 by nontemporal half lines and 51 by whole lines
+// through the caches; 4096 x 4096 x 4096 54, 56, 56. (Residuals loaded by whole lines and turned back in
+// registers gained nothing.)
+template <bool BF>
+__device__ __forceinline__ void store_lines(const GemmArgs& a, int m0, int n64, int r16, int g, const Channels<16>& ch,
+                                            const int (&sum)[16]) {
+    if (n64 + 64 > a.N) {  // the same for all lanes
+        store_run<BF>(a, m0 + r16, n64 + 16 * g, ch, sum);
+        return;
+    }
+    half8 o[2];
+    finish_run<BF>(a, min(m0 + r16, a.M - 1), n64 + 16 * g, ch, sum, o);
+    rows_of_eight(o[0], o[1]);
 #pragma unroll
-            for (int i = 0; i < W; ++i) o[i] = act_cvt<BF>(v[W * h + i]);
-            typename Vec16<W>::unaligned* to = reinterpret_cast<typename Vec16<W>::unaligned*>(a.out + at + W * h);
-            if constexpr (NT) __builtin_nontemporal_store(o, to);
-            else *to = o;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < RL; ++i) {
-            if (n + i < a.N) {
-                if (a.residual != nullptr) v[i] += act_get<BF>(half8{a.residual[at + i]}, 0);
-                a.out[at + i] = act_cvt<BF>(v[i]);
-            }
-        }
+    for (int p = 0; p < 2; ++p) {
+        const int m = m0 + 8 * p + (r16 & 7);
+        if (m < a.M) __builtin_nontemporal_store(o[p], reinterpret_cast<half8u*>(a.out + at_of(a, m, n64 + 16 * g + 8 * (r16 >> 3))));
     }
 }
 
@@ -165,7 +211,7 @@ __global__ __launch_bounds__(256) void q8_rows_kernel(GemmArgs a) {
 #pragma unroll
     for (int v = 1; v < KW; ++v) acc += part[v][lane];
     const int n = 64 * (o / 4) + 16 * g + 4 * (o % 4);
-    store_run<BF, 4, false>(a, r16, n, Channels<4>(a, n), {acc[0], acc[1], acc[2], acc[3]});
+    store_run<BF, 4>(a, r16, n, Channels<4>(a, n), {acc[0], acc[1], acc[2], acc[3]});
 }
 
 // A workgroup computes 16 MF WM rows by 16 NU WN channels. Its waves are KS groups of WM x WN; wave (wm, wn) of a
@@ -296,7 +342,9 @@ __global__ __launch_bounds__(64 * WM * WN * KS) void q8_tile_kernel(GemmArgs a) 
                 int sum[4 * NE];
 #pragma unroll
                 for (int i = 0; i < 4 * NE; ++i) sum[i] = acc[u + i / 4][mf][i % 4];
-                store_run<BF, 4 * NE, true>(a, m0 + 16 * (MF * wm + mf) + r16, n, ch, sum);
+                const int row0 = m0 + 16 * (MF * wm + mf);
+                if constexpr (NE == 4) store_lines<BF>(a, row0, 16 * o, r16, g, ch, sum);
+                else store_run<BF>(a, row0 + r16, n, ch, sum);
             }
         }
     } else {
@@ -322,7 +370,7 @@ __global__ __launch_bounds__(64 * WM * WN * KS) void q8_tile_kernel(GemmArgs a) 
                 for (int i = 0; i < 4; ++i) sum[4 * e + i] = s[i];
             }
             const int o = o0 + NU * wn + u, n = 64 * (o / 4) + 16 * g + 4 * (o % 4);
-            store_run<BF, 4 * NE, false>(a, m0 + 16 * (MF * wm + mf) + r16, n, Channels<4 * NE>(a, n), sum);
+            store_run<BF>(a, m0 + 16 * (MF * wm + mf) + r16, n, Channels<4 * NE>(a, n), sum);
         }
     }
 }
@@ -351,9 +399,9 @@ __device__ __forceinline__ void dma_lds_untracked(uint4v rsrc, void* dst, uint32
 // ahead; scales and biases wait in LDS, the next tile's row scales and residual in registers. Results go
 // out as 16-byte buffer stores, whose range drops what lies past M and N, so that every tile issues the
 // same number of memory accesses and a tile's wait can count them. A weight operand's rows are picked so that
-// a store's four lanes of a row write 64 consecutive bytes. Without a residual the stores are nontemporal:
-// 65536 x 256 x 1024 takes 36 us with and 55 us without that; with a residual, read through the same caches,
-// it is as often slower (147456 x 128 x 512: 68.5 and 62.7 us).
+// four lanes hold 64 consecutive bytes of a row, which is how the residual is read; stores turn them into whole
+// lines and are nontemporal. 147456 x 128 x 512 takes 28.4 us (170 MB, 6.0 TB/s), 40 by nontemporal half lines,
+// 45 by whole lines through the caches; with a residual 57 us (321 MB, 5.6 TB/s), 62, 59.
 template <bool BF, int KB, int NU, int MF, int WN, bool RES>
 __global__ __launch_bounds__(256) void q8_stream_kernel(GemmArgs a) {
     constexpr int BR = 16 * MF, WM = 4 / WN, XT = MF * WM * KB, XL = (XT + 3) / 4, RING = 3, SLOT = 4096 * XL;
@@ -438,21 +486,32 @@ __global__ __launch_bounds__(256) void q8_stream_kernel(GemmArgs a) {
                 for (int mf = 0; mf < MF; ++mf) acc[u][mf] = mfma_i8(w[kb][u], x[mf], kb == 0 ? int4v{0, 0, 0, 0} : acc[u][mf]);
         }
 #pragma unroll
-        for (int h = 0; h < H; ++h) {
-            const int c = CW * wn + 64 * (h / 2) + 32 * (h % 2) + 8 * g;
-            const float8v sw = *reinterpret_cast<const float8v*>(params + c), bv = *reinterpret_cast<const float8v*>(params + CW * WN + c);
-            const int n = c0 + c;
+        for (int h = 0; h < H; h += 2) {
+            float8v sw[2], bv[2];
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const int c = CW * wn + 32 * (h + p) + 8 * g;
+                sw[p] = *reinterpret_cast<const float8v*>(params + c);
+                bv[p] = *reinterpret_cast<const float8v*>(params + CW * WN + c);
+            }
+            const int n = n0 + 32 * (h + (r16 >> 3)) + 8 * g;
 #pragma unroll
             for (int mf = 0; mf < MF; ++mf) {
-                half8 o;
+                half8 o[2];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    float v = scaled(acc[2 * h + i / 4][mf][i % 4], now.qs[mf], sw[i], bv[i]);
-                    if constexpr (RES) v += act_get<BF>(now.res[mf][h], i);
-                    o[i] = act_cvt<BF>(v);
+                for (int p = 0; p < 2; ++p)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        float v = scaled(acc[2 * (h + p) + i / 4][mf][i % 4], now.qs[mf], sw[p][i], bv[p][i]);
+                        if constexpr (RES) v += act_get<BF>(now.res[mf][h + p], i);
+                        o[p][i] = act_cvt<BF>(v);
+                    }
+                rows_of_eight(o[0], o[1]);
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uint4v, o[p]), ro,
+                                                           n < a.N ? ((uint32_t)(16 * mf + 8 * p + (r16 & 7)) * (uint32_t)a.N + (uint32_t)n) * 2u : kDrop, 0, 2);
                 }
-                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uint4v, o), ro,
-                                                       n < a.N ? ((uint32_t)(16 * mf + r16) * (uint32_t)a.N + (uint32_t)n) * 2u : kDrop, 0, RES ? 0 : 2);
             }
         }
     };
@@ -511,8 +570,8 @@ int best_tile(int64_t M, int64_t N, int64_t Kp) {
 }
 
 // Whether the kernel for many rows and short k takes a call. From 2048 rows on it was the faster one for all of
-// 27 shapes with k of 64 to 512 (147456 x 128 x 512: 41.9 against 74.8 us, 65536 x 512 x 2048: 82 against
-// 141, 4096 x 64 x 64: 3.6 against 4.2); at 1024 rows and below it loses as often as it wins. 16-byte stores need
+// 27 shapes with k of 64 to 512 (147456 x 128 x 512: 28.4 against 50.2 us, 65536 x 512 x 2048: 84 against
+// 110, 4096 x 64 x 64: 3.6 against 4.2); at 1024 rows and below it loses as often as it wins. 16-byte stores need
 // aligned rows of results.
 bool streams(const GemmArgs& a) {
     return a.M >= 2048 && a.M <= 1 << 30 && a.Kp <= 512 && a.N % 8 == 0 && a.N <= 1 << 20 && aligned16(a.out) &&
@@ -565,8 +624,8 @@ void launch(hipStream_t s, GemmArgs& a) {
     if (streams(a)) {
         // Operands a wave and workgroups, measured at 147456 and 65536 rows: with few channels, or none but
         // the results to move, small waves and more of them; with a residual at many channels, large ones
-        // (147456 x 128 x 512 with a residual: 63 us with 8 channel operands a wave and 512 workgroups, 69 to 71
-        // us with 4; without one 39 us with 4, 45 with 8).
+        // (147456 x 128 x 512 with a residual: 57 us with 8 channel operands a wave and 512 workgroups, 61 to 63
+        // us with 4; without one 28.4 us with 4, 31.4 with 8).
         const int kbs = a.Kp / 64;
         const bool res = a.residual != nullptr;
         if (kbs == 1) {
