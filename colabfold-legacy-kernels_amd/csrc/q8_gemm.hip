@@ -400,8 +400,10 @@ __device__ __forceinline__ void dma_lds_untracked(uint4v rsrc, void* dst, uint32
 // out as 16-byte buffer stores, whose range drops what lies past M and N, so that every tile issues the
 // same number of memory accesses and a tile's wait can count them. A weight operand's rows are picked so that
 // four lanes hold 64 consecutive bytes of a row, which is how the residual is read; stores turn them into whole
-// lines and are nontemporal. 147456 x 128 x 512 takes 28.4 us (170 MB, 6.0 TB/s), 40 by nontemporal half lines,
-// 45 by whole lines through the caches; with a residual 57 us (321 MB, 5.6 TB/s), 62, 59.
+// lines. Without a residual they are nontemporal: 147456 x 128 x 512 takes 28.4 us (170 MB, 6.0 TB/s), 40 by
+// nontemporal half lines, 45 by whole lines through the caches. With a residual, read through the same caches, they
+// go through them too: 59 us (321 MB, 5.4 TB/s; 57 by nontemporal ones), but 65536 rows and a norm of
+// the results take 46 us, 55 by nontemporal ones.
 template <bool BF, int KB, int NU, int MF, int WN, bool RES>
 __global__ __launch_bounds__(256) void q8_stream_kernel(GemmArgs a) {
     constexpr int BR = 16 * MF, WM = 4 / WN, XT = MF * WM * KB, XL = (XT + 3) / 4, RING = 3, SLOT = 4096 * XL;
@@ -510,7 +512,7 @@ __global__ __launch_bounds__(256) void q8_stream_kernel(GemmArgs a) {
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {
                     __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uint4v, o[p]), ro,
-                                                           n < a.N ? ((uint32_t)(16 * mf + 8 * p + (r16 & 7)) * (uint32_t)a.N + (uint32_t)n) * 2u : kDrop, 0, 2);
+                                                           n < a.N ? ((uint32_t)(16 * mf + 8 * p + (r16 & 7)) * (uint32_t)a.N + (uint32_t)n) * 2u : kDrop, 0, RES ? 0 : 2);
                 }
             }
         }

@@ -22,6 +22,7 @@ namespace {
 typedef half8 half8u __attribute__((aligned(2)));
 typedef half_t half_u __attribute__((aligned(2)));
 typedef float8v float8u __attribute__((aligned(4)));
+typedef float4v float4u __attribute__((aligned(4)));
 typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
 
 // Rows whose scale a / 127 would leave fp32's normal range count as zeros (then 127 / a is finite too).
@@ -171,9 +172,11 @@ __device__ __forceinline__ half8 cut8(half8 v, int col, int C) {
     }
     return v;
 }
+template <bool NT = false>
 __device__ __forceinline__ void store8(half_t* row, int col, int C, half8 v) {
     if (col + 8 <= C) {
-        *reinterpret_cast<half8u*>(row + col) = v;
+        if constexpr (NT) __builtin_nontemporal_store(v, reinterpret_cast<half8u*>(row + col));
+        else *reinterpret_cast<half8u*>(row + col) = v;
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -188,13 +191,15 @@ __device__ __forceinline__ float8v load8f(const float* row, int col, int C) {
         if (col + e < C) v[e] = row[col + e];
     return v;
 }
-__device__ __forceinline__ void store8f(float* row, int col, int C, float8v v) {
-    if (col + 8 <= C) {
-        *reinterpret_cast<float8u*>(row + col) = v;
+template <bool NT>
+__device__ __forceinline__ void store4f(float* to, int n, float4v v) {
+    if (n >= 4) {
+        if constexpr (NT) __builtin_nontemporal_store(v, reinterpret_cast<float4u*>(to));
+        else *reinterpret_cast<float4u*>(to) = v;
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (col + e < C) row[col + e] = v[e];
+        for (int e = 0; e < 4; ++e)
+            if (e < n) to[e] = v[e];
     }
 }
 __device__ __forceinline__ uint2v quant8(const float (&t)[8], float inv) {
@@ -719,26 +724,33 @@ struct DequantArgs {
     int64_t M, K, Kp;
 };
 
-// 2^shift threads a row, 8 values each at a time. [147456, 512] to fp16: 35 us (227 MB, 6.5 TB/s; part of q comes from
-// the far cache).
+// 2^shift threads a row, 16 bytes of results each at a time, so that a wave's store is a kilobyte in one piece ([16384,
+// 8192] to fp32: 121 us, 172 with 32 bytes a thread). Results past half of the 256 MB far cache (NT) go by it:
+// whoever reads them next finds little of them there, and the other arrays stay in it. [40000, 2048] quantised,
+// dequantised to fp16 and added to another array takes 168 us, 179 without; 12000 rows 58, 57 without. [147456,
+// 512] to fp16: 29 us (227 MB, part of it from the far cache).
 template <int T>
+constexpr int kDequant = T == kF32 ? 4 : 8;
+template <int T, bool NT>
 __global__ __launch_bounds__(256) void dequantize_kernel(DequantArgs a, int shift) {
+    constexpr int E = kDequant<T>;
+    typedef uint32_t words __attribute__((ext_vector_type(E / 4)));
     const int part = threadIdx.x & ((1 << shift) - 1), rows = 256 >> shift;
     for (int64_t row = (int64_t)blockIdx.x * rows + (threadIdx.x >> shift); row < a.M; row += (int64_t)gridDim.x * rows) {
         const float sc = a.scale[row];
-        for (int64_t c = 8 * part; c < a.K; c += 8 << shift) {
-            const uint2v q = *reinterpret_cast<const uint2v*>(a.q + row * a.Kp + c);
-            float v[8];
+        for (int64_t c = E * part; c < a.K; c += E << shift) {
+            const words q = *reinterpret_cast<const words*>(a.q + row * a.Kp + c);
+            float v[E];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)(q[e >> 2] >> 8 * (e & 3)) * sc;
-            const int left = (int)min<int64_t>(a.K - c, 8);
+            for (int e = 0; e < E; ++e) v[e] = (float)(int8_t)(q[e >> 2] >> 8 * (e & 3)) * sc;
+            const int left = (int)min<int64_t>(a.K - c, E);
             if constexpr (T == kF32) {
-                store8f(static_cast<float*>(a.out) + row * a.K + c, 0, left, float8v{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]});
+                store4f<NT>(static_cast<float*>(a.out) + row * a.K + c, left, float4v{v[0], v[1], v[2], v[3]});
             } else {
                 half8 h;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) h[e] = act_cvt<T == kBf16>(v[e]);
-                store8(static_cast<half_t*>(a.out) + row * a.K + c, 0, left, h);
+                for (int e = 0; e < E; ++e) h[e] = act_cvt<T == kBf16>(v[e]);
+                store8<NT>(static_cast<half_t*>(a.out) + row * a.K + c, 0, left, h);
             }
         }
     }
@@ -956,11 +968,16 @@ extern "C" int clk_dequantize_rows(clk_stream stream, const clk_buffer* q, const
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     stage_mark(s, 0);
     int shift = 3;
-    while (shift < 8 && (8 << shift) < K) ++shift;
+    while (shift < 8 && ((ot == CLK_F32 ? kDequant<kF32> : kDequant<kF16>) << shift) < K) ++shift;
     const dim3 grid(row_blocks(M, 1 << shift)), block(256);
-    if (ot == CLK_F32) hipLaunchKernelGGL(dequantize_kernel<kF32>, grid, block, 0, s, a, shift);
-    else if (ot == CLK_BF16) hipLaunchKernelGGL(dequantize_kernel<kBf16>, grid, block, 0, s, a, shift);
-    else hipLaunchKernelGGL(dequantize_kernel<kF16>, grid, block, 0, s, a, shift);
+    const auto launch = [&](auto t_) {
+        constexpr int T = decltype(t_)::value;
+        if (M * K >= (int64_t)(1 << 27) / (T == kF32 ? 4 : 2)) hipLaunchKernelGGL((dequantize_kernel<T, true>), grid, block, 0, s, a, shift);
+        else hipLaunchKernelGGL((dequantize_kernel<T, false>), grid, block, 0, s, a, shift);
+    };
+    if (ot == CLK_F32) launch(std::integral_constant<int, kF32>());
+    else if (ot == CLK_BF16) launch(std::integral_constant<int, kBf16>());
+    else launch(std::integral_constant<int, kF16>());
     stage_mark(s, 1);
     return launch_status("dequantize_rows");
 }
