@@ -103,71 +103,59 @@ struct Vec16<8> {
     typedef half8u unaligned;
 };
 __device__ __forceinline__ int64_t at_of(const GemmArgs& a, int m, int n) { return (int64_t)m * a.N + n; }
-// The results of row m, all of whose RL channels exist: with the residual, rounded
 template <bool BF, int RL>
-__device__ __forceinline__ void finish_run(const GemmArgs& a, int m, int n, const Channels<RL>& ch, const int (&sum)[RL],
-                                           typename Vec16<(RL < 8 ? RL : 8)>::type (&o)[RL < 8 ? 1 : RL / 8]) {
+__device__ __forceinline__ void store_run(const GemmArgs& a, int m, int n, const Channels<RL>& ch, const int (&sum)[RL]) {
     constexpr int W = RL < 8 ? RL : 8;  // channels an access
+    if (m >= a.M || n >= a.N) return;
     const float sx = a.qs[m];
     const int64_t at = at_of(a, m, n);
     float v[RL];
 #pragma unroll
     for (int i = 0; i < RL; ++i) v[i] = scaled(sum[i], sx, ch.sw[i], ch.b[i]);
-    if (a.residual != nullptr) {
-        typename Vec16<W>::type r[RL / W];
+    if (n + RL <= a.N) {
+        if (a.residual != nullptr) {
+            typename Vec16<W>::type r[RL / W];
 #pragma unroll
-        for (int h = 0; h < RL / W; ++h) r[h] = *reinterpret_cast<const typename Vec16<W>::unaligned*>(a.residual + at + W * h);
+            for (int h = 0; h < RL / W; ++h) r[h] = *reinterpret_cast<const typename Vec16<W>::unaligned*>(a.residual + at + W * h);
 #pragma unroll
-        for (int i = 0; i < RL; ++i) v[i] += act_get<BF>(half8{r[i / W][i % W]}, 0);
-    }
+            for (int i = 0; i < RL; ++i) v[i] += act_get<BF>(half8{r[i / W][i % W]}, 0);
+        }
 #pragma unroll
-    for (int i = 0; i < RL; ++i) o[i / W][i % W] = act_cvt<BF>(v[i]);
-}
-// the channels n .. below N of row m, one by one
-template <bool BF, int RL>
-__device__ __forceinline__ void store_few(const GemmArgs& a, int m, int n, const Channels<RL>& ch, const int (&sum)[RL]) {
-    const float sx = a.qs[m];
-    const int64_t at = at_of(a, m, n);
+        for (int h = 0; h < RL / W; ++h) {
+            typename Vec16<W>::type o;
 #pragma unroll
-    for (int i = 0; i < RL; ++i) {
-        if (n + i < a.N) {
-            float v = scaled(sum[i], sx, ch.sw[i], ch.b[i]);
-            if (a.residual != nullptr) v += act_get<BF>(half8{a.residual[at + i]}, 0);
-            a.out[at + i] = act_cvt<BF>(v);
+            for (int i = 0; i < W; ++i) o[i] = act_cvt<BF>(v[W * h + i]);
+            *reinterpret_cast<typename Vec16<W>::unaligned*>(a.out + at + W * h) = o;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < RL; ++i) {
+            if (n + i < a.N) {
+                if (a.residual != nullptr) v[i] += act_get<BF>(half8{a.residual[at + i]}, 0);
+                a.out[at + i] = act_cvt<BF>(v[i]);
+            }
         }
     }
 }
-template <bool BF, int RL>
-__device__ __forceinline__ void store_run(const GemmArgs& a, int m, int n, const Channels<RL>& ch, const int (&sum)[RL]) {
-    constexpr int W = RL < 8 ? RL : 8;
-    if (m >= a.M || n >= a.N) return;
-    if (n + RL > a.N) {
-        store_few<BF>(a, m, n, ch, sum);
-        return;
-    }
-    typename Vec16<W>::type o[RL / W];
-    finish_run<BF>(a, m, n, ch, sum, o);
-#pragma unroll
-    for (int h = 0; h < RL / W; ++h) *reinterpret_cast<typename Vec16<W>::unaligned*>(a.out + at_of(a, m, n) + W * h) = o[h];
-}
-// The same for a wave's 16 rows m0 + r16 and 64 channels n64 .. (16 g .. a lane), with nontemporal stores of whole
-// lines: 20000 x 1024 x 1024 with a residual takes 37 us, 38 by nontemporal half lines and 51 by whole lines
-// through the caches; 4096 x 4096 x 4096 54, 56, 56. (Residuals loaded by whole lines and turned back in
-// registers gained nothing.)
-template <bool BF>
-__device__ __forceinline__ void store_lines(const GemmArgs& a, int m0, int n64, int r16, int g, const Channels<16>& ch,
-                                            const int (&sum)[16]) {
-    if (n64 + 64 > a.N) {  // the same for all lanes
-        store_run<BF>(a, m0 + r16, n64 + 16 * g, ch, sum);
-        return;
-    }
+// The same for a wave's rows m0 .. m0 + 15 and 64 channels that all exist (16 a lane), with their residual (ADD), by
+// nontemporal stores of whole lines: 20000 x 1024 x 1024 with a residual takes 37 us, 38 by nontemporal half
+// lines and 51 by whole lines through the caches; 4096 x 4096 x 4096 54, 56, 56.
+template <bool BF, bool ADD>
+__device__ __forceinline__ void store_lines(const GemmArgs& a, int m0, int n, int r16, const Channels<16>& ch, const int (&sum)[16],
+                                            const half8 (&res)[2]) {
+    const float sx = a.qs[min(m0 + r16, a.M - 1)];
     half8 o[2];
-    finish_run<BF>(a, min(m0 + r16, a.M - 1), n64 + 16 * g, ch, sum, o);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        float v = scaled(sum[i], sx, ch.sw[i], ch.b[i]);
+        if constexpr (ADD) v += act_get<BF>(res[i / 8], i % 8);
+        o[i / 8][i % 8] = act_cvt<BF>(v);
+    }
     rows_of_eight(o[0], o[1]);
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
         const int m = m0 + 8 * p + (r16 & 7);
-        if (m < a.M) __builtin_nontemporal_store(o[p], reinterpret_cast<half8u*>(a.out + at_of(a, m, n64 + 16 * g + 8 * (r16 >> 3))));
+        if (m < a.M) __builtin_nontemporal_store(o[p], reinterpret_cast<half8u*>(a.out + at_of(a, m, n + 8 * (r16 >> 3))));
     }
 }
 
@@ -337,14 +325,47 @@ __global__ __launch_bounds__(64 * WM * WN * KS) void q8_tile_kernel(GemmArgs a) 
         for (int u = 0; u < NU; u += NE) {
             const int o = o0 + NU * wn + u, n = 64 * (o / 4) + 16 * g + 4 * (o % 4);
             const Channels<4 * NE> ch(a, n);
+            const auto sums = [&](int mf, int (&sum)[4 * NE]) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < 4 * NE; ++i) sum[i] = acc[u + i / 4][mf][i % 4];
+            };
+            const int row0 = m0 + 16 * MF * wm;
+            if constexpr (NE == 4) {
+                if (16 * o + 64 <= a.N) {  // the same for all lanes
+                    // residuals three groups of rows ahead: 8192 x 8192 x 8192 takes 426 us with and 445 without that,
+                    // 8192 x 1024 x 8192 107 and 127 (two ahead 427 and 111; by whole lines, turned back in
+                    // registers, the same)
+                    constexpr int AHEAD = MF < 3 ? MF : 3;
+                    const auto rows = [&](auto add_) __attribute__((always_inline)) {
+                        constexpr bool ADD = decltype(add_)::value;
+                        half8 res[AHEAD + 1][2];
+                        const auto read = [&](int mf) __attribute__((always_inline)) {
+                            if constexpr (ADD)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h)
+                                    res[mf % (AHEAD + 1)][h] = *reinterpret_cast<const half8u*>(a.residual + at_of(a, min(row0 + 16 * mf + r16, a.M - 1), n) + 8 * h);
+                        };
+#pragma unroll
+                        for (int mf = 0; mf < AHEAD; ++mf) read(mf);
+#pragma unroll
+                        for (int mf = 0; mf < MF; ++mf) {
+                            if (mf + AHEAD < MF) read(mf + AHEAD);
+                            __builtin_amdgcn_sched_barrier(0);
+                            int sum[16];
+                            sums(mf, sum);
+                            store_lines<BF, ADD>(a, row0 + 16 * mf, n, r16, ch, sum, res[mf % (AHEAD + 1)]);
+                        }
+                    };
+                    if (a.residual != nullptr) rows(std::true_type());
+                    else rows(std::false_type());
+                    continue;
+                }
+            }
 #pragma unroll
             for (int mf = 0; mf < MF; ++mf) {
                 int sum[4 * NE];
-#pragma unroll
-                for (int i = 0; i < 4 * NE; ++i) sum[i] = acc[u + i / 4][mf][i % 4];
-                const int row0 = m0 + 16 * (MF * wm + mf);
-                if constexpr (NE == 4) store_lines<BF>(a, row0, 16 * o, r16, g, ch, sum);
-                else store_run<BF>(a, row0 + r16, n, ch, sum);
+                sums(mf, sum);
+                store_run<BF>(a, row0 + 16 * mf + r16, n, ch, sum);
             }
         }
     } else {
