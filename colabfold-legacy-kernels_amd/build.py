@@ -30,6 +30,11 @@ HIP_FLAGS = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=" + ARCH,
              "-mllvm", "-amdgpu-mfma-vgpr-form",
              "-Wall", "-Wno-unused-result", "-Wno-unused-function"]
 
+# The 8-bit path's results do not depend on the kernel that a call's size picks. Without this the compiler rounds some
+# products and fmas to fp16 at once (v_fma_mixlo_f16) and others to fp32 first, lane by lane as it likes.
+ONE_ROUNDING = ["-Xclang", "-target-feature", "-Xclang", "-fma-mix-insts"]
+SOURCE_FLAGS = {"q8_gemm.hip": ONE_ROUNDING, "rows8.hip": ONE_ROUNDING}
+
 
 def hipcc():
     for cand in (os.environ.get("HIPCC"), "/opt/rocm/bin/hipcc", shutil.which("hipcc")):
@@ -45,12 +50,13 @@ def sources():
 def compile_one(cc, src, verbose):
     obj = os.path.join(BUILD_DIR, os.path.basename(src) + ".o")
     # every source is compiled as HIP: the .cc files hold host code only, but share the headers
-    cmd = [cc, "-x", "hip"] + HIP_FLAGS + ["-I", INCLUDE, "-I", CSRC, "-c", src, "-o", obj]
+    cmd = [cc, "-x", "hip"] + HIP_FLAGS + SOURCE_FLAGS.get(os.path.basename(src), []) + \
+        ["-I", INCLUDE, "-I", CSRC, "-c", src, "-o", obj]
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)
     out = (r.stdout + r.stderr).strip()
-    # hipcc's host pass does not know the packed-fp32-ops feature; that warning is expected
+    # hipcc's host pass does not know these target features; that warning is expected
     lines = [l for l in out.splitlines() if "packed-fp32-ops" not in l and "not a recognized feature" not in l]
     if r.returncode != 0:
         raise RuntimeError("compile failed: %s\n%s" % (src, "\n".join(lines)))

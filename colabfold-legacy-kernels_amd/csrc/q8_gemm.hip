@@ -47,6 +47,7 @@ struct GemmArgs {
     half_t* out;
     int M, N, Kp;
     int mtiles, ntiles;
+    bool lines;  // each 64 channels of a row are a whole line of out
 };
 
 template <typename P>
@@ -138,9 +139,10 @@ __device__ __forceinline__ void store_run(const GemmArgs& a, int m, int n, const
     }
 }
 // The same for a wave's rows m0 .. m0 + 15 and 64 channels that all exist (16 a lane), with their residual (ADD), by
-// nontemporal stores of whole lines: 20000 x 1024 x 1024 with a residual takes 37 us, 38 by nontemporal half
-// lines and 51 by whole lines through the caches; 4096 x 4096 x 4096 54, 56, 56.
-template <bool BF, bool ADD>
+// stores of whole lines, nontemporal where they are such in memory too (LINES): 20000 x 1024 x 1024 with a residual
+// takes 37 us, 38 by nontemporal half lines and 51 by whole lines through the caches; 4096 x 1024 x 4094 26 us
+// through the caches and 35 by nontemporal stores.
+template <bool BF, bool ADD, bool LINES>
 __device__ __forceinline__ void store_lines(const GemmArgs& a, int m0, int n, int r16, const Channels<16>& ch, const int (&sum)[16],
                                             const half8 (&res)[2]) {
     const float sx = a.qs[min(m0 + r16, a.M - 1)];
@@ -155,7 +157,10 @@ __device__ __forceinline__ void store_lines(const GemmArgs& a, int m0, int n, in
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
         const int m = m0 + 8 * p + (r16 & 7);
-        if (m < a.M) __builtin_nontemporal_store(o[p], reinterpret_cast<half8u*>(a.out + at_of(a, m, n + 8 * (r16 >> 3))));
+        if (m >= a.M) continue;
+        half8u* to = reinterpret_cast<half8u*>(a.out + at_of(a, m, n + 8 * (r16 >> 3)));
+        if constexpr (LINES) __builtin_nontemporal_store(o[p], to);
+        else *to = o[p];
     }
 }
 
@@ -336,8 +341,8 @@ __global__ __launch_bounds__(64 * WM * WN * KS) void q8_tile_kernel(GemmArgs a) 
                     // 8192 x 1024 x 8192 107 and 127 (two ahead 427 and 111; by whole lines, turned back in
                     // registers, the same)
                     constexpr int AHEAD = MF < 3 ? MF : 3;
-                    const auto rows = [&](auto add_) __attribute__((always_inline)) {
-                        constexpr bool ADD = decltype(add_)::value;
+                    const auto rows = [&](auto add_, auto lines_) __attribute__((always_inline)) {
+                        constexpr bool ADD = decltype(add_)::value, LINES = decltype(lines_)::value;
                         half8 res[AHEAD + 1][2];
                         const auto read = [&](int mf) __attribute__((always_inline)) {
                             if constexpr (ADD)
@@ -353,11 +358,11 @@ __global__ __launch_bounds__(64 * WM * WN * KS) void q8_tile_kernel(GemmArgs a) 
                             __builtin_amdgcn_sched_barrier(0);
                             int sum[16];
                             sums(mf, sum);
-                            store_lines<BF, ADD>(a, row0 + 16 * mf, n, r16, ch, sum, res[mf % (AHEAD + 1)]);
+                            store_lines<BF, ADD, LINES>(a, row0 + 16 * mf, n, r16, ch, sum, res[mf % (AHEAD + 1)]);
                         }
                     };
-                    if (a.residual != nullptr) rows(std::true_type());
-                    else rows(std::false_type());
+                    if (a.residual != nullptr) a.lines ? rows(std::true_type(), std::true_type()) : rows(std::true_type(), std::false_type());
+                    else a.lines ? rows(std::false_type(), std::true_type()) : rows(std::false_type(), std::false_type());
                     continue;
                 }
             }
@@ -421,11 +426,13 @@ __device__ __forceinline__ void dma_lds_untracked(uint4v rsrc, void* dst, uint32
 // out as 16-byte buffer stores, whose range drops what lies past M and N, so that every tile issues the
 // same number of memory accesses and a tile's wait can count them. A weight operand's rows are picked so that
 // four lanes hold 64 consecutive bytes of a row, which is how the residual is read; stores turn them into whole
-// lines. Without a residual they are nontemporal: 147456 x 128 x 512 takes 28.4 us (170 MB, 6.0 TB/s), 40 by
-// nontemporal half lines, 45 by whole lines through the caches. With a residual, read through the same caches, they
-// go through them too: 59 us (321 MB, 5.4 TB/s; 57 by nontemporal ones), but 65536 rows and a norm of
-// the results take 46 us, 55 by nontemporal ones.
-template <bool BF, int KB, int NU, int MF, int WN, bool RES>
+// lines. Where rows are whole lines and there is no residual they are nontemporal: 147456 x 128 x 512 takes 28.4 us
+// (170 MB, 6.0 TB/s), 40 by nontemporal half lines, 45 by whole lines through the caches; 147456 x 128 x 520,
+// whose stores end inside lines, 53 through the caches and 89 nontemporal. With a residual, read through the same
+// caches, they go through them too: 59 us (321 MB, 5.4 TB/s; 57 by nontemporal ones), but 65536 rows and a norm
+// of the results take 46 us, 55 by nontemporal ones. A row's last piece, cut at an even channel, goes out by its
+// words: 147456 x 128 x 510 52 us.
+template <bool BF, int KB, int NU, int MF, int WN, bool RES, bool NT>
 __global__ __launch_bounds__(256) void q8_stream_kernel(GemmArgs a) {
     constexpr int BR = 16 * MF, WM = 4 / WN, XT = MF * WM * KB, XL = (XT + 3) / 4, RING = 3, SLOT = 4096 * XL;
     constexpr int CW = 16 * NU, H = NU / 2;  // channels a wave; 16-byte pieces of a lane's results a row
@@ -437,6 +444,7 @@ __global__ __launch_bounds__(256) void q8_stream_kernel(GemmArgs a) {
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int r16 = lane & 15, g = lane >> 4, wm = wave / WN, wn = wave % WN;
     const int c0 = CW * WN * nt, n0 = c0 + CW * wn;  // the workgroup's and the wave's first channel
+    const bool tail = a.N % 8 != 0 && n0 < a.N && n0 + CW > a.N;  // one of its pieces is cut
     for (int i = threadIdx.x; i < CW * WN; i += 256) {
         params[i] = c0 + i < a.N ? a.ws[c0 + i] : 0.f;
         params[CW * WN + i] = a.b != nullptr && c0 + i < a.N ? a.b[c0 + i] : 0.f;
@@ -532,8 +540,15 @@ __global__ __launch_bounds__(256) void q8_stream_kernel(GemmArgs a) {
                 rows_of_eight(o[0], o[1]);
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {
-                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uint4v, o[p]), ro,
-                                                           n < a.N ? ((uint32_t)(16 * mf + 8 * p + (r16 & 7)) * (uint32_t)a.N + (uint32_t)n) * 2u : kDrop, 0, RES ? 0 : 2);
+                    const uint32_t to = ((uint32_t)(16 * mf + 8 * p + (r16 & 7)) * (uint32_t)a.N + (uint32_t)n) * 2u;
+                    const uint4v words = __builtin_bit_cast(uint4v, o[p]);
+                    __builtin_amdgcn_raw_buffer_store_b128(words, ro, n + 8 <= a.N ? to : kDrop, 0, NT ? 2 : 0);
+                    if (tail) {
+#pragma unroll
+                        for (int i = 0; i < 3; ++i) {
+                            __builtin_amdgcn_raw_buffer_store_b32(words[i], ro, n + 8 > a.N && n + 2 * i < a.N ? to + 4 * i : kDrop, 0, 0);
+                        }
+                    }
                 }
             }
         }
@@ -593,11 +608,11 @@ int best_tile(int64_t M, int64_t N, int64_t Kp) {
 }
 
 // Whether the kernel for many rows and short k takes a call. From 2048 rows on it was the faster one for all of
-// 27 shapes with k of 64 to 512 (147456 x 128 x 512: 28.4 against 50.2 us, 65536 x 512 x 2048: 84 against
-// 110, 4096 x 64 x 64: 3.6 against 4.2); at 1024 rows and below it loses as often as it wins. 16-byte stores need
-// aligned rows of results.
+// 27 shapes with k of 64 to 512 (147456 x 128 x 512: 28.4 against 50.2 us, 147456 x 128 x 510: 52 against 86, 65536 x 512 x 2048: 84
+// against 110, 4096 x 64 x 64: 3.6 against 4.2); at 1024 rows and below it loses as often as it wins. Buffer
+// accesses need rows of results at multiples of 4 bytes.
 bool streams(const GemmArgs& a) {
-    return a.M >= 2048 && a.M <= 1 << 30 && a.Kp <= 512 && a.N % 8 == 0 && a.N <= 1 << 20 && aligned16(a.out) &&
+    return a.M >= 2048 && a.M <= 1 << 30 && a.Kp <= 512 && a.N % 2 == 0 && a.N <= 1 << 20 && aligned16(a.out) &&
            aligned16(a.residual);
 }
 
@@ -608,8 +623,9 @@ void launch_stream(hipStream_t s, GemmArgs& a, int workgroups) {
         a.ntiles = (a.N + 16 * NU * WN - 1) / (16 * NU * WN);
         const int rows = 16 * MF * (4 / WN), mtiles = (a.M + rows - 1) / rows;
         const int most = std::max(1, workgroups / a.ntiles);
-        hipLaunchKernelGGL((q8_stream_kernel<BF, KB, NU, MF, WN, RES>), dim3((unsigned)(std::min(mtiles, most) * a.ntiles)),
-                           dim3(256), 0, s, a);
+        const dim3 grid((unsigned)(std::min(mtiles, most) * a.ntiles)), block(256);
+        if (!RES && a.lines) hipLaunchKernelGGL((q8_stream_kernel<BF, KB, NU, MF, WN, RES, !RES>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((q8_stream_kernel<BF, KB, NU, MF, WN, RES, false>), grid, block, 0, s, a);
     };
     if (a.N <= 16 * NU) go(std::integral_constant<int, 1>());
     else if (a.N <= 32 * NU) go(std::integral_constant<int, 2>());
@@ -711,7 +727,8 @@ extern "C" int clk_q8_projection(clk_stream stream, const clk_buffer* q, const c
                static_cast<const int8_t*>(wq->data), static_cast<const float*>(w_scale->data),
                has_b ? static_cast<const float*>(b->data) : nullptr,
                has_residual ? static_cast<const half_t*>(residual->data) : nullptr, static_cast<half_t*>(out->data),
-               (int)M, (int)N, (int)Kp, 0, 0};
+               (int)M, (int)N, (int)Kp, 0, 0,
+               N % 64 == 0 && (reinterpret_cast<uintptr_t>(out->data) & 127u) == 0};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     stage_mark(s, 0);
     act == CLK_BF16 ? launch<true>(s, a) : launch<false>(s, a);

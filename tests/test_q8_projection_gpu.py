@@ -101,6 +101,47 @@ def test_many_rows_short_k(hip, m, n, k):
     assert torch.equal(call(hip, rows, "bf16"), want[7:60])  # a row's result is the same in a batch of any size
 
 
+@pytest.mark.parametrize("k", [64, 128, 256, 500])
+@pytest.mark.parametrize("m,n", [(2048, 2), (2049, 6), (2100, 62), (2500, 130), (3001, 254), (5003, 258), (20011, 42),
+                                 (2300, 1030), (2048, 510)])
+def test_many_rows_even_channels(hip, m, n, k):
+    """As above with rows that end inside a 16-byte piece: the cut piece and what lies behind the last row."""
+    for kind, b, residual in (("f16", True, True), ("bf16", True, False), ("bf16", False, True)):
+        t = operands(m, k, n, kind, b, residual)
+        out, ok = guarded((m, n), DT[kind], 7.0)
+        check(call(hip, t, kind, out=out), t, kind)
+        assert ok()
+    res = t["residual"].clone()
+    assert torch.equal(call(hip, dict(t, residual=res), "bf16", out=res), out)
+    rows = dict(t, q=t["q"][7:60].contiguous(), qs=t["qs"][7:60].contiguous(), residual=t["residual"][7:60].contiguous())
+    assert torch.equal(call(hip, rows, "bf16"), out[7:60])
+
+
+@pytest.mark.parametrize("m,k,n", [(3000, 128, 256), (300, 1024, 512), (700, 192, 130), (2304, 640, 2304)])
+@pytest.mark.parametrize("residual", [False, True])
+def test_results_off_lines(hip, m, k, n, residual):
+    """Results that start 16 bytes (or 2) into a line are the same bits."""
+    t = operands(m, k, n, "f16", True, residual)
+    want = call(hip, t, "f16")
+    check(want, t, "f16")
+    for by in (1, 8, 40):
+        flat = torch.full((m * n + 128,), 7.0, dtype=torch.float16, device="cuda")
+        out = flat[by:by + m * n].view(m, n)
+        assert torch.equal(call(hip, t, "f16", out=out), want)
+        assert (flat[:by] == 7).all() and (flat[by + m * n:] == 7).all()
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("k,n", [(128, 512), (500, 254), (1024, 1024), (1000, 511)])
+@pytest.mark.parametrize("b,residual", [(False, False), (True, False), (False, True), (True, True)])
+def test_a_row_is_the_same_in_calls_of_any_size(hip, kind, k, n, b, residual):
+    t = operands(9000, k, n, kind, b, residual)
+    want = call(hip, t, kind)
+    for lo, hi in ((0, 1), (5, 8), (100, 148), (300, 500), (1000, 1700), (2000, 5000), (8, 9000)):
+        part = dict(t, q=t["q"][lo:hi], qs=t["qs"][lo:hi].clone(), residual=t["residual"][lo:hi].clone() if residual else None)
+        assert torch.equal(call(hip, part, kind), want[lo:hi])
+
+
 @pytest.mark.parametrize("m", [1, 20, 70, 300, 600])
 def test_sums_are_exact(hip, m):
     """The longest rows of the largest integers: the sums reach 131008 * 128 * 128, just under 2^31, and one
