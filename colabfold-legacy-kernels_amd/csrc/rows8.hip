@@ -673,7 +673,8 @@ __device__ __forceinline__ void floats8(const Raw8<T>& r, int col, int K, float 
     }
 }
 
-// As the norm: a row in registers, bound by memory. relu of [147456, 512] fp16: 50 us (227 MB, 4.6 TB/s).
+// As the norm: a row in registers, bound by memory. relu of [147456, 512] fp16: 45 to 54 us (227 MB, 4.2 to 5.0 TB/s;
+// the less of it is left in the far cache by what ran before, the more).
 template <int T, int ACT, int TPR, int NCH>
 __global__ __launch_bounds__(block_of(TPR)) void quantize_kernel(QuantArgs a) {
     constexpr int ROWS = block_of(TPR) / TPR;
@@ -728,7 +729,7 @@ struct DequantArgs {
 // 8192] to fp32: 121 us, 172 with 32 bytes a thread). Results past half of the 256 MB far cache (NT) go by it:
 // whoever reads them next finds little of them there, and the other arrays stay in it. [40000, 2048] quantised,
 // dequantised to fp16 and added to another array takes 168 us, 179 without; 12000 rows 58, 57 without. [147456,
-// 512] to fp16: 29 us (227 MB, part of it from the far cache).
+// 512] to fp16: 34 us (227 MB, 6.7 TB/s, part of it from the far cache).
 template <int T>
 constexpr int kDequant = T == kF32 ? 4 : 8;
 template <int T, bool NT>
