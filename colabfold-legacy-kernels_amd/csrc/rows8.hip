@@ -209,7 +209,7 @@ __device__ __forceinline__ uint2v quant8(const float (&t)[8], float inv) {
     return uint2v{pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7])};
 }
 
-// Sum and maximum over the 256 threads of a block, for the kernels that take a row of any length.
+// Sum and maximum over the threads of a block, for the kernels that take a row of any length.
 template <int THREADS>
 __device__ __forceinline__ float block_sum(float v, float* slot) {
     v = lanes_sum<kWave>(v);
@@ -233,16 +233,6 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* slot) {
     return s;
 }
 
-template <bool BF>
-__device__ __forceinline__ float get16(const half_t* p) {
-    const half_t h = *p;
-    if constexpr (BF) {
-        return (float)__builtin_bit_cast(__bf16, h);
-    } else {
-        return (float)h;
-    }
-}
-
 // ---- RMS norm -----------------------------------------------------------------------------
 
 struct RmsArgs {
@@ -257,57 +247,76 @@ struct RmsArgs {
     float inv_c, eps;
 };
 
-// Rows of any length: a block a row, two passes over it (the second from cache where it fits).
+constexpr int kAny = 1024;  // threads of the kernels for rows of any length
+
+// Rows of any length (past 16384 values): a block a row, two passes over it (the second from cache where it fits).
+// [1024, 40000] bf16 with the residual 73 us (328 MB, 4.5 TB/s), as 8-bit rows 71; [4096, 20000] 149 and 155, where
+// 1024 threads with 4 chunks of a row in registers take 222 and 536 (they spill).
 template <bool BF, bool RES, bool Q8>
-__global__ __launch_bounds__(256) void rms_norm_any_kernel(RmsArgs a) {
-    __shared__ float fslot[4];
-    __shared__ uint32_t uslot[4];
+__global__ __launch_bounds__(kAny) void rms_norm_any_kernel(RmsArgs a) {
+    __shared__ float fslot[kAny / kWave];
+    __shared__ uint32_t uslot[kAny / kWave];
+    const int C = (int)a.C, Kp = (int)a.Kp, first = 8 * threadIdx.x;
     for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
         const half_t* xr = a.x + row * a.C;
         const half_t* rr = a.residual + row * a.C;
         half_t* sr = a.sum + row * a.C;
+        const half_t* vr = RES ? sr : xr;  // each thread reads back only what it wrote
         float ss = 0.f;
         uint32_t m = 0, mt = 0;
-        for (int64_t c = threadIdx.x; c < a.C; c += 256) {
-            float v = get16<BF>(xr + c);
-            if constexpr (RES) {
-                const half_t h = act_cvt<BF>(v + get16<BF>(rr + c));
-                sr[c] = h;
-                v = get16<BF>(&h);
+        const auto collect = [&](int c, half8 v, float d) __attribute__((always_inline)) {
+            float8v w = {};
+            if constexpr (Q8) w = load8f(a.w, c, C);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float f = act_get<BF>(v, e) * d;
+                ss += f * f;
+                m = max(m, abs_bits(f));
+                if constexpr (Q8) mt = max(mt, abs_bits(f * w[e]));
             }
-            ss += v * v;
-            m = max(m, abs_bits(v));
-            if constexpr (Q8) mt = max(mt, abs_bits(v * a.w[c]));
+        };
+        for (int c = first; c < C; c += 8 * kAny) {
+            half8 v = cut8(load8(xr, c, C), c, C);
+            if constexpr (RES) {
+                const half8 r = cut8(load8(rr, c, C), c, C);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = act_cvt<BF>(act_get<BF>(v, e) + act_get<BF>(r, e));
+                store8(sr, c, C, v);
+            }
+            collect(c, v, 1.f);
         }
-        const half_t* vr = RES ? sr : xr;  // each thread reads back only what it wrote
-        ss = block_sum<256>(ss, fslot);
-        m = block_max<256>(m, uslot);
+        ss = block_sum<kAny>(ss, fslot);
+        m = block_max<kAny>(m, uslot);
         const float d = BF ? row_shift(m, a.eps) : 1.f;
         if (d != 1.f) {
             ss = 0.f;
             mt = 0;
-            for (int64_t c = threadIdx.x; c < a.C; c += 256) {
-                const float v = get16<BF>(vr + c) * d;
-                ss += v * v;
-                if constexpr (Q8) mt = max(mt, abs_bits(v * a.w[c]));
-            }
-            ss = block_sum<256>(ss, fslot);
+            for (int c = first; c < C; c += 8 * kAny) collect(c, cut8(load8(vr, c, C), c, C), d);
+            ss = block_sum<kAny>(ss, fslot);
         }
         const float r = inv_rms(ss, a.inv_c, a.eps * d * d);
         if constexpr (Q8) {
-            mt = block_max<256>(max(mt, m >= kInfBits ? m : 0u), uslot);
+            mt = block_max<kAny>(mt, uslot);
             float inv, scale;
             row_scale(mt, r, inv, scale);
             if (threadIdx.x == 0) a.stat[row] = scale;
-            int8_t* qr = a.q + row * a.Kp;
-            for (int64_t c = threadIdx.x; c < a.Kp; c += 256) {
-                qr[c] = c < a.C ? (int8_t)quant(get16<BF>(vr + c) * d * a.w[c], inv) : (int8_t)0;
+            for (int c = first; c < Kp; c += 8 * kAny) {
+                const half8 v = cut8(load8(vr, c, C), c, C);
+                const float8v w = load8f(a.w, c, C);
+                float t[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) t[e] = act_get<BF>(v, e) * d * w[e];
+                *reinterpret_cast<uint2v*>(a.q + row * a.Kp + c) = quant8(t, inv);
             }
         } else {
             if (threadIdx.x == 0 && a.stat != nullptr) a.stat[row] = r * d;
-            half_t* orow = a.out + row * a.C;
-            for (int64_t c = threadIdx.x; c < a.C; c += 256) {
-                orow[c] = act_cvt<BF>(get16<BF>(vr + c) * d * r * a.w[c]);
+            for (int c = first; c < C; c += 8 * kAny) {
+                const half8 v = cut8(load8(vr, c, C), c, C);
+                const float8v w = load8f(a.w, c, C);
+                half8 o;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] = act_cvt<BF>(act_get<BF>(v, e) * d * r * w[e]);
+                store8(a.out + row * a.C, c, C, o);
             }
         }
     }
@@ -412,24 +421,37 @@ struct RmsBwdArgs {
     float inv_c;
 };
 
-// Rows of any length: a block a row for ds; dw by columns in a kernel of its own, which reads s and dout again.
+// Rows of any length (past 16384 values): a block a row for ds; dw by columns in a kernel of its own, which reads s and
+// dout again. [1024, 40000] bf16 with dsum: 107 us (492 MB read and written, 4.6 TB/s).
 template <bool BF>
-__global__ __launch_bounds__(256) void rms_norm_bwd_any_kernel(RmsBwdArgs a) {
-    __shared__ float slot[4];
+__global__ __launch_bounds__(kAny) void rms_norm_bwd_any_kernel(RmsBwdArgs a) {
+    __shared__ float slot[kAny / kWave];
+    const int C = (int)a.C, first = 8 * threadIdx.x;
     for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
         const float r = a.rstd[row];
         const half_t* sr = a.s + row * a.C;
         const half_t* dr = a.dout + row * a.C;
         float dot = 0.f;
-        for (int64_t c = threadIdx.x; c < a.C; c += 256) {
-            dot += get16<BF>(dr + c) * a.w[c] * (get16<BF>(sr + c) * r);
+        for (int c = first; c < C; c += 8 * kAny) {
+            const half8 s = cut8(load8(sr, c, C), c, C), dy = cut8(load8(dr, c, C), c, C);
+            const float8v w = load8f(a.w, c, C);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dot += act_get<BF>(dy, e) * w[e] * (act_get<BF>(s, e) * r);
         }
-        dot = block_sum<256>(dot, slot) * a.inv_c;
-        for (int64_t c = threadIdx.x; c < a.C; c += 256) {
-            const float dy = get16<BF>(dr + c), xh = get16<BF>(sr + c) * r;
-            float d = r * (dy * a.w[c] - xh * dot);
-            if (a.dsum != nullptr) d += get16<BF>(a.dsum + row * a.C + c);
-            a.ds[row * a.C + c] = act_cvt<BF>(d);
+        dot = block_sum<kAny>(dot, slot) * a.inv_c;
+        for (int c = first; c < C; c += 8 * kAny) {
+            const half8 s = cut8(load8(sr, c, C), c, C), dy = cut8(load8(dr, c, C), c, C);
+            const float8v w = load8f(a.w, c, C);
+            half8 dz = {};
+            if (a.dsum != nullptr) dz = cut8(load8(a.dsum + row * a.C, c, C), c, C);
+            half8 o;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                float d = r * (act_get<BF>(dy, e) * w[e] - act_get<BF>(s, e) * r * dot);
+                if (a.dsum != nullptr) d += act_get<BF>(dz, e);
+                o[e] = act_cvt<BF>(d);
+            }
+            store8(a.ds + row * a.C, c, C, o);
         }
     }
 }
@@ -569,17 +591,15 @@ Route route_of(int64_t Kp) {
     if (Kp <= 8192) return {512, 2};
     if (Kp <= 12288) return {512, 3};
     if (Kp <= 16384) return {1024, 2};
-    if (Kp <= 32768) return {1024, 4};
     return {0, 0};
 }
-#define CLK_ROUTES(X_) X_(8, 1) X_(16, 1) X_(32, 1) X_(64, 1) X_(64, 2) X_(256, 1) X_(256, 2) X_(256, 3) X_(512, 2) X_(512, 3) X_(1024, 2) X_(1024, 4)
+#define CLK_ROUTES(X_) X_(8, 1) X_(16, 1) X_(32, 1) X_(64, 1) X_(64, 2) X_(256, 1) X_(256, 2) X_(256, 3) X_(512, 2) X_(512, 3) X_(1024, 2)
 
 int64_t padded64(int64_t k) { return (k + 63) / 64 * 64; }
 
 // The gradients hold twice the registers: for [4096, 12000] 512 threads with 3 chunks take 100 us, 1024 with 2 88 us.
 Route bwd_route(int64_t C) {
     const Route rt = route_of(padded64(C));
-    if (rt.nch == 4) return {0, 0};
     return rt.nch == 3 && rt.tpr == 512 ? Route{1024, 2} : rt;
 }
 
@@ -609,43 +629,8 @@ struct QuantArgs {
 enum { kF16, kBf16, kF32 };
 enum { kActNone, kActRelu, kActSwish };
 
-template <int T>
-__device__ __forceinline__ float get_any(const void* p, int64_t i) {
-    if constexpr (T == kF32) {
-        return static_cast<const float*>(p)[i];
-    } else {
-        return get16<T == kBf16>(static_cast<const half_t*>(p) + i);
-    }
-}
-
 // relu keeps a NaN (a row that holds one is NaN as a whole)
 __device__ __forceinline__ float relu(float v) { return v < 0.f ? 0.f : v; }
-
-template <int T, int ACT>
-__device__ __forceinline__ float hidden(const void* x, int64_t row, int64_t k, int64_t K) {
-    if constexpr (ACT == kActSwish) {
-        const float g = get_any<T>(x, row * 2 * K + k), u = get_any<T>(x, row * 2 * K + K + k);
-        return g * sigmoid_fast(g) * u;
-    } else {
-        const float v = get_any<T>(x, row * K + k);
-        return ACT == kActRelu ? relu(v) : v;
-    }
-}
-
-template <int T, int ACT>
-__global__ __launch_bounds__(256) void quantize_any_kernel(QuantArgs a) {
-    __shared__ uint32_t slot[4];
-    for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
-        uint32_t m = 0;
-        for (int64_t k = threadIdx.x; k < a.K; k += 256) m = max(m, abs_bits(hidden<T, ACT>(a.x, row, k, a.K)));
-        float inv, scale;
-        row_scale(block_max<256>(m, slot), 1.f, inv, scale);
-        if (threadIdx.x == 0) a.scale[row] = scale;
-        for (int64_t k = threadIdx.x; k < a.Kp; k += 256) {
-            a.q[row * a.Kp + k] = k < a.K ? (int8_t)quant(hidden<T, ACT>(a.x, row, k, a.K), inv) : (int8_t)0;
-        }
-    }
-}
 
 // 8 values from column col of a row of h: read, and made of what was read
 template <int T>
@@ -670,6 +655,46 @@ __device__ __forceinline__ void floats8(const Raw8<T>& r, int col, int K, float 
         const half8 v = cut8(r.v, col, K);
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] = act_get<T == kBf16>(v, e);
+    }
+}
+
+// h's 8 values from column c of the row that starts at x[at]
+template <int T, int ACT>
+__device__ __forceinline__ void hidden8(const void* x, int64_t at, int c, int K, float (&h)[8]) {
+    Raw8<T> raw, up;
+    read8(x, at, c, K, raw);
+    if constexpr (ACT == kActSwish) read8(x, at + K, c, K, up);
+    floats8(raw, c, K, h);
+    float u[8];
+    if constexpr (ACT == kActSwish) floats8(up, c, K, u);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if constexpr (ACT == kActSwish) h[e] = h[e] * sigmoid_fast(h[e]) * u[e];
+        if constexpr (ACT == kActRelu) h[e] = relu(h[e]);
+    }
+}
+
+// Rows of any length, read twice. [1024, 40000] bf16: 30 us (123 MB, 4.1 TB/s).
+template <int T, int ACT>
+__global__ __launch_bounds__(kAny) void quantize_any_kernel(QuantArgs a) {
+    __shared__ uint32_t slot[kAny / kWave];
+    const int K = (int)a.K, Kp = (int)a.Kp, first = 8 * threadIdx.x;
+    for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
+        const int64_t at = row * (ACT == kActSwish ? 2 * a.K : a.K);
+        uint32_t m = 0;
+        float h[8];
+        for (int c = first; c < K; c += 8 * kAny) {
+            hidden8<T, ACT>(a.x, at, c, K, h);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m = max(m, abs_bits(h[e]));
+        }
+        float inv, scale;
+        row_scale(block_max<kAny>(m, slot), 1.f, inv, scale);
+        if (threadIdx.x == 0) a.scale[row] = scale;
+        for (int c = first; c < Kp; c += 8 * kAny) {
+            hidden8<T, ACT>(a.x, at, c, K, h);
+            *reinterpret_cast<uint2v*>(a.q + row * a.Kp + c) = quant8(h, inv);
+        }
     }
 }
 
@@ -814,7 +839,7 @@ int rms_forward(const char* what, clk_stream stream, const clk_buffer* x, const 
     const auto launch = [&](auto bf_, auto q8_) {
         constexpr bool BF = decltype(bf_)::value, Q8 = decltype(q8_)::value;
         if (rt.tpr == 0) {
-            const dim3 grid(any_blocks(M)), block(256);
+            const dim3 grid(any_blocks(M)), block(kAny);
             if (has_residual) hipLaunchKernelGGL((rms_norm_any_kernel<BF, true, Q8>), grid, block, 0, s, a);
             else hipLaunchKernelGGL((rms_norm_any_kernel<BF, false, Q8>), grid, block, 0, s, a);
             return;
@@ -886,9 +911,9 @@ extern "C" int clk_rms_norm_bwd(clk_stream stream, const clk_buffer* s, const cl
     if (M > 0) {
         const Route rt = bwd_route(C);
 #define CLK_BWD_RT(TPR_, NCH_)                                                                                        \
-    if (rt.tpr == TPR_ && rt.nch == NCH_ && NCH_ < 4) {                                                               \
-        if (has_dsum) hipLaunchKernelGGL((rms_norm_bwd_kernel<BF, TPR_, NCH_ < 4 ? NCH_ : 1, true>), grid, block, 0, st, a);         \
-        else hipLaunchKernelGGL((rms_norm_bwd_kernel<BF, TPR_, NCH_ < 4 ? NCH_ : 1, false>), grid, block, 0, st, a);                 \
+    if (rt.tpr == TPR_ && rt.nch == NCH_) {                                                               \
+        if (has_dsum) hipLaunchKernelGGL((rms_norm_bwd_kernel<BF, TPR_, NCH_, true>), grid, block, 0, st, a);         \
+        else hipLaunchKernelGGL((rms_norm_bwd_kernel<BF, TPR_, NCH_, false>), grid, block, 0, st, a);                 \
     }
         const auto launch = [&](auto bf_) {
             constexpr bool BF = decltype(bf_)::value;
@@ -896,7 +921,7 @@ extern "C" int clk_rms_norm_bwd(clk_stream stream, const clk_buffer* s, const cl
                 // dw first: ds may overwrite dout
                 hipLaunchKernelGGL(rms_norm_dw_any_kernel<BF>, dim3((unsigned)((C + 2047) / 2048), a.P), dim3(256), 0, st, a);
                 stage_mark(st, ++stage);
-                hipLaunchKernelGGL(rms_norm_bwd_any_kernel<BF>, dim3(any_blocks(M)), dim3(256), 0, st, a);
+                hipLaunchKernelGGL(rms_norm_bwd_any_kernel<BF>, dim3(any_blocks(M)), dim3(kAny), 0, st, a);
                 return;
             }
             const dim3 grid(a.P), block(block_of(rt.tpr));
@@ -936,7 +961,7 @@ extern "C" int clk_quantize_rows(clk_stream stream, const clk_buffer* x, const c
     if (rt.tpr == TPR_ && rt.nch == NCH_) hipLaunchKernelGGL((quantize_kernel<T, A, TPR_, NCH_>), grid, block, 0, s, a);
     const auto launch = [&](auto t_, auto a_) {
         constexpr int T = decltype(t_)::value, A = decltype(a_)::value;
-        const dim3 grid(rt.tpr == 0 ? any_blocks(M) : row_blocks(M, rt.tpr)), block(rt.tpr == 0 ? 256 : block_of(rt.tpr));
+        const dim3 grid(rt.tpr == 0 ? any_blocks(M) : row_blocks(M, rt.tpr)), block(rt.tpr == 0 ? kAny : block_of(rt.tpr));
         if (rt.tpr == 0) hipLaunchKernelGGL((quantize_any_kernel<T, A>), grid, block, 0, s, a);
         CLK_ROUTES(CLK_QR_RT)
     };
