@@ -214,11 +214,21 @@ def transition(x, scale, offset, w1, b1, w2, b2, keep=None, add_input=False, eps
 # ---- RMS norm and the 8-bit path (no counterpart in the reference) ----------------------------
 
 class _RmsNorm(torch.autograd.Function):
+    """x and residual come in as the caller has them and are flattened in here: reshaped around this
+    node, their gradients would reach the leaves as two views of ds, each of which autograd takes for
+    a leaf's own and adds to in place. As one tensor for both inputs it is copied where a leaf keeps
+    it, as an addition's gradient is."""
+
     @staticmethod
     def forward(ctx, x, scale, residual, eps):
-        out, total, rstd = hip.rms_norm(x, scale, residual, eps, want_rstd=True)
+        x2 = _matrix(x)
+        out = x2.new_empty(x.shape)  # of the results' own shape: a view of a result could not be changed in place
+        total = None if residual is None else x2.new_empty(x.shape)
+        _, _, rstd = hip.rms_norm(x2, scale, None if residual is None else _matrix(residual), eps, want_rstd=True,
+                                  out=_matrix(out), sum_out=None if residual is None else _matrix(total))
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x if residual is None else total, scale, rstd)
+        ctx.shape = x.shape
+        ctx.save_for_backward(x2 if residual is None else total, scale, rstd)
         return out if residual is None else (out, total)
 
     @staticmethod
@@ -229,7 +239,9 @@ class _RmsNorm(torch.autograd.Function):
         if dout is None:  # only the sum was used
             ds, dscale = dsum, torch.zeros_like(scale)
         else:
-            ds, dscale = hip.rms_norm_bwd(s, scale, rstd, dout.to(s.dtype).contiguous(), dsum)
+            ds, dscale = s.new_empty(ctx.shape), torch.empty_like(scale)
+            hip.rms_norm_bwd(_matrix(s), scale, rstd, _matrix(dout.to(s.dtype)), None if dsum is None else _matrix(dsum),
+                             grads=(_matrix(ds), dscale))
         need = ctx.needs_input_grad
         return ds if need[0] else None, dscale if need[1] else None, ds if need[2] else None, None
 
@@ -250,18 +262,13 @@ def rms_norm(x, scale, residual=None, eps=1e-5):
     if differentiated and x.is_cuda and torch.cuda.is_current_stream_capturing():
         raise hip.InvalidArgument(hip.INVALID_ARGUMENT, "rms_norm: a differentiated call cannot be captured into a "
                                   "graph; capture hip.rms_norm and hip.rms_norm_bwd")
-    shape = x.shape
-    x2 = _matrix(x)
-    r2 = None if residual is None else _matrix(residual)
     w = scale.float().contiguous()
     if differentiated:
-        res = _RmsNorm.apply(x2, w, r2, float(eps))
-    else:
-        res = hip.rms_norm(x2, w, r2, eps)
-        res = res[0] if residual is None else res[:2]
-    if len(shape) == 2:
-        return res
-    return res.reshape(shape) if residual is None else tuple(t.reshape(shape) for t in res)
+        return _RmsNorm.apply(x, w, residual, float(eps))
+    out, total, _ = hip.rms_norm(_matrix(x), w, None if residual is None else _matrix(residual), eps)
+    if x.dim() != 2:
+        out, total = out.reshape(x.shape), None if total is None else total.reshape(x.shape)
+    return out if residual is None else (out, total)
 
 
 def _matrix(x):

@@ -249,3 +249,84 @@ def test_shapes_are_refused():
 
 def test_padded_k():
     assert [H.padded_k(k) for k in (1, 63, 64, 65, 128, 8191)] == [64, 64, 64, 128, 128, 8192]
+
+
+# ---- torch_ops.rms_norm under autograd, with torch operations in the kernels' place --------------
+
+@pytest.fixture
+def kernels_on_cpu(monkeypatch):
+    """hip.rms_norm and hip.rms_norm_bwd by torch operations, with the entry points' own shapes."""
+    def forward(x, scale, residual=None, eps=1e-5, want_rstd=False, out=None, sum_out=None, rstd=None):
+        assert x.dim() == 2 and (out is None or out.shape == x.shape)
+        s = x if residual is None else (x.float() + residual.float()).to(x.dtype)
+        r = 1 / torch.sqrt(s.float().square().mean(1) + eps)
+        y = (s.float() * r[:, None] * scale.reshape(-1)).to(x.dtype)
+        y = y if out is None else out.copy_(y)
+        if residual is not None and sum_out is not None:
+            s = sum_out.copy_(s)
+        return y, None if residual is None else s, r if want_rstd else None
+
+    def backward(s, scale, rstd, dout, dsum=None, workspace=None, grads=None):
+        assert s.dim() == 2 and dout.shape == s.shape and (dsum is None or dsum.shape == s.shape)
+        g, xh = dout.float() * scale.reshape(-1), s.float() * rstd[:, None]
+        ds = rstd[:, None] * (g - xh * (g * xh).mean(1, keepdim=True)) + (0 if dsum is None else dsum.float())
+        ds, dscale = ds.to(s.dtype), (dout.float() * xh).sum(0).reshape(scale.shape)
+        return (ds, dscale) if grads is None else (grads[0].copy_(ds), grads[1].copy_(dscale))
+
+    monkeypatch.setattr(H, "rms_norm", forward)
+    monkeypatch.setattr(H, "rms_norm_bwd", backward)
+
+
+def norm_leaves(shape, dtype=torch.float16):
+    gen = torch.Generator().manual_seed(3)
+    x, res = (torch.randn(shape, generator=gen).to(dtype).requires_grad_() for _ in range(2))
+    w = (1 + 0.2 * torch.randn(shape[-1], generator=gen)).requires_grad_()
+    return x, res, w, torch.randn(shape, generator=gen).to(dtype), torch.randn(shape, generator=gen).to(dtype)
+
+
+@pytest.mark.parametrize("shape", [(64,), (6, 64), (2, 3, 64), (2, 3, 2, 8), (1, 1, 64), (0, 3, 64)])
+@pytest.mark.parametrize("used", ["both", "norm", "sum"])
+def test_gradients_accumulate_leaf_by_leaf(kernels_on_cpu, shape, used):
+    """Two passes into both leaves: twice one pass's gradient in each, in memory of its own."""
+    x, res, w, dy, ds = norm_leaves(shape)
+
+    def one_pass():
+        y, total = torch_ops.rms_norm(x, w, res)
+        assert y.shape == x.shape and total.shape == x.shape
+        outs, grads = {"both": ((y, total), (dy, ds)), "norm": ((y,), (dy,)), "sum": ((total,), (ds,))}[used]
+        torch.autograd.backward(outs, grads)
+
+    given = dy.clone(), ds.clone()
+    one_pass()
+    once = x.grad.clone(), res.grad.clone()
+    assert torch.equal(*once) and x.grad.shape == x.shape
+    one_pass()
+    for leaf, g in zip((x, res), once):
+        assert torch.equal(leaf.grad, 2 * g)
+    if x.numel():
+        owners = [t.data_ptr() for t in (x.grad, res.grad, dy, ds)]
+        assert len(set(owners)) == 4
+    x.grad.zero_()
+    assert torch.equal(res.grad, 2 * once[1]) and torch.equal(dy, given[0]) and torch.equal(ds, given[1])
+
+
+@pytest.mark.parametrize("shape", [(6, 64), (2, 3, 64)])
+def test_results_of_a_differentiated_norm_are_plain_tensors(kernels_on_cpu, shape):
+    """The results may be changed in place as any operation's, what the gradient needs of them is checked,
+    and strided inputs get gradients of their own."""
+    x, res, w, dy, ds = norm_leaves(shape)
+    y, total = torch_ops.rms_norm(x, w, res)
+    y.mul_(2)
+    y.backward(dy)
+    want = x.grad.clone()
+    x.grad = None
+    torch_ops.rms_norm(x, w, res)[0].backward(2 * dy)
+    assert torch.equal(want, x.grad)
+    y, total = torch_ops.rms_norm(x, w, res)
+    total.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(dy)
+    xt, rt = (t.detach().transpose(0, -1).contiguous().transpose(0, -1).requires_grad_() for t in (x, res))
+    assert not xt.is_contiguous()
+    torch_ops.rms_norm(xt, w, rt)[0].backward(2 * dy)
+    assert torch.equal(xt.grad, want) and torch.equal(rt.grad, want)
