@@ -29,6 +29,7 @@ Everything runs on the GPU through the built library; there is no CPU path. The 
 fp16 or bf16 activations, with weights and biases cast to fp16 for the kernels.
 """
 import torch
+from torch.autograd import forward_ad
 
 from . import hip
 from . import layouts
@@ -249,7 +250,8 @@ class _RmsNorm(torch.autograd.Function):
 def rms_norm(x, scale, residual=None, eps=1e-5):
     """y [..., c] = s / sqrt(mean(s^2) + eps) * scale with s = x, or (y, s) with s = x + residual
     rounded to x's type: the residual stream, which the next block adds to. x and residual fp16 or
-    bf16, one shape; scale [c]. Differentiable in x, residual and scale (once).
+    bf16, one shape; scale [c]. Differentiable in x, residual and scale (once, in reverse mode; a dual tensor is
+    refused).
 
     A call that needs gradients is refused while a HIP graph is being captured: torch may order such a
     backward against the streams of an eager pass over the same leaves, which a capture cannot
@@ -263,12 +265,18 @@ def rms_norm(x, scale, residual=None, eps=1e-5):
         raise hip.InvalidArgument(hip.INVALID_ARGUMENT, "rms_norm: a differentiated call cannot be captured into a "
                                   "graph; capture hip.rms_norm and hip.rms_norm_bwd")
     w = scale.float().contiguous()
-    if differentiated:
+    if differentiated or any(_has_tangent(t) for t in (x, scale, residual)):
         return _RmsNorm.apply(x, w, residual, float(eps))
     out, total, _ = hip.rms_norm(_matrix(x), w, None if residual is None else _matrix(residual), eps)
     if x.dim() != 2:
         out, total = out.reshape(x.shape), None if total is None else total.reshape(x.shape)
     return out if residual is None else (out, total)
+
+
+def _has_tangent(t):
+    """Whether t is a dual tensor of the open forward-mode level: the autograd node refuses those, which have
+    no requires_grad"""
+    return t is not None and forward_ad.unpack_dual(t).tangent is not None
 
 
 def _matrix(x):

@@ -330,3 +330,19 @@ def test_results_of_a_differentiated_norm_are_plain_tensors(kernels_on_cpu, shap
     assert not xt.is_contiguous()
     torch_ops.rms_norm(xt, w, rt)[0].backward(2 * dy)
     assert torch.equal(xt.grad, want) and torch.equal(rt.grad, want)
+
+
+@pytest.mark.parametrize("which", ["x", "scale", "residual"])
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(kernels_on_cpu, which, grad):
+    """A dual tensor has no requires_grad of its own; its tangent must not vanish. Without a tangent, a call
+    inside a dual level is an ordinary one."""
+    from torch.autograd import forward_ad
+    x, res, w, _, _ = (t.detach() for t in norm_leaves((2, 3, 64)))
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        want = torch_ops.rms_norm(x, w, res)
+        args = dict(x=x, scale=w, residual=res)
+        args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(RuntimeError, match="jvp|forward"):
+            torch_ops.rms_norm(**args)
+    assert all(torch.equal(a, b) for a, b in zip(torch_ops.rms_norm(x, w, res), want))
