@@ -236,6 +236,7 @@ class _RmsNorm(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, dsum=None):
         s, scale, rstd = ctx.saved_tensors
+        _refuse_capture(s)
         dsum = None if dsum is None else dsum.to(s.dtype).contiguous()
         if dout is None:  # only the sum was used
             ds, dscale = dsum, torch.zeros_like(scale)
@@ -253,17 +254,17 @@ def rms_norm(x, scale, residual=None, eps=1e-5):
     bf16, one shape; scale [c]. Differentiable in x, residual and scale (once, in reverse mode; a dual tensor is
     refused).
 
-    A call that needs gradients is refused while a HIP graph is being captured: torch may order such a
-    backward against the streams of an eager pass over the same leaves, which a capture cannot
-    hold. Capture hip.rms_norm and hip.rms_norm_bwd instead, which take their buffers."""
+    While a HIP graph is being captured, a call that needs gradients is refused, and so is the backward of an
+    earlier one on the capturing stream: a leaf that an eager pass has used keeps that pass's stream, torch makes it
+    wait for the capture's work when the gradient reaches it, and nothing in a call tells whether one of its leaves
+    is such a one. Capture hip.rms_norm and hip.rms_norm_bwd instead, which take their buffers."""
     if residual is not None and residual.shape != x.shape:
         raise hip.InvalidArgument(hip.INVALID_ARGUMENT, "rms_norm: residual must be like x, got %s and %s"
                                   % (tuple(residual.shape), tuple(x.shape)))
     differentiated = torch.is_grad_enabled() and (x.requires_grad or scale.requires_grad or (
         residual is not None and residual.requires_grad))
-    if differentiated and x.is_cuda and torch.cuda.is_current_stream_capturing():
-        raise hip.InvalidArgument(hip.INVALID_ARGUMENT, "rms_norm: a differentiated call cannot be captured into a "
-                                  "graph; capture hip.rms_norm and hip.rms_norm_bwd")
+    if differentiated:
+        _refuse_capture(x)
     w = scale.float().contiguous()
     if differentiated or any(_has_tangent(t) for t in (x, scale, residual)):
         return _RmsNorm.apply(x, w, residual, float(eps))
@@ -271,6 +272,16 @@ def rms_norm(x, scale, residual=None, eps=1e-5):
     if x.dim() != 2:
         out, total = out.reshape(x.shape), None if total is None else total.reshape(x.shape)
     return out if residual is None else (out, total)
+
+
+def _capturing(t):
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
+def _refuse_capture(t):
+    if _capturing(t):
+        raise hip.InvalidArgument(hip.INVALID_ARGUMENT, "rms_norm: a differentiated call cannot be captured into a "
+                                  "graph; capture hip.rms_norm and hip.rms_norm_bwd")
 
 
 def _has_tangent(t):

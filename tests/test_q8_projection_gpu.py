@@ -386,3 +386,26 @@ def test_differentiated_call_is_refused_under_capture(hip):
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(y, torch_ops.rms_norm(static, w))
+
+
+def test_backward_of_an_eager_forward_is_refused_under_capture(hip):
+    """The backward node runs on its forward's stream; captured there, it raises before any gradient reaches a leaf."""
+    x, _, w = inputs(4, 64, "f16", False)
+    dy = torch.ones_like(x)
+    x.requires_grad_()
+    static = x.detach().clone()
+    torch_ops.rms_norm(static, w)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        y = torch_ops.rms_norm(x, w)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        with pytest.raises(hip.InvalidArgument, match="cannot be captured"):
+            y.backward(dy)
+        captured = torch_ops.rms_norm(static, w)
+    assert x.grad is None
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(captured, torch_ops.rms_norm(static, w))

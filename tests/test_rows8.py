@@ -346,3 +346,22 @@ def test_forward_mode_is_refused(kernels_on_cpu, which, grad):
         with pytest.raises(RuntimeError, match="jvp|forward"):
             torch_ops.rms_norm(**args)
     assert all(torch.equal(a, b) for a, b in zip(torch_ops.rms_norm(x, w, res), want))
+
+
+def test_backward_is_refused_under_capture(kernels_on_cpu, monkeypatch):
+    """An eager forward whose backward runs into a capture, for each result that may be used; the same graph's
+    backward outside of the capture still runs."""
+    x, res, w, dy, ds = norm_leaves((2, 3, 64))
+    y, total = torch_ops.rms_norm(x, w, res)
+    alone = torch_ops.rms_norm(x, w)
+    with monkeypatch.context() as m:
+        m.setattr(torch_ops, "_capturing", lambda t: True)
+        for outs, grads in (((y, total), (dy, ds)), ((y,), (dy,)), ((total,), (ds,)), ((alone,), (dy,))):
+            with pytest.raises(H.InvalidArgument, match="cannot be captured"):
+                torch.autograd.backward(outs, grads, retain_graph=True)
+        with pytest.raises(H.InvalidArgument, match="cannot be captured"):
+            torch_ops.rms_norm(x, w, res)
+        torch_ops.rms_norm(x.detach(), w.detach())
+    assert x.grad is None and res.grad is None and w.grad is None
+    torch.autograd.backward((y, total), (dy, ds))
+    assert x.grad is not None
