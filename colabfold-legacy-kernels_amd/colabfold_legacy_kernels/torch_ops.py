@@ -258,9 +258,7 @@ def rms_norm(x, scale, residual=None, eps=1e-5):
     earlier one on the capturing stream: a leaf that an eager pass has used keeps that pass's stream, torch makes it
     wait for the capture's work when the gradient reaches it, and nothing in a call tells whether one of its leaves
     is such a one. Capture hip.rms_norm and hip.rms_norm_bwd instead, which take their buffers."""
-    if residual is not None and residual.shape != x.shape:
-        raise hip.InvalidArgument(hip.INVALID_ARGUMENT, "rms_norm: residual must be like x, got %s and %s"
-                                  % (tuple(residual.shape), tuple(x.shape)))
+    _residual_like("rms_norm", "x", residual, x.shape)
     differentiated = torch.is_grad_enabled() and (x.requires_grad or scale.requires_grad or (
         residual is not None and residual.requires_grad))
     if differentiated:
@@ -272,6 +270,21 @@ def rms_norm(x, scale, residual=None, eps=1e-5):
     if x.dim() != 2:
         out, total = out.reshape(x.shape), None if total is None else total.reshape(x.shape)
     return out if residual is None else (out, total)
+
+
+def _residual_like(name, what, residual, shape):
+    if residual is not None and residual.shape != shape:
+        raise hip.InvalidArgument(hip.INVALID_ARGUMENT, "%s: residual must be like %s, got %s and %s"
+                                  % (name, what, tuple(residual.shape), tuple(shape)))
+
+
+def _residual_rows(name, what, residual, shape):
+    """residual as rows: of `shape`, or given as rows [M, C] (whose M and C the entry point checks)"""
+    if residual is None:
+        return None
+    if residual.dim() != 2:
+        _residual_like(name, what, residual, shape)
+    return _rows(residual)[0]
 
 
 def _capturing(t):
@@ -303,7 +316,7 @@ def rms_norm_q8(x, scale, residual=None, eps=1e-5):
     """(q, q_scale, s): rms_norm with its result as 8-bit rows, q [..., hip.padded_k(c)] int8 and
     q_scale [...] fp32; s as in rms_norm, None without a residual."""
     x2, lead = _rows(x)
-    r2 = None if residual is None else _rows(residual)[0]
+    r2 = _residual_rows("rms_norm_q8", "x", residual, x.shape)
     q, q_scale, total = hip.rms_norm_q8(x2, scale.float().contiguous(), r2, eps)
     return _q8_lead(q, q_scale, lead) + (None if total is None else total.reshape(x.shape),)
 
@@ -340,7 +353,7 @@ def q8_projection(q, q_scale, weights, b=None, residual=None, dtype=torch.float1
     q8_weights(w); in residual's type, or `dtype` without one."""
     wq, w_scale = weights
     q2, lead = _rows(q)
-    r2 = None if residual is None else _rows(residual)[0]
+    r2 = _residual_rows("q8_projection", "the result", residual, q.shape[:-1] + w_scale.shape[:1])
     out = hip.q8_projection(q2, q_scale.reshape(-1).contiguous(), wq, w_scale, None if b is None else b.float().contiguous(),
                             r2, dtype if r2 is None else r2.dtype)
     return out.reshape(lead + (out.shape[-1],))

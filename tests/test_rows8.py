@@ -365,3 +365,19 @@ def test_backward_is_refused_under_capture(kernels_on_cpu, monkeypatch):
     assert x.grad is None and res.grad is None and w.grad is None
     torch.autograd.backward((y, total), (dy, ds))
     assert x.grad is not None
+
+
+def test_residuals_of_another_shape_are_refused():
+    """Also where they hold as many values: [3, 2, 64] is not added to [2, 3, 64] by position in memory. Rows [M, C]
+    pass to the entry point, which checks them."""
+    x, w = torch.zeros((2, 3, 64), dtype=torch.float16), torch.ones(64)
+    q, s = torch.zeros((2, 3, 64), dtype=torch.int8), torch.ones((2, 3))
+    weights = layouts.q8_blocked(torch.zeros((8, 64), dtype=torch.int8)), torch.ones(8)
+    for other in ((3, 2, 64), (1, 6, 64), (2, 3, 32), (2, 3, 65), (64,)):
+        with pytest.raises(H.InvalidArgument, match="residual must be like x"):
+            torch_ops.rms_norm_q8(x, w, torch.zeros(other, dtype=torch.float16))
+        with pytest.raises(H.InvalidArgument, match="residual must be like x"):
+            torch_ops.q8_transition(x, w, weights, None, weights, None, torch.zeros(other, dtype=torch.float16))
+    for other in ((3, 2, 8), (1, 6, 8), (2, 3, 9), (2, 3, 64), (8,)):
+        with pytest.raises(H.InvalidArgument, match="residual must be like the result"):
+            torch_ops.q8_projection(q, s, weights, residual=torch.zeros(other, dtype=torch.float16))
