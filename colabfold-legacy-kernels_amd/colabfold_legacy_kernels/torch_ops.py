@@ -279,10 +279,10 @@ def _residual_like(name, what, residual, shape):
 
 
 def _residual_rows(name, what, residual, shape):
-    """residual as rows: of `shape`, or given as rows [M, C] (whose M and C the entry point checks)"""
+    """residual as rows: of `shape`, or given as rows [M, C] or a row (whose M and C the entry point checks)"""
     if residual is None:
         return None
-    if residual.dim() != 2:
+    if residual.dim() > 2:
         _residual_like(name, what, residual, shape)
     return _rows(residual)[0]
 
