@@ -2,10 +2,10 @@
 // LayerNorm and feed the 8-bit matrix product (q8_gemm.hip).
 //
 //   rms_norm        s = round16(x + residual), y = round16(s r w), r = 1 / sqrt(mean(s^2) + eps)
-//   rms_norm_q8     t = s w, a = max |t|; q = rint(t (127 / a)), scale = a r / 127: r cancels in q, so
+//   rms_norm_q8     t = s w, a = max |t|; q = 127 t / a to the nearest, scale = a r / 127: r cancels in q, so
 //                   the integers depend on s and w alone
 //   rms_norm_bwd    g = dy w, xh = s r: ds = r (g - xh mean(g xh)) + dsum, dw = sum over rows of dy xh
-//   quantize_rows   h = x, relu(x) or swish(x[:, :K]) x[:, K:]; q = rint(h (127 / a)), scale = a / 127
+//   quantize_rows   h = x, relu(x) or swish(x[:, :K]) x[:, K:]; q = 127 h / a to the nearest, scale = a / 127
 //   dequantize_rows out = q scale
 //
 // All of them are bound by memory: each value is read once and written once, statistics and products
@@ -33,10 +33,10 @@ constexpr uint32_t kInfBits = 0x7f800000u;
 // where a float maximum drops NaN
 __device__ __forceinline__ uint32_t abs_bits(float t) { return __builtin_bit_cast(uint32_t, t) & 0x7fffffffu; }
 
-// What a row of largest magnitude `bits` is multiplied by before the rounding, and its scale times r.
-// A row with an infinity or NaN is zeros with scale NaN, so everything computed from it is NaN.
-__device__ __forceinline__ void row_scale(uint32_t bits, float r, float& inv, float& scale) {
-    const float a = __builtin_bit_cast(float, bits);
+// A row of largest magnitude `bits`: that as a float, what its values are multiplied by before the rounding, and its
+// scale times r. A row with an infinity or NaN is zeros with scale NaN, so everything computed from it is NaN.
+__device__ __forceinline__ void row_scale(uint32_t bits, float r, float& a, float& inv, float& scale) {
+    a = __builtin_bit_cast(float, bits);
     if (bits >= kInfBits) {
         inv = 0.f;
         scale = __builtin_nanf("");
@@ -49,12 +49,22 @@ __device__ __forceinline__ void row_scale(uint32_t bits, float r, float& inv, fl
     }
 }
 
-// rint(t inv) as an integer, ties to even; |t| <= a bounds it by 127, and inv = 0 (a row of zeros)
-// gives 0 also for a t that is not finite
-__device__ __forceinline__ int quant(float t, float inv) { return inv == 0.f ? 0 : (int)__builtin_rintf(t * inv); }
+// The integer nearest to 127 t / a, ties to even, where it lies within 2^-15 of a half: t inv carries inv's rounding, 127
+// 2^-24 at most, which decides there. n = t inv to the nearest, f what t inv lies past it. Of 127 t - m a, m the
+// half, the sign counts: 127 t is taken in two parts, m a has to be rounded nowhere (fma), and what is left of
+// the two is a multiple of a's last bit too small to be rounded. Rows of huge values are taken times 2^-64 for it.
+__device__ __forceinline__ int settle_half(float t, float a, float n, float f) {
+    const float s = a > 0x1p100f ? 0x1p-64f : 1.f, ts = t * s;
+    const float hi = 127.f * ts, lo = __builtin_fmaf(127.f, ts, -hi);
+    const float e = __builtin_fmaf(-(n + __builtin_copysignf(0.5f, f)), a * s, hi) + lo;
+    const int below = (int)n - (f < 0.f);
+    return below + (e > 0.f || (e == 0.f && (below & 1)));
+}
+constexpr float kNearHalf = 0.5f - 0x1p-15f;
 
-__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
-    return (uint32_t)(a & 255) | (uint32_t)(b & 255) << 8 | (uint32_t)(c & 255) << 16 | (uint32_t)d << 24;
+// The low bytes of four registers
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __builtin_amdgcn_perm(b, a, 0x0c0c0400u) | __builtin_amdgcn_perm(d, c, 0x04000c0cu);
 }
 
 // 1 / sqrt(ss / C + eps) from a row's sum of squares
@@ -202,11 +212,31 @@ __device__ __forceinline__ void store4f(float* to, int n, float4v v) {
             if (e < n) to[e] = v[e];
     }
 }
-__device__ __forceinline__ uint2v quant8(const float (&t)[8], float inv) {
-    int q[8];
+// 8 values of a row of largest magnitude a, inv = 127 / a, as the integers nearest to 127 t / a. |t| <= a bounds them by
+// 127, so t inv + 1.5 2^23, rounded once, has the integer nearest to t inv in its low byte. What may lie at a half
+// is looked at again: one value in 16000 does where values are spread. inv = 0 (a row of zeros) gives 0 also
+// for a t that is not finite.
+__device__ __forceinline__ uint2v quant8(const float (&t)[8], float a, float inv) {
+    constexpr float kUnits = 0x1.8p23f;  // its last bit is 1
+    uint32_t q[8];
+    float far = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q[e] = quant(t[e], inv);
-    return uint2v{pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7])};
+    for (int e = 0; e < 8; ++e) {
+        const float r = __builtin_fmaf(t[e], inv, kUnits);
+        q[e] = __builtin_bit_cast(uint32_t, r);
+        far = fmaxf(far, fabsf(__builtin_fmaf(t[e], inv, kUnits - r)));
+    }
+    if (__any(far > kNearHalf)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float n = __builtin_bit_cast(float, q[e]) - kUnits, f = __builtin_fmaf(t[e], inv, -n);
+            const uint32_t settled = (uint32_t)settle_half(t[e], a, n, f);
+            q[e] = fabsf(f) > kNearHalf ? settled : q[e];
+            __builtin_amdgcn_sched_barrier(0);  // one by one, in few registers
+        }
+    }
+    const uint2v words{pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7])};
+    return inv == 0.f ? uint2v{0, 0} : words;
 }
 
 // Sum and maximum over the threads of a block, for the kernels that take a row of any length.
@@ -297,8 +327,8 @@ __global__ __launch_bounds__(kAny) void rms_norm_any_kernel(RmsArgs a) {
         const float r = inv_rms(ss, a.inv_c, a.eps * d * d);
         if constexpr (Q8) {
             mt = block_max<kAny>(mt, uslot);
-            float inv, scale;
-            row_scale(mt, r, inv, scale);
+            float top, inv, scale;
+            row_scale(mt, r, top, inv, scale);
             if (threadIdx.x == 0) a.stat[row] = scale;
             for (int c = first; c < Kp; c += 8 * kAny) {
                 const half8 v = cut8(load8(vr, c, C), c, C);
@@ -306,7 +336,7 @@ __global__ __launch_bounds__(kAny) void rms_norm_any_kernel(RmsArgs a) {
                 float t[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) t[e] = act_get<BF>(v, e) * d * w[e];
-                *reinterpret_cast<uint2v*>(a.q + row * a.Kp + c) = quant8(t, inv);
+                *reinterpret_cast<uint2v*>(a.q + row * a.Kp + c) = quant8(t, top, inv);
             }
         } else {
             if (threadIdx.x == 0 && a.stat != nullptr) a.stat[row] = r * d;
@@ -381,8 +411,8 @@ __global__ __launch_bounds__(block_of(TPR)) void rms_norm_kernel(RmsArgs a) {
         }
         const float r = inv_rms(s.sum, a.inv_c, a.eps * d * d);
         if constexpr (Q8) {
-            float inv, scale;
-            row_scale(s.max1, r, inv, scale);
+            float top, inv, scale;
+            row_scale(s.max1, r, top, inv, scale);
             if (part == 0 && in) a.stat[row] = scale;
 #pragma unroll
             for (int j = 0; j < NCH; ++j) {
@@ -390,7 +420,7 @@ __global__ __launch_bounds__(block_of(TPR)) void rms_norm_kernel(RmsArgs a) {
                 float t[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) t[e] = act_get<BF>(v[j], e) * d * w[j][e];
-                if (in && col < Kp) *reinterpret_cast<uint2v*>(a.q + row * Kp + col) = quant8(t, inv);
+                if (in && col < Kp) *reinterpret_cast<uint2v*>(a.q + row * Kp + col) = quant8(t, top, inv);
             }
         } else {
             if (part == 0 && in && a.stat != nullptr) a.stat[row] = r * d;
@@ -688,12 +718,12 @@ __global__ __launch_bounds__(kAny) void quantize_any_kernel(QuantArgs a) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) m = max(m, abs_bits(h[e]));
         }
-        float inv, scale;
-        row_scale(block_max<kAny>(m, slot), 1.f, inv, scale);
+        float top, inv, scale;
+        row_scale(block_max<kAny>(m, slot), 1.f, top, inv, scale);
         if (threadIdx.x == 0) a.scale[row] = scale;
         for (int c = first; c < Kp; c += 8 * kAny) {
             hidden8<T, ACT>(a.x, at, c, K, h);
-            *reinterpret_cast<uint2v*>(a.q + row * a.Kp + c) = quant8(h, inv);
+            *reinterpret_cast<uint2v*>(a.q + row * a.Kp + c) = quant8(h, top, inv);
         }
     }
 }
@@ -732,13 +762,13 @@ __global__ __launch_bounds__(block_of(TPR)) void quantize_kernel(QuantArgs a) {
             }
         }
         s = row_all<TPR>(s, share, turn);
-        float inv, scale;
-        row_scale(s.max0, 1.f, inv, scale);
+        float top, inv, scale;
+        row_scale(s.max0, 1.f, top, inv, scale);
         if (part == 0 && in) a.scale[row] = scale;
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
             const int col = 8 * (part + TPR * j);
-            if (in && col < Kp) *reinterpret_cast<uint2v*>(a.q + row * Kp + col) = quant8(h[j], inv);
+            if (in && col < Kp) *reinterpret_cast<uint2v*>(a.q + row * Kp + col) = quant8(h[j], top, inv);
         }
     }
 }

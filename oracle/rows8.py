@@ -76,3 +76,16 @@ def project(q, sx, w, sw, b=None, residual=None):
             out = out + np.asarray(t, np.float64)
             mag = mag + np.abs(np.asarray(t, np.float64))
     return out, mag
+
+
+def nearest(t):
+    """127 t / a of rows t of fp32 values to the nearest integer, ties to even, without a rounding before it: 127 t and
+    (n + 1/2) a are exact in float64."""
+    t = np.asarray(t, np.float64)
+    a = np.abs(t).max(1, keepdims=True)
+    live = a >= TINY
+    num, a = np.where(live, 127.0 * t, 0.0), np.where(live, a, 1.0)
+    n = np.rint(num / a)
+    odd = n % 2 == 1
+    up, down = num - (n + 0.5) * a, num - (n - 0.5) * a
+    return n + ((up > 0) | (odd & (up == 0))) - ((down < 0) | (odd & (down == 0)))

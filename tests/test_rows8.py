@@ -381,3 +381,21 @@ def test_residuals_of_another_shape_are_refused():
     for other in ((3, 2, 8), (1, 6, 8), (2, 3, 9), (2, 3, 64)):
         with pytest.raises(H.InvalidArgument, match="residual must be like the result"):
             torch_ops.q8_projection(q, s, weights, residual=torch.zeros(other, dtype=torch.float16))
+
+
+def test_nearest():
+    """Against Python's fractions: values on and next to halves, one of the tiniest rows, one too tiny, zeros."""
+    from fractions import Fraction
+    rng = np.random.default_rng(5)
+    a = (rng.uniform(1, 2, (40, 1)) * 2.0 ** rng.integers(-118, 120, (40, 1))).astype(np.float32)
+    t = (a.astype(np.float64) * (2 * rng.integers(-127, 127, (40, 50)) + 1) / 254).astype(np.float32)
+    t = (t.view(np.int32) + rng.integers(-2, 3, t.shape).astype(np.int32)).view(np.float32)
+    t[:, 0], t[:, 1], t[:, 2] = a[:, 0], a[:, 0] / 2, -a[:, 0] / 2
+    t[3] *= np.float32(2.0 ** -119) / a[3, 0]
+    t[4] *= np.float32(2.0 ** -121) / a[4, 0]
+    t[5] = 0
+    got = orr.nearest(t)
+    for row, q in zip(t, got):
+        top = max(Fraction(abs(float(v))) for v in row)
+        for v, n in zip(row, q):
+            assert n == (round(127 * Fraction(float(v)) / top) if top >= Fraction(2) ** -119 else 0)

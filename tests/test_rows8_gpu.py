@@ -371,3 +371,58 @@ def test_offsets_past_2_31(hip):
     ds, _ = hip.rms_norm_bwd(x, w, rstd, x)
     ds1, _ = hip.rms_norm_bwd(y1, w, rstd1, y1)
     assert torch.equal(ds[-3:], ds1)
+
+
+# ---- the integers themselves, against 127 t / a without a rounding before the nearest ---------------
+
+def check_nearest(q, t):
+    """q's first columns are the nearest integers to 127 t / a, bit for bit (t: fp32 values)."""
+    assert np.array_equal(q.cpu().numpy()[:, :t.shape[1]].astype(np.float64), orr.nearest(t))
+
+
+def norm_products(x, w):
+    return (x.float().cpu().numpy() * w.cpu().numpy()[None]).astype(np.float64)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("c", [13, 64, 512, 1000, 2050, 8200, 16384, 20001])
+def test_nearest_integers(hip, c, kind):
+    for m in (3, 4000000 // c // 8):
+        x, res, w = inputs(m, c, kind, kind != "f32", seed=11)
+        for act in (0, 1):
+            check_nearest(hip.quantize_rows(x, act)[0], orr.hidden(host(x), act))
+        if kind != "f32":
+            check_nearest(hip.rms_norm_q8(x, w)[0], norm_products(x, w))
+            q, _, total = hip.rms_norm_q8(x, w, res)
+            check_nearest(q, norm_products(total, w))
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_half_of_the_largest(hip, kind):
+    """t = a / 2, so 127 t / a = 63.5, for every 16-bit a above the type's smallest hundred: 64, whatever 127 / a rounds
+    to; and a row of both signs."""
+    bits = torch.arange(101 if kind == "f16" else 0x500, int(torch.tensor(float("inf"), dtype=DT[kind]).view(torch.int16)),
+                        dtype=torch.int16)
+    a = bits.view(DT[kind])
+    x = torch.stack([a, a / 2, -a / 2, -a, a / 4, torch.zeros_like(a)], 1).cuda()
+    x = x[(x[:, 1] * 2 == x[:, 0]) & (x[:, 0] >= 2.0 ** -119)]
+    q, _ = hip.quantize_rows(x)
+    assert len(x) > 20000 and (q[:, :4].cpu() == torch.tensor([127, 64, -64, -127])).all()
+    check_nearest(q, host(x))
+    check_nearest(hip.rms_norm_q8(x, torch.ones(6, device="cuda"))[0], host(x))
+
+
+@pytest.mark.parametrize("k", [61, 1000, 9000, 40000])
+@pytest.mark.parametrize("low,high", [(-10, 10), (-118, -100), (110, 127), (-119, 127)])
+def test_next_to_halves(hip, k, low, high):
+    """fp32 values on, and up to three steps beside, the halves of a row's scale."""
+    rng = np.random.default_rng(k + 300 + low)
+    m = 200000 // k + 1
+    a = (rng.uniform(1, 2, (m, 1)) * 2.0 ** rng.integers(low, high + 1, (m, 1))).astype(np.float32)
+    t = (a.astype(np.float64) * (2 * rng.integers(-127, 127, (m, k)) + 1) / 254).astype(np.float32)
+    t = (t.view(np.int32) + rng.integers(-3, 4, (m, k)).astype(np.int32)).view(np.float32)
+    t[:, 0] = a[:, 0]
+    t[:, k // 2] = -a[:, 0] / 2
+    assert np.abs(t).max() < np.inf and (np.abs(t).max(1) == a[:, 0]).all()
+    q, _ = hip.quantize_rows(torch.from_numpy(t).cuda())
+    check_nearest(q, t)
