@@ -79,6 +79,13 @@ __device__ __forceinline__ float row_shift(uint32_t bits, float eps) {
     return a >= 0x1p40f ? 0x1p-90f : a < 0x1p-40f && eps < 0x1p-100f ? 0x1p90f : 1.f;
 }
 
+// Whether a row taken times d is turned to 8 bits from its values as they are: huge ones whose products with w, of largest
+// magnitude `bits` as they were taken, would lose low bits (or, under 2^-119, the row) by that. Those products
+// are under 1 without d, and the scale is multiplied by d in the end.
+__device__ __forceinline__ bool as_they_are(float d, uint32_t bits) {
+    return d < 1.f && __builtin_bit_cast(float, bits) < 0x1p-90f;
+}
+
 // v of the lane that DPP control CTRL names
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp(uint32_t v) {
@@ -318,6 +325,7 @@ __global__ __launch_bounds__(kAny) void rms_norm_any_kernel(RmsArgs a) {
         ss = block_sum<kAny>(ss, fslot);
         m = block_max<kAny>(m, uslot);
         const float d = BF ? row_shift(m, a.eps) : 1.f;
+        const uint32_t plain = mt;
         if (d != 1.f) {
             ss = 0.f;
             mt = 0;
@@ -327,15 +335,19 @@ __global__ __launch_bounds__(kAny) void rms_norm_any_kernel(RmsArgs a) {
         const float r = inv_rms(ss, a.inv_c, a.eps * d * d);
         if constexpr (Q8) {
             mt = block_max<kAny>(mt, uslot);
-            float top, inv, scale;
+            float dt = d, top, inv, scale;
+            if (as_they_are(d, mt)) {
+                dt = 1.f;
+                mt = block_max<kAny>(plain, uslot);
+            }
             row_scale(mt, r, top, inv, scale);
-            if (threadIdx.x == 0) a.stat[row] = scale;
+            if (threadIdx.x == 0) a.stat[row] = dt == d ? scale : scale * d;
             for (int c = first; c < Kp; c += 8 * kAny) {
                 const half8 v = cut8(load8(vr, c, C), c, C);
                 const float8v w = load8f(a.w, c, C);
                 float t[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) t[e] = act_get<BF>(v, e) * d * w[e];
+                for (int e = 0; e < 8; ++e) t[e] = act_get<BF>(v, e) * dt * w[e];
                 *reinterpret_cast<uint2v*>(a.q + row * a.Kp + c) = quant8(t, top, inv);
             }
         } else {
@@ -404,22 +416,30 @@ __global__ __launch_bounds__(block_of(TPR)) void rms_norm_kernel(RmsArgs a) {
             s = row_all<TPR>(s, share, turn);
         };
         collect(1.f);
-        float d = 1.f;
+        float d = 1.f, dt = 1.f;  // of the squares and results, of the products that go to 8 bits
         if constexpr (BF) {
             d = row_shift(s.max0, a.eps);
-            if (d != 1.f) collect(d);
+            if (d != 1.f) {
+                const uint32_t plain = s.max1;
+                collect(d);
+                dt = d;
+                if (Q8 && as_they_are(d, s.max1)) {
+                    dt = 1.f;
+                    s.max1 = plain;
+                }
+            }
         }
         const float r = inv_rms(s.sum, a.inv_c, a.eps * d * d);
         if constexpr (Q8) {
             float top, inv, scale;
             row_scale(s.max1, r, top, inv, scale);
-            if (part == 0 && in) a.stat[row] = scale;
+            if (part == 0 && in) a.stat[row] = dt == d ? scale : scale * d;
 #pragma unroll
             for (int j = 0; j < NCH; ++j) {
                 const int col = 8 * (part + TPR * j);
                 float t[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) t[e] = act_get<BF>(v[j], e) * d * w[j][e];
+                for (int e = 0; e < 8; ++e) t[e] = act_get<BF>(v[j], e) * dt * w[j][e];
                 if (in && col < Kp) *reinterpret_cast<uint2v*>(a.q + row * Kp + col) = quant8(t, top, inv);
             }
         } else {

@@ -220,7 +220,8 @@ int clk_opm_outer(clk_stream stream, const clk_buffer* left, const clk_buffer* r
  * the columns past K zero; column k of row r stands for q[r,k] * scale[r]. A row is quantised by its
  * largest magnitude a: q = 127 t / a to the nearest integer (ties to even) and scale = a / 127, so q lies
  * in -127..127. A row whose a is under 2^-119 (its scale would leave fp32's normal range) is all
- * zeros with scale 0; a row that holds an infinity or NaN is all zeros with scale NaN. */
+ * zeros with scale 0; a row that holds an infinity or NaN is all zeros with scale NaN. (A norm's bf16 row
+ * of values under 2^-40 with eps under 2^-100, which is taken times 2^90, is zeros under 2^-209 only.) */
 
 /* out [M,C] = s / sqrt(mean(s^2) + eps) * scale over the last axis, with s = x, or with has_residual
  * s = x + residual rounded to the activation type, which is also written to sum [M,C] (the residual

@@ -426,3 +426,24 @@ def test_next_to_halves(hip, k, low, high):
     assert np.abs(t).max() < np.inf and (np.abs(t).max(1) == a[:, 0]).all()
     q, _ = hip.quantize_rows(torch.from_numpy(t).cuda())
     check_nearest(q, t)
+
+
+@pytest.mark.parametrize("c", [13, 128, 1000, 9000, 40000])
+@pytest.mark.parametrize("wexp", [-50, -80, -100, -126, -150])
+def test_huge_rows_of_tiny_weights(hip, c, wexp):
+    """bf16 rows past 2^40 times weights of any size: a row is zeros where its own largest product is under 2^-119, not
+    where that of the values as they are taken for their squares is."""
+    x, _, w = inputs(6, c, "bf16", False)
+    x = x * 2.0 ** 60
+    x[1] = x[1] * 2.0 ** 60
+    w = w * 2.0 ** (wexp / 2) * 2.0 ** (wexp / 2)
+    x[2] = 0
+    x[2, 0] = 2.0 ** 41
+    q, qs, _ = hip.rms_norm_q8(x, w)
+    t = norm_products(x, w)
+    check_nearest(q, t)
+    quot, scale = orr.quotients(t)
+    assert wexp < -126 or (np.abs(quot).max(1) == 127).all()
+    want = scale * orr.rms_norm(host(x), host(w), 1e-5)[1]
+    # below fp32's normal range a scale is off by half its smallest step
+    assert (np.abs(host(qs) - want) <= (12 + seq(c)) * E * want + 2.0 ** -150).all()
