@@ -447,3 +447,48 @@ def test_huge_rows_of_tiny_weights(hip, c, wexp):
     want = scale * orr.rms_norm(host(x), host(w), 1e-5)[1]
     # below fp32's normal range a scale is off by half its smallest step
     assert (np.abs(host(qs) - want) <= (12 + seq(c)) * E * want + 2.0 ** -150).all()
+
+
+@pytest.mark.parametrize("m,c", [((1 << 25) + 5, 1), ((1 << 20) + 3, 1025)])
+def test_more_rows_than_a_grid_takes(hip, m, c):
+    """A grid has at most 2^20 workgroups (of 32 rows each where rows are shortest): the rows past it are their second
+    ones. Every row is compared with the same row in calls that fit a grid."""
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    x = torch.empty((m, c), dtype=torch.bfloat16, device="cuda").normal_(generator=gen)
+    w = torch.ones(c, device="cuda").normal_(generator=gen)
+    y, total, rstd = hip.rms_norm(x, w, x, want_rstd=True)
+    q, qs, _ = hip.rms_norm_q8(x, w)
+    h, hs = hip.quantize_rows(x, 1)
+    v = hip.dequantize_rows(h, hs, c)
+    step = m // 3 + 1
+    for lo in range(0, m, step):
+        part = x[lo:lo + step]
+        y1, total1, rstd1 = hip.rms_norm(part, w, part, want_rstd=True)
+        q1, qs1, _ = hip.rms_norm_q8(part, w)
+        h1, hs1 = hip.quantize_rows(part, 1)
+        v1 = hip.dequantize_rows(h1, hs1, c)
+        for whole, alone in ((y, y1), (total, total1), (rstd, rstd1), (q, q1), (qs, qs1), (h, h1), (hs, hs1), (v, v1)):
+            assert torch.equal(whole[lo:lo + step], alone)
+    last = slice(m - 70, m)
+    check_norm(y[last], rstd[last], host(total[last]), w, 1e-5, "bf16")
+    check_nearest(q[last], norm_products(x[last], w))
+
+
+def test_more_long_rows_than_a_grid_takes(hip):
+    """The same for the rows of any length, 34 GB of them: the last five against calls of their own."""
+    m, c = (1 << 20) + 5, 16385
+    x = torch.ones((m, c), dtype=torch.bfloat16, device="cuda")
+    tail, _, w = inputs(8, c, "bf16", False)
+    x[-8:] = tail
+    q, qs = hip.quantize_rows(x)
+    q1, qs1 = hip.quantize_rows(tail)
+    assert torch.equal(q[-8:], q1) and torch.equal(qs[-8:], qs1) and torch.equal(q[3], q[m - 9])
+    hip.rms_norm_q8(x, w, q=q, q_scale=qs)
+    q1, qs1, _ = hip.rms_norm_q8(tail, w)
+    assert torch.equal(q[-8:], q1) and torch.equal(qs[-8:], qs1) and torch.equal(q[3], q[m - 9])
+    del q
+    y1, _, rstd1 = hip.rms_norm(tail, w, want_rstd=True)
+    _, _, rstd = hip.rms_norm(x, w, want_rstd=True, out=x)
+    assert torch.equal(x[-8:], y1) and torch.equal(rstd[-8:], rstd1) and torch.equal(x[3], x[m - 9])
+    del x
+    torch.cuda.empty_cache()
