@@ -409,3 +409,39 @@ def test_backward_of_an_eager_forward_is_refused_under_capture(hip):
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(captured, torch_ops.rms_norm(static, w))
+
+
+def cancelling(m, k, n, turns):
+    """Rows and weights of [m, k] and [n, k] whose products add up to millions above 2^24, all of them again below zero, and
+    the product of two small odd numbers, which 16 bits hold. The two lie in k's two halves, or (turns) 64 inputs by
+    64 in turn, so that one of them is all that some parts of a divided sum have."""
+    rng = np.random.default_rng(m + k + n)
+    h = k // 2
+    row, chan = 2 * rng.integers(0, 8, m) + 1, (2 * rng.integers(0, 8, n) + 1) * rng.choice((-1, 1), n)
+    q = torch.from_numpy(rng.integers(64, 128, (m, h)).astype(np.int8)).cuda()
+    q[:, -1] = torch.from_numpy(row.astype(np.int8))
+    w = torch.from_numpy(rng.integers(64, 128, (n, h)).astype(np.int8)).cuda()
+    w[:, -1] = 0
+    less = -w
+    less[:, -1] = torch.from_numpy(chan.astype(np.int8))
+
+    def join(a, b):
+        if turns:
+            return torch.stack([a.view(len(a), -1, 64), b.view(len(a), -1, 64)], 2).reshape(len(a), k)
+        return torch.cat([a, b], 1)
+    return join(q, q).contiguous(), join(w, less).contiguous(), torch.from_numpy(np.outer(row, chan)).cuda()
+
+
+@pytest.mark.parametrize("turns", [False, True])
+@pytest.mark.parametrize("m,k,n", [(1, 16384, 70), (4, 130944, 70), (9, 16384, 70), (16, 130944, 70), (20, 16384, 70), (33, 16384, 130),
+                                   (64, 130944, 70), (20, 16384, 4200), (40, 16384, 4200), (60, 16384, 4200),
+                                   (70, 16384, 70), (300, 130944, 70), (700, 16384, 1100), (1531, 16384, 2050),
+                                   (2304, 16384, 4608)])
+def test_sums_that_cancel_are_exact(hip, m, k, n, turns):
+    """A sum in floating point, or one that is rounded to it before its parts are joined, is off by a few here."""
+    q, w, want = cancelling(m, k, n, turns)
+    ones = lambda r: torch.ones(r, device="cuda")  # noqa: E731
+    wq = layouts.q8_blocked(w)
+    for kind in ("f16", "bf16"):
+        out = hip.q8_projection(q, ones(m), wq, ones(n), dtype=DT[kind])
+        assert torch.equal(out, want.to(DT[kind]))
