@@ -414,7 +414,7 @@ __device__ __forceinline__ uint4v words_of(const P* p, uint32_t bytes) {
 __device__ __forceinline__ void dma_lds_untracked(uint4v rsrc, void* dst, uint32_t off) {
 #ifdef __HIP_DEVICE_COMPILE__
     const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)dst;
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc) : "memory", "m0");
 #else
     (void)rsrc, (void)dst, (void)off;
 #endif

@@ -399,3 +399,20 @@ def test_nearest():
         top = max(Fraction(abs(float(v))) for v in row)
         for v, n in zip(row, q):
             assert n == (round(127 * Fraction(float(v)) / top) if top >= Fraction(2) ** -119 else 0)
+
+
+def test_inline_assembly_names_the_m0_that_it_writes():
+    """m0 is the compiler's too (it holds the LDS address of the direct-to-LDS builtin, and lane indices): a block that
+    writes it has to say so."""
+    import glob
+    import os
+    import re
+    import build as pkg_build
+    writers = 0
+    for path in glob.glob(os.path.join(pkg_build.CSRC, "*.h*")):
+        for text in re.findall(r"asm(?:\s+volatile)?\s*\((.*?)\);", open(path).read(), re.S):
+            code, _, rest = text.partition("::") if "::" in text else text.partition(" :")
+            if re.search(r"\bs_\w+ m0\b", code):
+                writers += 1
+                assert '"m0"' in rest, os.path.basename(path)
+    assert writers == 1
