@@ -222,14 +222,15 @@ class _RmsNorm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, scale, residual, eps):
-        x2 = _matrix(x)
-        out = x2.new_empty(x.shape)  # of the results' own shape: a view of a result could not be changed in place
-        total = None if residual is None else x2.new_empty(x.shape)
-        _, _, rstd = hip.rms_norm(x2, scale, None if residual is None else _matrix(residual), eps, want_rstd=True,
-                                  out=_matrix(out), sum_out=None if residual is None else _matrix(total))
+        x = x.contiguous()
+        out, total = torch.empty_like(x), None  # of x's own shape: a view as a result could not be changed in place
+        if residual is None:
+            _, _, rstd = hip.rms_norm(_matrix(x), scale, None, eps, True, _matrix(out))
+        else:
+            total = torch.empty_like(x)
+            _, _, rstd = hip.rms_norm(_matrix(x), scale, _matrix(residual), eps, True, _matrix(out), _matrix(total))
         ctx.set_materialize_grads(False)
-        ctx.shape = x.shape
-        ctx.save_for_backward(x2 if residual is None else total, scale, rstd)
+        ctx.save_for_backward(x if residual is None else total, scale, rstd)
         return out if residual is None else (out, total)
 
     @staticmethod
@@ -241,7 +242,7 @@ class _RmsNorm(torch.autograd.Function):
         if dout is None:  # only the sum was used
             ds, dscale = dsum, torch.zeros_like(scale)
         else:
-            ds, dscale = s.new_empty(ctx.shape), torch.empty_like(scale)
+            ds, dscale = torch.empty_like(s), torch.empty_like(scale)
             hip.rms_norm_bwd(_matrix(s), scale, rstd, _matrix(dout.to(s.dtype)), None if dsum is None else _matrix(dsum),
                              grads=(_matrix(ds), dscale))
         need = ctx.needs_input_grad
@@ -264,7 +265,7 @@ def rms_norm(x, scale, residual=None, eps=1e-5):
     if differentiated:
         _refuse_capture(x)
     w = scale.float().contiguous()
-    if differentiated or any(_has_tangent(t) for t in (x, scale, residual)):
+    if differentiated or _any_tangent(x, scale, residual):
         return _RmsNorm.apply(x, w, residual, float(eps))
     out, total, _ = hip.rms_norm(_matrix(x), w, None if residual is None else _matrix(residual), eps)
     if x.dim() != 2:
@@ -297,10 +298,12 @@ def _refuse_capture(t):
                                   "graph; capture hip.rms_norm and hip.rms_norm_bwd")
 
 
-def _has_tangent(t):
-    """Whether t is a dual tensor of the open forward-mode level: the autograd node refuses those, which have
-    no requires_grad"""
-    return t is not None and forward_ad.unpack_dual(t).tangent is not None
+def _any_tangent(*tensors):
+    """Whether one of them is a dual tensor of the open forward-mode level: the autograd node refuses those,
+    which have no requires_grad. (Three looks with no level open are 1 us of a call's 9: the level first, where
+    torch has it under this name.)"""
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _matrix(x):
