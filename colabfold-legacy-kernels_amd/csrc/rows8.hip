@@ -219,27 +219,48 @@ __device__ __forceinline__ void store4f(float* to, int n, float4v v) {
             if (e < n) to[e] = v[e];
     }
 }
-// 8 values of a row of largest magnitude a, inv = 127 / a, as the integers nearest to 127 t / a. |t| <= a bounds them by
-// 127, so t inv + 1.5 2^23, rounded once, has the integer nearest to t inv in its low byte. What may lie at a half
-// is looked at again: one value in 16000 does where values are spread. inv = 0 (a row of zeros) gives 0 also
-// for a t that is not finite.
+// 8 values of a row of largest magnitude a, inv = 127 / a, as the integers nearest to 127 t / a, ties to even. |t| <= a
+// bounds them by 127, and the sum of one with 1.5 2^23 is rounded to integers and has them in its low byte.
+// inv = 0 (a row of zeros) gives 0 also for a t that is not finite.
+//
+// Values and a of 16 bits (IN16): 127 t / a lies on a half or, t being 2^i times an integer T < 2^11, at least 1 / (254
+// T) > 2^-19 of itself away from it, so the quotient rounded to fp32 (t inv, and t times what inv lacks, in one
+// fma) is on the same side, or on the half.
+// Other values: what may lie at a half is looked at again, one value in 16000 where they are spread. Half of a,
+// which values made of 16-bit ones hit far more often, is 63.5, so 64. (The norm of [4099, 5120] bf16 with weights
+// of 1 takes 28 us; 31 with that half settled like the others, 26.5 with halves as t inv has them.)
+template <bool IN16>
 __device__ __forceinline__ uint2v quant8(const float (&t)[8], float a, float inv) {
-    constexpr float kUnits = 0x1.8p23f;  // its last bit is 1
+    constexpr float kUnits = 0x1.8p23f;
     uint32_t q[8];
-    float far = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float r = __builtin_fmaf(t[e], inv, kUnits);
-        q[e] = __builtin_bit_cast(uint32_t, r);
-        far = fmaxf(far, fabsf(__builtin_fmaf(t[e], inv, kUnits - r)));
-    }
-    if (__any(far > kNearHalf)) {
+    if constexpr (IN16) {
+        const float lacks = __builtin_fmaf(-inv, a, 127.f) * inv * (1.f / 127.f);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float n = __builtin_bit_cast(float, q[e]) - kUnits, f = __builtin_fmaf(t[e], inv, -n);
-            const uint32_t settled = (uint32_t)settle_half(t[e], a, n, f);
-            q[e] = fabsf(f) > kNearHalf ? settled : q[e];
-            __builtin_amdgcn_sched_barrier(0);  // one by one, in few registers
+            q[e] = __builtin_bit_cast(uint32_t, __builtin_fmaf(t[e], inv, t[e] * lacks) + kUnits);
+        }
+    } else {
+        uint64_t near[8], any = 0;  // the lanes whose value e may lie at a half
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float r = __builtin_fmaf(t[e], inv, kUnits);
+            q[e] = __builtin_bit_cast(uint32_t, r);
+            near[e] = __ballot(fabsf(__builtin_fmaf(t[e], inv, kUnits - r)) > kNearHalf);
+            any |= near[e];
+        }
+        if (any != 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (near[e] == 0) continue;
+                const uint64_t half = __ballot(fabsf(t[e]) == 0.5f * a);
+                if ((near[e] & ~half) != 0) {
+                    const float n = __builtin_bit_cast(float, q[e]) - kUnits;
+                    const float f = __builtin_fmaf(t[e], inv, -n);
+                    const uint32_t settled = (uint32_t)settle_half(t[e], a, n, f);
+                    q[e] = fabsf(f) > kNearHalf ? settled : q[e];
+                }
+                if (fabsf(t[e]) == 0.5f * a) q[e] = t[e] < 0.f ? (uint32_t)-64 : 64u;
+            }
         }
     }
     const uint2v words{pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7])};
@@ -287,7 +308,7 @@ struct RmsArgs {
 constexpr int kAny = 1024;  // threads of the kernels for rows of any length
 
 // Rows of any length (past 16384 values): a block a row, two passes over it (the second from cache where it fits).
-// [1024, 40000] bf16 with the residual 73 us (328 MB, 4.5 TB/s), as 8-bit rows 71; [4096, 20000] 149 and 155, where
+// [1024, 40000] bf16 with the residual 73 us (328 MB, 4.5 TB/s), as 8-bit rows 70; [4096, 20000] 149 and 155, where
 // 1024 threads with 4 chunks of a row in registers take 222 and 536 (they spill).
 template <bool BF, bool RES, bool Q8>
 __global__ __launch_bounds__(kAny) void rms_norm_any_kernel(RmsArgs a) {
@@ -348,7 +369,7 @@ __global__ __launch_bounds__(kAny) void rms_norm_any_kernel(RmsArgs a) {
                 float t[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) t[e] = act_get<BF>(v, e) * dt * w[e];
-                *reinterpret_cast<uint2v*>(a.q + row * a.Kp + c) = quant8(t, top, inv);
+                *reinterpret_cast<uint2v*>(a.q + row * a.Kp + c) = quant8<false>(t, top, inv);
             }
         } else {
             if (threadIdx.x == 0 && a.stat != nullptr) a.stat[row] = r * d;
@@ -366,7 +387,7 @@ __global__ __launch_bounds__(kAny) void rms_norm_any_kernel(RmsArgs a) {
 
 // Rows of up to 8 TPR NCH values, held in registers: TPR threads a row, NCH chunks each, one pass over memory,
 // which bounds it. [16384, 8192] bf16 with the residual: 176 us (1.07 GB, 6.1 TB/s); [147456, 128] fp16: 13.8 us
-// (5.5 TB/s); 8-bit rows of [4099, 5120] bf16 with the residual: 27 us (5.4 TB/s).
+// (5.5 TB/s); 8-bit rows of [4099, 5120] bf16 with the residual: 28 us (5.2 TB/s).
 constexpr int block_of(int tpr) { return tpr < 256 ? 256 : tpr; }
 
 template <bool BF, int TPR, int NCH, bool RES, bool Q8>
@@ -440,7 +461,7 @@ __global__ __launch_bounds__(block_of(TPR)) void rms_norm_kernel(RmsArgs a) {
                 float t[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) t[e] = act_get<BF>(v[j], e) * dt * w[j][e];
-                if (in && col < Kp) *reinterpret_cast<uint2v*>(a.q + row * Kp + col) = quant8(t, top, inv);
+                if (in && col < Kp) *reinterpret_cast<uint2v*>(a.q + row * Kp + col) = quant8<false>(t, top, inv);
             }
         } else {
             if (part == 0 && in && a.stat != nullptr) a.stat[row] = r * d;
@@ -724,7 +745,7 @@ __device__ __forceinline__ void hidden8(const void* x, int64_t at, int c, int K,
     }
 }
 
-// Rows of any length, read twice. [1024, 40000] bf16: 30 us (123 MB, 4.1 TB/s).
+// Rows of any length, read twice. [1024, 40000] bf16: 28 us (123 MB, 4.4 TB/s).
 template <int T, int ACT>
 __global__ __launch_bounds__(kAny) void quantize_any_kernel(QuantArgs a) {
     __shared__ uint32_t slot[kAny / kWave];
@@ -743,13 +764,14 @@ __global__ __launch_bounds__(kAny) void quantize_any_kernel(QuantArgs a) {
         if (threadIdx.x == 0) a.scale[row] = scale;
         for (int c = first; c < Kp; c += 8 * kAny) {
             hidden8<T, ACT>(a.x, at, c, K, h);
-            *reinterpret_cast<uint2v*>(a.q + row * a.Kp + c) = quant8(h, top, inv);
+            *reinterpret_cast<uint2v*>(a.q + row * a.Kp + c) = quant8<T != kF32 && ACT != kActSwish>(h, top, inv);
         }
     }
 }
 
 // As the norm: a row in registers, bound by memory. relu of [147456, 512] fp16: 45 to 54 us (227 MB, 4.2 to 5.0 TB/s;
-// the less of it is left in the far cache by what ran before, the more).
+// the less of it is left in the far cache by what ran before, the more); swish gate of [147456, 2 x 512] fp16 67 us (378
+// MB, 5.6 TB/s), [147456, 512] fp32 64 us (378 MB, 5.9 TB/s).
 template <int T, int ACT, int TPR, int NCH>
 __global__ __launch_bounds__(block_of(TPR)) void quantize_kernel(QuantArgs a) {
     constexpr int ROWS = block_of(TPR) / TPR;
@@ -788,7 +810,7 @@ __global__ __launch_bounds__(block_of(TPR)) void quantize_kernel(QuantArgs a) {
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
             const int col = 8 * (part + TPR * j);
-            if (in && col < Kp) *reinterpret_cast<uint2v*>(a.q + row * Kp + col) = quant8(h[j], top, inv);
+            if (in && col < Kp) *reinterpret_cast<uint2v*>(a.q + row * Kp + col) = quant8<T != kF32 && !GATE>(h[j], top, inv);
         }
     }
 }

@@ -5,11 +5,13 @@ Written from the definitions; the operators have no counterpart in the reference
   rms_norm_bwd   g = dy w, xh = s r: ds = r (g - xh mean(g xh)) + dsum, dw = sum over rows of dy xh
   quotients      127 t / a of each row t with largest magnitude a: 8-bit rows hold its nearest
                  integers, and a / 127 as their scale
+  nearest        those integers of fp32 values, ties to even, exactly
   hidden         x, relu(x), or swish of x's first half times its second
   project        (q w^T) sx sw + b + residual, the sum of integers exact
 
 Pinned by (tests/test_rows8.py): the gradients against central differences of rms_norm, the rounding to
-16 bits against torch's conversions, and the matrix product against an explicit sum.
+16 bits against torch's conversions, the matrix product against an explicit sum and the
+nearest integers against fractions.
 """
 import numpy as np
 
