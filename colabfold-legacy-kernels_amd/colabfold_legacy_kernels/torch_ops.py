@@ -223,12 +223,13 @@ class _RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, scale, residual, eps):
         x = x.contiguous()
-        out, total = torch.empty_like(x), None  # of x's own shape: a view as a result could not be changed in place
-        if residual is None:
-            _, _, rstd = hip.rms_norm(_matrix(x), scale, None, eps, True, _matrix(out))
-        else:
-            total = torch.empty_like(x)
-            _, _, rstd = hip.rms_norm(_matrix(x), scale, _matrix(residual), eps, True, _matrix(out), _matrix(total))
+        residual = None if residual is None else residual.contiguous()
+        if x.dim() == 2:
+            out, total, rstd = hip.rms_norm(x, scale, residual, eps, True)
+        else:  # results of x's own shape: as views of rows they could not be changed in place
+            out, total = torch.empty_like(x), None if residual is None else torch.empty_like(x)
+            rstd = hip.rms_norm(_matrix(x), scale, None if residual is None else _matrix(residual), eps, True,
+                                _matrix(out), None if residual is None else _matrix(total))[2]
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x if residual is None else total, scale, rstd)
         return out if residual is None else (out, total)
@@ -242,9 +243,13 @@ class _RmsNorm(torch.autograd.Function):
         if dout is None:  # only the sum was used
             ds, dscale = dsum, torch.zeros_like(scale)
         else:
-            ds, dscale = torch.empty_like(s), torch.empty_like(scale)
-            hip.rms_norm_bwd(_matrix(s), scale, rstd, _matrix(dout.to(s.dtype)), None if dsum is None else _matrix(dsum),
-                             grads=(_matrix(ds), dscale))
+            dout = dout.to(s.dtype).contiguous()
+            if s.dim() == 2:
+                ds, dscale = hip.rms_norm_bwd(s, scale, rstd, dout, dsum)
+            else:
+                ds, dscale = torch.empty_like(s), torch.empty_like(scale)
+                hip.rms_norm_bwd(_matrix(s), scale, rstd, _matrix(dout), None if dsum is None else _matrix(dsum),
+                                 grads=(_matrix(ds), dscale))
         need = ctx.needs_input_grad
         return ds if need[0] else None, dscale if need[1] else None, ds if need[2] else None, None
 
