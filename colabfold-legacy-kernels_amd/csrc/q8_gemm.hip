@@ -217,7 +217,7 @@ __global__ __launch_bounds__(256) void q8_rows_kernel(GemmArgs a) {
 //   rows     16 rows of 64 bytes a load, position p of row r holding its 16-byte chunk p ^ swizzle(r). (Loaded
 //            straight in operand order, 16 bytes of 16 rows after each other, the same kilobyte takes three times
 //            as long: 16 bytes a clock and CU against 44.)
-// Large products are bound by power: 8192 x 8192 x 8192 with a residual takes 416 to 445 us (2.47 to 2.64 POP/s), machine
+// Large products are bound by power: 8192 x 8192 x 8192 with a residual takes 426 to 462 us (2.38 to 2.58 POP/s), machine
 // by machine, with the matrix cores busy for 75% of the cycles at 1.64 to 1.77 GHz (2.4 in kernels that memory
 // bounds). Few rows are bound by the weights' reading (48 x 4096 x 8192: 8.7 us, 34 MB at 3.9 TB/s), medium ones
 // by the fill and tail of one round of workgroups (1531 x 1100 x 2050 with a residual: 10.6 us, 0.65 POP/s).
