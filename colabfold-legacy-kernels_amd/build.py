@@ -33,7 +33,7 @@ HIP_FLAGS = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=" + ARCH,
 # The 8-bit path's results do not depend on the kernel that a call's size picks. Without this the compiler rounds some
 # products and fmas to fp16 at once (v_fma_mixlo_f16) and others to fp32 first, lane by lane as it likes.
 ONE_ROUNDING = ["-Xclang", "-target-feature", "-Xclang", "-fma-mix-insts"]
-SOURCE_FLAGS = {"q8_gemm.hip": ONE_ROUNDING, "rows8.hip": ONE_ROUNDING}
+SOURCE_FLAGS = {"q8_gemm.hip": ONE_ROUNDING, "rows8.hip": ONE_ROUNDING, "heads.hip": ONE_ROUNDING}
 
 
 def hipcc():

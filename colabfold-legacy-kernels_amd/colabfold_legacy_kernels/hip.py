@@ -19,6 +19,10 @@ and, without a counterpart in the reference, the RMS norm and the 8-bit serving 
   rms_norm_q8                 the same norm with 8-bit rows as its result
   quantize_rows, dequantize_rows  8-bit rows of a matrix (or of its relu or swish gate), and back
   q8_projection               8-bit rows times 8-bit weights, scales, bias and residual
+  qk_norm_rope, qk_norm_rope_bwd  RMS norm of each query and key head with the position rotation, and its gradients
+  qk_norm_rope_cache          the same with keys and values written into a paged cache, in 16 or 8 bits
+  kv_cache, kv_cache_write, kv_cache_read  that cache, and keys and values into it and back
+  paged_attention             one new token's attention over the cache
 
 Results are allocated here with torch (as XLA preallocates them) unless passed in, which is how a
 caller aliases an output to its residual / input. The fused ops take fp16 or bf16 activations
@@ -27,6 +31,7 @@ back in the activation type. A rejected call raises InvalidArgument (the
 FFI's InvalidArgument) and a launch failure KernelError (Internal), with the library's message.
 There is no CPU fallback: without the built library every call raises.
 """
+import collections
 import ctypes
 import functools
 import struct
@@ -89,6 +94,14 @@ _SIGNATURES = {
     "clk_quantize_rows": [ctypes.c_void_p] + [_P] * 3 + [ctypes.c_int64],
     "clk_dequantize_rows": [ctypes.c_void_p] + [_P] * 3,
     "clk_q8_projection": [ctypes.c_void_p] + [_P] * 7 + [ctypes.c_int32, ctypes.c_int32],
+    "clk_qk_norm_rope": [ctypes.c_void_p] + [_P] * 8 + [ctypes.c_float, ctypes.c_int32],
+    "clk_qk_norm_rope_bwd": [ctypes.c_void_p] + [_P] * 11 +
+                            [ctypes.c_float, ctypes.c_int32, ctypes.c_void_p, ctypes.c_size_t],
+    "clk_qk_norm_rope_cache": [ctypes.c_void_p] + [_P] * 11 + [ctypes.c_float, ctypes.c_int32],
+    "clk_kv_cache_write": [ctypes.c_void_p] + [_P] * 7,
+    "clk_kv_cache_read": [ctypes.c_void_p] + [_P] * 7,
+    "clk_paged_attention": [ctypes.c_void_p] + [_P] * 9 +
+                           [ctypes.c_float, ctypes.c_int32, ctypes.c_void_p, ctypes.c_size_t],
 }
 
 
@@ -110,6 +123,10 @@ def lib():
         handle.clk_attention_bwd_plan.restype = ctypes.c_int
         handle.clk_rms_norm_bwd_workspace_size.argtypes = [_P]
         handle.clk_rms_norm_bwd_workspace_size.restype = ctypes.c_size_t
+        handle.clk_qk_norm_rope_bwd_workspace_size.argtypes = [_P, _P]
+        handle.clk_qk_norm_rope_bwd_workspace_size.restype = ctypes.c_size_t
+        handle.clk_paged_attention_workspace_size.argtypes = [_P, _P, _P]
+        handle.clk_paged_attention_workspace_size.restype = ctypes.c_size_t
         handle.clk_attention_bwd_noalloc_scratch_size.argtypes = []
         handle.clk_attention_bwd_noalloc_scratch_size.restype = ctypes.c_size_t
         _lib = handle
@@ -530,3 +547,134 @@ def q8_projection(q, q_scale, wq, w_scale, b=None, residual=None, dtype=torch.fl
     _call("clk_q8_projection", (q, q_scale, wq, w_scale, w_scale if b is None else b, out if residual is None else residual,
                                 out), int(b is not None), int(residual is not None))
     return out
+
+
+# ---- heads, the key-value cache and its attention (no counterpart in the reference) -----------
+
+KVCache = collections.namedtuple("KVCache", "k v k_scale v_scale")
+KVCache.__doc__ = """A paged cache: k, v [pages, heads, page, D] in the order that layouts.keys_blocked and values_blocked make, F16, BF16
+or S8; k_scale, v_scale [pages, heads, page] F32 for S8, else None. Any such four in a tuple serve."""
+
+
+def kv_cache(pages, heads, page, d, dtype=torch.int8, device="cuda"):
+    """A cache of `pages` pages of `page` tokens, a multiple of 16, filled with zeros; d a multiple of 32. dtype:
+    float16, bfloat16, or int8 for 8-bit rows."""
+    k, v = (torch.zeros((pages, heads, page, d), dtype=dtype, device=device) for _ in range(2))
+    if dtype != torch.int8:
+        return KVCache(k, v, None, None)
+    return KVCache(k, v, *(torch.zeros((pages, heads, page), dtype=torch.float32, device=device) for _ in range(2)))
+
+
+def _cache_buffers(name, cache):
+    k, v, k_scale, v_scale = cache
+    if (k_scale is None) != (v_scale is None) or (k_scale is None) == (k.dtype is torch.int8):
+        raise InvalidArgument(INVALID_ARGUMENT, "%s: an 8-bit cache has scales, and no other has" % name)
+    if k_scale is None:
+        k_scale = v_scale = _one(k, torch.float32)
+    return k, v, k_scale, v_scale
+
+
+def _rank3(name, t):
+    if t.dim() != 3:
+        raise InvalidArgument(INVALID_ARGUMENT, "%s: expected [tokens, heads, D], got shape %s" % (name, tuple(t.shape)))
+    return t.shape
+
+
+def _scratch(name, workspace, like, need):
+    """(workspace, its bytes): the caller's, or one of `need` bytes"""
+    if workspace is None:
+        workspace = like.new_empty(max(need, 1), dtype=torch.uint8)
+    elif workspace.device != like.device or not workspace.is_contiguous():
+        raise InvalidArgument(INVALID_ARGUMENT, "%s: workspace must be contiguous, on the tensors' GPU" % name)
+    return workspace, workspace.numel() * workspace.element_size()
+
+
+def qk_norm_rope(qkv, q_norm, k_norm, rope, positions, kv_heads, eps=1e-5, interleaved=False, out=None):
+    """(q, k, v): the heads of a projection's result qkv [T, Hq + 2 kv_heads, D], apart: q [T,Hq,D], k, v
+    [T,kv_heads,D]. Queries and keys have each head's RMS norm with the weights q_norm, k_norm [D] F32, then the first R
+    channels rotated by the angles of positions [T] S32 in rope [P,R] F32 (layouts.rope_table): halves as pairs, or
+    neighbours (interleaved). Written into `out` = (q, k, v) when given."""
+    t, h, d = _rank3("qk_norm_rope", qkv)
+    if out is None:
+        if not 0 < 2 * kv_heads < h:
+            raise InvalidArgument(INVALID_ARGUMENT, "qk_norm_rope: qkv has %d heads, of which 2 * %d cannot be keys and values"
+                                  % (h, kv_heads))
+        out = qkv.new_empty((t, h - 2 * kv_heads, d)), qkv.new_empty((t, kv_heads, d)), qkv.new_empty((t, kv_heads, d))
+    _call("clk_qk_norm_rope", (qkv, q_norm, k_norm, rope, positions) + tuple(out), float(eps), int(bool(interleaved)))
+    return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_of(name, *shapes):
+    arrays = [(ctypes.c_int64 * max(len(s), 1))(*s) for s in shapes]
+    bufs = [Buffer(None, CLK_F16, len(s), a) for s, a in zip(shapes, arrays)]
+    return int(getattr(lib(), name)(*(ctypes.byref(b) for b in bufs)))
+
+
+def qk_norm_rope_bwd_workspace(qkv, dk):
+    """Bytes of workspace qk_norm_rope_bwd needs for qkv [T,H,D] and dk [T,Hkv,D]."""
+    return _workspace_of("clk_qk_norm_rope_bwd_workspace_size", tuple(qkv.shape), tuple(dk.shape))
+
+
+def qk_norm_rope_bwd(qkv, q_norm, k_norm, rope, positions, dq, dk, dv, eps=1e-5, interleaved=False, workspace=None, grads=None):
+    """(dqkv, dq_norm, dk_norm): the gradients of qk_norm_rope; written into `grads` when given."""
+    if grads is None:
+        grads = torch.empty_like(qkv), torch.empty_like(q_norm), torch.empty_like(k_norm)
+    workspace, size = _scratch("qk_norm_rope_bwd", workspace, qkv, qk_norm_rope_bwd_workspace(qkv, dk))
+    _call("clk_qk_norm_rope_bwd", (qkv, q_norm, k_norm, rope, positions, dq, dk, dv) + tuple(grads), float(eps),
+          int(bool(interleaved)), ctypes.c_void_p(workspace.data_ptr()), size)
+    return grads
+
+
+def qk_norm_rope_cache(qkv, q_norm, k_norm, rope, positions, slots, cache, eps=1e-5, interleaved=False, q=None):
+    """q [T,Hq,D]: qk_norm_rope with keys and values written into the cache, token t at slot slots[t] (S32: page * tokens of a
+    page + place in the page). A token whose slot the cache does not have, a negative one for a padded row, is not
+    written; slots of a call must differ from one another."""
+    t, h, d = _rank3("qk_norm_rope_cache", qkv)
+    bufs = _cache_buffers("qk_norm_rope_cache", cache)
+    if q is None:
+        heads = h - 2 * bufs[0].shape[1] if bufs[0].dim() == 4 else 1
+        q = qkv.new_empty((t, max(heads, 1), d))
+    _call("clk_qk_norm_rope_cache", (qkv, q_norm, k_norm, rope, positions, slots, q) + bufs, float(eps), int(bool(interleaved)))
+    return q
+
+
+def kv_cache_write(k, v, slots, cache):
+    """k, v [T,heads,D] into the cache as they are, token t at slot slots[t], with qk_norm_rope_cache's rules."""
+    _call("clk_kv_cache_write", (k, v, slots) + _cache_buffers("kv_cache_write", cache))
+
+
+def kv_cache_read(cache, slots, dtype=None, out=None):
+    """(k, v) [T,heads,D]: what the slots hold, zeros for a slot that the cache does not have. dtype: the cache's, or F16
+    (the default) or BF16 for an 8-bit cache."""
+    bufs = _cache_buffers("kv_cache_read", cache)
+    if out is None:
+        if bufs[0].dim() != 4:
+            raise InvalidArgument(INVALID_ARGUMENT, "kv_cache_read: a cache must be [pages,heads,page,D]")
+        if dtype is None:
+            dtype = torch.float16 if bufs[0].dtype is torch.int8 else bufs[0].dtype
+        shape = (slots.shape[0], bufs[0].shape[1], bufs[0].shape[3])
+        out = bufs[0].new_empty(shape, dtype=dtype), bufs[0].new_empty(shape, dtype=dtype)
+    _call("clk_kv_cache_read", bufs + (slots,) + tuple(out))
+    return out
+
+
+def paged_attention_workspace(q, cache, page_table):
+    """Bytes of workspace paged_attention needs."""
+    return _workspace_of("clk_paged_attention_workspace_size", tuple(q.shape), tuple(cache[0].shape), tuple(page_table.shape))
+
+
+def paged_attention(q, cache, page_table, lengths, scale=None, want_lse=False, out=None, lse=None, workspace=None):
+    """(out, lse): attention of one new token a sequence, q [B,Hq,D], over the lengths[b] (S32) tokens that the pages
+    page_table[b,:] (S32 [B,N]) of the cache hold; lse [B,Hq] F32 in the log2 domain, None without want_lse. scale
+    defaults to D^-1/2. A sequence of no tokens gives zeros and -inf."""
+    b, h, d = _rank3("paged_attention", q)
+    bufs = _cache_buffers("paged_attention", cache)
+    out = torch.empty_like(q) if out is None else out
+    want_lse = want_lse or lse is not None
+    if want_lse and lse is None:
+        lse = q.new_empty((b, h), dtype=torch.float32)
+    workspace, size = _scratch("paged_attention", workspace, q, paged_attention_workspace(q, cache, page_table))
+    _call("clk_paged_attention", (q,) + bufs + (page_table, lengths, out, lse if want_lse else _one(q, torch.float32)),
+          float(d ** -0.5 if scale is None else scale), int(want_lse), ctypes.c_void_p(workspace.data_ptr()), size)
+    return out, (lse if want_lse else None)

@@ -17,8 +17,13 @@ and the layout of the 8-bit projection's weights, which has no counterpart there
   q8_projection       q [N, Kp] (8-bit rows of w^T, Kp a multiple of 64) ->
                       wq [ceil(N/64), Kp/64, 4, 4, 16, 16]
 
+and what the heads' rotation and the key-value cache hold, which have none either:
+
+  rope_table          [positions, r]: the cosines and sines of each position's angles
+  keys_blocked, values_blocked  [pages, heads, page, d] in the order of the tokens -> in the cache's
+
 Each function takes and returns torch tensors (any device) or numpy arrays, and returns a
-contiguous result of the input's dtype.
+contiguous result of the input's dtype (rope_table makes a torch tensor).
 """
 
 HIDDEN_CHUNK = 64  # rows of w2 per block of the transition's blocked layout
@@ -111,3 +116,54 @@ def q8_unblocked(wq, n):
     p = wq.reshape(blocks, kbs, 4, 4, 4, 4, 16)
     p = p.permute(0, 4, 2, 5, 1, 3, 6) if hasattr(p, "permute") else p.transpose(0, 4, 2, 5, 1, 3, 6)
     return _contig(p.reshape(blocks * Q8_BLOCK, kbs * Q8_BLOCK)[:n])
+
+
+def rope_table(positions, r, base=10000.0, device="cpu"):
+    """rope [positions, r] fp32 (hip.qk_norm_rope): row p holds cos(p f_i), i < r / 2, then sin(p f_i), f_i = base^(-2 i / r),
+    computed in float64."""
+    import torch
+    f = float(base) ** (-torch.arange(0, r, 2, dtype=torch.float64) / r)
+    angles = torch.arange(positions, dtype=torch.float64)[:, None] * f
+    return torch.cat([angles.cos(), angles.sin()], 1).to(torch.float32).to(device)
+
+
+CACHE_BLOCK = 16  # tokens of a block of the cache
+
+
+def _cache_dims(x):
+    if x.ndim != 4 or x.shape[2] % CACHE_BLOCK or x.shape[3] % 32:
+        raise ValueError("expected [pages, heads, page, d], page a multiple of 16 and d of 32, got shape %s" % (tuple(x.shape),))
+    item = x.element_size() if hasattr(x, "element_size") else x.dtype.itemsize
+    p, h, n, d = x.shape
+    return p, h, n // CACHE_BLOCK, d, 16 if item == 1 else 8, 4 if item == 1 and d % 64 == 0 else 2
+
+
+def _reordered(x, shape, order):
+    y = x.reshape(shape)
+    return _contig((y.permute(*order) if hasattr(y, "permute") else y.transpose(order)).reshape(x.shape))
+
+
+def keys_blocked(k):
+    """k [pages, heads, page, d] -> the cache's order: blocks of 16 tokens as [d / w][16][w], w = 8 (16 bits) or 16 (8 bits)
+    channels."""
+    p, h, blocks, d, w, _ = _cache_dims(k)
+    return _reordered(k, (p, h, blocks, 16, d // w, w), (0, 1, 2, 4, 3, 5))
+
+
+def keys_unblocked(k):
+    """The inverse of keys_blocked."""
+    p, h, blocks, d, w, _ = _cache_dims(k)
+    return _reordered(k, (p, h, blocks, d // w, 16, w), (0, 1, 2, 4, 3, 5))
+
+
+def values_blocked(v):
+    """v [pages, heads, page, d] -> the cache's order: blocks of 16 tokens as [d / (16 c)][4 g][16 i][c e][4 j], token 4 g + j,
+    channel 16 (c b + e) + i; c = 2, or 4 for 8 bits where d is a multiple of 64."""
+    p, h, blocks, d, _, c = _cache_dims(v)
+    return _reordered(v, (p, h, blocks, 4, 4, d // (16 * c), c, 16), (0, 1, 2, 5, 3, 7, 6, 4))
+
+
+def values_unblocked(v):
+    """The inverse of values_blocked."""
+    p, h, blocks, d, _, c = _cache_dims(v)
+    return _reordered(v, (p, h, blocks, d // (16 * c), 4, 16, c, 4), (0, 1, 2, 4, 7, 3, 6, 5))

@@ -23,6 +23,11 @@ provides on top of `hip` (the C ABI binding):
   rms_norm_q8, quantize_rows, dequantize_rows, q8_weights, q8_projection, q8_transition
                    the 8-bit serving path: norms and activations as 8-bit rows, weights quantised
                    once, projections and an MLP in 8-bit products (no counterpart in the reference)
+  qk_norm_rope     a projection's queries, keys and values apart, queries and keys with each head's RMS norm and the
+                   position rotation, differentiable
+  cache_slots, qk_norm_rope_cache, kv_cache_write, kv_cache_read, paged_attention
+                   attention over a paged key-value cache, in 16 or 8 bits, one new token a sequence (no counterpart
+                   in the reference)
 
 Everything runs on the GPU through the built library; there is no CPU path. The fused and the
 8-bit wrappers are forward only (the reference's callers take their gradients from jnp references). They take
@@ -297,10 +302,10 @@ def _capturing(t):
     return t.is_cuda and torch.cuda.is_current_stream_capturing()
 
 
-def _refuse_capture(t):
+def _refuse_capture(t, name="rms_norm"):
     if _capturing(t):
-        raise hip.InvalidArgument(hip.INVALID_ARGUMENT, "rms_norm: a differentiated call cannot be captured into a "
-                                  "graph; capture hip.rms_norm and hip.rms_norm_bwd")
+        raise hip.InvalidArgument(hip.INVALID_ARGUMENT, "%s: a differentiated call cannot be captured into a "
+                                  "graph; capture hip.%s and hip.%s_bwd" % (name, name, name))
 
 
 def _any_tangent(*tensors):
@@ -377,3 +382,128 @@ def q8_transition(x, scale, w1, b1, w2, b2, residual=None, activation="relu", ad
     h = q8_projection(q, q_scale, w1, b1, dtype=x.dtype)
     out = q8_projection(*quantize_rows(h, activation), w2, b2, residual=s if add_input else None, dtype=x.dtype)
     return out if residual is None else (out, s)
+
+
+# ---- heads, the key-value cache and its attention (no counterpart in the reference) -----------
+
+class _QkNormRope(torch.autograd.Function):
+    """qkv [..., H, D] is flattened in here, as in _RmsNorm."""
+
+    @staticmethod
+    def forward(ctx, qkv, q_norm, k_norm, rope, positions, kv_heads, eps, interleaved):
+        qkv = qkv.contiguous()
+        lead, (h, d) = qkv.shape[:-2], qkv.shape[-2:]
+        out = tuple(qkv.new_empty(lead + (n, d)) for n in (h - 2 * kv_heads, kv_heads, kv_heads))
+        hip.qk_norm_rope(_heads(qkv), q_norm, k_norm, rope, positions, kv_heads, eps, interleaved, tuple(map(_heads, out)))
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(qkv, q_norm, k_norm, rope, positions)
+        ctx.rule = kv_heads, eps, interleaved
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        qkv, q_norm, k_norm, rope, positions = ctx.saved_tensors
+        kv_heads, eps, interleaved = ctx.rule
+        _refuse_capture(qkv, "qk_norm_rope")
+        lead, (h, d) = qkv.shape[:-2], qkv.shape[-2:]
+        grads = [qkv.new_zeros(lead + (n, d)) if g is None else g.to(qkv.dtype).contiguous()
+                 for g, n in zip(grads, (h - 2 * kv_heads, kv_heads, kv_heads))]
+        dqkv, dq_norm, dk_norm = torch.empty_like(qkv), torch.empty_like(q_norm), torch.empty_like(k_norm)
+        hip.qk_norm_rope_bwd(_heads(qkv), q_norm, k_norm, rope, positions, *map(_heads, grads), eps, interleaved,
+                             grads=(_heads(dqkv), dq_norm, dk_norm))
+        need = ctx.needs_input_grad
+        return (dqkv if need[0] else None, dq_norm if need[1] else None, dk_norm if need[2] else None) + (None,) * 5
+
+
+def _heads(x):
+    """x [..., H, D] as [T, H, D]; x itself where it is that"""
+    return x if x.dim() == 3 else x.reshape((-1,) + x.shape[-2:])
+
+
+def _tokens(name, what, t, lead):
+    """One value a token: of the leading shape, or one that broadcasts to it, as [T]"""
+    try:
+        return t.expand(lead).reshape(-1)
+    except RuntimeError:
+        raise hip.InvalidArgument(hip.INVALID_ARGUMENT, "%s: %s must be of the tokens' shape %s, got %s"
+                                  % (name, what, tuple(lead), tuple(t.shape))) from None
+
+
+def _check_heads(name, x, what):
+    if x.dim() < 3:
+        raise hip.InvalidArgument(hip.INVALID_ARGUMENT, "%s: %s must be [..., heads, D], got shape %s" % (name, what, tuple(x.shape)))
+
+
+def _head_rows(name, x, what):
+    _check_heads(name, x, what)
+    return _heads(x.contiguous())
+
+
+def qk_norm_rope(qkv, q_norm, k_norm, rope, positions, kv_heads, eps=1e-5, interleaved=False):
+    """(q [..., Hq, D], k, v [..., kv_heads, D]): the heads of a projection's result qkv [..., Hq + 2 kv_heads, D], apart;
+    queries and keys with each head's RMS norm, weights q_norm, k_norm [D], then the first R channels rotated by the
+    angles of positions [...] int32 (or a shape that broadcasts to it) in rope [P, R] fp32 = layouts.rope_table(P, R): channels
+    i and i + R / 2 as pairs, or neighbours (interleaved). fp16 or bf16. Differentiable in qkv, q_norm and
+    k_norm (once, in reverse mode; a dual tensor is refused); like rms_norm, not while a HIP graph is captured: capture
+    hip.qk_norm_rope and hip.qk_norm_rope_bwd instead."""
+    _check_heads("qk_norm_rope", qkv, "qkv")
+    h = qkv.shape[-2]
+    if not 0 < 2 * kv_heads < h:
+        raise hip.InvalidArgument(hip.INVALID_ARGUMENT, "qk_norm_rope: qkv has %d heads, of which 2 * %d cannot be keys and values"
+                                  % (h, kv_heads))
+    positions = _tokens("qk_norm_rope", "positions", positions, qkv.shape[:-2])
+    wq, wk = q_norm.float().contiguous(), k_norm.float().contiguous()
+    differentiated = torch.is_grad_enabled() and (qkv.requires_grad or q_norm.requires_grad or k_norm.requires_grad)
+    if differentiated:
+        _refuse_capture(qkv, "qk_norm_rope")
+    if differentiated or _any_tangent(qkv, q_norm, k_norm, rope):
+        return _QkNormRope.apply(qkv, wq, wk, rope, positions, int(kv_heads), float(eps), bool(interleaved))
+    out = hip.qk_norm_rope(_head_rows("qk_norm_rope", qkv, "qkv"), wq, wk, rope, positions, int(kv_heads), eps, interleaved)
+    return out if qkv.dim() == 3 else tuple(t.reshape(qkv.shape[:-2] + t.shape[1:]) for t in out)
+
+
+def cache_slots(page_table, positions, page):
+    """The slots [B] or [B, S] int32 of positions [B] or [B, S] of B sequences whose pages are page_table [B, N], `page` tokens
+    a page: -1 for a negative position (a padded row), one past the table, or a page that is negative."""
+    at = positions.reshape(positions.shape[0], -1).long()
+    col = at.div(page, rounding_mode="floor")
+    known = (at >= 0) & (col < page_table.shape[1])
+    pages = page_table.long().gather(1, torch.where(known, col, torch.zeros_like(col)))
+    slots = torch.where(known & (pages >= 0), pages * page + at % page, torch.full_like(at, -1))
+    return slots.to(torch.int32).reshape(positions.shape)
+
+
+def qk_norm_rope_cache(qkv, q_norm, k_norm, rope, positions, slots, cache, eps=1e-5, interleaved=False):
+    """q [..., Hq, D]: qk_norm_rope with keys and values written into `cache` = hip.kv_cache(...), each token at its slot
+    (cache_slots; positions and slots [...] int32). A token with a slot that the cache does not have is not written;
+    the slots of a call must differ from one another. Forward only."""
+    rows = _head_rows("qk_norm_rope_cache", qkv, "qkv")
+    lead = qkv.shape[:-2]
+    q = hip.qk_norm_rope_cache(rows, q_norm.float().contiguous(), k_norm.float().contiguous(), rope,
+                               _tokens("qk_norm_rope_cache", "positions", positions, lead),
+                               _tokens("qk_norm_rope_cache", "slots", slots, lead), cache, eps, interleaved)
+    return q.reshape(lead + q.shape[1:])
+
+
+def kv_cache_write(k, v, slots, cache):
+    """k, v [..., heads, D] into the cache as they are, each token at its slot (qk_norm_rope_cache's rules)."""
+    if k.shape != v.shape:
+        raise hip.InvalidArgument(hip.INVALID_ARGUMENT, "kv_cache_write: k and v must be alike, got %s and %s"
+                                  % (tuple(k.shape), tuple(v.shape)))
+    k, v, lead = _head_rows("kv_cache_write", k, "k"), _head_rows("kv_cache_write", v, "v"), k.shape[:-2]
+    hip.kv_cache_write(k, v, _tokens("kv_cache_write", "slots", slots, lead), cache)
+
+
+def kv_cache_read(cache, slots, dtype=None):
+    """(k, v) [..., heads, D]: what slots [...] int32 of the cache hold, zeros for a slot that it does not have."""
+    k, v = hip.kv_cache_read(cache, slots.reshape(-1), dtype)
+    return k.reshape(slots.shape + k.shape[1:]), v.reshape(slots.shape + v.shape[1:])
+
+
+def paged_attention(q, cache, page_table, lengths, scale=None, want_lse=False):
+    """softmax(scale q K^T) V for one new token a sequence, q [B, Hq, D], over the lengths[b] tokens that the pages
+    page_table[b] of the cache hold (both int32); with want_lse (out, lse [B, Hq] fp32, log2 domain). scale defaults to
+    D^-1/2. Forward only."""
+    out, lse = hip.paged_attention(q.contiguous(), cache, page_table.contiguous(), lengths.contiguous(), scale, want_lse)
+    return (out, lse) if want_lse else out

@@ -68,6 +68,35 @@ __device__ __forceinline__ half_t act_cvt(float v) {
     }
 }
 
+// Raw 16-bit patterns that are moved, selected or put together one by one are held as integers: a half vector made of
+// single values is packed by v_pack_b32_f16, which quiets fp16's signalling NaNs, and those are bf16 values past
+// 2^121. Results are therefore converted as whole vectors.
+typedef uint16_t raw8 __attribute__((ext_vector_type(8)));
+typedef uint16_t raw4 __attribute__((ext_vector_type(4)));
+template <bool BF>
+__device__ __forceinline__ raw8 act_cvt8(const float (&f)[8]) {
+    if constexpr (BF) {
+        bf16x8 v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (__bf16)f[e];
+        return __builtin_bit_cast(raw8, v);
+    } else {
+        half8 v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (half_t)f[e];
+        return __builtin_bit_cast(raw8, v);
+    }
+}
+template <bool BF>
+__device__ __forceinline__ raw4 act_cvt4(float4v f) {
+    if constexpr (BF) {
+        typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+        return __builtin_bit_cast(raw4, bf16x4{(__bf16)f[0], (__bf16)f[1], (__bf16)f[2], (__bf16)f[3]});
+    } else {
+        return __builtin_bit_cast(raw4, half4{(half_t)f[0], (half_t)f[1], (half_t)f[2], (half_t)f[3]});
+    }
+}
+
 // LDS row of tile row x, for operand tiles whose A row r of block b is
 //   x = per (r / 4) + 4 b + r % 4:
 // stored at row 16 b + r, a 16-lane group reads 16 consecutive rows, which with a row stride of

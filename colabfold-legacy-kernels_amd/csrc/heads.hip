@@ -1,0 +1,809 @@
+// Queries, keys and values on their way from a projection to attention, for gfx950 (CDNA4). No counterpart in the
+// reference.
+//
+//   qk_norm_rope        x [T, Hq + 2 Hkv, D]: each query and key head n = x r w, r = 1 / sqrt(mean(x^2) + eps), then its
+//                       first R channels rotated in pairs (a, b) -> (a cos - b sin, a sin + b cos) by the angles of
+//                       the token's position; values as they are; q, k and v apart
+//   qk_norm_rope_bwd    g' = the gradient rotated back, xh = x r, g = g' w: dx = r (g - xh mean(g xh)), dw = sum over tokens
+//                       and heads of g' xh
+//   qk_norm_rope_cache  the forward with keys and values written into the cache, in 16 bits or as 8-bit rows of a
+//                       token's head (each value rounded once, from fp32)
+//   kv_cache_write, kv_cache_read  keys and values into the cache as they are, and back
+//
+// All of them are bound by memory: each value is read once and written once, statistics and products are fp32.
+//
+// A head is a group of LG lanes (the power of two at or past D / 8) with 8 channels each, the two halves of its pairs: a
+// lane whose channels are rotated by halves holds channels 4 j .. + 3 and R / 2 + 4 j .. + 3, so that pairs never
+// cross lanes; all others hold 8 j .. + 7. A workgroup takes 256 / LG tokens of up to HPG heads of one kind, and
+// reads a token's cosines and sines once for them.
+#include "kv_cache.h"
+#include "rows8_dev.h"
+
+#include <algorithm>
+#include <type_traits>
+
+#pragma clang fp contract(off)  // every kernel rounds alike, whichever of them a call's size picks
+
+namespace clk {
+
+namespace {
+
+constexpr int kThreads = 256;
+enum { kQuery, kKey, kValue };
+
+struct HeadsArgs {
+    const half_t* x;  // [T, Hq + 2 Hkv, D]
+    const float* qn;
+    const float* kn;
+    const float* rope;  // [P, R]
+    const int32_t* pos;
+    const int32_t* slots;
+    half_t* q;
+    half_t* k;
+    half_t* v;
+    void* kc;  // the cache
+    void* vc;
+    float* ks;
+    float* vs;
+    const half_t* dq;
+    const half_t* dk;
+    const half_t* dv;
+    half_t* dx;
+    float* partial;
+    float* dqn;
+    float* dkn;
+    int64_t T;
+    int Hq, Hkv, D, R, P;
+    int cq, ck;          // chunks of heads: queries', keys' (values' as keys')
+    int parts;           // the backward's workgroups a chunk
+    int page, slots_end;  // the cache's page, and its tokens
+    FastDiv by_page;
+    float inv_d, eps;
+    bool interleaved;
+};
+
+// A lane's 8 channels of its head: two runs of four
+struct Lane {
+    int c0, c1;
+    bool in, turned;
+};
+__device__ __forceinline__ Lane lane_of(int j, int D, int R, bool interleaved) {
+    Lane l;
+    l.in = 8 * j < D;
+    l.turned = 8 * j < R;
+    const bool halves = l.turned && !interleaved;
+    l.c0 = !l.in ? 0 : halves ? 4 * j : 8 * j;
+    l.c1 = !l.in ? 4 : halves ? R / 2 + 4 * j : 8 * j + 4;
+    return l;
+}
+
+__device__ __forceinline__ raw8 load_head(const half_t* row, const Lane& l) {
+    const raw4 a = *reinterpret_cast<const raw4*>(row + l.c0), b = *reinterpret_cast<const raw4*>(row + l.c1);
+    const raw8 v{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    return l.in ? v : raw8{};
+}
+__device__ __forceinline__ void store_head(half_t* row, const Lane& l, raw8 v) {
+    *reinterpret_cast<raw4*>(row + l.c0) = raw4{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<raw4*>(row + l.c1) = raw4{v[4], v[5], v[6], v[7]};
+}
+template <bool BF>
+__device__ __forceinline__ void floats(raw8 v, float (&f)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = act_get<BF>(__builtin_bit_cast(half8, v), e);
+}
+__device__ __forceinline__ void load_weight(const float* w, const Lane& l, float (&f)[8]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        f[e] = l.in ? w[l.c0 + e] : 0.f;
+        f[4 + e] = l.in ? w[l.c1 + e] : 0.f;
+    }
+}
+
+// The angles of lane j's four pairs at a position, (1, 0) where it has none; false at a position that the table does not have
+struct Angles {
+    float4v cos, sin;
+};
+__device__ __forceinline__ bool load_angles(const HeadsArgs& a, int pos, int j, bool turned, Angles& t) {
+    const bool ok = (uint32_t)pos < (uint32_t)a.P;
+    const float* row = a.rope + (int64_t)(ok ? pos : 0) * a.R;
+    const int at = turned ? 4 * j : 0;
+    t.cos = *reinterpret_cast<const float4v*>(row + at);
+    t.sin = *reinterpret_cast<const float4v*>(row + a.R / 2 + at);
+    return ok;
+}
+
+// A lane's pairs by the angles' (cos, sin), or back by (cos, -sin)
+template <bool BACK>
+__device__ __forceinline__ void turn(float (&f)[8], const Angles& t, const Lane& l, bool interleaved) {
+    float a[4], b[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        a[e] = interleaved ? f[2 * e] : f[e];
+        b[e] = interleaved ? f[2 * e + 1] : f[4 + e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float s = BACK ? -t.sin[e] : t.sin[e];
+        const float x = __builtin_fmaf(a[e], t.cos[e], -(b[e] * s)), y = __builtin_fmaf(a[e], s, b[e] * t.cos[e]);
+        a[e] = x;
+        b[e] = y;
+    }
+    if (!l.turned) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        f[interleaved ? 2 * e : e] = a[e];
+        f[interleaved ? 2 * e + 1 : 4 + e] = b[e];
+    }
+}
+
+// f times r = 1 / sqrt(mean(f^2) + eps), and r. bf16 heads whose squares leave fp32's range are taken times a
+// power of two, as rows are (row_shift).
+template <bool BF, int LG>
+__device__ __forceinline__ float normalise(float (&f)[8], float inv_d, float eps) {
+    const auto squares = [&] {
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = __builtin_fmaf(f[e], f[e], s);
+        return lanes_sum<LG>(s);
+    };
+    float ss = squares(), d = 1.f;
+    if constexpr (BF) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = max(m, abs_bits(f[e]));
+        d = row_shift(lanes_max<LG>(m), eps);
+        if (__any(d != 1.f)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] *= d;
+            ss = squares();
+        }
+    }
+    const float r = inv_rms(ss, inv_d, eps * d * d);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] *= r;
+    return r * d;
+}
+
+// The heads of workgroup row `chunk`: their kind, the first of them among their kind, and how many
+struct Heads {
+    int kind, first, count;
+};
+template <int HPG>
+__device__ __forceinline__ Heads heads_of(const HeadsArgs& a, int chunk) {
+    Heads h;
+    h.kind = chunk < a.cq ? kQuery : chunk < a.cq + a.ck ? kKey : kValue;
+    const int i = h.kind == kQuery ? chunk : h.kind == kKey ? chunk - a.cq : chunk - a.cq - a.ck;
+    h.first = i * HPG;
+    h.count = min(HPG, (h.kind == kQuery ? a.Hq : a.Hkv) - h.first);
+    return h;
+}
+__device__ __forceinline__ int head_at(const HeadsArgs& a, int kind) {
+    return kind == kQuery ? 0 : kind == kKey ? a.Hq : a.Hq + a.Hkv;
+}
+
+// ---- the cache ------------------------------------------------------------------------------
+
+// Where a token's head lies: its block, and its row in it
+struct Place {
+    int64_t block;  // in values
+    int64_t scale;
+    int t;
+};
+__device__ __forceinline__ Place place_of(const HeadsArgs& a, int slot, int head) {
+    const int page = fdiv(slot, a.by_page), in = slot - page * a.page;
+    const int64_t row = (int64_t)page * a.Hkv + head;
+    return Place{(row * a.page + (in & ~15)) * a.D, row * a.page + in, in & 15};
+}
+
+// A lane's 8 channels of a key (l) or value (8 j ..) into the cache, in 16 bits
+__device__ __forceinline__ void cache_key16(void* kc, const Place& p, const Lane& l, raw8 v) {
+    uint16_t* at = static_cast<uint16_t*>(kc) + p.block;
+    *reinterpret_cast<raw4*>(at + key_place(false, p.t, l.c0)) = raw4{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<raw4*>(at + key_place(false, p.t, l.c1)) = raw4{v[4], v[5], v[6], v[7]};
+}
+__device__ __forceinline__ void cache_value16(void* vc, const Place& p, int c, raw8 v) {
+    uint16_t* at = static_cast<uint16_t*>(vc) + p.block + value_place(2, p.t, c);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) at[8 * e] = v[e];
+}
+// and as 8-bit rows: f in fp32, of 16-bit values where IN16. Every lane of the group comes here.
+template <int LG, bool IN16>
+__device__ __forceinline__ uint2v to_row8(const float (&f)[8], float& scale) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = max(m, abs_bits(f[e]));
+    float top, inv;
+    row_scale(lanes_max<LG>(m), 1.f, top, inv, scale);
+    return quant8<IN16>(f, top, inv);
+}
+__device__ __forceinline__ void cache_key8(void* kc, const Place& p, const Lane& l, uint2v w) {
+    int8_t* at = static_cast<int8_t*>(kc) + p.block;
+    *reinterpret_cast<uint32_t*>(at + key_place(true, p.t, l.c0)) = w[0];
+    *reinterpret_cast<uint32_t*>(at + key_place(true, p.t, l.c1)) = w[1];
+}
+__device__ __forceinline__ void cache_value8(void* vc, const Place& p, int group, int c, uint2v w) {
+    int8_t* at = static_cast<int8_t*>(vc) + p.block + value_place(group, p.t, c);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) at[4 * group * e] = (int8_t)(w[e >> 2] >> 8 * (e & 3));
+}
+
+// ---- forward --------------------------------------------------------------------------------
+
+enum { kApart, kCache16, kCache8 };
+
+template <bool BF, int LG, int OUT, int HPG>
+__global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(HeadsArgs a) {
+    constexpr int TOKENS = kThreads / LG;
+    const int j = threadIdx.x % LG, sub = threadIdx.x / LG;
+    const Heads h = heads_of<HPG>(a, blockIdx.y);
+    const Lane l = lane_of(j, a.D, h.kind == kValue ? 0 : a.R, a.interleaved);
+    const int H = a.Hq + 2 * a.Hkv, group = value_group(OUT == kCache8, a.D);
+    float w[8];
+    if (h.kind != kValue) load_weight(h.kind == kQuery ? a.qn : a.kn, l, w);
+    for (int64_t t0 = (int64_t)blockIdx.x * TOKENS; t0 < a.T; t0 += (int64_t)gridDim.x * TOKENS) {
+        const int64_t t = t0 + sub, from = min(t, a.T - 1);  // past T: the last token, unused
+        const half_t* row = a.x + (from * H + head_at(a, h.kind) + h.first) * a.D;
+        raw8 raw[HPG];
+#pragma unroll
+        for (int i = 0; i < HPG; ++i) raw[i] = load_head(row + (int64_t)min(i, h.count - 1) * a.D, l);
+        Angles angles;
+        bool ok = true;
+        if (h.kind != kValue) ok = load_angles(a, a.pos[from], j, l.turned, angles);
+        int slot = -1;
+        if (OUT != kApart && h.kind != kQuery) slot = a.slots[from];
+        const bool live = t < a.T && l.in && (OUT == kApart || h.kind == kQuery || (uint32_t)slot < (uint32_t)a.slots_end);
+#pragma unroll
+        for (int i = 0; i < HPG; ++i) {
+            if (i >= h.count) break;
+            const int head = h.first + i;
+            if (h.kind == kValue) {
+                if constexpr (OUT == kApart) {
+                    if (live) store_head(a.v + (t * a.Hkv + head) * a.D, l, raw[i]);
+                } else if constexpr (OUT == kCache16) {
+                    if (live) cache_value16(a.vc, place_of(a, slot, head), l.c0, raw[i]);
+                } else {
+                    float f[8], scale;
+                    floats<BF>(raw[i], f);
+                    const uint2v q = to_row8<LG, true>(f, scale);
+                    if (live) {
+                        const Place p = place_of(a, slot, head);
+                        cache_value8(a.vc, p, group, l.c0, q);
+                        if (j == 0) a.vs[p.scale] = scale;
+                    }
+                }
+                continue;
+            }
+            float f[8];
+            floats<BF>(raw[i], f);
+            normalise<BF, LG>(f, a.inv_d, a.eps);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] *= w[e];
+            turn<false>(f, angles, l, a.interleaved);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = ok ? f[e] : __builtin_nanf("");
+            const raw8 y = act_cvt8<BF>(f);
+            if (OUT == kApart || h.kind == kQuery) {
+                half_t* out = h.kind == kQuery ? a.q + (t * a.Hq + head) * a.D : a.k + (t * a.Hkv + head) * a.D;
+                if (live) store_head(out, l, y);
+            } else if constexpr (OUT == kCache16) {
+                if (live) cache_key16(a.kc, place_of(a, slot, head), l, y);
+            } else {
+                float scale;
+                const uint2v q = to_row8<LG, false>(f, scale);
+                if (live) {
+                    const Place p = place_of(a, slot, head);
+                    cache_key8(a.kc, p, l, q);
+                    if (j == 0) a.ks[p.scale] = scale;
+                }
+            }
+        }
+    }
+}
+
+// ---- backward -------------------------------------------------------------------------------
+
+constexpr int kBwdHeads = 4;  // heads a workgroup row
+
+template <bool BF, int LG>
+__global__ __launch_bounds__(kThreads) void qk_norm_rope_bwd_kernel(HeadsArgs a) {
+    constexpr int TOKENS = kThreads / LG, HPG = kBwdHeads;
+    __shared__ float sums[TOKENS][LG * 8 + 1];
+    const int j = threadIdx.x % LG, sub = threadIdx.x / LG;
+    const Heads h = heads_of<HPG>(a, blockIdx.y);
+    const Lane l = lane_of(j, a.D, h.kind == kValue ? 0 : a.R, a.interleaved);
+    const int H = a.Hq + 2 * a.Hkv, mine = h.kind == kQuery ? a.Hq : a.Hkv;
+    const half_t* dy = h.kind == kQuery ? a.dq : h.kind == kKey ? a.dk : a.dv;
+    float w[8], dw[8] = {};
+    if (h.kind != kValue) load_weight(h.kind == kQuery ? a.qn : a.kn, l, w);
+    for (int64_t t0 = (int64_t)blockIdx.x * TOKENS; t0 < a.T; t0 += (int64_t)a.parts * TOKENS) {
+        const int64_t t = t0 + sub, from = min(t, a.T - 1);
+        const bool in = t < a.T && l.in;
+        const half_t* row = a.x + (from * H + head_at(a, h.kind) + h.first) * a.D;
+        const half_t* gow = dy + (from * mine + h.first) * a.D;
+        half_t* out = a.dx + (from * H + head_at(a, h.kind) + h.first) * a.D;
+        raw8 raw[HPG], graw[HPG];
+#pragma unroll
+        for (int i = 0; i < HPG; ++i) {
+            const int64_t at = (int64_t)min(i, h.count - 1) * a.D;
+            if (h.kind != kValue) raw[i] = load_head(row + at, l);
+            graw[i] = load_head(gow + at, l);
+        }
+        Angles angles;
+        bool ok = true;
+        if (h.kind != kValue) ok = load_angles(a, a.pos[from], j, l.turned, angles);
+#pragma unroll
+        for (int i = 0; i < HPG; ++i) {
+            if (i >= h.count) break;
+            raw8 o = graw[i];
+            if (h.kind != kValue) {
+                float f[8], g[8], dot = 0.f;
+                floats<BF>(raw[i], f);
+                floats<BF>(graw[i], g);
+                const float r = normalise<BF, LG>(f, a.inv_d, a.eps);
+                turn<true>(g, angles, l, a.interleaved);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (!ok) g[e] = __builtin_nanf("");
+                    if (t < a.T) dw[e] = __builtin_fmaf(g[e], f[e], dw[e]);
+                    g[e] *= w[e];
+                    dot = __builtin_fmaf(g[e], f[e], dot);
+                }
+                dot = lanes_sum<LG>(dot) * a.inv_d;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) g[e] = r * __builtin_fmaf(-f[e], dot, g[e]);
+                o = act_cvt8<BF>(g);
+            }
+            if (in) store_head(out + (int64_t)i * a.D, l, o);
+        }
+    }
+    if (h.kind == kValue) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (l.in) {
+            sums[sub][l.c0 + e] = dw[e];
+            sums[sub][l.c1 + e] = dw[4 + e];
+        }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.D; c += kThreads) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < TOKENS; ++i) s += sums[i][c];
+        a.partial[((int64_t)blockIdx.y * a.parts + blockIdx.x) * a.D + c] = s;
+    }
+}
+
+// dqn and dkn (blockIdx.y): the sums of their partial rows, 16 interleaved groups of them, each in order, then the
+// groups.
+__global__ __launch_bounds__(kThreads) void qk_norm_dw_kernel(HeadsArgs a) {
+    __shared__ float sums[16][16];
+    const int col = threadIdx.x & 15, grp = threadIdx.x >> 4, c = blockIdx.x * 16 + col;
+    const int first = blockIdx.y ? a.cq * a.parts : 0, n = (blockIdx.y ? a.ck : a.cq) * a.parts;
+    float v = 0.f;
+    if (c < a.D) {
+        const float* p = a.partial + (int64_t)first * a.D + c;
+        int i = grp;
+        for (; i + 7 * 16 < n; i += 8 * 16) {
+            float u[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) u[k] = p[(int64_t)(i + 16 * k) * a.D];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v += u[k];
+        }
+        for (; i < n; i += 16) v += p[(int64_t)i * a.D];
+    }
+    sums[grp][col] = v;
+    __syncthreads();
+    if (grp == 0 && c < a.D) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t += sums[i][col];
+        (blockIdx.y ? a.dkn : a.dqn)[c] = t;
+    }
+}
+
+// ---- cache in, cache out --------------------------------------------------------------------
+
+// blockIdx.y: a head of keys, then of values
+template <bool BF, int LG, bool Q8>
+__global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(HeadsArgs a) {
+    constexpr int TOKENS = kThreads / LG;
+    const int j = threadIdx.x % LG, sub = threadIdx.x / LG, group = value_group(Q8, a.D);
+    const bool values = (int)blockIdx.y >= a.Hkv;
+    const int head = values ? blockIdx.y - a.Hkv : blockIdx.y;
+    const Lane l = lane_of(j, a.D, 0, false);
+    const half_t* x = values ? a.dv : a.dk;
+    for (int64_t t0 = (int64_t)blockIdx.x * TOKENS; t0 < a.T; t0 += (int64_t)gridDim.x * TOKENS) {
+        const int64_t t = t0 + sub, from = min(t, a.T - 1);
+        const int slot = a.slots[from];
+        const bool live = t < a.T && l.in && (uint32_t)slot < (uint32_t)a.slots_end;
+        const raw8 raw = load_head(x + (from * a.Hkv + head) * a.D, l);
+        if constexpr (Q8) {
+            float f[8], scale;
+            floats<BF>(raw, f);
+            const uint2v q = to_row8<LG, true>(f, scale);
+            if (!live) continue;
+            const Place p = place_of(a, slot, head);
+            if (values) cache_value8(a.vc, p, group, l.c0, q);
+            else cache_key8(a.kc, p, l, q);
+            if (j == 0) (values ? a.vs : a.ks)[p.scale] = scale;
+        } else {
+            if (!live) continue;
+            const Place p = place_of(a, slot, head);
+            if (values) cache_value16(a.vc, p, l.c0, raw);
+            else cache_key16(a.kc, p, l, raw);
+        }
+    }
+}
+
+template <bool BF, int LG, bool Q8>
+__global__ __launch_bounds__(kThreads) void kv_cache_read_kernel(HeadsArgs a) {
+    constexpr int TOKENS = kThreads / LG;
+    const int j = threadIdx.x % LG, sub = threadIdx.x / LG, group = value_group(Q8, a.D);
+    const bool values = (int)blockIdx.y >= a.Hkv;
+    const int head = values ? blockIdx.y - a.Hkv : blockIdx.y;
+    const Lane l = lane_of(j, a.D, 0, false);
+    half_t* out = values ? a.v : a.k;
+    for (int64_t t0 = (int64_t)blockIdx.x * TOKENS; t0 < a.T; t0 += (int64_t)gridDim.x * TOKENS) {
+        const int64_t t = t0 + sub;
+        if (t >= a.T || !l.in) continue;
+        const int slot = a.slots[t];
+        raw8 v = {};
+        if ((uint32_t)slot < (uint32_t)a.slots_end) {
+            const Place p = place_of(a, slot, head);
+            if constexpr (Q8) {
+                const float scale = (values ? a.vs : a.ks)[p.scale];
+                const int8_t* at = static_cast<const int8_t*>(values ? a.vc : a.kc) + p.block;
+                at += values ? value_place(group, p.t, l.c0) : key_place(true, p.t, l.c0);
+                const int step = values ? 4 * group : 1;
+                float f[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = (float)at[step * e] * scale;
+                v = act_cvt8<BF>(f);
+            } else {
+                const uint16_t* at = static_cast<const uint16_t*>(values ? a.vc : a.kc) + p.block;
+                at += values ? value_place(2, p.t, l.c0) : key_place(false, p.t, l.c0);
+                const int step = values ? 8 : 1;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = at[step * e];
+            }
+        }
+        store_head(out + (t * a.Hkv + head) * a.D, l, v);
+    }
+}
+
+// ---- host -----------------------------------------------------------------------------------
+
+int lanes_of(int64_t D) {
+    int lg = 1;
+    while (8 * lg < D) lg *= 2;
+    return lg;
+}
+int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+// Workgroups for T tokens: a launch takes fewer than 2^32 threads, and the kernels go round
+unsigned token_blocks(int64_t T, int lg) { return (unsigned)std::min<int64_t>((T + kThreads / lg - 1) / (kThreads / lg), 1 << 20); }
+
+#define CLK_LANES(X_) X_(1) X_(2) X_(4) X_(8) X_(16) X_(32)
+#define CLK_CACHE_LANES(X_) X_(4) X_(8) X_(16) X_(32)
+
+constexpr int64_t kMostHeads = 16384;
+
+// T, H and D of packed heads, the norms' weights and the angles: the checks of the norm's entry points
+int check_heads(const char* what, const clk_buffer* qkv, int64_t hkv, const clk_buffer* qn, const clk_buffer* kn,
+                const clk_buffer* rope, const clk_buffer* pos, float eps, HeadsArgs& a) {
+    const std::string w(what);
+    const int64_t T = qkv->dims[0], H = qkv->dims[1], D = qkv->dims[2];
+    if (D < 8 || D > 256 || D % 8) return invalid(w + ": D must be a multiple of 8 up to 256, got " + std::to_string(D));
+    if (hkv < 1 || H - 2 * hkv < 1) {
+        return invalid(w + ": qkv must be [T,Hq+2*Hkv,D] with at least one query and one key head, got " + std::to_string(H) +
+                       " heads and Hkv = " + std::to_string(hkv));
+    }
+    if (T < 0 || T > INT32_MAX || H > kMostHeads) return invalid(w + ": too large");
+    if (elements(qn) != D || elements(kn) != D) return invalid(w + ": q_norm and k_norm must be [D]");
+    if (rope->rank != 2 || rope->dims[0] < 1 || rope->dims[0] > INT32_MAX || rope->dims[1] < 8 || rope->dims[1] > D ||
+        rope->dims[1] % 8) {
+        return invalid(w + ": rope must be [P,R] with a row at least and R a multiple of 8 up to D");
+    }
+    if (pos->rank != 1 || pos->dims[0] != T) return invalid(w + ": positions must be [T]");
+    if (!(eps >= 0.f)) return invalid(w + ": eps must not be negative");
+    a.x = static_cast<const half_t*>(qkv->data);
+    a.qn = static_cast<const float*>(qn->data);
+    a.kn = static_cast<const float*>(kn->data);
+    a.rope = static_cast<const float*>(rope->data);
+    a.pos = static_cast<const int32_t*>(pos->data);
+    a.T = T;
+    a.Hq = (int)(H - 2 * hkv);
+    a.Hkv = (int)hkv;
+    a.D = (int)D;
+    a.R = (int)rope->dims[1];
+    a.P = (int)rope->dims[0];
+    a.inv_d = 1.f / (float)D;
+    a.eps = eps;
+    return CLK_OK;
+}
+bool is_heads(const clk_buffer* b, int64_t T, int64_t H, int64_t D) { return b->rank == 3 && dims_are(b, T, H, D); }
+
+int check_aligned(const char* what, std::initializer_list<const clk_buffer*> bufs) {
+    for (const clk_buffer* b : bufs) {
+        if (elements(b) > 0 && !aligned16(b->data)) return invalid(std::string(what) + ": buffers must be 16-byte aligned");
+    }
+    return CLK_OK;
+}
+void set_cache(HeadsArgs& a, const CacheShape& c, const clk_buffer* k, const clk_buffer* v, const clk_buffer* ks,
+               const clk_buffer* vs, const clk_buffer* slots) {
+    a.kc = k->data;
+    a.vc = v->data;
+    a.ks = static_cast<float*>(ks->data);
+    a.vs = static_cast<float*>(vs->data);
+    a.slots = static_cast<const int32_t*>(slots->data);
+    a.page = (int)c.page;
+    a.slots_end = (int)(c.pages * c.page);
+    a.by_page = fast_div(c.page);
+}
+
+template <int OUT>
+void launch_forward(HeadsArgs& a, bool bf, hipStream_t s) {
+    const int lg = lanes_of(a.D);
+    // Four heads a workgroup share a token's angles and keep four loads in flight; few tokens are spread over more
+    // workgroups instead.
+    const bool wide = a.T * (a.Hq + 2 * a.Hkv) * lg >= 4 * 256 * 1024;
+    const int hpg = wide ? 4 : 1;
+    a.cq = ceil_div(a.Hq, hpg);
+    a.ck = ceil_div(a.Hkv, hpg);
+    const dim3 grid(token_blocks(a.T, lg), a.cq + 2 * a.ck), block(kThreads);
+    const auto launch = [&](auto bf_, auto lg_) {
+        constexpr bool BF = decltype(bf_)::value;
+        constexpr int LG = decltype(lg_)::value;
+        if (wide) hipLaunchKernelGGL((qk_norm_rope_kernel<BF, LG, OUT, 4>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((qk_norm_rope_kernel<BF, LG, OUT, 1>), grid, block, 0, s, a);
+    };
+#define CLK_L(LG_)                                                                                  \
+    if (lg == LG_) {                                                                                \
+        if (bf) launch(std::true_type(), std::integral_constant<int, LG_>());                       \
+        else launch(std::false_type(), std::integral_constant<int, LG_>());                         \
+    }
+    if constexpr (OUT == kApart) {
+        CLK_LANES(CLK_L)
+    } else {
+        CLK_CACHE_LANES(CLK_L)
+    }
+#undef CLK_L
+}
+
+// The backward's workgroups a chunk of heads: a rule on the shape alone, so that results do not depend on the device.
+// About two rounds of what 256 CUs hold in all.
+int bwd_parts(int64_t T, int64_t Hq, int64_t Hkv, int64_t D) {
+    const int chunks = ceil_div(Hq, kBwdHeads) + 2 * ceil_div(Hkv, kBwdHeads), tokens = kThreads / lanes_of(D);
+    return (int)std::min<int64_t>((T + tokens - 1) / tokens, std::max(1, 2048 / chunks));
+}
+
+}  // namespace
+
+int check_cache(const char* what, const clk_buffer* k, const clk_buffer* v, const clk_buffer* ks, const clk_buffer* vs, int act,
+                CacheShape& c) {
+    const std::string w(what);
+    const int held = k != nullptr && k->dtype == CLK_S8 ? CLK_S8 : act;
+    const clk_buffer* bufs[] = {k, v, ks, vs};
+    const int types[] = {held, held, CLK_F32, CLK_F32};
+    if (int st = check_types((w + ": cache").c_str(), bufs, types, 4)) return st;
+    if (k->rank != 4 || !same_shape(k, v)) return invalid(w + ": k_cache and v_cache must be [pages,heads,page,D], alike");
+    c = CacheShape{k->dims[0], k->dims[1], k->dims[2], k->dims[3], held == CLK_S8};
+    if (c.D < 32 || c.D > 256 || c.D % 32) return invalid(w + ": a cache's D must be a multiple of 32 up to 256, got " + std::to_string(c.D));
+    if (c.page < 16 || c.page % 16) return invalid(w + ": a cache's page must be a multiple of 16, got " + std::to_string(c.page));
+    if (c.pages < 1 || c.heads < 1) return invalid(w + ": a cache must have a page and a head at least");
+    if (c.heads > 16384 || c.page > (1 << 20) || c.pages > INT32_MAX / c.page) return invalid(w + ": too large");
+    if (c.q8) {
+        for (const clk_buffer* s : {ks, vs}) {
+            if (s->rank != 3 || !dims_are(s, c.pages, c.heads, c.page)) return invalid(w + ": an 8-bit cache's scales must be [pages,heads,page]");
+        }
+    }
+    if (k->data == v->data) return invalid(w + ": k_cache and v_cache must not be the same buffer");
+    if (!aligned16(k->data) || !aligned16(v->data) || (c.q8 && (!aligned16(ks->data) || !aligned16(vs->data)))) {
+        return invalid(w + ": a cache's buffers must be 16-byte aligned");
+    }
+    return CLK_OK;
+}
+
+}  // namespace clk
+
+using namespace clk;
+
+extern "C" int clk_qk_norm_rope(clk_stream stream, const clk_buffer* qkv, const clk_buffer* q_norm, const clk_buffer* k_norm,
+                                const clk_buffer* rope, const clk_buffer* positions, const clk_buffer* q, const clk_buffer* k,
+                                const clk_buffer* v, float eps, int32_t interleaved) {
+    const int act = qkv != nullptr && qkv->dtype == CLK_BF16 ? CLK_BF16 : CLK_F16;
+    const clk_buffer* bufs[] = {qkv, q_norm, k_norm, rope, positions, q, k, v};
+    const int types[] = {act, CLK_F32, CLK_F32, CLK_F32, CLK_S32, act, act, act};
+    if (int st = check_types("qk_norm_rope", bufs, types, 8)) return st;
+    if (qkv->rank != 3 || k->rank != 3) return invalid("qk_norm_rope: qkv must be [T,Hq+2*Hkv,D], k [T,Hkv,D]");
+    HeadsArgs a{};
+    if (int st = check_heads("qk_norm_rope", qkv, k->dims[1], q_norm, k_norm, rope, positions, eps, a)) return st;
+    if (!is_heads(q, a.T, a.Hq, a.D) || !is_heads(k, a.T, a.Hkv, a.D) || !is_heads(v, a.T, a.Hkv, a.D)) {
+        return invalid("qk_norm_rope: q must be [T,Hq,D], k and v [T,Hkv,D]");
+    }
+    if (int st = check_aligned("qk_norm_rope", {qkv, rope, q, k, v})) return st;
+    if (a.T == 0) return ok();
+    a.q = static_cast<half_t*>(q->data);
+    a.k = static_cast<half_t*>(k->data);
+    a.v = static_cast<half_t*>(v->data);
+    a.interleaved = interleaved != 0;
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    stage_mark(s, 0);
+    launch_forward<kApart>(a, act == CLK_BF16, s);
+    stage_mark(s, 1);
+    return launch_status("qk_norm_rope");
+}
+
+extern "C" int clk_qk_norm_rope_cache(clk_stream stream, const clk_buffer* qkv, const clk_buffer* q_norm, const clk_buffer* k_norm,
+                                      const clk_buffer* rope, const clk_buffer* positions, const clk_buffer* slots,
+                                      const clk_buffer* q, const clk_buffer* k_cache, const clk_buffer* v_cache,
+                                      const clk_buffer* k_scale, const clk_buffer* v_scale, float eps, int32_t interleaved) {
+    const char* what = "qk_norm_rope_cache";
+    const int act = qkv != nullptr && qkv->dtype == CLK_BF16 ? CLK_BF16 : CLK_F16;
+    const clk_buffer* bufs[] = {qkv, q_norm, k_norm, rope, positions, slots, q};
+    const int types[] = {act, CLK_F32, CLK_F32, CLK_F32, CLK_S32, CLK_S32, act};
+    if (int st = check_types(what, bufs, types, 7)) return st;
+    CacheShape c;
+    if (int st = check_cache(what, k_cache, v_cache, k_scale, v_scale, act, c)) return st;
+    if (qkv->rank != 3) return invalid("qk_norm_rope_cache: qkv must be [T,Hq+2*Hkv,D]");
+    HeadsArgs a{};
+    if (int st = check_heads(what, qkv, c.heads, q_norm, k_norm, rope, positions, eps, a)) return st;
+    if (c.D != a.D) return invalid("qk_norm_rope_cache: qkv and the cache must have the same D");
+    if (!is_heads(q, a.T, a.Hq, a.D)) return invalid("qk_norm_rope_cache: q must be [T,Hq,D]");
+    if (slots->rank != 1 || slots->dims[0] != a.T) return invalid("qk_norm_rope_cache: slots must be [T]");
+    if (int st = check_aligned(what, {qkv, rope, q})) return st;
+    if (a.T == 0) return ok();
+    a.q = static_cast<half_t*>(q->data);
+    a.interleaved = interleaved != 0;
+    set_cache(a, c, k_cache, v_cache, k_scale, v_scale, slots);
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    stage_mark(s, 0);
+    if (c.q8) launch_forward<kCache8>(a, act == CLK_BF16, s);
+    else launch_forward<kCache16>(a, act == CLK_BF16, s);
+    stage_mark(s, 1);
+    return launch_status(what);
+}
+
+extern "C" size_t clk_qk_norm_rope_bwd_workspace_size(const clk_buffer* qkv, const clk_buffer* dk) {
+    if (qkv == nullptr || dk == nullptr || qkv->rank != 3 || dk->rank != 3 || qkv->dims == nullptr || dk->dims == nullptr) return 0;
+    const int64_t T = qkv->dims[0], H = qkv->dims[1], D = qkv->dims[2], hkv = dk->dims[1], hq = H - 2 * hkv;
+    if (T < 1 || T > INT32_MAX || H > kMostHeads || hkv < 1 || hq < 1 || D < 8 || D > 256 || D % 8) return 0;
+    const size_t rows = (size_t)bwd_parts(T, hq, hkv, D) * (ceil_div(hq, kBwdHeads) + ceil_div(hkv, kBwdHeads));
+    return (rows * D * 4 + 255) / 256 * 256;
+}
+
+extern "C" int clk_qk_norm_rope_bwd(clk_stream stream, const clk_buffer* qkv, const clk_buffer* q_norm, const clk_buffer* k_norm,
+                                    const clk_buffer* rope, const clk_buffer* positions, const clk_buffer* dq,
+                                    const clk_buffer* dk, const clk_buffer* dv, const clk_buffer* dqkv, const clk_buffer* dq_norm,
+                                    const clk_buffer* dk_norm, float eps, int32_t interleaved, void* workspace,
+                                    size_t workspace_bytes) {
+    const char* what = "qk_norm_rope_bwd";
+    const int act = qkv != nullptr && qkv->dtype == CLK_BF16 ? CLK_BF16 : CLK_F16;
+    const clk_buffer* bufs[] = {qkv, q_norm, k_norm, rope, positions, dq, dk, dv, dqkv, dq_norm, dk_norm};
+    const int types[] = {act, CLK_F32, CLK_F32, CLK_F32, CLK_S32, act, act, act, act, CLK_F32, CLK_F32};
+    if (int st = check_types(what, bufs, types, 11)) return st;
+    if (qkv->rank != 3 || dk->rank != 3) return invalid("qk_norm_rope_bwd: qkv must be [T,Hq+2*Hkv,D], dk [T,Hkv,D]");
+    HeadsArgs a{};
+    if (int st = check_heads(what, qkv, dk->dims[1], q_norm, k_norm, rope, positions, eps, a)) return st;
+    if (!is_heads(dq, a.T, a.Hq, a.D) || !is_heads(dk, a.T, a.Hkv, a.D) || !is_heads(dv, a.T, a.Hkv, a.D)) {
+        return invalid("qk_norm_rope_bwd: dq must be [T,Hq,D], dk and dv [T,Hkv,D]");
+    }
+    if (!same_shape(dqkv, qkv)) return invalid("qk_norm_rope_bwd: dqkv must be like qkv");
+    if (elements(dq_norm) != a.D || elements(dk_norm) != a.D) return invalid("qk_norm_rope_bwd: dq_norm and dk_norm must be [D]");
+    if (int st = check_aligned(what, {qkv, rope, dq, dk, dv, dqkv})) return st;
+    const size_t need = clk_qk_norm_rope_bwd_workspace_size(qkv, dk);
+    if (workspace_bytes < need || (need > 0 && workspace == nullptr)) {
+        return invalid("qk_norm_rope_bwd: workspace of " + std::to_string(workspace_bytes) + " bytes, needs " + std::to_string(need));
+    }
+    if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return invalid("qk_norm_rope_bwd: workspace must be 256-byte aligned");
+    a.dq = static_cast<const half_t*>(dq->data);
+    a.dk = static_cast<const half_t*>(dk->data);
+    a.dv = static_cast<const half_t*>(dv->data);
+    a.dx = static_cast<half_t*>(dqkv->data);
+    a.dqn = static_cast<float*>(dq_norm->data);
+    a.dkn = static_cast<float*>(dk_norm->data);
+    a.partial = static_cast<float*>(workspace);
+    a.interleaved = interleaved != 0;
+    a.cq = ceil_div(a.Hq, kBwdHeads);
+    a.ck = ceil_div(a.Hkv, kBwdHeads);
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    int stage = 0;
+    stage_mark(s, stage);
+    if (a.T > 0) {
+        a.parts = bwd_parts(a.T, a.Hq, a.Hkv, a.D);
+        const dim3 grid(a.parts, a.cq + 2 * a.ck), block(kThreads);
+        const int lg = lanes_of(a.D);
+#define CLK_L(LG_)                                                                                                    \
+    if (lg == LG_) {                                                                                                  \
+        if (act == CLK_BF16) hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<true, LG_>), grid, block, 0, s, a);          \
+        else hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<false, LG_>), grid, block, 0, s, a);                         \
+    }
+        CLK_LANES(CLK_L)
+#undef CLK_L
+        stage_mark(s, ++stage);
+    }
+    hipLaunchKernelGGL(qk_norm_dw_kernel, dim3(ceil_div(a.D, 16), 2), dim3(kThreads), 0, s, a);
+    stage_mark(s, ++stage);
+    return launch_status(what);
+}
+
+namespace clk {
+
+namespace {
+
+// What kv_cache_write and kv_cache_read share: k, v [T,Hkv,D] beside the cache
+int check_moved(const char* what, const clk_buffer* k, const clk_buffer* v, const clk_buffer* slots, const clk_buffer* k_cache,
+                const clk_buffer* v_cache, const clk_buffer* k_scale, const clk_buffer* v_scale, HeadsArgs& a, bool& q8, bool& bf) {
+    const int act = k != nullptr && k->dtype == CLK_BF16 ? CLK_BF16 : CLK_F16;
+    const clk_buffer* bufs[] = {k, v, slots};
+    const int types[] = {act, act, CLK_S32};
+    if (int st = check_types(what, bufs, types, 3)) return st;
+    CacheShape c;
+    if (int st = check_cache(what, k_cache, v_cache, k_scale, v_scale, act, c)) return st;
+    const int64_t T = k->rank == 3 ? k->dims[0] : -1;
+    if (T < 0 || !is_heads(k, T, c.heads, c.D) || !is_heads(v, T, c.heads, c.D)) {
+        return invalid(std::string(what) + ": k and v must be [T,heads,D], heads and D the cache's");
+    }
+    if (T > INT32_MAX) return invalid(std::string(what) + ": too large");
+    if (slots->rank != 1 || slots->dims[0] != T) return invalid(std::string(what) + ": slots must be [T]");
+    if (int st = check_aligned(what, {k, v})) return st;
+    a.T = T;
+    a.Hkv = (int)c.heads;
+    a.D = (int)c.D;
+    set_cache(a, c, k_cache, v_cache, k_scale, v_scale, slots);
+    q8 = c.q8;
+    bf = act == CLK_BF16;
+    return CLK_OK;
+}
+
+}  // namespace
+
+}  // namespace clk
+
+#define CLK_MOVE(KERNEL_)                                                                                              \
+    const int lg = lanes_of(a.D);                                                                                      \
+    const dim3 grid(token_blocks(a.T, lg), 2 * a.Hkv), block(kThreads);                                                \
+    const auto launch = [&](auto bf_, auto lg_) {                                                                      \
+        constexpr bool BF = decltype(bf_)::value;                                                                      \
+        constexpr int LG = decltype(lg_)::value;                                                                       \
+        if (q8) hipLaunchKernelGGL((KERNEL_<BF, LG, true>), grid, block, 0, s, a);                                     \
+        else hipLaunchKernelGGL((KERNEL_<BF, LG, false>), grid, block, 0, s, a);                                       \
+    };                                                                                                                 \
+    CLK_CACHE_LANES(CLK_L)
+#define CLK_L(LG_)                                                                                                     \
+    if (lg == LG_) {                                                                                                   \
+        if (bf) launch(std::true_type(), std::integral_constant<int, LG_>());                                          \
+        else launch(std::false_type(), std::integral_constant<int, LG_>());                                            \
+    }
+
+extern "C" int clk_kv_cache_write(clk_stream stream, const clk_buffer* k, const clk_buffer* v, const clk_buffer* slots,
+                                  const clk_buffer* k_cache, const clk_buffer* v_cache, const clk_buffer* k_scale,
+                                  const clk_buffer* v_scale) {
+    HeadsArgs a{};
+    bool q8, bf;
+    if (int st = check_moved("kv_cache_write", k, v, slots, k_cache, v_cache, k_scale, v_scale, a, q8, bf)) return st;
+    if (a.T == 0) return ok();
+    a.dk = static_cast<const half_t*>(k->data);
+    a.dv = static_cast<const half_t*>(v->data);
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    stage_mark(s, 0);
+    CLK_MOVE(kv_cache_write_kernel)
+    stage_mark(s, 1);
+    return launch_status("kv_cache_write");
+}
+
+extern "C" int clk_kv_cache_read(clk_stream stream, const clk_buffer* k_cache, const clk_buffer* v_cache, const clk_buffer* k_scale,
+                                 const clk_buffer* v_scale, const clk_buffer* slots, const clk_buffer* k, const clk_buffer* v) {
+    HeadsArgs a{};
+    bool q8, bf;
+    if (int st = check_moved("kv_cache_read", k, v, slots, k_cache, v_cache, k_scale, v_scale, a, q8, bf)) return st;
+    if (a.T == 0) return ok();
+    a.k = static_cast<half_t*>(k->data);
+    a.v = static_cast<half_t*>(v->data);
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    stage_mark(s, 0);
+    CLK_MOVE(kv_cache_read_kernel)
+    stage_mark(s, 1);
+    return launch_status("kv_cache_read");
+}

@@ -273,6 +273,84 @@ int clk_q8_projection(clk_stream stream, const clk_buffer* q, const clk_buffer* 
                       const clk_buffer* residual, const clk_buffer* out, int32_t has_b,
                       int32_t has_residual);
 
+/* ---- heads, the key-value cache and its attention (no counterpart in the reference) ------ */
+
+/* Activations (qkv, q, k, v, out and the gradients) are F16 or BF16, all of a call's one type, their buffers 16-byte
+ * aligned.
+ *
+ * A cache is a pair of buffers k_cache, v_cache [pages,heads,page,D], D a multiple of 32 up to 256 and page, the tokens of a
+ * page, a multiple of 16: of the activations' type, or S8 with k_scale, v_scale [pages,heads,page] F32 (for 16 bits any F32
+ * buffers, unread and unwritten). Token s % page of page s / page is slot s, and a cache holds fewer than 2^31. An 8-bit
+ * cache holds each token's head as an 8-bit row. Within a page's head, blocks of 16 tokens lie one after another:
+ *   keys    [D / W][16][W], W = 8 (16-bit) or 16 (8-bit) channels
+ *   values  [D / (16 C)][4][16][C][4]: token 4 g + j, channel 16 (C b + e) + i at [b][g][i][e][j], C = 2, or 4 for 8 bits
+ *           where D is a multiple of 64 */
+
+/* The queries, keys and values of a projection, qkv [T,Hq+2*Hkv,D] (query heads, then keys', then values'), apart and ready
+ * for attention: q [T,Hq,D], k and v [T,Hkv,D]. Each query and key head n = x / sqrt(mean(x^2) + eps) * w, w = q_norm or
+ * k_norm [D] F32, and its first R channels rotated by the angles of the token's position: pairs (a, b) = channels (i, i +
+ * R/2), or with interleaved (2 i, 2 i + 1), become (a cos - b sin, a sin + b cos), rounded once. Values are copied. rope [P,R] F32: the
+ * cosines of a position's R/2 angles, then their sines; positions [T] S32. A token whose position the table does not have
+ * gets NaN for its queries and keys. D and R multiples of 8, D up to 256, R up to D. */
+int clk_qk_norm_rope(clk_stream stream, const clk_buffer* qkv, const clk_buffer* q_norm,
+                     const clk_buffer* k_norm, const clk_buffer* rope, const clk_buffer* positions,
+                     const clk_buffer* q, const clk_buffer* k, const clk_buffer* v, float eps,
+                     int32_t interleaved);
+
+/* Its gradients: dq [T,Hq,D], dk, dv [T,Hkv,D] -> dqkv [T,Hq+2*Hkv,D] and dq_norm, dk_norm [D] F32, the sums over tokens and
+ * heads (zeros for T = 0). workspace: device scratch of at least clk_qk_norm_rope_bwd_workspace_size() bytes, 256-byte
+ * aligned, not shared by two calls in flight. Bit-identical from run to run (no atomics). */
+int clk_qk_norm_rope_bwd(clk_stream stream, const clk_buffer* qkv, const clk_buffer* q_norm,
+                         const clk_buffer* k_norm, const clk_buffer* rope,
+                         const clk_buffer* positions, const clk_buffer* dq, const clk_buffer* dk,
+                         const clk_buffer* dv, const clk_buffer* dqkv, const clk_buffer* dq_norm,
+                         const clk_buffer* dk_norm, float eps, int32_t interleaved,
+                         void* workspace, size_t workspace_bytes);
+
+/* Bytes of workspace clk_qk_norm_rope_bwd needs (0 on shapes that it would reject). */
+size_t clk_qk_norm_rope_bwd_workspace_size(const clk_buffer* qkv, const clk_buffer* dk);
+
+/* clk_qk_norm_rope with keys and values written into the cache, token t at slot slots[t] (S32 [T]), and q [T,Hq,D] beside.
+ * Keys of an 8-bit cache are quantised from fp32. A token whose slot the cache does not have (a negative one, as in
+ * the rows of a padded batch) writes nothing there. Two tokens of a call must not have the same slot: what it
+ * holds afterwards may be of either, value by value. */
+int clk_qk_norm_rope_cache(clk_stream stream, const clk_buffer* qkv, const clk_buffer* q_norm,
+                           const clk_buffer* k_norm, const clk_buffer* rope,
+                           const clk_buffer* positions, const clk_buffer* slots,
+                           const clk_buffer* q, const clk_buffer* k_cache,
+                           const clk_buffer* v_cache, const clk_buffer* k_scale,
+                           const clk_buffer* v_scale, float eps, int32_t interleaved);
+
+/* k, v [T,heads,D] into the cache as they are, token t at slot slots[t], with the rules of clk_qk_norm_rope_cache. */
+int clk_kv_cache_write(clk_stream stream, const clk_buffer* k, const clk_buffer* v,
+                       const clk_buffer* slots, const clk_buffer* k_cache,
+                       const clk_buffer* v_cache, const clk_buffer* k_scale,
+                       const clk_buffer* v_scale);
+
+/* k, v [T,heads,D] = what the slots hold, zeros for a slot that the cache does not have; 8-bit rows in k's type. A slot may
+ * be read any number of times. */
+int clk_kv_cache_read(clk_stream stream, const clk_buffer* k_cache, const clk_buffer* v_cache,
+                      const clk_buffer* k_scale, const clk_buffer* v_scale, const clk_buffer* slots,
+                      const clk_buffer* k, const clk_buffer* v);
+
+/* One new token's attention for each of B sequences: out [B,Hq,D] = softmax(scale q K^T) V over the first lengths[b] tokens of
+ * the pages page_table[b,:], query head h on the cache's head h / (Hq / heads). q [B,Hq,D]; page_table [B,N], lengths [B] S32;
+ * lse [B,Hq] F32 (with want_lse) = log2 of the sum of exp(scale q k), in the log2 domain. Statistics and sums are fp32. A
+ * sequence of no tokens (or a negative length) gives zeros, and -inf as lse. Entries of page_table past a sequence's last
+ * token are not read; a page among the others that the cache does not have, or a length past N pages, makes the
+ * sequence's results NaN. What pages hold past the last token does not matter. workspace: device scratch of at
+ * least clk_paged_attention_workspace_size() bytes, 256-byte aligned, not shared by two calls in flight.
+ * Bit-identical from run to run. */
+int clk_paged_attention(clk_stream stream, const clk_buffer* q, const clk_buffer* k_cache,
+                        const clk_buffer* v_cache, const clk_buffer* k_scale,
+                        const clk_buffer* v_scale, const clk_buffer* page_table,
+                        const clk_buffer* lengths, const clk_buffer* out, const clk_buffer* lse,
+                        float scale, int32_t want_lse, void* workspace, size_t workspace_bytes);
+
+/* Bytes of workspace clk_paged_attention needs (0 where it needs none, and on shapes that it would reject). */
+size_t clk_paged_attention_workspace_size(const clk_buffer* q, const clk_buffer* k_cache,
+                                          const clk_buffer* page_table);
+
 #ifdef __cplusplus
 }
 #endif
