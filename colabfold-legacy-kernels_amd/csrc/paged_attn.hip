@@ -23,9 +23,22 @@ namespace {
 
 typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
+typedef int int4v __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
 constexpr int kTile = 32;  // tokens a wave takes at a time
+constexpr int kChunk = kWaves * kTile;
+constexpr int kDirect = 512;
+
+// Workgroups a CU that the kernels' registers are kept for
+constexpr int occupancy(int64_t D) { return D <= 128 ? 3 : 2; }
+constexpr int kMostSplit = 256 * 3;
+
+// Weights are taken times 2^bias, which their sum has too and which cancels: fp16 ones so that small ones keep their bits (a
+// weight of 2^-25 of the largest, of which a long sequence may have millions, would be 0), bf16 ones so that
+// sums of values near the type's largest stay in fp32's range.
+template <bool MBF>
+constexpr float kBias = MBF ? -24.f : 15.f;
 
 struct AttnArgs {
     const half_t* q;  // [B, Hq, D]
@@ -37,10 +50,15 @@ struct AttnArgs {
     const int32_t* len;    // [B]
     half_t* out;
     float* lse;  // may be null
-    int B, Hkv, G, blocks;  // G query heads a head of keys, in blocks of 16
+    int B, Hkv, G, blocks, heads;  // G query heads a head of keys, in blocks of 16; heads = Hkv blocks: a sequence's items
     int per, pages, page;
-    FastDiv by_page, by_blocks, by_hkv;
+    FastDiv by_page, by_blocks, by_heads;
     float scale2;  // scale log2 e
+    // of a split call
+    int W;          // workgroups
+    float* part_o;  // [2 W][16][D]
+    float* part_s;  // [2 W][2][16]: running maximum, sum
+    int4v* meta;    // [B, Hkv, blocks]: the first and last workgroup of an item, and the first one's slot
 };
 
 template <bool BF>
@@ -99,25 +117,40 @@ struct Tile {
     float4v ks[2], vs[2];
 };
 
+// One item, the query heads 16 rb .. + 15 of head of keys h of sequence b, and tokens of it
+struct Span {
+    int b, h, rb, rows, from, to;
+    int64_t qrow;
+};
+__device__ __forceinline__ Span span_of(const AttnArgs& a, int b, int hr, int from, int to) {
+    Span s;
+    s.b = b;
+    s.h = fdiv(hr, a.by_blocks);
+    s.rb = hr - s.h * a.blocks;
+    s.rows = min(16, a.G - 16 * s.rb);
+    s.qrow = ((int64_t)b * a.Hkv + s.h) * a.G + 16 * s.rb;
+    s.from = from;
+    s.to = to;
+    return s;
+}
+
+// A wave's running maximum, sum and results: for query l % 16, o[e] channels 16 e + 4 g .. + 3
+template <int D>
+struct State {
+    float4v o[D / 16];
+    float m, l;
+    bool bad;  // a page that the cache does not have
+};
+
+// The wave's tiles of a span: every kWaves-th
 template <bool BF, bool Q8, int D>
-__global__ __launch_bounds__(kWaves * kWave) void paged_attn_kernel(AttnArgs a) {
+__device__ __forceinline__ void attend(const AttnArgs& a, const Span& sp, int wave, State<D>& st) {
     typedef Tile<Q8, D> T;
     constexpr int KS = D / 32, DB = D / 16, SIZE = Q8 ? 1 : 2;
-    constexpr bool MBF = BF || Q8;       // the products' operands are bf16
-    constexpr bool QLO = Q8 && !BF;      // fp16 queries in two bf16 parts, which is exact
-    constexpr float kBias = MBF ? -24.f : 15.f;
-    __shared__ float stat[kWaves][2][16];
-    __shared__ float acc[2][16][D + 4];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, i16 = lane & 15, g = lane >> 4;
-    int item = blockIdx.x;
-    const int seq_head = fdiv(item, a.by_blocks), rb = item - seq_head * a.blocks;
-    const int b = fdiv(seq_head, a.by_hkv), h = seq_head - b * a.Hkv;
-    const int rows = min(16, a.G - 16 * rb);
-    const int64_t qrow = ((int64_t)b * a.Hkv + h) * a.G + 16 * rb;
-    const int len = max(a.len[b], 0);
-    const int32_t* table = a.table + (int64_t)b * a.per;
-    bool bad = (int64_t)len > (int64_t)a.per * a.page;
-    const int keys = bad ? 0 : len;
+    constexpr bool MBF = BF || Q8;   // the products' operands are bf16
+    constexpr bool QLO = Q8 && !BF;  // fp16 queries in two bf16 parts, which is exact
+    const int lane = threadIdx.x % kWave, i16 = lane & 15, g = lane >> 4, keys = sp.to;
+    const int32_t* table = a.table + (int64_t)sp.b * a.per;
 
     // the queries' operands; channels in the order of the keys'
     half8 q[KS], qlo[QLO ? KS : 1];
@@ -126,7 +159,7 @@ __global__ __launch_bounds__(kWaves * kWave) void paged_attn_kernel(AttnArgs a) 
         const bool pair = Q8 && (s / 2 * 64 + 64 <= D);
         const int d = pair ? s / 2 * 64 + 16 * g + 8 * (s & 1) : 32 * s + 8 * g;
         uint4v raw{};
-        if (i16 < rows) raw = *reinterpret_cast<const uint4v*>(a.q + (qrow + i16) * D + d);
+        if (i16 < sp.rows) raw = *reinterpret_cast<const uint4v*>(a.q + (sp.qrow + i16) * D + d);
         q[s] = __builtin_bit_cast(half8, raw);
         if constexpr (QLO) {
             bf16x8 hi, lo;
@@ -141,12 +174,13 @@ __global__ __launch_bounds__(kWaves * kWave) void paged_attn_kernel(AttnArgs a) 
         }
     }
 
-    float4v o[DB];
 #pragma unroll
-    for (int e = 0; e < DB; ++e) o[e] = float4v{};
-    float m = -__builtin_inff(), l = 0.f;
+    for (int e = 0; e < DB; ++e) st.o[e] = float4v{};
+    st.m = -__builtin_inff();
+    st.l = 0.f;
+    st.bad = false;
 
-    for (int k0 = wave * kTile; k0 < keys; k0 += kWaves * kTile) {
+    for (int k0 = sp.from + wave * kTile; k0 < keys; k0 += kWaves * kTile) {
         T t;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
@@ -154,10 +188,10 @@ __global__ __launch_bounds__(kWaves * kWave) void paged_attn_kernel(AttnArgs a) 
             const int p = fdiv(at, a.by_page);
             int page = table[p];  // one that the cache does not have: page 0, and NaN in the end
             if ((uint32_t)page >= (uint32_t)a.pages) {
-                bad = true;
+                st.bad = true;
                 page = 0;
             }
-            const int64_t row = ((int64_t)page * a.Hkv + h) * a.page + (at - p * a.page);
+            const int64_t row = ((int64_t)page * a.Hkv + sp.h) * a.page + (at - p * a.page);
             const char* kb = a.kc + row * (D * SIZE);
             const char* vb = a.vc + row * (D * SIZE);
 #pragma unroll
@@ -211,20 +245,20 @@ __global__ __launch_bounds__(kWaves * kWave) void paged_attn_kernel(AttnArgs a) 
             }
         }
         top = wave_xor_max4(top);
-        const float m_new = fmaxf(m, top);
-        const float base = (m_new == -__builtin_inff() ? 0.f : m_new) - kBias;
-        const float alpha = exp2_fast(m - kBias - base);
-        l *= alpha;
+        const float m_new = fmaxf(st.m, top);
+        const float base = (m_new == -__builtin_inff() ? 0.f : m_new) - kBias<MBF>;
+        const float alpha = exp2_fast(st.m - kBias<MBF> - base);
+        st.l *= alpha;
 #pragma unroll
-        for (int e = 0; e < DB; ++e) o[e] *= alpha;
-        m = m_new;
+        for (int e = 0; e < DB; ++e) st.o[e] *= alpha;
+        st.m = m_new;
         float pf[8];
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float x = exp2_fast(s2[n][i] - base);
-                l += x;
+                st.l += x;
                 if constexpr (Q8) x = k0 + 16 * n + 4 * g + i < keys ? x * t.vs[n][i] : 0.f;
                 pf[4 * n + i] = x;
             }
@@ -251,50 +285,276 @@ __global__ __launch_bounds__(kWaves * kWave) void paged_attn_kernel(AttnArgs a) 
             } else {
                 op = join(bf16_of_bytes(t.v[0][s][c]), bf16_of_bytes(t.v[1][s][c]));
             }
-            o[e] = mfma<MBF>(op, p, o[e]);
-            o[e] = mfma<MBF>(op, plo, o[e]);
+            st.o[e] = mfma<MBF>(op, p, st.o[e]);
+            st.o[e] = mfma<MBF>(op, plo, st.o[e]);
         }
     }
+}
 
-    // the waves' parts, joined in LDS
-    l = wave_xor_sum4(l);
+// The waves' states as one, in wave 0 (its m and l are of the query l % 16 in every lane)
+template <int D>
+struct WaveShare {
+    float stat[kWaves][2][16];
+    float acc[2][16][D + 4];
+};
+template <int D>
+__device__ __forceinline__ void join_waves(State<D>& st, int wave, WaveShare<D>& share) {
+    const int lane = threadIdx.x % kWave, i16 = lane & 15, g = lane >> 4;
+    const float l = wave_xor_sum4(st.l);
     if (g == 0) {
-        stat[wave][0][i16] = m;
-        stat[wave][1][i16] = bad ? __builtin_nanf("") : l;
+        share.stat[wave][0][i16] = st.m;
+        share.stat[wave][1][i16] = st.bad ? __builtin_nanf("") : l;
     }
     __syncthreads();
     float m_all = -__builtin_inff(), l_all = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) m_all = fmaxf(m_all, stat[w][0][i16]);
+    for (int w = 0; w < kWaves; ++w) m_all = fmaxf(m_all, share.stat[w][0][i16]);
     const float m_ref = m_all == -__builtin_inff() ? 0.f : m_all;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) l_all += stat[w][1][i16] * exp2_fast(stat[w][0][i16] - m_ref);
-    const float mine = exp2_fast(m - m_ref);
+    for (int w = 0; w < kWaves; ++w) l_all += share.stat[w][1][i16] * exp2_fast(share.stat[w][0][i16] - m_ref);
+    const float mine = exp2_fast(st.m - m_ref);
 #pragma unroll
-    for (int e = 0; e < DB; ++e) o[e] *= mine;
+    for (int e = 0; e < D / 16; ++e) st.o[e] *= mine;
 #pragma unroll
-    for (int half = 2; half >= 1; half /= 2) {
+    for (int half = kWaves / 2; half >= 1; half /= 2) {
         if (wave >= half && wave < 2 * half) {
 #pragma unroll
-            for (int e = 0; e < DB; ++e) *reinterpret_cast<float4v*>(&acc[wave - half][i16][16 * e + 4 * g]) = o[e];
+            for (int e = 0; e < D / 16; ++e) *reinterpret_cast<float4v*>(&share.acc[wave - half][i16][16 * e + 4 * g]) = st.o[e];
         }
         __syncthreads();
         if (wave < half) {
 #pragma unroll
-            for (int e = 0; e < DB; ++e) o[e] += *reinterpret_cast<const float4v*>(&acc[wave][i16][16 * e + 4 * g]);
+            for (int e = 0; e < D / 16; ++e) st.o[e] += *reinterpret_cast<const float4v*>(&share.acc[wave][i16][16 * e + 4 * g]);
         }
         __syncthreads();
     }
-    if (wave != 0 || i16 >= rows) return;
-    const bool none = len == 0;
-    const float inv = 1.f / l_all;
+    st.m = m_all;
+    st.l = l_all;
+}
+
+// Results from a whole span's state
+template <bool BF, bool Q8, int D>
+__device__ __forceinline__ void finish(const AttnArgs& a, const Span& sp, const State<D>& st) {
+    const int lane = threadIdx.x % kWave, i16 = lane & 15, g = lane >> 4;
+    if (i16 >= sp.rows) return;
+    const float inv = 1.f / st.l;
 #pragma unroll
-    for (int e = 0; e < DB; ++e) {
-        float4v r = o[e] * inv;
-        if (none) r = float4v{};
-        *reinterpret_cast<raw4*>(a.out + (qrow + i16) * D + 16 * e + 4 * g) = act_cvt4<BF>(r);
+    for (int e = 0; e < D / 16; ++e) {
+        *reinterpret_cast<raw4*>(a.out + (sp.qrow + i16) * D + 16 * e + 4 * g) = act_cvt4<BF>(st.o[e] * inv);
     }
-    if (a.lse != nullptr && g == 0) a.lse[qrow + i16] = none ? -__builtin_inff() : m_all + (__builtin_amdgcn_logf(l_all) - kBias);
+    if (a.lse != nullptr && g == 0) a.lse[sp.qrow + i16] = st.m + (__builtin_amdgcn_logf(st.l) - kBias<BF || Q8>);
+}
+
+// Results of a sequence of no tokens (zeros), or of one with more than its pages hold (NaN), for columns from `col` on
+template <bool BF, int D>
+__device__ __forceinline__ void finish_empty(const AttnArgs& a, const Span& sp, bool bad, int first, int last) {
+    const float v = bad ? __builtin_nanf("") : 0.f;
+    const raw4 r = act_cvt4<BF>(float4v{v, v, v, v});
+    const int cols = (last - first) / 4;
+    for (int i = threadIdx.x; i < sp.rows * cols; i += kWaves * kWave) {
+        *reinterpret_cast<raw4*>(a.out + (sp.qrow + i / cols) * D + first + i % cols * 4) = r;
+    }
+    if (a.lse != nullptr && first == 0 && (int)threadIdx.x < sp.rows) a.lse[sp.qrow + threadIdx.x] = bad ? v : -__builtin_inff();
+}
+
+// A workgroup an item: for caches that no sequence can have more than kDirect tokens in
+template <bool BF, bool Q8, int D>
+__global__ __launch_bounds__(kWaves* kWave, occupancy(D)) void paged_attn_kernel(AttnArgs a) {
+    __shared__ WaveShare<D> share;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int b = fdiv(blockIdx.x, a.by_heads);
+    const int len = a.len[b];
+    const bool bad = (int64_t)len > (int64_t)a.per * a.page;
+    const Span sp = span_of(a, b, blockIdx.x - b * a.heads, 0, len);
+    if (bad || len <= 0) {
+        finish_empty<BF, D>(a, sp, bad, 0, D);
+        return;
+    }
+    State<D> st;
+    attend<BF, Q8, D>(a, sp, wave, st);
+    join_waves<D>(st, wave, share);
+    if (wave == 0) finish<BF, Q8, D>(a, sp, st);
+}
+
+// Chunks of a sequence: what the workgroups of a split call are dealt
+__device__ __forceinline__ int chunks_of(const AttnArgs& a, int b) {
+    const int len = a.len[b];
+    return len <= 0 || (int64_t)len > (int64_t)a.per * a.page ? 0 : (len + kChunk - 1) / kChunk;
+}
+
+// All items' chunks, one after another, in W equal runs, one a workgroup: however the lengths differ, every workgroup reads as
+// much. An item that one workgroup has whole is finished there; of one that several have, each leaves its part for
+// paged_attn_join_kernel, in its slot 0 if the run begins with it and 1 if not. meta says which.
+template <bool BF, bool Q8, int D>
+__global__ __launch_bounds__(kWaves* kWave, occupancy(D)) void paged_attn_split_kernel(AttnArgs a) {
+    constexpr int THREADS = kWaves * kWave;
+    __shared__ WaveShare<D> share;
+    __shared__ int64_t wave_sums[kWaves];
+    __shared__ int64_t begin[2];  // the sequence that the run begins in, and the chunks before that sequence
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
+    // chunks before each thread's sequences, and of all
+    const int per = (a.B + THREADS - 1) / THREADS, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
+    int64_t mine = 0;
+    for (int b = b0; b < b1; ++b) mine += chunks_of(a, b);
+    int64_t upto = mine;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        const int64_t v = __shfl_up(upto, d);
+        if (lane >= d) upto += v;
+    }
+    if (lane == kWave - 1) wave_sums[wave] = upto;
+    __syncthreads();
+    int64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        if (w < wave) upto += wave_sums[w];
+        total += wave_sums[w];
+    }
+    const int64_t U = total * a.heads, W = min<int64_t>(a.W, U);  // each of W has a chunk at least
+    if (blockIdx.x >= W) return;
+    const int64_t start = U * blockIdx.x / W, end = U * (blockIdx.x + 1) / W;
+    {
+        int64_t before = upto - mine;
+        if (before * a.heads <= start && start < upto * a.heads) {
+            int b = b0;
+            for (int n = chunks_of(a, b); (before + n) * a.heads <= start; n = chunks_of(a, ++b)) before += n;
+            begin[0] = b;
+            begin[1] = before;
+        }
+    }
+    __syncthreads();
+    int b = __builtin_amdgcn_readfirstlane((int)begin[0]);
+    int n = __builtin_amdgcn_readfirstlane(chunks_of(a, b));
+    const uint64_t in = (uint64_t)(start - begin[1] * a.heads);
+    int hr = __builtin_amdgcn_readfirstlane((int)(in / (uint32_t)n)), chunk = __builtin_amdgcn_readfirstlane((int)(in - (uint64_t)hr * n));
+    int64_t left = end - start;
+    for (bool first = true; left > 0; first = false) {
+        const int take = (int)min<int64_t>(left, n - chunk);
+        const Span sp = span_of(a, b, hr, chunk * kChunk, min(a.len[b], (chunk + take) * kChunk));
+        State<D> st;
+        attend<BF, Q8, D>(a, sp, wave, st);
+        join_waves<D>(st, wave, share);
+        const int64_t slot = 2 * (int64_t)blockIdx.x + !first;
+        if (wave == 0) {
+            const int i16 = lane & 15, g = lane >> 4;
+            if (chunk == 0 && take == n) {
+                finish<BF, Q8, D>(a, sp, st);
+            } else if (i16 < sp.rows) {
+#pragma unroll
+                for (int e = 0; e < D / 16; ++e) {
+                    *reinterpret_cast<float4v*>(a.part_o + (slot * 16 + i16) * D + 16 * e + 4 * g) = st.o[e];
+                }
+                if (g == 0) {
+                    a.part_s[slot * 32 + i16] = st.m;
+                    a.part_s[slot * 32 + 16 + i16] = st.l;
+                }
+            }
+            if (chunk == 0 && lane == 0) {
+                const uint64_t last = (uint64_t)(end - left) + n;  // one past the item's chunks
+                a.meta[(int64_t)b * a.heads + hr] = int4v{(int)blockIdx.x, (int)((last * (uint64_t)W - 1) / (uint64_t)U), (int)!first, 0};
+            }
+        }
+        left -= take;
+        chunk = 0;
+        if (++hr == a.heads && left > 0) {
+            hr = 0;
+            do n = __builtin_amdgcn_readfirstlane(chunks_of(a, ++b));
+            while (n == 0);
+        }
+    }
+}
+
+// The parts of an item that several workgroups had, in their order; 32 channels of it a workgroup (blockIdx.y)
+template <bool BF, bool MBF, int D>
+__global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
+    constexpr int GROUPS = 8;
+    __shared__ float weight[kMostSplit + 1][16];
+    __shared__ float sums[16][17];
+    __shared__ float m_of[16], l_of[16];
+    __shared__ float parts[GROUPS][16][33];
+    const int tid = threadIdx.x, b = fdiv(blockIdx.x, a.by_heads);
+    const int len = a.len[b];
+    const bool bad = (int64_t)len > (int64_t)a.per * a.page;
+    const Span sp = span_of(a, b, blockIdx.x - b * a.heads, 0, len);
+    const int d0 = 32 * blockIdx.y;
+    if (bad || len <= 0) {
+        finish_empty<BF, D>(a, sp, bad, d0, d0 + 32);
+        return;
+    }
+    const int4v meta = a.meta[blockIdx.x];
+    const int n = meta[1] - meta[0] + 1;
+    if (n == 1) return;
+    const auto slot = [&](int p) { return 2 * (int64_t)(meta[0] + p) + (p == 0 ? meta[2] : 0); };
+    {  // thread (p0, r): parts p0, p0 + 16, .. of row r
+        const int r = tid & 15, p0 = tid >> 4;
+        float m = -__builtin_inff(), l = 0.f;
+        for (int p = p0; p < n; p += 16) {
+            const float v = r < sp.rows ? a.part_s[slot(p) * 32 + r] : 0.f;
+            weight[p][r] = v;
+            m = fmaxf(m, v);
+        }
+        sums[p0][r] = m;
+        __syncthreads();
+        for (int i = 0; i < 16; ++i) m = fmaxf(m, sums[i][r]);
+        const float ref = m == -__builtin_inff() ? 0.f : m;
+        for (int p = p0; p < n; p += 16) {
+            const float w = exp2_fast(weight[p][r] - ref);
+            weight[p][r] = w;
+            l += w * (r < sp.rows ? a.part_s[slot(p) * 32 + 16 + r] : 0.f);
+        }
+        __syncthreads();
+        sums[p0][r] = l;
+        __syncthreads();
+        if (p0 == 0) {
+            l = 0.f;
+            for (int i = 0; i < 16; ++i) l += sums[i][r];
+            m_of[r] = m;
+            l_of[r] = l;
+        }
+    }
+    const int c = tid & 31, grp = tid >> 5;
+    for (int r = 0; r < sp.rows; ++r) {
+        float o = 0.f;
+        for (int p = grp; p < n; p += GROUPS) o = __builtin_fmaf(weight[p][r], a.part_o[(slot(p) * 16 + r) * D + d0 + c], o);
+        parts[grp][r][c] = o;
+    }
+    __syncthreads();
+    for (int i = tid; i < sp.rows * 8; i += 256) {
+        const int r = i >> 3, at = (i & 7) * 4;
+        const float inv = 1.f / l_of[r];
+        float4v v{};
+#pragma unroll
+        for (int k = 0; k < GROUPS; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += parts[k][r][at + e];
+        *reinterpret_cast<raw4*>(a.out + (sp.qrow + r) * D + d0 + at) = act_cvt4<BF>(v * inv);
+    }
+    if (a.lse != nullptr && d0 == 0 && tid < sp.rows) a.lse[sp.qrow + tid] = m_of[tid] + (__builtin_amdgcn_logf(l_of[tid]) - kBias<MBF>);
+}
+
+// ---- host -----------------------------------------------------------------------------------
+
+// How a call is run: a rule on the shapes alone, so that results do not depend on the device
+struct Plan {
+    int64_t items = 0;  // 0: a shape that the entry point rejects
+    int W = 0;          // workgroups of a split call, 0: one an item
+    size_t o = 0, s = 0, meta = 0;
+    size_t bytes() const { return o + s + meta; }
+};
+Plan plan_of(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t per, int64_t page) {
+    Plan p;
+    if (B < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || per < 1 || page < 16 || page % 16 || D < 32 || D > 256 || D % 32) return p;
+    const int64_t blocks = (Hq / Hkv + 15) / 16;
+    if (Hkv > 16384 || blocks > 16384 || Hkv * blocks > 16384 || B > (1 << 23) / (Hkv * blocks) || per > (1 << 30) / page) return p;
+    p.items = B * Hkv * blocks;
+    const int64_t chunks = (per * page + kChunk - 1) / kChunk;
+    if (chunks * kChunk > kDirect) {
+        p.W = (int)std::min<int64_t>(std::max<int64_t>(1, p.items) * chunks, 256 * occupancy(D));
+        p.o = (size_t)2 * p.W * 16 * D * 4;
+        p.s = (size_t)2 * p.W * 32 * 4;
+        p.meta = (size_t)(p.items * 16 + 255) / 256 * 256;
+    }
+    return p;
 }
 
 }  // namespace
@@ -304,7 +564,11 @@ __global__ __launch_bounds__(kWaves * kWave) void paged_attn_kernel(AttnArgs a) 
 using namespace clk;
 
 extern "C" size_t clk_paged_attention_workspace_size(const clk_buffer* q, const clk_buffer* k_cache, const clk_buffer* page_table) {
-    return 0;
+    for (const clk_buffer* b : {q, k_cache, page_table}) {
+        if (b == nullptr || b->dims == nullptr) return 0;
+    }
+    if (q->rank != 3 || k_cache->rank != 4 || page_table->rank != 2) return 0;
+    return plan_of(q->dims[0], q->dims[1], k_cache->dims[1], k_cache->dims[3], page_table->dims[1], k_cache->dims[2]).bytes();
 }
 
 extern "C" int clk_paged_attention(clk_stream stream, const clk_buffer* q, const clk_buffer* k_cache, const clk_buffer* v_cache,
@@ -330,11 +594,15 @@ extern "C" int clk_paged_attention(clk_stream stream, const clk_buffer* q, const
     if (want_lse && (lse->rank != 2 || lse->dims[0] != B || lse->dims[1] != Hq)) return invalid("paged_attention: lse must be [B,Hq]");
     if (!(scale == scale) || scale - scale != 0.f) return invalid("paged_attention: scale must be finite");
     const int64_t G = Hq / c.heads, blocks = (G + 15) / 16;
-    if (B > INT32_MAX / (c.heads * blocks) || B * c.heads * blocks >= (1 << 24) || page_table->dims[1] > (1 << 30) / c.page) {
-        return invalid("paged_attention: too large");
-    }
+    const Plan plan = plan_of(B, Hq, c.heads, c.D, page_table->dims[1], c.page);
+    if (B > 0 && plan.items == 0) return invalid("paged_attention: too large");
     if (B > 0 && (!aligned16(q->data) || !aligned16(out->data))) return invalid("paged_attention: q and out must be 16-byte aligned");
     if (B == 0) return ok();
+    const size_t need = plan.bytes();
+    if (workspace_bytes < need || (need > 0 && workspace == nullptr)) {
+        return invalid("paged_attention: workspace of " + std::to_string(workspace_bytes) + " bytes, needs " + std::to_string(need));
+    }
+    if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return invalid("paged_attention: workspace must be 256-byte aligned");
     AttnArgs a{};
     a.q = static_cast<const half_t*>(q->data);
     a.kc = static_cast<const char*>(k_cache->data);
@@ -354,20 +622,32 @@ extern "C" int clk_paged_attention(clk_stream stream, const clk_buffer* q, const
     a.page = (int)c.page;
     a.by_page = fast_div(c.page);
     a.by_blocks = fast_div(blocks);
-    a.by_hkv = fast_div(c.heads);
+    a.heads = (int)(c.heads * blocks);
+    a.by_heads = fast_div(a.heads);
     a.scale2 = scale * kLog2e;
+    a.W = plan.W;
+    char* ws = static_cast<char*>(workspace);
+    a.part_o = reinterpret_cast<float*>(ws);
+    a.part_s = reinterpret_cast<float*>(ws + plan.o);
+    a.meta = reinterpret_cast<int4v*>(ws + plan.o + plan.s);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    stage_mark(s, 0);
-    const dim3 grid((unsigned)(B * c.heads * blocks)), block(kWaves * kWave);
-    const auto launch = [&](auto d_) {
+    int stage = 0;
+    stage_mark(s, stage);
+    const dim3 block(kWaves * kWave);
+    const auto kernels = [&](auto bf_, auto q8_, auto d_) {
+        constexpr bool BF = decltype(bf_)::value, Q8 = decltype(q8_)::value;
         constexpr int D = decltype(d_)::value;
-        if (act == CLK_BF16) {
-            if (c.q8) hipLaunchKernelGGL((paged_attn_kernel<true, true, D>), grid, block, 0, s, a);
-            else hipLaunchKernelGGL((paged_attn_kernel<true, false, D>), grid, block, 0, s, a);
-        } else {
-            if (c.q8) hipLaunchKernelGGL((paged_attn_kernel<false, true, D>), grid, block, 0, s, a);
-            else hipLaunchKernelGGL((paged_attn_kernel<false, false, D>), grid, block, 0, s, a);
+        if (plan.W == 0) {
+            hipLaunchKernelGGL((paged_attn_kernel<BF, Q8, D>), dim3((unsigned)plan.items), block, 0, s, a);
+            return;
         }
+        hipLaunchKernelGGL((paged_attn_split_kernel<BF, Q8, D>), dim3(plan.W), block, 0, s, a);
+        stage_mark(s, ++stage);
+        hipLaunchKernelGGL((paged_attn_join_kernel<BF, BF || Q8, D>), dim3((unsigned)plan.items, D / 32), dim3(256), 0, s, a);
+    };
+    const auto launch = [&](auto d_) {
+        if (act == CLK_BF16) c.q8 ? kernels(std::true_type(), std::true_type(), d_) : kernels(std::true_type(), std::false_type(), d_);
+        else c.q8 ? kernels(std::false_type(), std::true_type(), d_) : kernels(std::false_type(), std::false_type(), d_);
     };
     switch (c.D) {
     case 32: launch(std::integral_constant<int, 32>()); break;
@@ -379,6 +659,6 @@ extern "C" int clk_paged_attention(clk_stream stream, const clk_buffer* q, const
     case 224: launch(std::integral_constant<int, 224>()); break;
     default: launch(std::integral_constant<int, 256>()); break;
     }
-    stage_mark(s, 1);
+    stage_mark(s, ++stage);
     return launch_status(what);
 }

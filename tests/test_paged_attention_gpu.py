@@ -105,6 +105,10 @@ def test_lengths_and_heads(hip, lengths, hq, hkv, d, page, bits, kind):
         c.check(out, lse, scale)
         again, none = hip.paged_attention(c.q, c.cache, c.table, c.len, scale)
         assert none is None and torch.equal(again, out)
+        wide = torch.nn.functional.pad(c.table, (0, 1 + 5000 // page), value=-7)  # room for long sequences: split calls
+        out, lse = hip.paged_attention(c.q, c.cache, wide, c.len, scale, want_lse=True)
+        c.check(out, lse, scale)
+        assert torch.equal(hip.paged_attention(c.q, c.cache, wide, c.len, scale)[0], out)
 
 
 @pytest.mark.parametrize("kind", TYPES)
@@ -125,8 +129,9 @@ def test_batches(hip, b, bits, kind):
 def test_many_short_sequences(hip, bits):
     lengths = [i % 5 for i in range(4100)]
     c = Case(lengths, 2, 1, 32, 16, bits, "f16")
-    out, lse = hip.paged_attention(c.q, c.cache, c.table, c.len, want_lse=True)
-    c.check(out, lse, 32 ** -0.5, only=list(range(0, 4100, 37)) + [4099])
+    for table in (c.table, torch.nn.functional.pad(c.table, (0, 40), value=-1)):
+        out, lse = hip.paged_attention(c.q, c.cache, table, c.len, want_lse=True)
+        c.check(out, lse, 32 ** -0.5, only=list(range(0, 4100, 37)) + [4099])
 
 
 @pytest.mark.parametrize("kind", TYPES)
