@@ -58,7 +58,7 @@ struct AttnArgs {
     int W;          // workgroups
     float* part_o;  // [2 W][16][D]
     float* part_s;  // [2 W][2][16]: running maximum, sum
-    int4v* meta;    // [B, Hkv, blocks]: the first and last workgroup of an item, and the first one's slot
+    int4v* meta;    // [W]: the item that a workgroup began and did not finish, its parts (0: none), the first one's slot
 };
 
 template <bool BF>
@@ -345,16 +345,13 @@ __device__ __forceinline__ void finish(const AttnArgs& a, const Span& sp, const 
     if (a.lse != nullptr && g == 0) a.lse[sp.qrow + i16] = st.m + (__builtin_amdgcn_logf(st.l) - kBias<BF || Q8>);
 }
 
-// Results of a sequence of no tokens (zeros), or of one with more than its pages hold (NaN), for columns from `col` on
+// Results of a sequence of no tokens (zeros), or of one with more than its pages hold (NaN)
 template <bool BF, int D>
-__device__ __forceinline__ void finish_empty(const AttnArgs& a, const Span& sp, bool bad, int first, int last) {
+__device__ __forceinline__ void finish_empty(const AttnArgs& a, const Span& sp, bool bad) {
     const float v = bad ? __builtin_nanf("") : 0.f;
     const raw4 r = act_cvt4<BF>(float4v{v, v, v, v});
-    const int cols = (last - first) / 4;
-    for (int i = threadIdx.x; i < sp.rows * cols; i += kWaves * kWave) {
-        *reinterpret_cast<raw4*>(a.out + (sp.qrow + i / cols) * D + first + i % cols * 4) = r;
-    }
-    if (a.lse != nullptr && first == 0 && (int)threadIdx.x < sp.rows) a.lse[sp.qrow + threadIdx.x] = bad ? v : -__builtin_inff();
+    for (int i = threadIdx.x; i < sp.rows * (D / 4); i += kWaves * kWave) *reinterpret_cast<raw4*>(a.out + sp.qrow * D + 4 * i) = r;
+    if (a.lse != nullptr && (int)threadIdx.x < sp.rows) a.lse[sp.qrow + threadIdx.x] = bad ? v : -__builtin_inff();
 }
 
 // A workgroup an item: for caches that no sequence can have more than kDirect tokens in
@@ -367,7 +364,7 @@ __global__ __launch_bounds__(kWaves* kWave, occupancy(D)) void paged_attn_kernel
     const bool bad = (int64_t)len > (int64_t)a.per * a.page;
     const Span sp = span_of(a, b, blockIdx.x - b * a.heads, 0, len);
     if (bad || len <= 0) {
-        finish_empty<BF, D>(a, sp, bad, 0, D);
+        finish_empty<BF, D>(a, sp, bad);
         return;
     }
     State<D> st;
@@ -384,7 +381,8 @@ __device__ __forceinline__ int chunks_of(const AttnArgs& a, int b) {
 
 // All items' chunks, one after another, in W equal runs, one a workgroup: however the lengths differ, every workgroup reads as
 // much. An item that one workgroup has whole is finished there; of one that several have, each leaves its part for
-// paged_attn_join_kernel, in its slot 0 if the run begins with it and 1 if not. meta says which.
+// paged_attn_join_kernel, in its slot 0 if the run begins with it and 1 if not. meta says which. Sequences of no tokens
+// are nobody's and get their results from every W-th workgroup.
 template <bool BF, bool Q8, int D>
 __global__ __launch_bounds__(kWaves* kWave, occupancy(D)) void paged_attn_split_kernel(AttnArgs a) {
     constexpr int THREADS = kWaves * kWave;
@@ -411,7 +409,16 @@ __global__ __launch_bounds__(kWaves* kWave, occupancy(D)) void paged_attn_split_
         total += wave_sums[w];
     }
     const int64_t U = total * a.heads, W = min<int64_t>(a.W, U);  // each of W has a chunk at least
-    if (blockIdx.x >= W) return;
+    for (int b = blockIdx.x; b < a.B; b += a.W) {
+        if (chunks_of(a, b) != 0) continue;
+        const bool bad = a.len[b] > 0;
+        for (int hr = 0; hr < a.heads; ++hr) finish_empty<BF, D>(a, span_of(a, b, hr, 0, 0), bad);
+    }
+    int4v unfinished{};
+    if (blockIdx.x >= W) {
+        if (tid == 0) a.meta[blockIdx.x] = unfinished;
+        return;
+    }
     const int64_t start = U * blockIdx.x / W, end = U * (blockIdx.x + 1) / W;
     {
         int64_t before = upto - mine;
@@ -449,9 +456,9 @@ __global__ __launch_bounds__(kWaves* kWave, occupancy(D)) void paged_attn_split_
                     a.part_s[slot * 32 + 16 + i16] = st.l;
                 }
             }
-            if (chunk == 0 && lane == 0) {
+            if (chunk == 0 && take < n) {
                 const uint64_t last = (uint64_t)(end - left) + n;  // one past the item's chunks
-                a.meta[(int64_t)b * a.heads + hr] = int4v{(int)blockIdx.x, (int)((last * (uint64_t)W - 1) / (uint64_t)U), (int)!first, 0};
+                unfinished = int4v{b * a.heads + hr, (int)((last * (uint64_t)W - 1) / (uint64_t)U) - (int)blockIdx.x + 1, (int)!first, 0};
             }
         }
         left -= take;
@@ -462,74 +469,78 @@ __global__ __launch_bounds__(kWaves* kWave, occupancy(D)) void paged_attn_split_
             while (n == 0);
         }
     }
+    if (tid == 0) a.meta[blockIdx.x] = unfinished;
 }
 
-// The parts of an item that several workgroups had, in their order; 32 channels of it a workgroup (blockIdx.y)
+// The parts of the item that workgroup blockIdx.x of the split began and did not finish, in their order: one of its rows
+// (blockIdx.y) a workgroup, its parts dealt to four waves. What it waits for is a chain of loads, so the first
+// parts' results are on their way before the weights are known, and eight a wave from then on.
 template <bool BF, bool MBF, int D>
-__global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
-    constexpr int GROUPS = 8;
-    __shared__ float weight[kMostSplit + 1][16];
-    __shared__ float sums[16][17];
-    __shared__ float m_of[16], l_of[16];
-    __shared__ float parts[GROUPS][16][33];
-    const int tid = threadIdx.x, b = fdiv(blockIdx.x, a.by_heads);
-    const int len = a.len[b];
-    const bool bad = (int64_t)len > (int64_t)a.per * a.page;
-    const Span sp = span_of(a, b, blockIdx.x - b * a.heads, 0, len);
-    const int d0 = 32 * blockIdx.y;
-    if (bad || len <= 0) {
-        finish_empty<BF, D>(a, sp, bad, d0, d0 + 32);
-        return;
-    }
+__global__ __launch_bounds__(kWaves* kWave) void paged_attn_join_kernel(AttnArgs a) {
+    constexpr int COLS = D <= 128 ? 2 : 4, EARLY = 4, AT_ONCE = 8;  // channels a lane; parts a wave
+    typedef float cols __attribute__((ext_vector_type(COLS)));
+    __shared__ float weight[kMostSplit + 1];
+    __shared__ float red[2][kWaves];
+    __shared__ float parts[kWaves][D];
     const int4v meta = a.meta[blockIdx.x];
-    const int n = meta[1] - meta[0] + 1;
-    if (n == 1) return;
-    const auto slot = [&](int p) { return 2 * (int64_t)(meta[0] + p) + (p == 0 ? meta[2] : 0); };
-    {  // thread (p0, r): parts p0, p0 + 16, .. of row r
-        const int r = tid & 15, p0 = tid >> 4;
-        float m = -__builtin_inff(), l = 0.f;
-        for (int p = p0; p < n; p += 16) {
-            const float v = r < sp.rows ? a.part_s[slot(p) * 32 + r] : 0.f;
-            weight[p][r] = v;
-            m = fmaxf(m, v);
-        }
-        sums[p0][r] = m;
-        __syncthreads();
-        for (int i = 0; i < 16; ++i) m = fmaxf(m, sums[i][r]);
-        const float ref = m == -__builtin_inff() ? 0.f : m;
-        for (int p = p0; p < n; p += 16) {
-            const float w = exp2_fast(weight[p][r] - ref);
-            weight[p][r] = w;
-            l += w * (r < sp.rows ? a.part_s[slot(p) * 32 + 16 + r] : 0.f);
-        }
-        __syncthreads();
-        sums[p0][r] = l;
-        __syncthreads();
-        if (p0 == 0) {
-            l = 0.f;
-            for (int i = 0; i < 16; ++i) l += sums[i][r];
-            m_of[r] = m;
-            l_of[r] = l;
-        }
+    const int n = meta[1], r = blockIdx.y;
+    if (n == 0) return;
+    const int b = fdiv(meta[0], a.by_heads);
+    const Span sp = span_of(a, b, meta[0] - b * a.heads, 0, 0);
+    if (r >= sp.rows) return;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
+    const auto slot = [&](int p) { return 2 * (int64_t)(blockIdx.x + p) + (p == 0 ? meta[2] : 0); };
+    const int col = min(lane * COLS, D - COLS);
+    const auto part = [&](int p) { return *reinterpret_cast<const cols*>(a.part_o + (slot(p) * 16 + r) * D + col); };
+    cols early[EARLY];
+#pragma unroll
+    for (int k = 0; k < EARLY; ++k) early[k] = part(min(wave + kWaves * k, n - 1));
+    float m = -__builtin_inff(), l = 0.f;
+    for (int p = tid; p < n; p += kWaves * kWave) {
+        weight[p] = a.part_s[slot(p) * 32 + r];
+        m = fmaxf(m, weight[p]);
     }
-    const int c = tid & 31, grp = tid >> 5;
-    for (int r = 0; r < sp.rows; ++r) {
-        float o = 0.f;
-        for (int p = grp; p < n; p += GROUPS) o = __builtin_fmaf(weight[p][r], a.part_o[(slot(p) * 16 + r) * D + d0 + c], o);
-        parts[grp][r][c] = o;
-    }
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
+    if (lane == 0) red[0][wave] = m;
     __syncthreads();
-    for (int i = tid; i < sp.rows * 8; i += 256) {
-        const int r = i >> 3, at = (i & 7) * 4;
-        const float inv = 1.f / l_of[r];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, red[0][w]);
+    const float ref = m == -__builtin_inff() ? 0.f : m;
+    for (int p = tid; p < n; p += kWaves * kWave) {
+        const float w = exp2_fast(weight[p] - ref);
+        weight[p] = w;
+        l += w * a.part_s[slot(p) * 32 + 16 + r];
+    }
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) l += __shfl_xor(l, d);
+    if (lane == 0) red[1][wave] = l;
+    __syncthreads();
+    l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+    cols o{};
+#pragma unroll
+    for (int k = 0; k < EARLY; ++k) {
+        const int p = wave + kWaves * k;
+        if (p < n) o += early[k] * weight[p];
+    }
+    for (int p = wave + kWaves * EARLY; p < n; p += kWaves * AT_ONCE) {
+        cols v[AT_ONCE];
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) v[k] = part(min(p + kWaves * k, n - 1));
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+            if (p + kWaves * k < n) o += v[k] * weight[p + kWaves * k];
+        }
+    }
+    *reinterpret_cast<cols*>(&parts[wave][col]) = o;
+    __syncthreads();
+    if (tid < D / 4) {
         float4v v{};
 #pragma unroll
-        for (int k = 0; k < GROUPS; ++k)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] += parts[k][r][at + e];
-        *reinterpret_cast<raw4*>(a.out + (sp.qrow + r) * D + d0 + at) = act_cvt4<BF>(v * inv);
+        for (int w = 0; w < kWaves; ++w) v += *reinterpret_cast<const float4v*>(&parts[w][4 * tid]);
+        *reinterpret_cast<raw4*>(a.out + (sp.qrow + r) * D + 4 * tid) = act_cvt4<BF>(v * (1.f / l));
     }
-    if (a.lse != nullptr && d0 == 0 && tid < sp.rows) a.lse[sp.qrow + tid] = m_of[tid] + (__builtin_amdgcn_logf(l_of[tid]) - kBias<MBF>);
+    if (a.lse != nullptr && tid == 0) a.lse[sp.qrow + r] = m + (__builtin_amdgcn_logf(l) - kBias<MBF>);
 }
 
 // ---- host -----------------------------------------------------------------------------------
@@ -552,7 +563,7 @@ Plan plan_of(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t per, int64_t
         p.W = (int)std::min<int64_t>(std::max<int64_t>(1, p.items) * chunks, 256 * occupancy(D));
         p.o = (size_t)2 * p.W * 16 * D * 4;
         p.s = (size_t)2 * p.W * 32 * 4;
-        p.meta = (size_t)(p.items * 16 + 255) / 256 * 256;
+        p.meta = (size_t)p.W * 16;
     }
     return p;
 }
@@ -643,7 +654,7 @@ extern "C" int clk_paged_attention(clk_stream stream, const clk_buffer* q, const
         }
         hipLaunchKernelGGL((paged_attn_split_kernel<BF, Q8, D>), dim3(plan.W), block, 0, s, a);
         stage_mark(s, ++stage);
-        hipLaunchKernelGGL((paged_attn_join_kernel<BF, BF || Q8, D>), dim3((unsigned)plan.items, D / 32), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((paged_attn_join_kernel<BF, BF || Q8, D>), dim3(plan.W, (unsigned)std::min<int64_t>(G, 16)), block, 0, s, a);
     };
     const auto launch = [&](auto d_) {
         if (act == CLK_BF16) c.q8 ? kernels(std::true_type(), std::true_type(), d_) : kernels(std::true_type(), std::false_type(), d_);
