@@ -61,6 +61,16 @@ struct AttnArgs {
     int4v* meta;    // [W]: the item that a workgroup began and did not finish, its parts (0: none), the first one's slot
 };
 
+// A wave-uniform value on the scalar unit, and a scalar load from an array that the kernel does not write: a page's number
+// by a vector load would be waited for behind all keys and values in flight.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    return (int64_t)((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v));
+}
+__device__ __forceinline__ int scalar_load(const int32_t* p, int64_t i) {
+    return reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p))[i];
+}
+
 template <bool BF>
 __device__ __forceinline__ float4v mfma(half8 a, half8 b, float4v c) {
     if constexpr (BF) {
@@ -142,11 +152,76 @@ struct State {
     bool bad;  // a page that the cache does not have
 };
 
-// The wave's tiles of a span: every kWaves-th
+// Where a tile's two blocks lie in the cache, in tokens x heads, and whether they hold tokens of the span: a block past it (or
+// on a page that the cache does not have, which sets bad) is loaded as zeros, by a buffer of no bytes
+struct Where {
+    int64_t row[2];
+    bool in[2];
+};
+__device__ __forceinline__ Where where_of(const AttnArgs& a, const Span& sp, const int32_t* table, int k0, int keys, bool& bad) {
+    Where w;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const int at = k0 + 16 * n;
+        w.in[n] = at < keys;
+        const int in_span = w.in[n] ? at : sp.from, p = fdiv(in_span, a.by_page), page = scalar_load(table, p);
+        if ((uint32_t)page >= (uint32_t)a.pages) {
+            w.in[n] = false;
+            bad = true;
+        }
+        w.row[n] = w.in[n] ? ((int64_t)page * a.Hkv + sp.h) * a.page + (in_span - p * a.page) : 0;
+    }
+    return w;
+}
+template <typename P>
+__device__ __forceinline__ auto rsrc_of(const P* p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<P*>(p), 0, bytes, 0x00020000);
+}
+template <typename Rsrc>
+__device__ __forceinline__ uint4v load16(Rsrc r, uint32_t off) {
+    return __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+}
+template <typename Rsrc>
+__device__ __forceinline__ uint4v load8(Rsrc r, uint32_t off) {
+    const uint2v w = __builtin_bit_cast(uint2v, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
+    return uint4v{w[0], w[1], 0, 0};
+}
+template <bool Q8, int D>
+__device__ __forceinline__ void load_keys(const AttnArgs& a, const Where& at, int lane, Tile<Q8, D>& t) {
+    constexpr int SIZE = Q8 ? 1 : 2;
+    const int i16 = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const auto r = rsrc_of(a.kc + at.row[n] * (D * SIZE), at.in[n] ? 16 * D * SIZE : 0);
+#pragma unroll
+        for (int s = 0; s < Tile<Q8, D>::NK; ++s) {
+            if (!Q8 || s * 64 + 64 <= D) t.k[n][s] = load16(r, lane * 16 + s * 1024);
+            else t.k[n][s] = load8(r, (g >> 1) * 256 + i16 * 16 + (g & 1) * 8 + s * 1024);
+        }
+        if constexpr (Q8) t.ks[n] = __builtin_bit_cast(float4v, load16(rsrc_of(a.ks + at.row[n], at.in[n] ? 64 : 0), g * 16));
+    }
+}
+template <bool Q8, int D>
+__device__ __forceinline__ void load_values(const AttnArgs& a, const Where& at, int lane, Tile<Q8, D>& t) {
+    constexpr int SIZE = Q8 ? 1 : 2;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const auto r = rsrc_of(a.vc + at.row[n] * (D * SIZE), at.in[n] ? 16 * D * SIZE : 0);
+#pragma unroll
+        for (int s = 0; s < Tile<Q8, D>::NV; ++s) {
+            if constexpr (Tile<Q8, D>::C * SIZE == 4) t.v[n][s] = load16(r, lane * 16 + s * 1024);
+            else t.v[n][s] = load8(r, lane * 8 + s * 512);
+        }
+        if constexpr (Q8) t.vs[n] = __builtin_bit_cast(float4v, load16(rsrc_of(a.vs + at.row[n], at.in[n] ? 64 : 0), (lane >> 4) * 16));
+    }
+}
+
+// The wave's tiles of a span: every kWaves-th. The next tile's keys are loaded as soon as this one's scores have been
+// computed, into the same registers, and its values as soon as the results have: each load has half a tile's work to arrive in.
 template <bool BF, bool Q8, int D>
 __device__ __forceinline__ void attend(const AttnArgs& a, const Span& sp, int wave, State<D>& st) {
     typedef Tile<Q8, D> T;
-    constexpr int KS = D / 32, DB = D / 16, SIZE = Q8 ? 1 : 2;
+    constexpr int KS = D / 32, DB = D / 16;
     constexpr bool MBF = BF || Q8;   // the products' operands are bf16
     constexpr bool QLO = Q8 && !BF;  // fp16 queries in two bf16 parts, which is exact
     const int lane = threadIdx.x % kWave, i16 = lane & 15, g = lane >> 4, keys = sp.to;
@@ -180,45 +255,14 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Span& sp, int wa
     st.l = 0.f;
     st.bad = false;
 
-    for (int k0 = sp.from + wave * kTile; k0 < keys; k0 += kWaves * kTile) {
-        T t;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const int at = k0 + 16 * n < keys ? k0 + 16 * n : k0;
-            const int p = fdiv(at, a.by_page);
-            int page = table[p];  // one that the cache does not have: page 0, and NaN in the end
-            if ((uint32_t)page >= (uint32_t)a.pages) {
-                st.bad = true;
-                page = 0;
-            }
-            const int64_t row = ((int64_t)page * a.Hkv + sp.h) * a.page + (at - p * a.page);
-            const char* kb = a.kc + row * (D * SIZE);
-            const char* vb = a.vc + row * (D * SIZE);
-#pragma unroll
-            for (int s = 0; s < T::NK; ++s) {
-                if constexpr (!Q8) {
-                    t.k[n][s] = *reinterpret_cast<const uint4v*>(kb + s * 1024 + lane * 16);
-                } else if (s * 64 + 64 <= D) {
-                    t.k[n][s] = *reinterpret_cast<const uint4v*>(kb + s * 1024 + lane * 16);
-                } else {
-                    const uint2v w = *reinterpret_cast<const uint2v*>(kb + s * 1024 + (g >> 1) * 256 + i16 * 16 + (g & 1) * 8);
-                    t.k[n][s] = uint4v{w[0], w[1], 0, 0};
-                }
-            }
-#pragma unroll
-            for (int s = 0; s < T::NV; ++s) {
-                if constexpr (T::C * SIZE == 4) {
-                    t.v[n][s] = *reinterpret_cast<const uint4v*>(vb + s * 1024 + lane * 16);
-                } else {
-                    const uint2v w = *reinterpret_cast<const uint2v*>(vb + s * 512 + lane * 8);
-                    t.v[n][s] = uint4v{w[0], w[1], 0, 0};
-                }
-            }
-            if constexpr (Q8) {
-                t.ks[n] = *reinterpret_cast<const float4v*>(a.ks + row + 4 * g);
-                t.vs[n] = *reinterpret_cast<const float4v*>(a.vs + row + 4 * g);
-            }
-        }
+    int k0 = sp.from + wave * kTile;
+    if (k0 >= keys) return;
+    T t;
+    Where at = where_of(a, sp, table, k0, keys, st.bad);
+    load_keys<Q8, D>(a, at, lane, t);
+    load_values<Q8, D>(a, at, lane, t);
+    for (;;) {
+        const Where next = where_of(a, sp, table, k0 + kWaves * kTile, keys, st.bad);
         float s2[2][4], top = -__builtin_inff();
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
@@ -244,14 +288,17 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Span& sp, int wa
                 top = fmaxf(top, s2[n][i]);
             }
         }
+        load_keys<Q8, D>(a, next, lane, t);
         top = wave_xor_max4(top);
-        const float m_new = fmaxf(st.m, top);
-        const float base = (m_new == -__builtin_inff() ? 0.f : m_new) - kBias<MBF>;
-        const float alpha = exp2_fast(st.m - kBias<MBF> - base);
-        st.l *= alpha;
+        if (__any(top > st.m)) {
+            const float m_new = fmaxf(st.m, top);
+            const float alpha = m_new == st.m ? 1.f : exp2_fast(st.m - m_new);
+            st.l *= alpha;
 #pragma unroll
-        for (int e = 0; e < DB; ++e) st.o[e] *= alpha;
-        st.m = m_new;
+            for (int e = 0; e < DB; ++e) st.o[e] *= alpha;
+            st.m = m_new;
+        }
+        const float base = (st.m == -__builtin_inff() ? 0.f : st.m) - kBias<MBF>;
         float pf[8];
 #pragma unroll
         for (int n = 0; n < 2; ++n)
@@ -288,6 +335,9 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Span& sp, int wa
             st.o[e] = mfma<MBF>(op, p, st.o[e]);
             st.o[e] = mfma<MBF>(op, plo, st.o[e]);
         }
+        k0 += kWaves * kTile;
+        if (k0 >= keys) return;
+        load_values<Q8, D>(a, next, lane, t);
     }
 }
 
@@ -358,9 +408,9 @@ __device__ __forceinline__ void finish_empty(const AttnArgs& a, const Span& sp, 
 template <bool BF, bool Q8, int D>
 __global__ __launch_bounds__(kWaves* kWave, occupancy(D)) void paged_attn_kernel(AttnArgs a) {
     __shared__ WaveShare<D> share;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int wave = uniform((int)(threadIdx.x / kWave));
     const int b = fdiv(blockIdx.x, a.by_heads);
-    const int len = a.len[b];
+    const int len = scalar_load(a.len, b);
     const bool bad = (int64_t)len > (int64_t)a.per * a.page;
     const Span sp = span_of(a, b, blockIdx.x - b * a.heads, 0, len);
     if (bad || len <= 0) {
@@ -374,10 +424,10 @@ __global__ __launch_bounds__(kWaves* kWave, occupancy(D)) void paged_attn_kernel
 }
 
 // Chunks of a sequence: what the workgroups of a split call are dealt
-__device__ __forceinline__ int chunks_of(const AttnArgs& a, int b) {
-    const int len = a.len[b];
+__device__ __forceinline__ int chunks_in(const AttnArgs& a, int len) {
     return len <= 0 || (int64_t)len > (int64_t)a.per * a.page ? 0 : (len + kChunk - 1) / kChunk;
 }
+__device__ __forceinline__ int chunks_of(const AttnArgs& a, int b) { return chunks_in(a, a.len[b]); }
 
 // All items' chunks, one after another, in W equal runs, one a workgroup: however the lengths differ, every workgroup reads as
 // much. An item that one workgroup has whole is finished there; of one that several have, each leaves its part for
@@ -389,7 +439,7 @@ __global__ __launch_bounds__(kWaves* kWave, occupancy(D)) void paged_attn_split_
     __shared__ WaveShare<D> share;
     __shared__ int64_t wave_sums[kWaves];
     __shared__ int64_t begin[2];  // the sequence that the run begins in, and the chunks before that sequence
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
+    const int tid = threadIdx.x, wave = uniform((int)(tid / kWave)), lane = tid % kWave;
     // chunks before each thread's sequences, and of all
     const int per = (a.B + THREADS - 1) / THREADS, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
     int64_t mine = 0;
@@ -408,6 +458,7 @@ __global__ __launch_bounds__(kWaves* kWave, occupancy(D)) void paged_attn_split_
         if (w < wave) upto += wave_sums[w];
         total += wave_sums[w];
     }
+    total = uniform(total);
     const int64_t U = total * a.heads, W = min<int64_t>(a.W, U);  // each of W has a chunk at least
     for (int b = blockIdx.x; b < a.B; b += a.W) {
         if (chunks_of(a, b) != 0) continue;
@@ -430,14 +481,14 @@ __global__ __launch_bounds__(kWaves* kWave, occupancy(D)) void paged_attn_split_
         }
     }
     __syncthreads();
-    int b = __builtin_amdgcn_readfirstlane((int)begin[0]);
-    int n = __builtin_amdgcn_readfirstlane(chunks_of(a, b));
-    const uint64_t in = (uint64_t)(start - begin[1] * a.heads);
-    int hr = __builtin_amdgcn_readfirstlane((int)(in / (uint32_t)n)), chunk = __builtin_amdgcn_readfirstlane((int)(in - (uint64_t)hr * n));
+    int b = uniform((int)begin[0]);
+    int len = scalar_load(a.len, b), n = chunks_in(a, len);
+    const uint64_t in = (uint64_t)(start - uniform(begin[1]) * a.heads);
+    int hr = uniform((int)(in / (uint32_t)n)), chunk = uniform((int)(in - (uint64_t)hr * n));
     int64_t left = end - start;
     for (bool first = true; left > 0; first = false) {
-        const int take = (int)min<int64_t>(left, n - chunk);
-        const Span sp = span_of(a, b, hr, chunk * kChunk, min(a.len[b], (chunk + take) * kChunk));
+        const int take = uniform((int)min<int64_t>(left, n - chunk));
+        const Span sp = span_of(a, b, hr, chunk * kChunk, min(len, (chunk + take) * kChunk));
         State<D> st;
         attend<BF, Q8, D>(a, sp, wave, st);
         join_waves<D>(st, wave, share);
@@ -465,8 +516,10 @@ __global__ __launch_bounds__(kWaves* kWave, occupancy(D)) void paged_attn_split_
         chunk = 0;
         if (++hr == a.heads && left > 0) {
             hr = 0;
-            do n = __builtin_amdgcn_readfirstlane(chunks_of(a, ++b));
-            while (n == 0);
+            do {
+                len = scalar_load(a.len, ++b);
+                n = chunks_in(a, len);
+            } while (n == 0);
         }
     }
     if (tid == 0) a.meta[blockIdx.x] = unfinished;
@@ -488,7 +541,7 @@ __global__ __launch_bounds__(kWaves* kWave) void paged_attn_join_kernel(AttnArgs
     const int b = fdiv(meta[0], a.by_heads);
     const Span sp = span_of(a, b, meta[0] - b * a.heads, 0, 0);
     if (r >= sp.rows) return;
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
+    const int tid = threadIdx.x, wave = uniform((int)(tid / kWave)), lane = tid % kWave;
     const auto slot = [&](int p) { return 2 * (int64_t)(blockIdx.x + p) + (p == 0 ? meta[2] : 0); };
     const int col = min(lane * COLS, D - COLS);
     const auto part = [&](int p) { return *reinterpret_cast<const cols*>(a.part_o + (slot(p) * 16 + r) * D + col); };
