@@ -55,10 +55,11 @@ struct AttnArgs {
     FastDiv by_page, by_blocks, by_heads;
     float scale2;  // scale log2 e
     // of a split call
-    int W;          // workgroups
+    int W;          // workgroups that fill the chip
     float* part_o;  // [2 W][16][D]
     float* part_s;  // [2 W][2][16]: running maximum, sum
-    int4v* meta;    // [W]: the item that a workgroup began and did not finish, its parts (0: none), the first one's slot
+    int4v* split;   // [W]: an item in parts, its first part and how many it has
+    int* meta;      // the items in parts
 };
 
 // A wave-uniform value on the scalar unit, and a scalar load from an array that the kernel does not write: a page's number
@@ -341,58 +342,51 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Span& sp, int wa
     }
 }
 
-// The waves' states as one, in wave 0 (its m and l are of the query l % 16 in every lane)
+// What the workgroup's waves have of a span, summed: each of the rows' channels by one thread, four at a time, as results
+// (part_o null) or as a part for paged_attn_join_kernel. One barrier.
 template <int D>
 struct WaveShare {
     float stat[kWaves][2][16];
-    float acc[2][16][D + 4];
+    float acc[kWaves][16][D + 4];
 };
-template <int D>
-__device__ __forceinline__ void join_waves(State<D>& st, int wave, WaveShare<D>& share) {
+template <bool BF, bool MBF, int D>
+__device__ __forceinline__ void join_waves(const AttnArgs& a, const Span& sp, const State<D>& st, int wave, WaveShare<D>& share,
+                                           float* part_o, float* part_s) {
     const int lane = threadIdx.x % kWave, i16 = lane & 15, g = lane >> 4;
     const float l = wave_xor_sum4(st.l);
-    if (g == 0) {
-        share.stat[wave][0][i16] = st.m;
-        share.stat[wave][1][i16] = st.bad ? __builtin_nanf("") : l;
+    if (i16 < sp.rows) {
+        if (g == 0) {
+            share.stat[wave][0][i16] = st.m;
+            share.stat[wave][1][i16] = st.bad ? __builtin_nanf("") : l;
+        }
+#pragma unroll
+        for (int e = 0; e < D / 16; ++e) *reinterpret_cast<float4v*>(&share.acc[wave][i16][16 * e + 4 * g]) = st.o[e];
     }
     __syncthreads();
-    float m_all = -__builtin_inff(), l_all = 0.f;
+    for (int i = threadIdx.x; i < sp.rows * (D / 4); i += kWaves * kWave) {
+        const int r = i / (D / 4), d = 4 * (i % (D / 4));
+        float m = share.stat[0][0][r], sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) m_all = fmaxf(m_all, share.stat[w][0][i16]);
-    const float m_ref = m_all == -__builtin_inff() ? 0.f : m_all;
+        for (int w = 1; w < kWaves; ++w) m = fmaxf(m, share.stat[w][0][r]);
+        const float ref = m == -__builtin_inff() ? 0.f : m;
+        float4v o{};
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) l_all += share.stat[w][1][i16] * exp2_fast(share.stat[w][0][i16] - m_ref);
-    const float mine = exp2_fast(st.m - m_ref);
-#pragma unroll
-    for (int e = 0; e < D / 16; ++e) st.o[e] *= mine;
-#pragma unroll
-    for (int half = kWaves / 2; half >= 1; half /= 2) {
-        if (wave >= half && wave < 2 * half) {
-#pragma unroll
-            for (int e = 0; e < D / 16; ++e) *reinterpret_cast<float4v*>(&share.acc[wave - half][i16][16 * e + 4 * g]) = st.o[e];
+        for (int w = 0; w < kWaves; ++w) {
+            const float f = exp2_fast(share.stat[w][0][r] - ref);
+            sum += f * share.stat[w][1][r];
+            o += f * *reinterpret_cast<const float4v*>(&share.acc[w][r][d]);
         }
-        __syncthreads();
-        if (wave < half) {
-#pragma unroll
-            for (int e = 0; e < D / 16; ++e) st.o[e] += *reinterpret_cast<const float4v*>(&share.acc[wave][i16][16 * e + 4 * g]);
+        if (part_o != nullptr) {
+            *reinterpret_cast<float4v*>(part_o + r * D + d) = o;
+            if (d == 0) {
+                part_s[r] = m;
+                part_s[16 + r] = sum;
+            }
+        } else {
+            *reinterpret_cast<raw4*>(a.out + (sp.qrow + r) * D + d) = act_cvt4<BF>(o * (1.f / sum));
+            if (a.lse != nullptr && d == 0) a.lse[sp.qrow + r] = m + (__builtin_amdgcn_logf(sum) - kBias<MBF>);
         }
-        __syncthreads();
     }
-    st.m = m_all;
-    st.l = l_all;
-}
-
-// Results from a whole span's state
-template <bool BF, bool Q8, int D>
-__device__ __forceinline__ void finish(const AttnArgs& a, const Span& sp, const State<D>& st) {
-    const int lane = threadIdx.x % kWave, i16 = lane & 15, g = lane >> 4;
-    if (i16 >= sp.rows) return;
-    const float inv = 1.f / st.l;
-#pragma unroll
-    for (int e = 0; e < D / 16; ++e) {
-        *reinterpret_cast<raw4*>(a.out + (sp.qrow + i16) * D + 16 * e + 4 * g) = act_cvt4<BF>(st.o[e] * inv);
-    }
-    if (a.lse != nullptr && g == 0) a.lse[sp.qrow + i16] = st.m + (__builtin_amdgcn_logf(st.l) - kBias<BF || Q8>);
 }
 
 // Results of a sequence of no tokens (zeros), or of one with more than its pages hold (NaN)
@@ -419,114 +413,79 @@ __global__ __launch_bounds__(kWaves* kWave, occupancy(D)) void paged_attn_kernel
     }
     State<D> st;
     attend<BF, Q8, D>(a, sp, wave, st);
-    join_waves<D>(st, wave, share);
-    if (wave == 0) finish<BF, Q8, D>(a, sp, st);
+    join_waves<BF, BF || Q8, D>(a, sp, st, wave, share, nullptr, nullptr);
 }
 
-// Chunks of a sequence: what the workgroups of a split call are dealt
+// Chunks of a sequence
 __device__ __forceinline__ int chunks_in(const AttnArgs& a, int len) {
     return len <= 0 || (int64_t)len > (int64_t)a.per * a.page ? 0 : (len + kChunk - 1) / kChunk;
 }
-__device__ __forceinline__ int chunks_of(const AttnArgs& a, int b) { return chunks_in(a, a.len[b]); }
+// Parts of a sequence's items, c chunks each at most; a sequence of no tokens has one, which writes its results
+__device__ __forceinline__ int parts_in(int chunks, int c) { return chunks <= c ? 1 : (chunks - 1) / c + 1; }
 
-// All items' chunks, one after another, in W equal runs, one a workgroup: however the lengths differ, every workgroup reads as
-// much. An item that one workgroup has whole is finished there; of one that several have, each leaves its part for
-// paged_attn_join_kernel, in its slot 0 if the run begins with it and 1 if not. meta says which. Sequences of no tokens
-// are nobody's and get their results from every W-th workgroup.
+// Items in parts of about as many chunks, however the lengths differ, one a workgroup. c, the most chunks of a part, is what
+// fills W workgroups, all at once on the chip: items take up to half of them for their last, shorter parts. Items of one part are
+// finished here; parts of the others are numbered through and left for paged_attn_join_kernel.
+// (All chunks in W equal runs, one a workgroup, where a run could end one item and begin the next, was more even but a
+// workgroup had two short spans as often as one, each with its chain of loads: 61 sequences of up to 8192 over 8 bits
+// took 43 us.)
 template <bool BF, bool Q8, int D>
 __global__ __launch_bounds__(kWaves* kWave, occupancy(D)) void paged_attn_split_kernel(AttnArgs a) {
-    constexpr int THREADS = kWaves * kWave;
     __shared__ WaveShare<D> share;
-    __shared__ int64_t wave_sums[kWaves];
-    __shared__ int64_t begin[2];  // the sequence that the run begins in, and the chunks before that sequence
     const int tid = threadIdx.x, wave = uniform((int)(tid / kWave)), lane = tid % kWave;
-    // chunks before each thread's sequences, and of all
-    const int per = (a.B + THREADS - 1) / THREADS, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
-    int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) mine += chunks_of(a, b);
-    int64_t upto = mine;
+    // each wave looks at all lengths by itself: lane's are b0 .. b1 - 1
+    const int per = (a.B + kWave - 1) / kWave, b0 = min(lane * per, a.B), b1 = min(b0 + per, a.B);
+    int64_t total = 0;
+    for (int b = b0; b < b1; ++b) total += chunks_in(a, a.len[b]);
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) total += __shfl_xor(total, d);
+    const int64_t room = a.W - min<int64_t>((int64_t)a.B * a.heads, a.W / 2);
+    const int c = uniform((int)min<int64_t>(1 << 30, max<int64_t>(1, (uniform(total) * a.heads + room - 1) / room)));
+    // workgroups, parts among them and items in parts (bits 36, 18 and 0 on), of the lane's sequences and of those before
+    const auto count = [&](int len) {
+        const int k = parts_in(chunks_in(a, len), c);
+        return (uint64_t)k * (uint32_t)a.heads * (k > 1 ? 1ull << 36 | 1 << 18 : 1ull << 36) + (k > 1 ? a.heads : 0);
+    };
+    const auto groups = [](uint64_t v) { return (uint32_t)(v >> 36); };
+    uint64_t mine = 0;
+    for (int b = b0; b < b1; ++b) mine += count(a.len[b]);
+    uint64_t upto = mine;
 #pragma unroll
     for (int d = 1; d < kWave; d *= 2) {
-        const int64_t v = __shfl_up(upto, d);
+        const uint64_t v = __shfl_up(upto, d);
         if (lane >= d) upto += v;
     }
-    if (lane == kWave - 1) wave_sums[wave] = upto;
-    __syncthreads();
-    int64_t total = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        if (w < wave) upto += wave_sums[w];
-        total += wave_sums[w];
+    const uint32_t id = blockIdx.x;
+    const uint64_t all = (uint64_t)uniform((int64_t)__shfl(upto, kWave - 1));
+    if (id == 0 && tid == 0) a.meta[0] = (int)(all & 0x3ffff);
+    if (id >= groups(all)) return;
+    const int from = __builtin_ctzll(__ballot(groups(upto) > id));
+    uint64_t before = (uint64_t)uniform((int64_t)__shfl(upto - mine, from));
+    int b = from * per, len = scalar_load(a.len, b);
+    for (uint64_t n = count(len); groups(before + n) <= id; n = count(len)) {
+        before += n;
+        len = scalar_load(a.len, ++b);
     }
-    total = uniform(total);
-    const int64_t U = total * a.heads, W = min<int64_t>(a.W, U);  // each of W has a chunk at least
-    for (int b = blockIdx.x; b < a.B; b += a.W) {
-        if (chunks_of(a, b) != 0) continue;
-        const bool bad = a.len[b] > 0;
-        for (int hr = 0; hr < a.heads; ++hr) finish_empty<BF, D>(a, span_of(a, b, hr, 0, 0), bad);
-    }
-    int4v unfinished{};
-    if (blockIdx.x >= W) {
-        if (tid == 0) a.meta[blockIdx.x] = unfinished;
+    const int chunks = chunks_in(a, len), k = parts_in(chunks, c), at = (int)(id - groups(before));
+    const int hr = at / k, j = at - hr * k, each = (chunks - 1) / k + 1;
+    const Span sp = span_of(a, b, hr, j * each * kChunk, min(len, (j + 1) * each * kChunk));
+    if (chunks == 0) {
+        finish_empty<BF, D>(a, sp, len > 0);
         return;
     }
-    const int64_t start = U * blockIdx.x / W, end = U * (blockIdx.x + 1) / W;
-    {
-        int64_t before = upto - mine;
-        if (before * a.heads <= start && start < upto * a.heads) {
-            int b = b0;
-            for (int n = chunks_of(a, b); (before + n) * a.heads <= start; n = chunks_of(a, ++b)) before += n;
-            begin[0] = b;
-            begin[1] = before;
-        }
+    float *part_o = nullptr, *part_s = nullptr;
+    if (k > 1) {
+        const int slot = (int)(before >> 18 & 0x3ffff) + at;
+        part_o = a.part_o + (int64_t)slot * 16 * D;
+        part_s = a.part_s + slot * 32;
+        if (tid == 0 && j == 0) a.split[(before & 0x3ffff) + hr] = int4v{b * a.heads + hr, slot, k, 0};
     }
-    __syncthreads();
-    int b = uniform((int)begin[0]);
-    int len = scalar_load(a.len, b), n = chunks_in(a, len);
-    const uint64_t in = (uint64_t)(start - uniform(begin[1]) * a.heads);
-    int hr = uniform((int)(in / (uint32_t)n)), chunk = uniform((int)(in - (uint64_t)hr * n));
-    int64_t left = end - start;
-    for (bool first = true; left > 0; first = false) {
-        const int take = uniform((int)min<int64_t>(left, n - chunk));
-        const Span sp = span_of(a, b, hr, chunk * kChunk, min(len, (chunk + take) * kChunk));
-        State<D> st;
-        attend<BF, Q8, D>(a, sp, wave, st);
-        join_waves<D>(st, wave, share);
-        const int64_t slot = 2 * (int64_t)blockIdx.x + !first;
-        if (wave == 0) {
-            const int i16 = lane & 15, g = lane >> 4;
-            if (chunk == 0 && take == n) {
-                finish<BF, Q8, D>(a, sp, st);
-            } else if (i16 < sp.rows) {
-#pragma unroll
-                for (int e = 0; e < D / 16; ++e) {
-                    *reinterpret_cast<float4v*>(a.part_o + (slot * 16 + i16) * D + 16 * e + 4 * g) = st.o[e];
-                }
-                if (g == 0) {
-                    a.part_s[slot * 32 + i16] = st.m;
-                    a.part_s[slot * 32 + 16 + i16] = st.l;
-                }
-            }
-            if (chunk == 0 && take < n) {
-                const uint64_t last = (uint64_t)(end - left) + n;  // one past the item's chunks
-                unfinished = int4v{b * a.heads + hr, (int)((last * (uint64_t)W - 1) / (uint64_t)U) - (int)blockIdx.x + 1, (int)!first, 0};
-            }
-        }
-        left -= take;
-        chunk = 0;
-        if (++hr == a.heads && left > 0) {
-            hr = 0;
-            do {
-                len = scalar_load(a.len, ++b);
-                n = chunks_in(a, len);
-            } while (n == 0);
-        }
-    }
-    if (tid == 0) a.meta[blockIdx.x] = unfinished;
+    State<D> st;
+    attend<BF, Q8, D>(a, sp, wave, st);
+    join_waves<BF, BF || Q8, D>(a, sp, st, wave, share, part_o, part_s);
 }
 
-// The parts of the item that workgroup blockIdx.x of the split began and did not finish, in their order: one of its rows
-// (blockIdx.y) a workgroup, its parts dealt to four waves. What it waits for is a chain of loads, so the first
+// An item's parts, in their order: one of its rows (blockIdx.y) a workgroup, its parts dealt to four waves. What it waits for is a chain of loads, so the first
 // parts' results are on their way before the weights are known, and eight a wave from then on.
 template <bool BF, bool MBF, int D>
 __global__ __launch_bounds__(kWaves* kWave) void paged_attn_join_kernel(AttnArgs a) {
@@ -535,14 +494,13 @@ __global__ __launch_bounds__(kWaves* kWave) void paged_attn_join_kernel(AttnArgs
     __shared__ float weight[kMostSplit + 1];
     __shared__ float red[2][kWaves];
     __shared__ float parts[kWaves][D];
-    const int4v meta = a.meta[blockIdx.x];
-    const int n = meta[1], r = blockIdx.y;
-    if (n == 0) return;
-    const int b = fdiv(meta[0], a.by_heads);
-    const Span sp = span_of(a, b, meta[0] - b * a.heads, 0, 0);
+    const int4v item = a.split[blockIdx.x];
+    if ((int)blockIdx.x >= a.meta[0]) return;
+    const int first = item[1], n = item[2], r = blockIdx.y, b = fdiv(item[0], a.by_heads);
+    const Span sp = span_of(a, b, item[0] - b * a.heads, 0, 0);
     if (r >= sp.rows) return;
     const int tid = threadIdx.x, wave = uniform((int)(tid / kWave)), lane = tid % kWave;
-    const auto slot = [&](int p) { return 2 * (int64_t)(blockIdx.x + p) + (p == 0 ? meta[2] : 0); };
+    const auto slot = [&](int p) { return (int64_t)first + p; };
     const int col = min(lane * COLS, D - COLS);
     const auto part = [&](int p) { return *reinterpret_cast<const cols*>(a.part_o + (slot(p) * 16 + r) * D + col); };
     cols early[EARLY];
@@ -601,22 +559,27 @@ __global__ __launch_bounds__(kWaves* kWave) void paged_attn_join_kernel(AttnArgs
 // How a call is run: a rule on the shapes alone, so that results do not depend on the device
 struct Plan {
     int64_t items = 0;  // 0: a shape that the entry point rejects
-    int W = 0;          // workgroups of a split call, 0: one an item
-    size_t o = 0, s = 0, meta = 0;
-    size_t bytes() const { return o + s + meta; }
+    int W = 0;          // of a split call, 0: a workgroup an item
+    int64_t grid = 0;
+    size_t o = 0, s = 0, split = 0, meta = 0;
+    size_t bytes() const { return o + s + split + meta; }
 };
 Plan plan_of(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t per, int64_t page) {
     Plan p;
     if (B < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || per < 1 || page < 16 || page % 16 || D < 32 || D > 256 || D % 32) return p;
     const int64_t blocks = (Hq / Hkv + 15) / 16;
     if (Hkv > 16384 || blocks > 16384 || Hkv * blocks > 16384 || B > (1 << 23) / (Hkv * blocks) || per > (1 << 30) / page) return p;
-    p.items = B * Hkv * blocks;
-    const int64_t chunks = (per * page + kChunk - 1) / kChunk;
-    if (chunks * kChunk > kDirect) {
-        p.W = (int)std::min<int64_t>(std::max<int64_t>(1, p.items) * chunks, 256 * occupancy(D));
+    p.items = p.grid = B * Hkv * blocks;
+    if (per * page > kDirect && B > 0) {
+        p.W = 256 * occupancy(D);
+        // With c as the kernel takes it, all chunks / c <= room = W - min(items, W / 2), and an item has under its chunks / c + 1
+        // parts: under room + items workgroups; items of two parts and more have over c chunks: under room such items
+        // and 2 room parts.
+        p.grid = p.W - std::min<int64_t>(p.items, p.W / 2) + p.items;
         p.o = (size_t)2 * p.W * 16 * D * 4;
         p.s = (size_t)2 * p.W * 32 * 4;
-        p.meta = (size_t)p.W * 16;
+        p.split = (size_t)p.W * 16;
+        p.meta = 256;
     }
     return p;
 }
@@ -693,7 +656,8 @@ extern "C" int clk_paged_attention(clk_stream stream, const clk_buffer* q, const
     char* ws = static_cast<char*>(workspace);
     a.part_o = reinterpret_cast<float*>(ws);
     a.part_s = reinterpret_cast<float*>(ws + plan.o);
-    a.meta = reinterpret_cast<int4v*>(ws + plan.o + plan.s);
+    a.split = reinterpret_cast<int4v*>(ws + plan.o + plan.s);
+    a.meta = reinterpret_cast<int*>(ws + plan.o + plan.s + plan.split);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     int stage = 0;
     stage_mark(s, stage);
@@ -702,12 +666,12 @@ extern "C" int clk_paged_attention(clk_stream stream, const clk_buffer* q, const
         constexpr bool BF = decltype(bf_)::value, Q8 = decltype(q8_)::value;
         constexpr int D = decltype(d_)::value;
         if (plan.W == 0) {
-            hipLaunchKernelGGL((paged_attn_kernel<BF, Q8, D>), dim3((unsigned)plan.items), block, 0, s, a);
+            hipLaunchKernelGGL((paged_attn_kernel<BF, Q8, D>), dim3((unsigned)plan.grid), block, 0, s, a);
             return;
         }
-        hipLaunchKernelGGL((paged_attn_split_kernel<BF, Q8, D>), dim3(plan.W), block, 0, s, a);
+        hipLaunchKernelGGL((paged_attn_split_kernel<BF, Q8, D>), dim3((unsigned)plan.grid), block, 0, s, a);
         stage_mark(s, ++stage);
-        hipLaunchKernelGGL((paged_attn_join_kernel<BF, BF || Q8, D>), dim3(plan.W, (unsigned)std::min<int64_t>(G, 16)), block, 0, s, a);
+        hipLaunchKernelGGL((paged_attn_join_kernel<BF, BF || Q8, D>), dim3((unsigned)std::min<int64_t>(plan.items, plan.W), (unsigned)std::min<int64_t>(G, 16)), block, 0, s, a);
     };
     const auto launch = [&](auto d_) {
         if (act == CLK_BF16) c.q8 ? kernels(std::true_type(), std::true_type(), d_) : kernels(std::true_type(), std::false_type(), d_);
