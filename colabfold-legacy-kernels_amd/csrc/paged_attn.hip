@@ -6,7 +6,7 @@
 // Every cached byte is needed once, which bounds it: 4 Hq / Hkv operations a cached value are far under the matrix
 // cores' rate up to some hundred query heads a head of keys.
 //
-// A wave takes 32 tokens at a time, two blocks of the cache (kv_cache.h), for 16 query heads of one head of keys
+// A wave takes two or four blocks of 16 tokens of the cache (kv_cache.h) at a time, for 16 query heads of one head of keys
 // (rows past the group's last are zeros and cost nothing: the cache's bytes are what takes the time):
 //   S^T = K Q^T        K's operands are the cache's bytes as they lie; a lane gets tokens 4 g .. + 3 of each block for
 //                      query l % 16
@@ -26,13 +26,16 @@ typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 typedef int int4v __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
-constexpr int kTile = 32;  // tokens a wave takes at a time
-constexpr int kChunk = kWaves * kTile;
 constexpr int kDirect = 512;
 
+// Blocks of 16 tokens a wave takes at a time, and the tokens of a workgroup's step. (Four blocks, where the registers hold
+// them, were slower with 8 bits and the same with 16.)
+constexpr int kBlocks = 2;
+constexpr int kChunk = kWaves * 16 * kBlocks;
+
 // Workgroups a CU that the kernels' registers are kept for
-constexpr int occupancy(int64_t D) { return D <= 128 ? 3 : 2; }
-constexpr int kMostSplit = 256 * 3;
+constexpr int occupancy(int64_t D) { return D <= 64 ? 4 : D <= 128 ? 3 : 2; }
+constexpr int kMostSplit = 256 * 4 * 3;
 
 // Weights are taken times 2^bias, which their sum has too and which cancels: fp16 ones so that small ones keep their bits (a
 // weight of 2^-25 of the largest, of which a long sequence may have millions, would be 0), bf16 ones so that
@@ -71,6 +74,19 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
 __device__ __forceinline__ int scalar_load(const int32_t* p, int64_t i) {
     return reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p))[i];
 }
+
+// Sum over the wave, and inclusive sums, by DPP (a shuffle waits for LDS at each of its six steps)
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, true);   // row_shr 1, 2, 4, 8
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);  // row_bcast 15, 31
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
+__device__ __forceinline__ uint32_t wave_sum(uint32_t v) { return lane_value(wave_scan(v), kWave - 1); }
 
 template <bool BF>
 __device__ __forceinline__ float4v mfma(half8 a, half8 b, float4v c) {
@@ -118,14 +134,14 @@ __device__ __forceinline__ void two_parts(const float (&f)[8], half8& hi, half8&
 }
 
 // A tile's cached bytes as they were loaded: keys as operands, values as cells of four tokens a channel block
-template <bool Q8, int D>
+template <bool Q8, int D, int NB>
 struct Tile {
     static constexpr int NK = Q8 ? (D + 63) / 64 : D / 32;  // key loads a block
     static constexpr int C = value_group(Q8, D);            // channel blocks a value load
     static constexpr int NV = D / 16 / C;
-    uint4v k[2][NK];
-    uint4v v[2][NV];  // 8-byte loads (Q8, D no multiple of 64) in the low half
-    float4v ks[2], vs[2];
+    uint4v k[NB][NK];
+    uint4v v[NB][NV];  // 8-byte loads (Q8, D no multiple of 64) in the low half
+    float4v ks[NB], vs[NB];
 };
 
 // One item, the query heads 16 rb .. + 15 of head of keys h of sequence b, and tokens of it
@@ -153,76 +169,86 @@ struct State {
     bool bad;  // a page that the cache does not have
 };
 
-// Where a tile's two blocks lie in the cache, in tokens x heads, and whether they hold tokens of the span: a block past it (or
-// on a page that the cache does not have, which sets bad) is loaded as zeros, by a buffer of no bytes
-struct Where {
-    int64_t row[2];
-    bool in[2];
+// Where a tile's blocks lie in the cache, in tokens x heads, and whether they hold tokens of the span: a block past it (or on
+// a page that the cache does not have, which sets bad) is loaded as zeros, by a buffer of no bytes. The pages' numbers
+// are loaded first, all at once.
+template <int NB>
+struct Pages {
+    int page[NB];
 };
-__device__ __forceinline__ Where where_of(const AttnArgs& a, const Span& sp, const int32_t* table, int k0, int keys, bool& bad) {
-    Where w;
+template <int NB>
+__device__ __forceinline__ Pages<NB> pages_of(const AttnArgs& a, const Span& sp, const int32_t* table, int k0) {
+    Pages<NB> p;
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+    for (int n = 0; n < NB; ++n) {
         const int at = k0 + 16 * n;
-        w.in[n] = at < keys;
-        const int in_span = w.in[n] ? at : sp.from, p = fdiv(in_span, a.by_page), page = scalar_load(table, p);
-        if ((uint32_t)page >= (uint32_t)a.pages) {
-            w.in[n] = false;
-            bad = true;
-        }
-        w.row[n] = w.in[n] ? ((int64_t)page * a.Hkv + sp.h) * a.page + (in_span - p * a.page) : 0;
+        p.page[n] = scalar_load(table, fdiv(at < sp.to ? at : sp.from, a.by_page));
     }
+    return p;
+}
+struct Where {
+    int64_t row;
+    bool in;
+};
+__device__ __forceinline__ Where where_of(const AttnArgs& a, const Span& sp, int at, int page, bool& bad) {
+    Where w;
+    const bool have = (uint32_t)page < (uint32_t)a.pages;
+    bad |= at < sp.to && !have;
+    w.in = at < sp.to && have;
+    const int in_page = at - fdiv(at, a.by_page) * a.page;
+    w.row = w.in ? ((int64_t)page * a.Hkv + sp.h) * a.page + in_page : 0;
     return w;
 }
 template <typename P>
 __device__ __forceinline__ auto rsrc_of(const P* p, uint32_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<P*>(p), 0, bytes, 0x00020000);
 }
-template <typename Rsrc>
+template <bool NT, typename Rsrc>
 __device__ __forceinline__ uint4v load16(Rsrc r, uint32_t off) {
-    return __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+    return __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, NT ? 2 : 0));
 }
-template <typename Rsrc>
+template <bool NT, typename Rsrc>
 __device__ __forceinline__ uint4v load8(Rsrc r, uint32_t off) {
-    const uint2v w = __builtin_bit_cast(uint2v, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
+    const uint2v w = __builtin_bit_cast(uint2v, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, NT ? 2 : 0));
     return uint4v{w[0], w[1], 0, 0};
 }
-template <bool Q8, int D>
-__device__ __forceinline__ void load_keys(const AttnArgs& a, const Where& at, int lane, Tile<Q8, D>& t) {
+template <bool NT, bool Q8, int D, int NB>
+__device__ __forceinline__ void load_keys(const AttnArgs& a, const Where (&at)[NB], int lane, Tile<Q8, D, NB>& t) {
     constexpr int SIZE = Q8 ? 1 : 2;
     const int i16 = lane & 15, g = lane >> 4;
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-        const auto r = rsrc_of(a.kc + at.row[n] * (D * SIZE), at.in[n] ? 16 * D * SIZE : 0);
+    for (int n = 0; n < NB; ++n) {
+        const auto r = rsrc_of(a.kc + at[n].row * (D * SIZE), at[n].in ? 16 * D * SIZE : 0);
 #pragma unroll
-        for (int s = 0; s < Tile<Q8, D>::NK; ++s) {
-            if (!Q8 || s * 64 + 64 <= D) t.k[n][s] = load16(r, lane * 16 + s * 1024);
-            else t.k[n][s] = load8(r, (g >> 1) * 256 + i16 * 16 + (g & 1) * 8 + s * 1024);
+        for (int s = 0; s < t.NK; ++s) {
+            if (!Q8 || s * 64 + 64 <= D) t.k[n][s] = load16<NT>(r, lane * 16 + s * 1024);
+            else t.k[n][s] = load8<NT>(r, (g >> 1) * 256 + i16 * 16 + (g & 1) * 8 + s * 1024);
         }
-        if constexpr (Q8) t.ks[n] = __builtin_bit_cast(float4v, load16(rsrc_of(a.ks + at.row[n], at.in[n] ? 64 : 0), g * 16));
+        if constexpr (Q8) t.ks[n] = __builtin_bit_cast(float4v, load16<NT>(rsrc_of(a.ks + at[n].row, at[n].in ? 64 : 0), g * 16));
     }
 }
-template <bool Q8, int D>
-__device__ __forceinline__ void load_values(const AttnArgs& a, const Where& at, int lane, Tile<Q8, D>& t) {
+template <bool NT, bool Q8, int D, int NB>
+__device__ __forceinline__ void load_values(const AttnArgs& a, const Where (&at)[NB], int lane, Tile<Q8, D, NB>& t) {
     constexpr int SIZE = Q8 ? 1 : 2;
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-        const auto r = rsrc_of(a.vc + at.row[n] * (D * SIZE), at.in[n] ? 16 * D * SIZE : 0);
+    for (int n = 0; n < NB; ++n) {
+        const auto r = rsrc_of(a.vc + at[n].row * (D * SIZE), at[n].in ? 16 * D * SIZE : 0);
 #pragma unroll
-        for (int s = 0; s < Tile<Q8, D>::NV; ++s) {
-            if constexpr (Tile<Q8, D>::C * SIZE == 4) t.v[n][s] = load16(r, lane * 16 + s * 1024);
-            else t.v[n][s] = load8(r, lane * 8 + s * 512);
+        for (int s = 0; s < t.NV; ++s) {
+            if constexpr (Tile<Q8, D, NB>::C * SIZE == 4) t.v[n][s] = load16<NT>(r, lane * 16 + s * 1024);
+            else t.v[n][s] = load8<NT>(r, lane * 8 + s * 512);
         }
-        if constexpr (Q8) t.vs[n] = __builtin_bit_cast(float4v, load16(rsrc_of(a.vs + at.row[n], at.in[n] ? 64 : 0), (lane >> 4) * 16));
+        if constexpr (Q8) t.vs[n] = __builtin_bit_cast(float4v, load16<NT>(rsrc_of(a.vs + at[n].row, at[n].in ? 64 : 0), (lane >> 4) * 16));
     }
 }
 
 // The wave's tiles of a span: every kWaves-th. The next tile's keys are loaded as soon as this one's scores have been
 // computed, into the same registers, and its values as soon as the results have: each load has half a tile's work to arrive in.
-template <bool BF, bool Q8, int D>
+template <bool BF, bool Q8, bool NT, int D>
 __device__ __forceinline__ void attend(const AttnArgs& a, const Span& sp, int wave, State<D>& st) {
-    typedef Tile<Q8, D> T;
-    constexpr int KS = D / 32, DB = D / 16;
+    constexpr int NB = kBlocks;
+    typedef Tile<Q8, D, NB> T;
+    constexpr int KS = D / 32, DB = D / 16, TILE = 16 * NB, STEP = kWaves * TILE;
     constexpr bool MBF = BF || Q8;   // the products' operands are bf16
     constexpr bool QLO = Q8 && !BF;  // fp16 queries in two bf16 parts, which is exact
     const int lane = threadIdx.x % kWave, i16 = lane & 15, g = lane >> 4, keys = sp.to;
@@ -256,17 +282,20 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Span& sp, int wa
     st.l = 0.f;
     st.bad = false;
 
-    int k0 = sp.from + wave * kTile;
+    int k0 = sp.from + wave * TILE;
     if (k0 >= keys) return;
     T t;
-    Where at = where_of(a, sp, table, k0, keys, st.bad);
-    load_keys<Q8, D>(a, at, lane, t);
-    load_values<Q8, D>(a, at, lane, t);
-    for (;;) {
-        const Where next = where_of(a, sp, table, k0 + kWaves * kTile, keys, st.bad);
-        float s2[2][4], top = -__builtin_inff();
+    Where at[NB];
+    Pages<NB> pages = pages_of<NB>(a, sp, table, k0);
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
+    for (int n = 0; n < NB; ++n) at[n] = where_of(a, sp, k0 + 16 * n, pages.page[n], st.bad);
+    load_keys<NT, Q8, D, NB>(a, at, lane, t);
+    load_values<NT, Q8, D, NB>(a, at, lane, t);
+    for (;;) {
+        pages = pages_of<NB>(a, sp, table, k0 + STEP);
+        float s2[NB][4], top = -__builtin_inff();
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
             float4v s{};
 #pragma unroll
             for (int c = 0; c < KS; ++c) {
@@ -289,7 +318,9 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Span& sp, int wa
                 top = fmaxf(top, s2[n][i]);
             }
         }
-        load_keys<Q8, D>(a, next, lane, t);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) at[n] = where_of(a, sp, k0 + STEP + 16 * n, pages.page[n], st.bad);
+        load_keys<NT, Q8, D, NB>(a, at, lane, t);
         top = wave_xor_max4(top);
         if (__any(top > st.m)) {
             const float m_new = fmaxf(st.m, top);
@@ -300,21 +331,9 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Span& sp, int wa
             st.m = m_new;
         }
         const float base = (st.m == -__builtin_inff() ? 0.f : st.m) - kBias<MBF>;
-        float pf[8];
+        if (!Q8 && k0 + TILE > keys) {  // values behind the last token may be anything: zeros
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float x = exp2_fast(s2[n][i] - base);
-                st.l += x;
-                if constexpr (Q8) x = k0 + 16 * n + 4 * g + i < keys ? x * t.vs[n][i] : 0.f;
-                pf[4 * n + i] = x;
-            }
-        half8 p, plo;
-        two_parts<MBF, !Q8>(pf, p, plo);
-        if (!Q8 && k0 + kTile > keys) {  // values behind the last token may be anything: zeros
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < NB; ++n)
 #pragma unroll
                 for (int s = 0; s < T::NV; ++s)
 #pragma unroll
@@ -325,20 +344,33 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Span& sp, int wa
                     }
         }
 #pragma unroll
-        for (int e = 0; e < DB; ++e) {
-            half8 op;
-            const int s = e / T::C, c = e % T::C;
-            if constexpr (!Q8) {
-                op = join(uint2v{t.v[0][s][2 * c], t.v[0][s][2 * c + 1]}, uint2v{t.v[1][s][2 * c], t.v[1][s][2 * c + 1]});
-            } else {
-                op = join(bf16_of_bytes(t.v[0][s][c]), bf16_of_bytes(t.v[1][s][c]));
+        for (int n = 0; n < NB; n += 2) {
+            float pf[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float x = exp2_fast(s2[n + i / 4][i % 4] - base);
+                st.l += x;
+                if constexpr (Q8) x = k0 + 16 * (n + i / 4) + 4 * g + i % 4 < keys ? x * t.vs[n + i / 4][i % 4] : 0.f;
+                pf[i] = x;
             }
-            st.o[e] = mfma<MBF>(op, p, st.o[e]);
-            st.o[e] = mfma<MBF>(op, plo, st.o[e]);
+            half8 p, plo;
+            two_parts<MBF, !Q8>(pf, p, plo);
+#pragma unroll
+            for (int e = 0; e < DB; ++e) {
+                half8 op;
+                const int s = e / T::C, c = e % T::C;
+                if constexpr (!Q8) {
+                    op = join(uint2v{t.v[n][s][2 * c], t.v[n][s][2 * c + 1]}, uint2v{t.v[n + 1][s][2 * c], t.v[n + 1][s][2 * c + 1]});
+                } else {
+                    op = join(bf16_of_bytes(t.v[n][s][c]), bf16_of_bytes(t.v[n + 1][s][c]));
+                }
+                st.o[e] = mfma<MBF>(op, p, st.o[e]);
+                st.o[e] = mfma<MBF>(op, plo, st.o[e]);
+            }
         }
-        k0 += kWaves * kTile;
+        k0 += STEP;
         if (k0 >= keys) return;
-        load_values<Q8, D>(a, next, lane, t);
+        load_values<NT, Q8, D, NB>(a, at, lane, t);
     }
 }
 
@@ -412,7 +444,7 @@ __global__ __launch_bounds__(kWaves* kWave, occupancy(D)) void paged_attn_kernel
         return;
     }
     State<D> st;
-    attend<BF, Q8, D>(a, sp, wave, st);
+    attend<BF, Q8, false, D>(a, sp, wave, st);
     join_waves<BF, BF || Q8, D>(a, sp, st, wave, share, nullptr, nullptr);
 }
 
@@ -423,50 +455,63 @@ __device__ __forceinline__ int chunks_in(const AttnArgs& a, int len) {
 // Parts of a sequence's items, c chunks each at most; a sequence of no tokens has one, which writes its results
 __device__ __forceinline__ int parts_in(int chunks, int c) { return chunks <= c ? 1 : (chunks - 1) / c + 1; }
 
-// Items in parts of about as many chunks, however the lengths differ, one a workgroup. c, the most chunks of a part, is what
-// fills W workgroups, all at once on the chip: items take up to half of them for their last, shorter parts. Items of one part are
-// finished here; parts of the others are numbered through and left for paged_attn_join_kernel.
+// Items in parts of about as many chunks, however the lengths differ, one a workgroup. c, the most chunks of a part, is the
+// least with which W workgroups, all at once on the chip, are enough, but at most what room = W - min(items, W / 2)
+// workgroups would need if parts were as long as that to the last (with so many items that theirs do not fit on the
+// chip at once anyway). Items of one part are finished here; parts of the others are numbered through and left for paged_attn_join_kernel.
 // (All chunks in W equal runs, one a workgroup, where a run could end one item and begin the next, was more even but a
 // workgroup had two short spans as often as one, each with its chain of loads: 61 sequences of up to 8192 over 8 bits
 // took 43 us.)
-template <bool BF, bool Q8, int D>
+template <bool BF, bool Q8, bool NT, int D>
 __global__ __launch_bounds__(kWaves* kWave, occupancy(D)) void paged_attn_split_kernel(AttnArgs a) {
     __shared__ WaveShare<D> share;
     const int tid = threadIdx.x, wave = uniform((int)(tid / kWave)), lane = tid % kWave;
-    // each wave looks at all lengths by itself: lane's are b0 .. b1 - 1
+    // each wave looks at all lengths by itself: lane's are b0 .. b1 - 1, and the first is kept
     const int per = (a.B + kWave - 1) / kWave, b0 = min(lane * per, a.B), b1 = min(b0 + per, a.B);
-    int64_t total = 0;
-    for (int b = b0; b < b1; ++b) total += chunks_in(a, a.len[b]);
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) total += __shfl_xor(total, d);
-    const int64_t room = a.W - min<int64_t>((int64_t)a.B * a.heads, a.W / 2);
-    const int c = uniform((int)min<int64_t>(1 << 30, max<int64_t>(1, (uniform(total) * a.heads + room - 1) / room)));
-    // workgroups, parts among them and items in parts (bits 36, 18 and 0 on), of the lane's sequences and of those before
-    const auto count = [&](int len) {
-        const int k = parts_in(chunks_in(a, len), c);
-        return (uint64_t)k * (uint32_t)a.heads * (k > 1 ? 1ull << 36 | 1 << 18 : 1ull << 36) + (k > 1 ? a.heads : 0);
+    const int len0 = b0 < b1 ? a.len[b0] : -1;
+    const auto over = [&](auto f) {  // f of the lane's lengths, in order
+        for (int b = b0; b < b1; ++b) f(b == b0 ? len0 : a.len[b]);
     };
-    const auto groups = [](uint64_t v) { return (uint32_t)(v >> 36); };
-    uint64_t mine = 0;
-    for (int b = b0; b < b1; ++b) mine += count(a.len[b]);
-    uint64_t upto = mine;
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-        const uint64_t v = __shfl_up(upto, d);
-        if (lane >= d) upto += v;
+    int64_t mine = 0;
+    over([&](int len) { mine += chunks_in(a, len); });
+    const int64_t room = a.W - min<int64_t>((int64_t)a.B * a.heads, a.W / 2);
+    const int64_t U = (((int64_t)wave_sum((uint32_t)(mine >> 24)) << 24) + wave_sum((uint32_t)mine & 0xffffffu)) * a.heads;
+    const auto most = [&](int64_t groups) {
+        if (U < 1 << 30) return max(1, (int)(((uint32_t)U + (uint32_t)groups - 1) / (uint32_t)groups));
+        return (int)min<int64_t>(1 << 30, (U + groups - 1) / groups);
+    };
+    int c = most(room);
+    for (int low = most(a.W); low < c;) {  // the least c, or this one, with at most W parts
+        const int mid = low + (c - low) / 2;
+        int64_t parts = 0;
+        over([&](int len) { parts += parts_in(chunks_in(a, len), mid); });
+        if ((int64_t)wave_sum((uint32_t)min<int64_t>(parts, 1 << 24)) * a.heads <= a.W) c = mid;  // (a lane's 2^24 are too many)
+        else low = mid + 1;
     }
-    const uint32_t id = blockIdx.x;
-    const uint64_t all = (uint64_t)uniform((int64_t)__shfl(upto, kWave - 1));
-    if (id == 0 && tid == 0) a.meta[0] = (int)(all & 0x3ffff);
-    if (id >= groups(all)) return;
-    const int from = __builtin_ctzll(__ballot(groups(upto) > id));
-    uint64_t before = (uint64_t)uniform((int64_t)__shfl(upto - mine, from));
-    int b = from * per, len = scalar_load(a.len, b);
-    for (uint64_t n = count(len); groups(before + n) <= id; n = count(len)) {
-        before += n;
+    // workgroups, and below them parts (16 bits) and items in parts, of the lane's sequences and of those before
+    const auto count = [&](int len, uint32_t& groups, uint32_t& parts) {
+        const int k = parts_in(chunks_in(a, len), c);
+        groups += (uint32_t)(k * a.heads);
+        if (k > 1) parts += (uint32_t)(k * a.heads) << 16 | (uint32_t)a.heads;
+    };
+    uint32_t groups = 0, parts = 0;
+    over([&](int len) { count(len, groups, parts); });
+    const uint32_t id = blockIdx.x, groups_to = wave_scan(groups), parts_to = wave_scan(parts);
+    if (id == 0 && tid == kWave - 1) a.meta[0] = (int)(parts_to & 0xffffu);
+    const uint64_t has = __ballot(groups_to > id);
+    if (has == 0) return;
+    const int from = __builtin_ctzll(has);
+    uint32_t before = lane_value(groups_to - groups, from), parts_before = lane_value(parts_to - parts, from);
+    int b = from * per, len = (int)lane_value((uint32_t)len0, from);
+    for (;;) {
+        uint32_t g = 0, p = 0;
+        count(len, g, p);
+        if (before + g > id) break;
+        before += g;
+        parts_before += p;
         len = scalar_load(a.len, ++b);
     }
-    const int chunks = chunks_in(a, len), k = parts_in(chunks, c), at = (int)(id - groups(before));
+    const int chunks = chunks_in(a, len), k = parts_in(chunks, c), at = (int)(id - before);
     const int hr = at / k, j = at - hr * k, each = (chunks - 1) / k + 1;
     const Span sp = span_of(a, b, hr, j * each * kChunk, min(len, (j + 1) * each * kChunk));
     if (chunks == 0) {
@@ -475,13 +520,13 @@ __global__ __launch_bounds__(kWaves* kWave, occupancy(D)) void paged_attn_split_
     }
     float *part_o = nullptr, *part_s = nullptr;
     if (k > 1) {
-        const int slot = (int)(before >> 18 & 0x3ffff) + at;
+        const int slot = (int)(parts_before >> 16) + at;
         part_o = a.part_o + (int64_t)slot * 16 * D;
         part_s = a.part_s + slot * 32;
-        if (tid == 0 && j == 0) a.split[(before & 0x3ffff) + hr] = int4v{b * a.heads + hr, slot, k, 0};
+        if (tid == 0 && j == 0) a.split[(parts_before & 0xffffu) + hr] = int4v{b * a.heads + hr, slot, k, 0};
     }
     State<D> st;
-    attend<BF, Q8, D>(a, sp, wave, st);
+    attend<BF, Q8, NT, D>(a, sp, wave, st);
     join_waves<BF, BF || Q8, D>(a, sp, st, wave, share, part_o, part_s);
 }
 
@@ -571,7 +616,10 @@ Plan plan_of(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t per, int64_t
     if (Hkv > 16384 || blocks > 16384 || Hkv * blocks > 16384 || B > (1 << 23) / (Hkv * blocks) || per > (1 << 30) / page) return p;
     p.items = p.grid = B * Hkv * blocks;
     if (per * page > kDirect && B > 0) {
-        p.W = 256 * occupancy(D);
+        // One round of workgroups, but where the items nearly make one already, three, so that the long among them are cut
+        // finely enough to fill the last round: 256 ragged sequences of up to 4096 on 8 heads 155 us, 166 with one; 61 on
+        // 4 heads 43 with one and 48 with three.
+        p.W = 256 * occupancy(D) * (p.items > 128 * occupancy(D) ? 3 : 1);
         // With c as the kernel takes it, all chunks / c <= room = W - min(items, W / 2), and an item has under its chunks / c + 1
         // parts: under room + items workgroups; items of two parts and more have over c chunks: under room such items
         // and 2 room parts.
@@ -662,6 +710,10 @@ extern "C" int clk_paged_attention(clk_stream stream, const clk_buffer* q, const
     int stage = 0;
     stage_mark(s, stage);
     const dim3 block(kWaves * kWave);
+    // Keys and values of a cache past half of the 256 MB far cache are loaded past the caches, unless more than one workgroup
+    // reads them: 61 sequences of 2600 over 8 bits (166 MB) 42.7 us, 46.9 through the caches; 256 of 4096 (4.2 GB) 691 and
+    // 752; but 61 of 650 (41 MB, of which a next call finds some) 20.4 and 19.5.
+    const bool past = blocks == 1 && 2 * elements(k_cache) * (c.q8 ? 1 : 2) >= (int64_t)1 << 27;
     const auto kernels = [&](auto bf_, auto q8_, auto d_) {
         constexpr bool BF = decltype(bf_)::value, Q8 = decltype(q8_)::value;
         constexpr int D = decltype(d_)::value;
@@ -669,7 +721,8 @@ extern "C" int clk_paged_attention(clk_stream stream, const clk_buffer* q, const
             hipLaunchKernelGGL((paged_attn_kernel<BF, Q8, D>), dim3((unsigned)plan.grid), block, 0, s, a);
             return;
         }
-        hipLaunchKernelGGL((paged_attn_split_kernel<BF, Q8, D>), dim3((unsigned)plan.grid), block, 0, s, a);
+        if (past) hipLaunchKernelGGL((paged_attn_split_kernel<BF, Q8, true, D>), dim3((unsigned)plan.grid), block, 0, s, a);
+        else hipLaunchKernelGGL((paged_attn_split_kernel<BF, Q8, false, D>), dim3((unsigned)plan.grid), block, 0, s, a);
         stage_mark(s, ++stage);
         hipLaunchKernelGGL((paged_attn_join_kernel<BF, BF || Q8, D>), dim3((unsigned)std::min<int64_t>(plan.items, plan.W), (unsigned)std::min<int64_t>(G, 16)), block, 0, s, a);
     };
