@@ -28,6 +28,8 @@ namespace clk {
 
 namespace {
 
+typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
+
 constexpr int kThreads = 256;
 enum { kQuery, kKey, kValue };
 
@@ -404,71 +406,220 @@ __global__ __launch_bounds__(kThreads) void qk_norm_dw_kernel(HeadsArgs a) {
 
 // ---- cache in, cache out --------------------------------------------------------------------
 
-// blockIdx.y: a head of keys, then of values
+// Sixteen tokens of a call from 16 w on, as the cache sees them. Where a block of the cache is filled by sixteen tokens in a
+// row, whichever token it begins with, the workgroup that has its first token moves it whole, with stores (or loads) of
+// whole lines; the other tokens go one by one.
+struct Window {
+    int first;      // the token that a whole block begins with, from 16 w on; -1: none does
+    uint32_t rest;  // the tokens that go one by one (one bit each, from 16 w on)
+};
+__device__ __forceinline__ Window window_of(const HeadsArgs& a, int64_t t0) {
+    const int64_t t = t0 - 15 + (int)(threadIdx.x % kWave);  // the wave's lanes: 15 tokens before, 16, 15 after
+    const auto slot_at = [&](int64_t i) { return i >= 0 && i < a.T ? a.slots[i] : -1; };
+    const int slot = slot_at(t), after = slot_at(t + 1);
+    const bool live = (uint32_t)slot < (uint32_t)a.slots_end;
+    const uint64_t all = __ballot(live), begins = __ballot(live && slot % kCacheBlock == 0);
+    uint64_t run = __ballot(live && after == slot + 1);  // the next token follows; then the next 2, 4, 8 and 15 do
+    run &= run >> 1;
+    run &= run >> 2;
+    run &= run >> 4;
+    const uint64_t whole = begins & run & run >> 7;
+    uint64_t covered = whole | whole << 1;
+    covered |= covered << 2;
+    covered |= covered << 4;
+    covered |= covered << 8;
+    const uint32_t mine = (uint32_t)(whole >> 15) & 0xffffu;  // one at most: the other tokens of a block begin none
+    return Window{mine ? __builtin_ctz(mine) : -1, (uint32_t)((all & ~covered) >> 15) & 0xffffu};
+}
+
+// Heads a workgroup moves for its 16 tokens, and the rounds it needs for them
+template <int LG>
+constexpr int kHeadsAtOnce = kThreads / LG / 16 > 0 ? kThreads / LG / 16 : 1;
+template <int LG>
+constexpr int kRounds = LG * 16 > kThreads ? LG * 16 / kThreads : 1;
+
+// A block of 16 tokens as rows in LDS, 16 bytes between rows more than they have
+template <int LG, bool Q8>
+struct BlockRows {
+    static constexpr int ROW = 8 * LG * (Q8 ? 1 : 2) + 16;
+    char rows[kHeadsAtOnce<LG>][16][ROW];
+};
+
+// 16 bytes of a block's values (or 8, where a lane's cell has two channels of 8 bits), from rows or to them: unit u of a head has
+// channels 16 (C b + e) + i of tokens 4 g + j with u = (4 b + g) 16 + i
+template <int C, typename F>
+__device__ __forceinline__ void value_unit(int u, F f) {
+    const int i = u & 15, g = u >> 4 & 3, b = u >> 6;
+#pragma unroll
+    for (int e = 0; e < C; ++e)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f(4 * e + j, 4 * g + j, 16 * (C * b + e) + i);
+}
+
+// blockIdx.y: heads of keys, then of values
 template <bool BF, int LG, bool Q8>
 __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(HeadsArgs a) {
-    constexpr int TOKENS = kThreads / LG;
-    const int j = threadIdx.x % LG, sub = threadIdx.x / LG, group = value_group(Q8, a.D);
-    const bool values = (int)blockIdx.y >= a.Hkv;
-    const int head = values ? blockIdx.y - a.Hkv : blockIdx.y;
+    constexpr int TOKENS = kThreads / LG, HEADS = kHeadsAtOnce<LG>, SIZE = Q8 ? 1 : 2;
+    __shared__ __attribute__((aligned(16))) BlockRows<LG, Q8> share;
+    const int j = threadIdx.x % LG, sub = threadIdx.x / LG, group = value_group(Q8, a.D), groups = (a.Hkv + HEADS - 1) / HEADS;
+    const bool values = (int)blockIdx.y >= groups;
+    const int h0 = (values ? blockIdx.y - groups : blockIdx.y) * HEADS, heads = min(HEADS, a.Hkv - h0);
     const Lane l = lane_of(j, a.D, 0, false);
     const half_t* x = values ? a.dv : a.dk;
-    for (int64_t t0 = (int64_t)blockIdx.x * TOKENS; t0 < a.T; t0 += (int64_t)gridDim.x * TOKENS) {
-        const int64_t t = t0 + sub, from = min(t, a.T - 1);
-        const int slot = a.slots[from];
-        const bool live = t < a.T && l.in && (uint32_t)slot < (uint32_t)a.slots_end;
-        const raw8 raw = load_head(x + (from * a.Hkv + head) * a.D, l);
-        if constexpr (Q8) {
-            float f[8], scale;
-            floats<BF>(raw, f);
-            const uint2v q = to_row8<LG, true>(f, scale);
-            if (!live) continue;
-            const Place p = place_of(a, slot, head);
-            if (values) cache_value8(a.vc, p, group, l.c0, q);
-            else cache_key8(a.kc, p, l, q);
-            if (j == 0) (values ? a.vs : a.ks)[p.scale] = scale;
-        } else {
-            if (!live) continue;
-            const Place p = place_of(a, slot, head);
-            if (values) cache_value16(a.vc, p, l.c0, raw);
-            else cache_key16(a.kc, p, l, raw);
+    char* cache = static_cast<char*>(values ? a.vc : a.kc);
+    float* scales = values ? a.vs : a.ks;
+    for (int64_t t0 = 16 * (int64_t)blockIdx.x; t0 < a.T; t0 += 16 * (int64_t)gridDim.x) {
+        const Window w = window_of(a, t0);
+        if (w.first >= 0) {
+            const int slot = a.slots[t0 + w.first];
+#pragma unroll
+            for (int round = 0; round < kRounds<LG>; ++round) {
+                const int n = sub + round * TOKENS, t = n & 15, hs = n >> 4;
+                const int head = h0 + min(hs, heads - 1);
+                const raw8 raw = load_head(x + ((t0 + w.first + t) * a.Hkv + head) * a.D, l);
+                if constexpr (Q8) {
+                    float f[8], scale;
+                    floats<BF>(raw, f);
+                    *reinterpret_cast<uint2v*>(&share.rows[hs][t][8 * j]) = to_row8<LG, true>(f, scale);
+                    if (j == 0 && hs < heads) scales[place_of(a, slot + t, head).scale] = scale;
+                } else {
+                    *reinterpret_cast<raw8*>(&share.rows[hs][t][16 * j]) = raw;
+                }
+            }
+            __syncthreads();
+            const int bytes = values && Q8 && group == 2 ? 8 : 16, units = 16 * a.D * SIZE / bytes;  // of a head
+            for (int n = threadIdx.x; n < units * heads; n += kThreads) {
+                const int hs = n / units, u = n - hs * units;
+                char* to = cache + place_of(a, slot, h0 + hs).block * SIZE + u * bytes;
+                if (!values) {
+                    *reinterpret_cast<raw8*>(to) = *reinterpret_cast<const raw8*>(&share.rows[hs][u & 15][16 * (u >> 4)]);
+                } else if constexpr (!Q8) {
+                    raw8 v;
+                    value_unit<2>(u, [&](int k, int t, int c) { v[k] = *reinterpret_cast<const uint16_t*>(&share.rows[hs][t][2 * c]); });
+                    *reinterpret_cast<raw8*>(to) = v;
+                } else {
+                    uint32_t v[4] = {};
+                    const auto byte = [&](int k, int t, int c) { v[k >> 2] |= (uint32_t)(uint8_t)share.rows[hs][t][c] << 8 * (k & 3); };
+                    if (group == 4) {
+                        value_unit<4>(u, byte);
+                        *reinterpret_cast<uint4v*>(to) = uint4v{v[0], v[1], v[2], v[3]};
+                    } else {
+                        value_unit<2>(u, byte);
+                        *reinterpret_cast<uint2v*>(to) = uint2v{v[0], v[1]};
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        if (w.rest == 0) continue;
+#pragma unroll
+        for (int round = 0; round < kRounds<LG>; ++round) {
+            const int n = sub + round * TOKENS, t = n & 15, hs = n >> 4;
+            const bool live = hs < heads && (w.rest >> t & 1);
+            const int64_t from = live ? t0 + t : t0;
+            const int head = h0 + min(hs, heads - 1), slot = a.slots[from];
+            const raw8 raw = load_head(x + (from * a.Hkv + head) * a.D, l);
+            if constexpr (Q8) {
+                float f[8], scale;
+                floats<BF>(raw, f);
+                const uint2v q = to_row8<LG, true>(f, scale);
+                if (!live || !l.in) continue;
+                const Place p = place_of(a, slot, head);
+                if (values) cache_value8(a.vc, p, group, l.c0, q);
+                else cache_key8(a.kc, p, l, q);
+                if (j == 0) scales[p.scale] = scale;
+            } else {
+                if (!live || !l.in) continue;
+                const Place p = place_of(a, slot, head);
+                if (values) cache_value16(a.vc, p, l.c0, raw);
+                else cache_key16(a.kc, p, l, raw);
+            }
         }
     }
 }
 
 template <bool BF, int LG, bool Q8>
 __global__ __launch_bounds__(kThreads) void kv_cache_read_kernel(HeadsArgs a) {
-    constexpr int TOKENS = kThreads / LG;
-    const int j = threadIdx.x % LG, sub = threadIdx.x / LG, group = value_group(Q8, a.D);
-    const bool values = (int)blockIdx.y >= a.Hkv;
-    const int head = values ? blockIdx.y - a.Hkv : blockIdx.y;
+    constexpr int TOKENS = kThreads / LG, HEADS = kHeadsAtOnce<LG>, SIZE = Q8 ? 1 : 2;
+    __shared__ __attribute__((aligned(16))) BlockRows<LG, Q8> share;
+    const int j = threadIdx.x % LG, sub = threadIdx.x / LG, group = value_group(Q8, a.D), groups = (a.Hkv + HEADS - 1) / HEADS;
+    const bool values = (int)blockIdx.y >= groups;
+    const int h0 = (values ? blockIdx.y - groups : blockIdx.y) * HEADS, heads = min(HEADS, a.Hkv - h0);
     const Lane l = lane_of(j, a.D, 0, false);
     half_t* out = values ? a.v : a.k;
-    for (int64_t t0 = (int64_t)blockIdx.x * TOKENS; t0 < a.T; t0 += (int64_t)gridDim.x * TOKENS) {
-        const int64_t t = t0 + sub;
-        if (t >= a.T || !l.in) continue;
-        const int slot = a.slots[t];
-        raw8 v = {};
-        if ((uint32_t)slot < (uint32_t)a.slots_end) {
-            const Place p = place_of(a, slot, head);
-            if constexpr (Q8) {
-                const float scale = (values ? a.vs : a.ks)[p.scale];
-                const int8_t* at = static_cast<const int8_t*>(values ? a.vc : a.kc) + p.block;
-                at += values ? value_place(group, p.t, l.c0) : key_place(true, p.t, l.c0);
-                const int step = values ? 4 * group : 1;
-                float f[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = (float)at[step * e] * scale;
-                v = act_cvt8<BF>(f);
-            } else {
-                const uint16_t* at = static_cast<const uint16_t*>(values ? a.vc : a.kc) + p.block;
-                at += values ? value_place(2, p.t, l.c0) : key_place(false, p.t, l.c0);
-                const int step = values ? 8 : 1;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = at[step * e];
+    const char* cache = static_cast<const char*>(values ? a.vc : a.kc);
+    const float* scales = values ? a.vs : a.ks;
+    for (int64_t t0 = 16 * (int64_t)blockIdx.x; t0 < a.T; t0 += 16 * (int64_t)gridDim.x) {
+        const Window w = window_of(a, t0);
+        if (w.first >= 0) {
+            const int slot = a.slots[t0 + w.first];
+            const int bytes = values && Q8 && group == 2 ? 8 : 16, units = 16 * a.D * SIZE / bytes;
+            for (int n = threadIdx.x; n < units * heads; n += kThreads) {
+                const int hs = n / units, u = n - hs * units;
+                const char* at = cache + place_of(a, slot, h0 + hs).block * SIZE + u * bytes;
+                if (!values) {
+                    *reinterpret_cast<raw8*>(&share.rows[hs][u & 15][16 * (u >> 4)]) = *reinterpret_cast<const raw8*>(at);
+                } else if constexpr (!Q8) {
+                    const raw8 v = *reinterpret_cast<const raw8*>(at);
+                    value_unit<2>(u, [&](int k, int t, int c) { *reinterpret_cast<uint16_t*>(&share.rows[hs][t][2 * c]) = v[k]; });
+                } else if (group == 4) {
+                    const uint4v v = *reinterpret_cast<const uint4v*>(at);
+                    value_unit<4>(u, [&](int k, int t, int c) { share.rows[hs][t][c] = (char)(v[k >> 2] >> 8 * (k & 3)); });
+                } else {
+                    const uint2v v = *reinterpret_cast<const uint2v*>(at);
+                    value_unit<2>(u, [&](int k, int t, int c) { share.rows[hs][t][c] = (char)(v[k >> 2] >> 8 * (k & 3)); });
+                }
             }
+            __syncthreads();
+#pragma unroll
+            for (int round = 0; round < kRounds<LG>; ++round) {
+                const int n = sub + round * TOKENS, t = n & 15, hs = n >> 4;
+                if (hs >= heads || !l.in) continue;
+                raw8 v;
+                if constexpr (Q8) {
+                    const float scale = scales[place_of(a, slot + t, h0 + hs).scale];
+                    const uint2v q = *reinterpret_cast<const uint2v*>(&share.rows[hs][t][8 * j]);
+                    float f[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[e] = (float)(int8_t)(q[e >> 2] >> 8 * (e & 3)) * scale;
+                    v = act_cvt8<BF>(f);
+                } else {
+                    v = *reinterpret_cast<const raw8*>(&share.rows[hs][t][16 * j]);
+                }
+                store_head(out + ((t0 + w.first + t) * a.Hkv + h0 + hs) * a.D, l, v);
+            }
+            __syncthreads();
         }
-        store_head(out + (t * a.Hkv + head) * a.D, l, v);
+        // the others, and zeros for tokens that have no slot (those are in no block)
+#pragma unroll
+        for (int round = 0; round < kRounds<LG>; ++round) {
+            const int n = sub + round * TOKENS, t = n & 15, hs = n >> 4;
+            if (hs >= heads || !l.in || t0 + t >= a.T) continue;
+            const int slot = a.slots[t0 + t], head = h0 + hs;
+            const bool live = (uint32_t)slot < (uint32_t)a.slots_end;
+            if (live && !(w.rest >> t & 1)) continue;  // a block's
+            raw8 v = {};
+            if (live) {
+                const Place p = place_of(a, slot, head);
+                if constexpr (Q8) {
+                    const float scale = scales[p.scale];
+                    const int8_t* at = reinterpret_cast<const int8_t*>(cache) + p.block;
+                    at += values ? value_place(group, p.t, l.c0) : key_place(true, p.t, l.c0);
+                    const int step = values ? 4 * group : 1;
+                    float f[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[e] = (float)at[step * e] * scale;
+                    v = act_cvt8<BF>(f);
+                } else {
+                    const uint16_t* at = reinterpret_cast<const uint16_t*>(cache) + p.block;
+                    at += values ? value_place(2, p.t, l.c0) : key_place(false, p.t, l.c0);
+                    const int step = values ? 8 : 1;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = at[step * e];
+                }
+            }
+            store_head(out + ((t0 + t) * a.Hkv + head) * a.D, l, v);
+        }
     }
 }
 
@@ -763,7 +914,8 @@ int check_moved(const char* what, const clk_buffer* k, const clk_buffer* v, cons
 
 #define CLK_MOVE(KERNEL_)                                                                                              \
     const int lg = lanes_of(a.D);                                                                                      \
-    const dim3 grid(token_blocks(a.T, lg), 2 * a.Hkv), block(kThreads);                                                \
+    const int at_once = std::max(1, kThreads / lg / 16);                                                               \
+    const dim3 grid((unsigned)std::min<int64_t>((a.T + 15) / 16, 1 << 20), 2 * ceil_div(a.Hkv, at_once)), block(kThreads); \
     const auto launch = [&](auto bf_, auto lg_) {                                                                      \
         constexpr bool BF = decltype(bf_)::value;                                                                      \
         constexpr int LG = decltype(lg_)::value;                                                                       \
