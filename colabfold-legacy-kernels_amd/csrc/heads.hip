@@ -84,6 +84,10 @@ __device__ __forceinline__ raw8 load_head(const half_t* row, const Lane& l) {
     const raw8 v{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     return l.in ? v : raw8{};
 }
+__device__ __forceinline__ raw8 load_once(const half_t* row, const Lane& l) {  // 8 channels in a row
+    const raw8 v = __builtin_nontemporal_load(reinterpret_cast<const raw8*>(row + l.c0));
+    return l.in ? v : raw8{};
+}
 __device__ __forceinline__ void store_head(half_t* row, const Lane& l, raw8 v) {
     *reinterpret_cast<raw4*>(row + l.c0) = raw4{v[0], v[1], v[2], v[3]};
     *reinterpret_cast<raw4*>(row + l.c1) = raw4{v[4], v[5], v[6], v[7]};
@@ -445,8 +449,8 @@ struct BlockRows {
     char rows[kHeadsAtOnce<LG>][16][ROW];
 };
 
-// 16 bytes of a block's values (or 8, where a lane's cell has two channels of 8 bits), from rows or to them: unit u of a head has
-// channels 16 (C b + e) + i of tokens 4 g + j with u = (4 b + g) 16 + i
+// Four tokens of C channels of a block's values, from rows or to them: unit u of a head has channels 16 (C b + e) + i of tokens
+// 4 g + j, with u = (4 b + g) 16 + i
 template <int C, typename F>
 __device__ __forceinline__ void value_unit(int u, F f) {
     const int i = u & 15, g = u >> 4 & 3, b = u >> 6;
@@ -456,83 +460,98 @@ __device__ __forceinline__ void value_unit(int u, F f) {
         for (int j = 0; j < 4; ++j) f(4 * e + j, 4 * g + j, 16 * (C * b + e) + i);
 }
 
-// blockIdx.y: heads of keys, then of values
+// Keys and values of kHeadsAtOnce heads (blockIdx.y) of a window
 template <bool BF, int LG, bool Q8>
 __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(HeadsArgs a) {
-    constexpr int TOKENS = kThreads / LG, HEADS = kHeadsAtOnce<LG>, SIZE = Q8 ? 1 : 2;
-    __shared__ __attribute__((aligned(16))) BlockRows<LG, Q8> share;
-    const int j = threadIdx.x % LG, sub = threadIdx.x / LG, group = value_group(Q8, a.D), groups = (a.Hkv + HEADS - 1) / HEADS;
-    const bool values = (int)blockIdx.y >= groups;
-    const int h0 = (values ? blockIdx.y - groups : blockIdx.y) * HEADS, heads = min(HEADS, a.Hkv - h0);
+    constexpr int TOKENS = kThreads / LG, HEADS = kHeadsAtOnce<LG>, ROUNDS = kRounds<LG>, SIZE = Q8 ? 1 : 2;
+    __shared__ __attribute__((aligned(16))) BlockRows<LG, Q8> share[2];
+    const int j = threadIdx.x % LG, sub = threadIdx.x / LG, group = value_group(Q8, a.D);
+    const int h0 = blockIdx.y * HEADS, heads = min(HEADS, a.Hkv - h0);
     const Lane l = lane_of(j, a.D, 0, false);
-    const half_t* x = values ? a.dv : a.dk;
-    char* cache = static_cast<char*>(values ? a.vc : a.kc);
-    float* scales = values ? a.vs : a.ks;
     for (int64_t t0 = 16 * (int64_t)blockIdx.x; t0 < a.T; t0 += 16 * (int64_t)gridDim.x) {
         const Window w = window_of(a, t0);
         if (w.first >= 0) {
             const int slot = a.slots[t0 + w.first];
+            raw8 raw[2][ROUNDS];
 #pragma unroll
-            for (int round = 0; round < kRounds<LG>; ++round) {
-                const int n = sub + round * TOKENS, t = n & 15, hs = n >> 4;
-                const int head = h0 + min(hs, heads - 1);
-                const raw8 raw = load_head(x + ((t0 + w.first + t) * a.Hkv + head) * a.D, l);
-                if constexpr (Q8) {
-                    float f[8], scale;
-                    floats<BF>(raw, f);
-                    *reinterpret_cast<uint2v*>(&share.rows[hs][t][8 * j]) = to_row8<LG, true>(f, scale);
-                    if (j == 0 && hs < heads) scales[place_of(a, slot + t, head).scale] = scale;
-                } else {
-                    *reinterpret_cast<raw8*>(&share.rows[hs][t][16 * j]) = raw;
-                }
+            for (int round = 0; round < ROUNDS; ++round) {
+                const int n = sub + round * TOKENS, head = h0 + min(n >> 4, heads - 1);
+                const int64_t from = ((t0 + w.first + (n & 15)) * a.Hkv + head) * a.D;
+                // past the caches, which the cache is left in: 134 MB written and read again 118 us through them, 100 so
+                raw[0][round] = load_once(a.dk + from, l);
+                raw[1][round] = load_once(a.dv + from, l);
             }
+#pragma unroll
+            for (int values = 0; values < 2; ++values)
+#pragma unroll
+                for (int round = 0; round < ROUNDS; ++round) {
+                    const int n = sub + round * TOKENS, t = n & 15, hs = n >> 4;
+                    char* row = share[values].rows[hs][t];
+                    if constexpr (Q8) {
+                        float f[8], scale;
+                        floats<BF>(raw[values][round], f);
+                        *reinterpret_cast<uint2v*>(row + 8 * j) = to_row8<LG, true>(f, scale);
+                        if (j == 0 && hs < heads) (values ? a.vs : a.ks)[place_of(a, slot + t, h0 + hs).scale] = scale;
+                    } else {
+                        *reinterpret_cast<raw8*>(row + 16 * j) = raw[values][round];
+                    }
+                }
             __syncthreads();
-            const int bytes = values && Q8 && group == 2 ? 8 : 16, units = 16 * a.D * SIZE / bytes;  // of a head
-            for (int n = threadIdx.x; n < units * heads; n += kThreads) {
-                const int hs = n / units, u = n - hs * units;
-                char* to = cache + place_of(a, slot, h0 + hs).block * SIZE + u * bytes;
-                if (!values) {
-                    *reinterpret_cast<raw8*>(to) = *reinterpret_cast<const raw8*>(&share.rows[hs][u & 15][16 * (u >> 4)]);
-                } else if constexpr (!Q8) {
+            for (int n = threadIdx.x; n < a.D * SIZE * heads; n += kThreads) {  // 16 D SIZE / 16 units of 16 bytes a head
+                const int hs = n / (a.D * SIZE), u = n - hs * a.D * SIZE;
+                const int64_t at = place_of(a, slot, h0 + hs).block * SIZE + u * 16;
+                *reinterpret_cast<raw8*>(static_cast<char*>(a.kc) + at) =
+                    *reinterpret_cast<const raw8*>(&share[0].rows[hs][u & 15][16 * (u >> 4)]);
+                const auto& rows = share[1].rows[hs];
+                char* to = static_cast<char*>(a.vc) + at;
+                if constexpr (!Q8) {
                     raw8 v;
-                    value_unit<2>(u, [&](int k, int t, int c) { v[k] = *reinterpret_cast<const uint16_t*>(&share.rows[hs][t][2 * c]); });
+                    value_unit<2>(u, [&](int k, int t, int c) { v[k] = *reinterpret_cast<const uint16_t*>(&rows[t][2 * c]); });
                     *reinterpret_cast<raw8*>(to) = v;
                 } else {
                     uint32_t v[4] = {};
-                    const auto byte = [&](int k, int t, int c) { v[k >> 2] |= (uint32_t)(uint8_t)share.rows[hs][t][c] << 8 * (k & 3); };
                     if (group == 4) {
-                        value_unit<4>(u, byte);
-                        *reinterpret_cast<uint4v*>(to) = uint4v{v[0], v[1], v[2], v[3]};
+                        value_unit<4>(u, [&](int k, int t, int c) { v[k >> 2] |= (uint32_t)(uint8_t)rows[t][c] << 8 * (k & 3); });
                     } else {
-                        value_unit<2>(u, byte);
-                        *reinterpret_cast<uint2v*>(to) = uint2v{v[0], v[1]};
+                        const auto byte = [&](int k, int t, int c) { v[k >> 2] |= (uint32_t)(uint8_t)rows[t][c] << 8 * (k & 3); };
+                        value_unit<2>(2 * u, byte);
+                        value_unit<2>(2 * u + 1, [&](int k, int t, int c) { byte(k + 8, t, c); });
                     }
+                    *reinterpret_cast<uint4v*>(to) = uint4v{v[0], v[1], v[2], v[3]};
                 }
             }
             __syncthreads();
         }
         if (w.rest == 0) continue;
 #pragma unroll
-        for (int round = 0; round < kRounds<LG>; ++round) {
+        for (int round = 0; round < ROUNDS; ++round) {
             const int n = sub + round * TOKENS, t = n & 15, hs = n >> 4;
             const bool live = hs < heads && (w.rest >> t & 1);
-            const int64_t from = live ? t0 + t : t0;
-            const int head = h0 + min(hs, heads - 1), slot = a.slots[from];
-            const raw8 raw = load_head(x + (from * a.Hkv + head) * a.D, l);
+            const int64_t token = live ? t0 + t : t0;
+            const int head = h0 + min(hs, heads - 1), slot = live ? a.slots[token] : 0;
+            const Place p = place_of(a, slot, head);
+            const int64_t from = (token * a.Hkv + head) * a.D;
+            const raw8 raw[2] = {load_head(a.dk + from, l), load_head(a.dv + from, l)};
             if constexpr (Q8) {
-                float f[8], scale;
-                floats<BF>(raw, f);
-                const uint2v q = to_row8<LG, true>(f, scale);
+                uint2v q[2];
+                float scale[2];
+#pragma unroll
+                for (int values = 0; values < 2; ++values) {
+                    float f[8];
+                    floats<BF>(raw[values], f);
+                    q[values] = to_row8<LG, true>(f, scale[values]);
+                }
                 if (!live || !l.in) continue;
-                const Place p = place_of(a, slot, head);
-                if (values) cache_value8(a.vc, p, group, l.c0, q);
-                else cache_key8(a.kc, p, l, q);
-                if (j == 0) scales[p.scale] = scale;
+                cache_key8(a.kc, p, l, q[0]);
+                cache_value8(a.vc, p, group, l.c0, q[1]);
+                if (j == 0) {
+                    a.ks[p.scale] = scale[0];
+                    a.vs[p.scale] = scale[1];
+                }
             } else {
                 if (!live || !l.in) continue;
-                const Place p = place_of(a, slot, head);
-                if (values) cache_value16(a.vc, p, l.c0, raw);
-                else cache_key16(a.kc, p, l, raw);
+                cache_key16(a.kc, p, l, raw[0]);
+                cache_value16(a.vc, p, l.c0, raw[1]);
             }
         }
     }
@@ -540,85 +559,97 @@ __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(HeadsArgs a) {
 
 template <bool BF, int LG, bool Q8>
 __global__ __launch_bounds__(kThreads) void kv_cache_read_kernel(HeadsArgs a) {
-    constexpr int TOKENS = kThreads / LG, HEADS = kHeadsAtOnce<LG>, SIZE = Q8 ? 1 : 2;
-    __shared__ __attribute__((aligned(16))) BlockRows<LG, Q8> share;
-    const int j = threadIdx.x % LG, sub = threadIdx.x / LG, group = value_group(Q8, a.D), groups = (a.Hkv + HEADS - 1) / HEADS;
-    const bool values = (int)blockIdx.y >= groups;
-    const int h0 = (values ? blockIdx.y - groups : blockIdx.y) * HEADS, heads = min(HEADS, a.Hkv - h0);
+    constexpr int TOKENS = kThreads / LG, HEADS = kHeadsAtOnce<LG>, ROUNDS = kRounds<LG>, SIZE = Q8 ? 1 : 2;
+    __shared__ __attribute__((aligned(16))) BlockRows<LG, Q8> share[2];
+    const int j = threadIdx.x % LG, sub = threadIdx.x / LG, group = value_group(Q8, a.D);
+    const int h0 = blockIdx.y * HEADS, heads = min(HEADS, a.Hkv - h0);
     const Lane l = lane_of(j, a.D, 0, false);
-    half_t* out = values ? a.v : a.k;
-    const char* cache = static_cast<const char*>(values ? a.vc : a.kc);
-    const float* scales = values ? a.vs : a.ks;
+    const auto times = [](uint2v q, float scale) {
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = (float)(int8_t)(q[e >> 2] >> 8 * (e & 3)) * scale;
+        return act_cvt8<BF>(f);
+    };
     for (int64_t t0 = 16 * (int64_t)blockIdx.x; t0 < a.T; t0 += 16 * (int64_t)gridDim.x) {
         const Window w = window_of(a, t0);
         if (w.first >= 0) {
             const int slot = a.slots[t0 + w.first];
-            const int bytes = values && Q8 && group == 2 ? 8 : 16, units = 16 * a.D * SIZE / bytes;
-            for (int n = threadIdx.x; n < units * heads; n += kThreads) {
-                const int hs = n / units, u = n - hs * units;
-                const char* at = cache + place_of(a, slot, h0 + hs).block * SIZE + u * bytes;
-                if (!values) {
-                    *reinterpret_cast<raw8*>(&share.rows[hs][u & 15][16 * (u >> 4)]) = *reinterpret_cast<const raw8*>(at);
-                } else if constexpr (!Q8) {
-                    const raw8 v = *reinterpret_cast<const raw8*>(at);
-                    value_unit<2>(u, [&](int k, int t, int c) { *reinterpret_cast<uint16_t*>(&share.rows[hs][t][2 * c]) = v[k]; });
-                } else if (group == 4) {
-                    const uint4v v = *reinterpret_cast<const uint4v*>(at);
-                    value_unit<4>(u, [&](int k, int t, int c) { share.rows[hs][t][c] = (char)(v[k >> 2] >> 8 * (k & 3)); });
+            float scale[2][ROUNDS];
+            if constexpr (Q8) {
+#pragma unroll
+                for (int round = 0; round < ROUNDS; ++round) {
+                    const int n = sub + round * TOKENS;
+                    const int64_t at = place_of(a, slot + (n & 15), h0 + min(n >> 4, heads - 1)).scale;
+                    scale[0][round] = a.ks[at];
+                    scale[1][round] = a.vs[at];
+                }
+            }
+            for (int n = threadIdx.x; n < a.D * SIZE * heads; n += kThreads) {
+                const int hs = n / (a.D * SIZE), u = n - hs * a.D * SIZE;
+                const int64_t at = place_of(a, slot, h0 + hs).block * SIZE + u * 16;
+                const raw8 key = *reinterpret_cast<const raw8*>(static_cast<const char*>(a.kc) + at);
+                const raw8 value = *reinterpret_cast<const raw8*>(static_cast<const char*>(a.vc) + at);
+                *reinterpret_cast<raw8*>(&share[0].rows[hs][u & 15][16 * (u >> 4)]) = key;
+                auto& rows = share[1].rows[hs];
+                if constexpr (!Q8) {
+                    value_unit<2>(u, [&](int k, int t, int c) { *reinterpret_cast<uint16_t*>(&rows[t][2 * c]) = value[k]; });
                 } else {
-                    const uint2v v = *reinterpret_cast<const uint2v*>(at);
-                    value_unit<2>(u, [&](int k, int t, int c) { share.rows[hs][t][c] = (char)(v[k >> 2] >> 8 * (k & 3)); });
+                    const uint4v v = __builtin_bit_cast(uint4v, value);
+                    const auto byte = [&](int k, int t, int c) { rows[t][c] = (char)(v[k >> 2] >> 8 * (k & 3)); };
+                    if (group == 4) {
+                        value_unit<4>(u, byte);
+                    } else {
+                        value_unit<2>(2 * u, byte);
+                        value_unit<2>(2 * u + 1, [&](int k, int t, int c) { byte(k + 8, t, c); });
+                    }
                 }
             }
             __syncthreads();
 #pragma unroll
-            for (int round = 0; round < kRounds<LG>; ++round) {
+            for (int round = 0; round < ROUNDS; ++round) {
                 const int n = sub + round * TOKENS, t = n & 15, hs = n >> 4;
                 if (hs >= heads || !l.in) continue;
-                raw8 v;
-                if constexpr (Q8) {
-                    const float scale = scales[place_of(a, slot + t, h0 + hs).scale];
-                    const uint2v q = *reinterpret_cast<const uint2v*>(&share.rows[hs][t][8 * j]);
-                    float f[8];
+                const int64_t to = ((t0 + w.first + t) * a.Hkv + h0 + hs) * a.D;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] = (float)(int8_t)(q[e >> 2] >> 8 * (e & 3)) * scale;
-                    v = act_cvt8<BF>(f);
-                } else {
-                    v = *reinterpret_cast<const raw8*>(&share.rows[hs][t][16 * j]);
+                for (int values = 0; values < 2; ++values) {
+                    const char* row = share[values].rows[hs][t];
+                    raw8 v;
+                    if constexpr (Q8) v = times(*reinterpret_cast<const uint2v*>(row + 8 * j), scale[values][round]);
+                    else v = *reinterpret_cast<const raw8*>(row + 16 * j);
+                    store_head((values ? a.v : a.k) + to, l, v);
                 }
-                store_head(out + ((t0 + w.first + t) * a.Hkv + h0 + hs) * a.D, l, v);
             }
             __syncthreads();
         }
         // the others, and zeros for tokens that have no slot (those are in no block)
 #pragma unroll
-        for (int round = 0; round < kRounds<LG>; ++round) {
+        for (int round = 0; round < ROUNDS; ++round) {
             const int n = sub + round * TOKENS, t = n & 15, hs = n >> 4;
             if (hs >= heads || !l.in || t0 + t >= a.T) continue;
             const int slot = a.slots[t0 + t], head = h0 + hs;
             const bool live = (uint32_t)slot < (uint32_t)a.slots_end;
             if (live && !(w.rest >> t & 1)) continue;  // a block's
-            raw8 v = {};
+            raw8 v[2] = {};
             if (live) {
                 const Place p = place_of(a, slot, head);
                 if constexpr (Q8) {
-                    const float scale = scales[p.scale];
-                    const int8_t* at = reinterpret_cast<const int8_t*>(cache) + p.block;
-                    at += values ? value_place(group, p.t, l.c0) : key_place(true, p.t, l.c0);
-                    const int step = values ? 4 * group : 1;
-                    float f[8];
+                    const uint2v key = *reinterpret_cast<const uint2v*>(static_cast<const int8_t*>(a.kc) + p.block + key_place(true, p.t, l.c0));
+                    const uint8_t* at = static_cast<const uint8_t*>(a.vc) + p.block + value_place(group, p.t, l.c0);
+                    uint2v value{};
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] = (float)at[step * e] * scale;
-                    v = act_cvt8<BF>(f);
+                    for (int e = 0; e < 8; ++e) value[e >> 2] |= (uint32_t)at[4 * group * e] << 8 * (e & 3);
+                    v[0] = times(key, a.ks[p.scale]);
+                    v[1] = times(value, a.vs[p.scale]);
                 } else {
-                    const uint16_t* at = reinterpret_cast<const uint16_t*>(cache) + p.block;
-                    at += values ? value_place(2, p.t, l.c0) : key_place(false, p.t, l.c0);
-                    const int step = values ? 8 : 1;
+                    v[0] = *reinterpret_cast<const raw8*>(static_cast<const uint16_t*>(a.kc) + p.block + key_place(false, p.t, l.c0));
+                    const uint16_t* at = static_cast<const uint16_t*>(a.vc) + p.block + value_place(2, p.t, l.c0);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = at[step * e];
+                    for (int e = 0; e < 8; ++e) v[1][e] = at[8 * e];
                 }
             }
-            store_head(out + ((t0 + t) * a.Hkv + head) * a.D, l, v);
+            const int64_t to = ((t0 + t) * a.Hkv + head) * a.D;
+            store_head(a.k + to, l, v[0]);
+            store_head(a.v + to, l, v[1]);
         }
     }
 }
@@ -915,7 +946,7 @@ int check_moved(const char* what, const clk_buffer* k, const clk_buffer* v, cons
 #define CLK_MOVE(KERNEL_)                                                                                              \
     const int lg = lanes_of(a.D);                                                                                      \
     const int at_once = std::max(1, kThreads / lg / 16);                                                               \
-    const dim3 grid((unsigned)std::min<int64_t>((a.T + 15) / 16, 1 << 20), 2 * ceil_div(a.Hkv, at_once)), block(kThreads); \
+    const dim3 grid((unsigned)std::min<int64_t>((a.T + 15) / 16, 1 << 20), ceil_div(a.Hkv, at_once)), block(kThreads);    \
     const auto launch = [&](auto bf_, auto lg_) {                                                                      \
         constexpr bool BF = decltype(bf_)::value;                                                                      \
         constexpr int LG = decltype(lg_)::value;                                                                       \
