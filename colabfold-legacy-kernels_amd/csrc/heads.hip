@@ -15,7 +15,7 @@
 // A head is a group of LG lanes (the power of two at or past D / 8) with 8 channels each, the two halves of its pairs: a
 // lane whose channels are rotated by halves holds channels 4 j .. + 3 and R / 2 + 4 j .. + 3, so that pairs never
 // cross lanes; all others hold 8 j .. + 7. A workgroup takes 256 / LG tokens of up to HPG heads of one kind, and
-// reads a token's cosines and sines once for them.
+// reads a token's cosines and sines once for them. Workgroups go through a token's heads first.
 #include "kv_cache.h"
 #include "rows8_dev.h"
 
@@ -57,7 +57,8 @@ struct HeadsArgs {
     int64_t T;
     int Hq, Hkv, D, R, P;
     int cq, ck;          // chunks of heads: queries', keys' (values' as keys')
-    int parts;           // the backward's workgroups a chunk
+    int parts;           // workgroups a chunk
+    FastDiv by_chunks;
     int page, slots_end;  // the cache's page, and its tokens
     FastDiv by_page;
     float inv_d, eps;
@@ -98,10 +99,12 @@ __device__ __forceinline__ void floats(raw8 v, float (&f)[8]) {
     for (int e = 0; e < 8; ++e) f[e] = act_get<BF>(__builtin_bit_cast(half8, v), e);
 }
 __device__ __forceinline__ void load_weight(const float* w, const Lane& l, float (&f)[8]) {
+    typedef float4v float4u __attribute__((aligned(4)));
+    const float4v a = *reinterpret_cast<const float4u*>(w + l.c0), b = *reinterpret_cast<const float4u*>(w + l.c1);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        f[e] = l.in ? w[l.c0 + e] : 0.f;
-        f[4 + e] = l.in ? w[l.c1 + e] : 0.f;
+        f[e] = l.in ? a[e] : 0.f;
+        f[4 + e] = l.in ? b[e] : 0.f;
     }
 }
 
@@ -241,12 +244,13 @@ template <bool BF, int LG, int OUT, int HPG>
 __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(HeadsArgs a) {
     constexpr int TOKENS = kThreads / LG;
     const int j = threadIdx.x % LG, sub = threadIdx.x / LG;
-    const Heads h = heads_of<HPG>(a, blockIdx.y);
+    const int block = fdiv(blockIdx.x, a.by_chunks);
+    const Heads h = heads_of<HPG>(a, blockIdx.x - block * a.by_chunks.d);
     const Lane l = lane_of(j, a.D, h.kind == kValue ? 0 : a.R, a.interleaved);
     const int H = a.Hq + 2 * a.Hkv, group = value_group(OUT == kCache8, a.D);
     float w[8];
     if (h.kind != kValue) load_weight(h.kind == kQuery ? a.qn : a.kn, l, w);
-    for (int64_t t0 = (int64_t)blockIdx.x * TOKENS; t0 < a.T; t0 += (int64_t)gridDim.x * TOKENS) {
+    for (int64_t t0 = (int64_t)block * TOKENS; t0 < a.T; t0 += (int64_t)a.parts * TOKENS) {
         const int64_t t = t0 + sub, from = min(t, a.T - 1);  // past T: the last token, unused
         const half_t* row = a.x + (from * H + head_at(a, h.kind) + h.first) * a.D;
         raw8 raw[HPG];
@@ -315,13 +319,14 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_bwd_kernel(HeadsArgs a)
     constexpr int TOKENS = kThreads / LG, HPG = kBwdHeads;
     __shared__ float sums[TOKENS][LG * 8 + 1];
     const int j = threadIdx.x % LG, sub = threadIdx.x / LG;
-    const Heads h = heads_of<HPG>(a, blockIdx.y);
+    const int block = fdiv(blockIdx.x, a.by_chunks), chunk = blockIdx.x - block * a.by_chunks.d;
+    const Heads h = heads_of<HPG>(a, chunk);
     const Lane l = lane_of(j, a.D, h.kind == kValue ? 0 : a.R, a.interleaved);
     const int H = a.Hq + 2 * a.Hkv, mine = h.kind == kQuery ? a.Hq : a.Hkv;
     const half_t* dy = h.kind == kQuery ? a.dq : h.kind == kKey ? a.dk : a.dv;
     float w[8], dw[8] = {};
     if (h.kind != kValue) load_weight(h.kind == kQuery ? a.qn : a.kn, l, w);
-    for (int64_t t0 = (int64_t)blockIdx.x * TOKENS; t0 < a.T; t0 += (int64_t)a.parts * TOKENS) {
+    for (int64_t t0 = (int64_t)block * TOKENS; t0 < a.T; t0 += (int64_t)a.parts * TOKENS) {
         const int64_t t = t0 + sub, from = min(t, a.T - 1);
         const bool in = t < a.T && l.in;
         const half_t* row = a.x + (from * H + head_at(a, h.kind) + h.first) * a.D;
@@ -375,7 +380,7 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_bwd_kernel(HeadsArgs a)
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < TOKENS; ++i) s += sums[i][c];
-        a.partial[((int64_t)blockIdx.y * a.parts + blockIdx.x) * a.D + c] = s;
+        a.partial[((int64_t)chunk * a.parts + block) * a.D + c] = s;
     }
 }
 
@@ -664,7 +669,9 @@ int lanes_of(int64_t D) {
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // Workgroups for T tokens: a launch takes fewer than 2^32 threads, and the kernels go round
-unsigned token_blocks(int64_t T, int lg) { return (unsigned)std::min<int64_t>((T + kThreads / lg - 1) / (kThreads / lg), 1 << 20); }
+int token_blocks(int64_t T, int lg, int chunks) {
+    return (int)std::min<int64_t>((T + kThreads / lg - 1) / (kThreads / lg), std::max(1, (1 << 22) / chunks));
+}
 
 #define CLK_LANES(X_) X_(1) X_(2) X_(4) X_(8) X_(16) X_(32)
 #define CLK_CACHE_LANES(X_) X_(4) X_(8) X_(16) X_(32)
@@ -733,7 +740,10 @@ void launch_forward(HeadsArgs& a, bool bf, hipStream_t s) {
     const int hpg = wide ? 4 : 1;
     a.cq = ceil_div(a.Hq, hpg);
     a.ck = ceil_div(a.Hkv, hpg);
-    const dim3 grid(token_blocks(a.T, lg), a.cq + 2 * a.ck), block(kThreads);
+    const int chunks = a.cq + 2 * a.ck;
+    a.by_chunks = fast_div(chunks);
+    a.parts = token_blocks(a.T, lg, chunks);
+    const dim3 grid(a.parts * chunks), block(kThreads);
     const auto launch = [&](auto bf_, auto lg_) {
         constexpr bool BF = decltype(bf_)::value;
         constexpr int LG = decltype(lg_)::value;
@@ -894,7 +904,8 @@ extern "C" int clk_qk_norm_rope_bwd(clk_stream stream, const clk_buffer* qkv, co
     stage_mark(s, stage);
     if (a.T > 0) {
         a.parts = bwd_parts(a.T, a.Hq, a.Hkv, a.D);
-        const dim3 grid(a.parts, a.cq + 2 * a.ck), block(kThreads);
+        a.by_chunks = fast_div(a.cq + 2 * a.ck);
+        const dim3 grid(a.parts * (a.cq + 2 * a.ck)), block(kThreads);
         const int lg = lanes_of(a.D);
 #define CLK_L(LG_)                                                                                                    \
     if (lg == LG_) {                                                                                                  \
