@@ -58,7 +58,8 @@ struct HeadsArgs {
     int Hq, Hkv, D, R, P;
     int cq, ck;          // chunks of heads: queries', keys' (values' as keys')
     int parts;           // workgroups a chunk
-    FastDiv by_chunks;
+    int windows;         // workgroups a group of cached heads
+    FastDiv by_chunks, by_groups;
     int page, slots_end;  // the cache's page, and its tokens
     FastDiv by_page;
     float inv_d, eps;
@@ -238,16 +239,26 @@ __device__ __forceinline__ void cache_value8(void* vc, const Place& p, int group
 
 // ---- forward --------------------------------------------------------------------------------
 
-enum { kApart, kCache16, kCache8 };
+// A query's or key's 8 channels (f) normed, weighted and rotated; NaN where the token has no position
+template <bool BF, int LG>
+__device__ __forceinline__ void norm_rope(const HeadsArgs& a, float (&f)[8], const float (&w)[8], const Angles& angles, bool ok, const Lane& l) {
+    normalise<BF, LG>(f, a.inv_d, a.eps);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] *= w[e];
+    turn<false>(f, angles, l, a.interleaved);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = ok ? f[e] : __builtin_nanf("");
+}
 
-template <bool BF, int LG, int OUT, int HPG>
-__global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(HeadsArgs a) {
+// Heads apart: `chunk` of them, for the tokens from block 256 / LG on and every a.parts-th such block
+template <bool BF, int LG, int HPG>
+__device__ __forceinline__ void heads_apart(const HeadsArgs& a, int block, int chunk) {
     constexpr int TOKENS = kThreads / LG;
     const int j = threadIdx.x % LG, sub = threadIdx.x / LG;
-    const int block = fdiv(blockIdx.x, a.by_chunks);
-    const Heads h = heads_of<HPG>(a, blockIdx.x - block * a.by_chunks.d);
+    const Heads h = heads_of<HPG>(a, chunk);
     const Lane l = lane_of(j, a.D, h.kind == kValue ? 0 : a.R, a.interleaved);
-    const int H = a.Hq + 2 * a.Hkv, group = value_group(OUT == kCache8, a.D);
+    const int H = a.Hq + 2 * a.Hkv, mine = h.kind == kQuery ? a.Hq : a.Hkv;
+    half_t* out = h.kind == kQuery ? a.q : h.kind == kKey ? a.k : a.v;
     float w[8];
     if (h.kind != kValue) load_weight(h.kind == kQuery ? a.qn : a.kn, l, w);
     for (int64_t t0 = (int64_t)block * TOKENS; t0 < a.T; t0 += (int64_t)a.parts * TOKENS) {
@@ -259,55 +270,24 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(HeadsArgs a) {
         Angles angles;
         bool ok = true;
         if (h.kind != kValue) ok = load_angles(a, a.pos[from], j, l.turned, angles);
-        int slot = -1;
-        if (OUT != kApart && h.kind != kQuery) slot = a.slots[from];
-        const bool live = t < a.T && l.in && (OUT == kApart || h.kind == kQuery || (uint32_t)slot < (uint32_t)a.slots_end);
 #pragma unroll
         for (int i = 0; i < HPG; ++i) {
             if (i >= h.count) break;
-            const int head = h.first + i;
-            if (h.kind == kValue) {
-                if constexpr (OUT == kApart) {
-                    if (live) store_head(a.v + (t * a.Hkv + head) * a.D, l, raw[i]);
-                } else if constexpr (OUT == kCache16) {
-                    if (live) cache_value16(a.vc, place_of(a, slot, head), l.c0, raw[i]);
-                } else {
-                    float f[8], scale;
-                    floats<BF>(raw[i], f);
-                    const uint2v q = to_row8<LG, true>(f, scale);
-                    if (live) {
-                        const Place p = place_of(a, slot, head);
-                        cache_value8(a.vc, p, group, l.c0, q);
-                        if (j == 0) a.vs[p.scale] = scale;
-                    }
-                }
-                continue;
+            if (h.kind != kValue) {
+                float f[8];
+                floats<BF>(raw[i], f);
+                norm_rope<BF, LG>(a, f, w, angles, ok, l);
+                raw[i] = act_cvt8<BF>(f);
             }
-            float f[8];
-            floats<BF>(raw[i], f);
-            normalise<BF, LG>(f, a.inv_d, a.eps);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] *= w[e];
-            turn<false>(f, angles, l, a.interleaved);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = ok ? f[e] : __builtin_nanf("");
-            const raw8 y = act_cvt8<BF>(f);
-            if (OUT == kApart || h.kind == kQuery) {
-                half_t* out = h.kind == kQuery ? a.q + (t * a.Hq + head) * a.D : a.k + (t * a.Hkv + head) * a.D;
-                if (live) store_head(out, l, y);
-            } else if constexpr (OUT == kCache16) {
-                if (live) cache_key16(a.kc, place_of(a, slot, head), l, y);
-            } else {
-                float scale;
-                const uint2v q = to_row8<LG, false>(f, scale);
-                if (live) {
-                    const Place p = place_of(a, slot, head);
-                    cache_key8(a.kc, p, l, q);
-                    if (j == 0) a.ks[p.scale] = scale;
-                }
-            }
+            if (t < a.T && l.in) store_head(out + (t * mine + h.first + i) * a.D, l, raw[i]);
         }
     }
+}
+
+template <bool BF, int LG, int HPG>
+__global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(HeadsArgs a) {
+    const int block = fdiv(blockIdx.x, a.by_chunks);
+    heads_apart<BF, LG, HPG>(a, block, blockIdx.x - block * a.by_chunks.d);
 }
 
 // ---- backward -------------------------------------------------------------------------------
@@ -465,42 +445,97 @@ __device__ __forceinline__ void value_unit(int u, F f) {
         for (int j = 0; j < 4; ++j) f(4 * e + j, 4 * g + j, 16 * (C * b + e) + i);
 }
 
-// Keys and values of kHeadsAtOnce heads (blockIdx.y) of a window
-template <bool BF, int LG, bool Q8>
-__global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(HeadsArgs a) {
+// A lane's 8 channels of a key and a value: as they come, and as the cache holds them
+struct Pair {
+    raw8 key, value;
+    Angles angles;
+    bool ok;
+};
+struct Pair8 {
+    uint2v key, value;
+    float key_scale, value_scale;
+};
+// What a token's heads of keys and values come from: the projection's row (STEP), or k and v
+template <bool STEP>
+__device__ __forceinline__ Pair fetch(const HeadsArgs& a, int64_t token, int head, int j, const Lane& lk, const Lane& lv) {
+    Pair p;
+    if constexpr (STEP) {
+        const half_t* row = a.x + (token * (a.Hq + 2 * a.Hkv) + a.Hq + head) * a.D;
+        p.key = load_head(row, lk);
+        p.value = load_head(row + (int64_t)a.Hkv * a.D, lv);
+        p.ok = load_angles(a, a.pos[token], j, lk.turned, p.angles);
+    } else {
+        // past the caches, which the cache is left in: 134 MB written and read again 118 us through them, 100 so
+        const int64_t at = (token * a.Hkv + head) * a.D;
+        p.key = load_once(a.dk + at, lk);
+        p.value = load_once(a.dv + at, lv);
+    }
+    return p;
+}
+// Norm and rotation of a step's key, and both as 8-bit rows (all lanes of the head come here)
+template <bool BF, int LG, bool Q8, bool STEP>
+__device__ __forceinline__ Pair8 held(const HeadsArgs& a, Pair& p, const float (&w)[8], const Lane& lk) {
+    Pair8 h{};
+    float f[8];
+    if constexpr (STEP || Q8) floats<BF>(p.key, f);
+    if constexpr (STEP) {
+        norm_rope<BF, LG>(a, f, w, p.angles, p.ok, lk);
+        p.key = act_cvt8<BF>(f);
+    }
+    if constexpr (Q8) {
+        h.key = to_row8<LG, !STEP>(f, h.key_scale);
+        floats<BF>(p.value, f);
+        h.value = to_row8<LG, true>(f, h.value_scale);
+    }
+    return h;
+}
+
+// Keys and values of the kHeadsAtOnce heads from h0 on into the cache, window by window
+template <bool BF, int LG, bool Q8, bool STEP>
+__device__ __forceinline__ void cache_windows(const HeadsArgs& a, BlockRows<LG, Q8> (&share)[2], int64_t window, int64_t step, int h0) {
     constexpr int TOKENS = kThreads / LG, HEADS = kHeadsAtOnce<LG>, ROUNDS = kRounds<LG>, SIZE = Q8 ? 1 : 2;
-    __shared__ __attribute__((aligned(16))) BlockRows<LG, Q8> share[2];
-    const int j = threadIdx.x % LG, sub = threadIdx.x / LG, group = value_group(Q8, a.D);
-    const int h0 = blockIdx.y * HEADS, heads = min(HEADS, a.Hkv - h0);
-    const Lane l = lane_of(j, a.D, 0, false);
-    for (int64_t t0 = 16 * (int64_t)blockIdx.x; t0 < a.T; t0 += 16 * (int64_t)gridDim.x) {
-        const Window w = window_of(a, t0);
-        if (w.first >= 0) {
-            const int slot = a.slots[t0 + w.first];
-            raw8 raw[2][ROUNDS];
+    const int j = threadIdx.x % LG, sub = threadIdx.x / LG, group = value_group(Q8, a.D), heads = min(HEADS, a.Hkv - h0);
+    const Lane lk = lane_of(j, a.D, STEP ? a.R : 0, a.interleaved), lv = lane_of(j, a.D, 0, false);
+    float w[8];
+    if constexpr (STEP) load_weight(a.kn, lk, w);
+    for (int64_t t0 = 16 * window; t0 < a.T; t0 += 16 * step) {
+        Pair own[ROUNDS];  // the window's own tokens, on their way before it is known which of them go one by one
+#pragma unroll
+        for (int round = 0; round < ROUNDS; ++round) {
+            const int n = sub + round * TOKENS;
+            own[round] = fetch<STEP>(a, min(t0 + (n & 15), a.T - 1), h0 + min(n >> 4, heads - 1), j, lk, lv);
+        }
+        const Window win = window_of(a, t0);
+        if (win.first >= 0) {
+            const int slot = a.slots[t0 + win.first];
+            Pair p[ROUNDS];
 #pragma unroll
             for (int round = 0; round < ROUNDS; ++round) {
-                const int n = sub + round * TOKENS, head = h0 + min(n >> 4, heads - 1);
-                const int64_t from = ((t0 + w.first + (n & 15)) * a.Hkv + head) * a.D;
-                // past the caches, which the cache is left in: 134 MB written and read again 118 us through them, 100 so
-                raw[0][round] = load_once(a.dk + from, l);
-                raw[1][round] = load_once(a.dv + from, l);
+                const int n = sub + round * TOKENS;
+                p[round] = own[round];
+                if (win.first > 0) p[round] = fetch<STEP>(a, t0 + win.first + (n & 15), h0 + min(n >> 4, heads - 1), j, lk, lv);
             }
 #pragma unroll
-            for (int values = 0; values < 2; ++values)
-#pragma unroll
-                for (int round = 0; round < ROUNDS; ++round) {
-                    const int n = sub + round * TOKENS, t = n & 15, hs = n >> 4;
-                    char* row = share[values].rows[hs][t];
-                    if constexpr (Q8) {
-                        float f[8], scale;
-                        floats<BF>(raw[values][round], f);
-                        *reinterpret_cast<uint2v*>(row + 8 * j) = to_row8<LG, true>(f, scale);
-                        if (j == 0 && hs < heads) (values ? a.vs : a.ks)[place_of(a, slot + t, h0 + hs).scale] = scale;
-                    } else {
-                        *reinterpret_cast<raw8*>(row + 16 * j) = raw[values][round];
+            for (int round = 0; round < ROUNDS; ++round) {
+                const int n = sub + round * TOKENS, t = n & 15, hs = n >> 4;
+                const Pair8 q = held<BF, LG, Q8, STEP>(a, p[round], w, lk);
+                char* key = share[0].rows[hs][t];
+                char* value = share[1].rows[hs][t];
+                if (!lk.in) continue;
+                if constexpr (Q8) {
+                    *reinterpret_cast<uint32_t*>(key + lk.c0) = q.key[0];
+                    *reinterpret_cast<uint32_t*>(key + lk.c1) = q.key[1];
+                    *reinterpret_cast<uint2v*>(value + 8 * j) = q.value;
+                    if (j == 0 && hs < heads) {
+                        const int64_t at = place_of(a, slot + t, h0 + hs).scale;
+                        a.ks[at] = q.key_scale;
+                        a.vs[at] = q.value_scale;
                     }
+                } else {
+                    store_head(reinterpret_cast<half_t*>(key), lk, p[round].key);
+                    *reinterpret_cast<raw8*>(value + 16 * j) = p[round].value;
                 }
+            }
             __syncthreads();
             for (int n = threadIdx.x; n < a.D * SIZE * heads; n += kThreads) {  // 16 D SIZE / 16 units of 16 bytes a head
                 const int hs = n / (a.D * SIZE), u = n - hs * a.D * SIZE;
@@ -515,10 +550,10 @@ __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(HeadsArgs a) {
                     *reinterpret_cast<raw8*>(to) = v;
                 } else {
                     uint32_t v[4] = {};
+                    const auto byte = [&](int k, int t, int c) { v[k >> 2] |= (uint32_t)(uint8_t)rows[t][c] << 8 * (k & 3); };
                     if (group == 4) {
-                        value_unit<4>(u, [&](int k, int t, int c) { v[k >> 2] |= (uint32_t)(uint8_t)rows[t][c] << 8 * (k & 3); });
+                        value_unit<4>(u, byte);
                     } else {
-                        const auto byte = [&](int k, int t, int c) { v[k >> 2] |= (uint32_t)(uint8_t)rows[t][c] << 8 * (k & 3); };
                         value_unit<2>(2 * u, byte);
                         value_unit<2>(2 * u + 1, [&](int k, int t, int c) { byte(k + 8, t, c); });
                     }
@@ -527,38 +562,47 @@ __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(HeadsArgs a) {
             }
             __syncthreads();
         }
-        if (w.rest == 0) continue;
+        if (win.rest == 0) continue;
 #pragma unroll
         for (int round = 0; round < ROUNDS; ++round) {
             const int n = sub + round * TOKENS, t = n & 15, hs = n >> 4;
-            const bool live = hs < heads && (w.rest >> t & 1);
-            const int64_t token = live ? t0 + t : t0;
-            const int head = h0 + min(hs, heads - 1), slot = live ? a.slots[token] : 0;
-            const Place p = place_of(a, slot, head);
-            const int64_t from = (token * a.Hkv + head) * a.D;
-            const raw8 raw[2] = {load_head(a.dk + from, l), load_head(a.dv + from, l)};
+            const bool live = hs < heads && (win.rest >> t & 1) && lk.in;
+            const Place p = place_of(a, live ? a.slots[t0 + t] : 0, h0 + min(hs, heads - 1));
+            const Pair8 q = held<BF, LG, Q8, STEP>(a, own[round], w, lk);
+            if (!live) continue;
             if constexpr (Q8) {
-                uint2v q[2];
-                float scale[2];
-#pragma unroll
-                for (int values = 0; values < 2; ++values) {
-                    float f[8];
-                    floats<BF>(raw[values], f);
-                    q[values] = to_row8<LG, true>(f, scale[values]);
-                }
-                if (!live || !l.in) continue;
-                cache_key8(a.kc, p, l, q[0]);
-                cache_value8(a.vc, p, group, l.c0, q[1]);
+                cache_key8(a.kc, p, lk, q.key);
+                cache_value8(a.vc, p, group, lv.c0, q.value);
                 if (j == 0) {
-                    a.ks[p.scale] = scale[0];
-                    a.vs[p.scale] = scale[1];
+                    a.ks[p.scale] = q.key_scale;
+                    a.vs[p.scale] = q.value_scale;
                 }
             } else {
-                if (!live || !l.in) continue;
-                cache_key16(a.kc, p, l, raw[0]);
-                cache_value16(a.vc, p, l.c0, raw[1]);
+                cache_key16(a.kc, p, lk, own[round].key);
+                cache_value16(a.vc, p, lv.c0, own[round].value);
             }
         }
+    }
+}
+
+// blockIdx.y: heads
+template <bool BF, int LG, bool Q8>
+__global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(HeadsArgs a) {
+    __shared__ __attribute__((aligned(16))) BlockRows<LG, Q8> share[2];
+    cache_windows<BF, LG, Q8, false>(a, share, blockIdx.x, gridDim.x, blockIdx.y * kHeadsAtOnce<LG>);
+}
+
+// The first a.parts a.cq workgroups take the queries, the others windows of keys and values
+template <bool BF, int LG, bool Q8, int HPG>
+__global__ __launch_bounds__(kThreads) void qk_norm_rope_cache_kernel(HeadsArgs a) {
+    __shared__ __attribute__((aligned(16))) BlockRows<LG, Q8> share[2];
+    const int queries = a.parts * a.cq;
+    if ((int)blockIdx.x < queries) {
+        const int block = fdiv(blockIdx.x, a.by_chunks);
+        heads_apart<BF, LG, HPG>(a, block, blockIdx.x - block * a.by_chunks.d);
+    } else {
+        const int n = blockIdx.x - queries, window = fdiv(n, a.by_groups);
+        cache_windows<BF, LG, Q8, true>(a, share, window, a.windows, (n - window * a.by_groups.d) * kHeadsAtOnce<LG>);
     }
 }
 
@@ -731,15 +775,21 @@ void set_cache(HeadsArgs& a, const CacheShape& c, const clk_buffer* k, const clk
     a.by_page = fast_div(c.page);
 }
 
-template <int OUT>
+// Heads a workgroup: four share a token's angles and keep four loads in flight; few tokens are spread over more workgroups
+// instead.
+bool wide(int64_t T, int heads, int lg) { return T * heads * lg >= 4 * 256 * 1024; }
+
+#define CLK_L(LG_)                                                                                  \
+    if (lg == LG_) {                                                                                \
+        if (bf) launch(std::true_type(), std::integral_constant<int, LG_>());                       \
+        else launch(std::false_type(), std::integral_constant<int, LG_>());                         \
+    }
+
 void launch_forward(HeadsArgs& a, bool bf, hipStream_t s) {
     const int lg = lanes_of(a.D);
-    // Four heads a workgroup share a token's angles and keep four loads in flight; few tokens are spread over more
-    // workgroups instead.
-    const bool wide = a.T * (a.Hq + 2 * a.Hkv) * lg >= 4 * 256 * 1024;
-    const int hpg = wide ? 4 : 1;
-    a.cq = ceil_div(a.Hq, hpg);
-    a.ck = ceil_div(a.Hkv, hpg);
+    const bool four = wide(a.T, a.Hq + 2 * a.Hkv, lg);
+    a.cq = ceil_div(a.Hq, four ? 4 : 1);
+    a.ck = ceil_div(a.Hkv, four ? 4 : 1);
     const int chunks = a.cq + 2 * a.ck;
     a.by_chunks = fast_div(chunks);
     a.parts = token_blocks(a.T, lg, chunks);
@@ -747,21 +797,40 @@ void launch_forward(HeadsArgs& a, bool bf, hipStream_t s) {
     const auto launch = [&](auto bf_, auto lg_) {
         constexpr bool BF = decltype(bf_)::value;
         constexpr int LG = decltype(lg_)::value;
-        if (wide) hipLaunchKernelGGL((qk_norm_rope_kernel<BF, LG, OUT, 4>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((qk_norm_rope_kernel<BF, LG, OUT, 1>), grid, block, 0, s, a);
+        if (four) hipLaunchKernelGGL((qk_norm_rope_kernel<BF, LG, 4>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((qk_norm_rope_kernel<BF, LG, 1>), grid, block, 0, s, a);
     };
-#define CLK_L(LG_)                                                                                  \
-    if (lg == LG_) {                                                                                \
-        if (bf) launch(std::true_type(), std::integral_constant<int, LG_>());                       \
-        else launch(std::false_type(), std::integral_constant<int, LG_>());                         \
-    }
-    if constexpr (OUT == kApart) {
-        CLK_LANES(CLK_L)
-    } else {
-        CLK_CACHE_LANES(CLK_L)
-    }
-#undef CLK_L
+    CLK_LANES(CLK_L)
 }
+
+// Workgroups for T tokens' windows of 16, and the heads that each takes
+int window_blocks(int64_t T, int groups) { return (int)std::min<int64_t>((T + 15) / 16, std::max(1, (1 << 22) / groups)); }
+int head_groups(int64_t heads, int lg) { return ceil_div(heads, std::max(1, kThreads / lg / 16)); }
+
+void launch_step(HeadsArgs& a, bool bf, bool q8, hipStream_t s) {
+    const int lg = lanes_of(a.D);
+    const bool four = wide(a.T, a.Hq, lg);
+    a.cq = ceil_div(a.Hq, four ? 4 : 1);
+    a.by_chunks = fast_div(a.cq);
+    a.parts = token_blocks(a.T, lg, a.cq);
+    const int groups = head_groups(a.Hkv, lg);
+    a.by_groups = fast_div(groups);
+    a.windows = window_blocks(a.T, groups);
+    const dim3 grid(a.parts * a.cq + a.windows * groups), block(kThreads);
+    const auto launch = [&](auto bf_, auto lg_) {
+        constexpr bool BF = decltype(bf_)::value;
+        constexpr int LG = decltype(lg_)::value;
+        if (q8) {
+            if (four) hipLaunchKernelGGL((qk_norm_rope_cache_kernel<BF, LG, true, 4>), grid, block, 0, s, a);
+            else hipLaunchKernelGGL((qk_norm_rope_cache_kernel<BF, LG, true, 1>), grid, block, 0, s, a);
+        } else {
+            if (four) hipLaunchKernelGGL((qk_norm_rope_cache_kernel<BF, LG, false, 4>), grid, block, 0, s, a);
+            else hipLaunchKernelGGL((qk_norm_rope_cache_kernel<BF, LG, false, 1>), grid, block, 0, s, a);
+        }
+    };
+    CLK_CACHE_LANES(CLK_L)
+}
+#undef CLK_L
 
 // The backward's workgroups a chunk of heads: a rule on the shape alone, so that results do not depend on the device.
 // About two rounds of what 256 CUs hold in all.
@@ -822,7 +891,7 @@ extern "C" int clk_qk_norm_rope(clk_stream stream, const clk_buffer* qkv, const 
     a.interleaved = interleaved != 0;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     stage_mark(s, 0);
-    launch_forward<kApart>(a, act == CLK_BF16, s);
+    launch_forward(a, act == CLK_BF16, s);
     stage_mark(s, 1);
     return launch_status("qk_norm_rope");
 }
@@ -851,8 +920,7 @@ extern "C" int clk_qk_norm_rope_cache(clk_stream stream, const clk_buffer* qkv, 
     set_cache(a, c, k_cache, v_cache, k_scale, v_scale, slots);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     stage_mark(s, 0);
-    if (c.q8) launch_forward<kCache8>(a, act == CLK_BF16, s);
-    else launch_forward<kCache16>(a, act == CLK_BF16, s);
+    launch_step(a, act == CLK_BF16, c.q8, s);
     stage_mark(s, 1);
     return launch_status(what);
 }
@@ -956,8 +1024,8 @@ int check_moved(const char* what, const clk_buffer* k, const clk_buffer* v, cons
 
 #define CLK_MOVE(KERNEL_)                                                                                              \
     const int lg = lanes_of(a.D);                                                                                      \
-    const int at_once = std::max(1, kThreads / lg / 16);                                                               \
-    const dim3 grid((unsigned)std::min<int64_t>((a.T + 15) / 16, 1 << 20), ceil_div(a.Hkv, at_once)), block(kThreads);    \
+    const int groups = head_groups(a.Hkv, lg);                                                                         \
+    const dim3 grid(window_blocks(a.T, groups), groups), block(kThreads);                                              \
     const auto launch = [&](auto bf_, auto lg_) {                                                                      \
         constexpr bool BF = decltype(bf_)::value;                                                                      \
         constexpr int LG = decltype(lg_)::value;                                                                       \
