@@ -94,6 +94,19 @@ __device__ __forceinline__ void store_head(half_t* row, const Lane& l, raw8 v) {
     *reinterpret_cast<raw4*>(row + l.c0) = raw4{v[0], v[1], v[2], v[3]};
     *reinterpret_cast<raw4*>(row + l.c1) = raw4{v[4], v[5], v[6], v[7]};
 }
+// Stores through a buffer over a block of tokens: heads past its tokens, lanes past a head and heads past a chunk are offsets
+// past the buffer, which the hardware drops. A store in a branch makes the compiler wait for all loads and stores in
+// flight at the next use of a load.
+__device__ __forceinline__ auto tokens_buffer(half_t* first, int64_t tokens, int64_t row_bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(first, 0, (uint32_t)(tokens * row_bytes), 0x00020000);
+}
+constexpr uint32_t kDropped = 0xffffffffu;
+template <typename Rsrc>
+__device__ __forceinline__ void store_head(Rsrc r, uint32_t at, const Lane& l, raw8 v) {
+    const uint4v w = __builtin_bit_cast(uint4v, v);
+    __builtin_amdgcn_raw_buffer_store_b64(uint2v{w[0], w[1]}, r, at == kDropped ? at : at + 2 * l.c0, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b64(uint2v{w[2], w[3]}, r, at == kDropped ? at : at + 2 * l.c1, 0, 0);
+}
 template <bool BF>
 __device__ __forceinline__ void floats(raw8 v, float (&f)[8]) {
 #pragma unroll
@@ -250,36 +263,36 @@ __device__ __forceinline__ void norm_rope(const HeadsArgs& a, float (&f)[8], con
     for (int e = 0; e < 8; ++e) f[e] = ok ? f[e] : __builtin_nanf("");
 }
 
-// Heads apart: `chunk` of them, for the tokens from block 256 / LG on and every a.parts-th such block
-template <bool BF, int LG, int HPG>
-__device__ __forceinline__ void heads_apart(const HeadsArgs& a, int block, int chunk) {
+// Heads apart: up to HPG of them (h), normed and rotated, or values copied, for the tokens from block 256 / LG on and
+// every a.parts-th such block
+template <bool BF, int LG, int HPG, bool NORM>
+__device__ __forceinline__ void heads_apart(const HeadsArgs& a, int block, const Heads& h) {
     constexpr int TOKENS = kThreads / LG;
     const int j = threadIdx.x % LG, sub = threadIdx.x / LG;
-    const Heads h = heads_of<HPG>(a, chunk);
-    const Lane l = lane_of(j, a.D, h.kind == kValue ? 0 : a.R, a.interleaved);
+    const Lane l = lane_of(j, a.D, NORM ? a.R : 0, a.interleaved);
     const int H = a.Hq + 2 * a.Hkv, mine = h.kind == kQuery ? a.Hq : a.Hkv;
+    const half_t* x = a.x + (int64_t)(head_at(a, h.kind) + h.first) * a.D;
     half_t* out = h.kind == kQuery ? a.q : h.kind == kKey ? a.k : a.v;
     float w[8];
-    if (h.kind != kValue) load_weight(h.kind == kQuery ? a.qn : a.kn, l, w);
+    if constexpr (NORM) load_weight(h.kind == kQuery ? a.qn : a.kn, l, w);
     for (int64_t t0 = (int64_t)block * TOKENS; t0 < a.T; t0 += (int64_t)a.parts * TOKENS) {
-        const int64_t t = t0 + sub, from = min(t, a.T - 1);  // past T: the last token, unused
-        const half_t* row = a.x + (from * H + head_at(a, h.kind) + h.first) * a.D;
+        const int64_t from = min(t0 + sub, a.T - 1);  // past T: the last token, unused
         raw8 raw[HPG];
 #pragma unroll
-        for (int i = 0; i < HPG; ++i) raw[i] = load_head(row + (int64_t)min(i, h.count - 1) * a.D, l);
+        for (int i = 0; i < HPG; ++i) raw[i] = load_head(x + (from * H + min(i, h.count - 1)) * a.D, l);
         Angles angles;
         bool ok = true;
-        if (h.kind != kValue) ok = load_angles(a, a.pos[from], j, l.turned, angles);
+        if constexpr (NORM) ok = load_angles(a, a.pos[from], j, l.turned, angles);
+        const auto to = tokens_buffer(out + t0 * mine * a.D, min<int64_t>(TOKENS, a.T - t0), (int64_t)mine * a.D * 2);
 #pragma unroll
         for (int i = 0; i < HPG; ++i) {
-            if (i >= h.count) break;
-            if (h.kind != kValue) {
+            if constexpr (NORM) {
                 float f[8];
                 floats<BF>(raw[i], f);
                 norm_rope<BF, LG>(a, f, w, angles, ok, l);
                 raw[i] = act_cvt8<BF>(f);
             }
-            if (t < a.T && l.in) store_head(out + (t * mine + h.first + i) * a.D, l, raw[i]);
+            store_head(to, l.in && i < h.count ? (uint32_t)((sub * mine + h.first + i) * a.D) * 2 : kDropped, l, raw[i]);
         }
     }
 }
@@ -287,7 +300,9 @@ __device__ __forceinline__ void heads_apart(const HeadsArgs& a, int block, int c
 template <bool BF, int LG, int HPG>
 __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(HeadsArgs a) {
     const int block = fdiv(blockIdx.x, a.by_chunks);
-    heads_apart<BF, LG, HPG>(a, block, blockIdx.x - block * a.by_chunks.d);
+    const Heads h = heads_of<HPG>(a, blockIdx.x - block * a.by_chunks.d);
+    if (h.kind == kValue) heads_apart<BF, LG, HPG, false>(a, block, h);
+    else heads_apart<BF, LG, HPG, true>(a, block, h);
 }
 
 // ---- backward -------------------------------------------------------------------------------
@@ -308,10 +323,9 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_bwd_kernel(HeadsArgs a)
     if (h.kind != kValue) load_weight(h.kind == kQuery ? a.qn : a.kn, l, w);
     for (int64_t t0 = (int64_t)block * TOKENS; t0 < a.T; t0 += (int64_t)a.parts * TOKENS) {
         const int64_t t = t0 + sub, from = min(t, a.T - 1);
-        const bool in = t < a.T && l.in;
         const half_t* row = a.x + (from * H + head_at(a, h.kind) + h.first) * a.D;
         const half_t* gow = dy + (from * mine + h.first) * a.D;
-        half_t* out = a.dx + (from * H + head_at(a, h.kind) + h.first) * a.D;
+        const auto to = tokens_buffer(a.dx + t0 * H * a.D, min<int64_t>(TOKENS, a.T - t0), (int64_t)H * a.D * 2);
         raw8 raw[HPG], graw[HPG];
 #pragma unroll
         for (int i = 0; i < HPG; ++i) {
@@ -324,7 +338,6 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_bwd_kernel(HeadsArgs a)
         if (h.kind != kValue) ok = load_angles(a, a.pos[from], j, l.turned, angles);
 #pragma unroll
         for (int i = 0; i < HPG; ++i) {
-            if (i >= h.count) break;
             raw8 o = graw[i];
             if (h.kind != kValue) {
                 float f[8], g[8], dot = 0.f;
@@ -335,7 +348,7 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_bwd_kernel(HeadsArgs a)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     if (!ok) g[e] = __builtin_nanf("");
-                    if (t < a.T) dw[e] = __builtin_fmaf(g[e], f[e], dw[e]);
+                    if (t < a.T && i < h.count) dw[e] = __builtin_fmaf(g[e], f[e], dw[e]);
                     g[e] *= w[e];
                     dot = __builtin_fmaf(g[e], f[e], dot);
                 }
@@ -344,7 +357,7 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_bwd_kernel(HeadsArgs a)
                 for (int e = 0; e < 8; ++e) g[e] = r * __builtin_fmaf(-f[e], dot, g[e]);
                 o = act_cvt8<BF>(g);
             }
-            if (in) store_head(out + (int64_t)i * a.D, l, o);
+            store_head(to, l.in && i < h.count ? (uint32_t)((sub * H + head_at(a, h.kind) + h.first + i) * a.D) * 2 : kDropped, l, o);
         }
     }
     if (h.kind == kValue) return;
@@ -599,7 +612,7 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_cache_kernel(HeadsArgs 
     const int queries = a.parts * a.cq;
     if ((int)blockIdx.x < queries) {
         const int block = fdiv(blockIdx.x, a.by_chunks);
-        heads_apart<BF, LG, HPG>(a, block, blockIdx.x - block * a.by_chunks.d);
+        heads_apart<BF, LG, HPG, true>(a, block, heads_of<HPG>(a, blockIdx.x - block * a.by_chunks.d));
     } else {
         const int n = blockIdx.x - queries, window = fdiv(n, a.by_groups);
         cache_windows<BF, LG, Q8, true>(a, share, window, a.windows, (n - window * a.by_groups.d) * kHeadsAtOnce<LG>);
