@@ -83,6 +83,17 @@ def test_backward(hip, t, hq, hkv, d, r, kind):
         assert all(torch.equal(a, b) for a, b in zip(got, again))
 
 
+@pytest.mark.parametrize("t,hq,hkv", [(1, 1, 1), (17, 5, 2), (600, 3, 1)])
+def test_backward_without_eps(hip, t, hq, hkv):
+    """Tokens and heads that only fill up a workgroup count as zeros also where eps is 0."""
+    x, qn, kn, rope, pos, dy = inputs(t, hq, hkv, 96, 48, "f16")
+    got = hip.qk_norm_rope_bwd(x, qn, kn, rope, pos, *dy, 0.0)
+    for w, g, lo, hi, dw in ((qn, dy[0], 0, hq, got[1]), (kn, dy[1], hq, hq + hkv, got[2])):
+        dx, terms, want, wterms = oh.norm_rope_bwd(np64(x)[:, lo:hi], np64(w), np64(rope), pos.cpu().numpy(), np64(g), 0.0, False)
+        close(got[0][:, lo:hi], dx, terms, torch.float16, 2.0 ** -19)
+        close(dw, want, wterms, None, 2.0 ** -17)
+
+
 def test_backward_of_no_tokens(hip):
     x, qn, kn, rope, pos, dy = inputs(0, 4, 2, 64, 32, "f16")
     dx, dq, dk = hip.qk_norm_rope_bwd(x, qn, kn, rope, pos, *dy)
