@@ -634,17 +634,17 @@ __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(HeadsArgs a) {
     cache_windows<BF, LG, Q8, false>(a, share, blockIdx.x, gridDim.x, blockIdx.y * kHeadsAtOnce<LG>);
 }
 
-// The first a.parts a.cq workgroups take the queries, the others windows of keys and values
+// The first workgroups take windows of keys and values, which take longer, the others queries
 template <bool BF, int LG, bool Q8, int HPG>
 __global__ __launch_bounds__(kThreads) void qk_norm_rope_cache_kernel(HeadsArgs a) {
     __shared__ __attribute__((aligned(16))) BlockRows<LG, Q8> share[2];
-    const int queries = a.parts * a.cq;
-    if ((int)blockIdx.x < queries) {
-        const int block = fdiv(blockIdx.x, a.by_chunks);
-        heads_apart<BF, LG, HPG, true>(a, block, heads_of<HPG>(a, blockIdx.x - block * a.by_chunks.d));
+    const int cached = a.windows * a.by_groups.d;
+    if ((int)blockIdx.x < cached) {
+        const int window = fdiv(blockIdx.x, a.by_groups);
+        cache_windows<BF, LG, Q8, true>(a, share, window, a.windows, (blockIdx.x - window * a.by_groups.d) * kHeadsAtOnce<LG>);
     } else {
-        const int n = blockIdx.x - queries, window = fdiv(n, a.by_groups);
-        cache_windows<BF, LG, Q8, true>(a, share, window, a.windows, (n - window * a.by_groups.d) * kHeadsAtOnce<LG>);
+        const int n = blockIdx.x - cached, block = fdiv(n, a.by_chunks);
+        heads_apart<BF, LG, HPG, true>(a, block, heads_of<HPG>(a, n - block * a.by_chunks.d));
     }
 }
 
