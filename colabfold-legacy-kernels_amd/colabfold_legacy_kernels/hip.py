@@ -581,12 +581,14 @@ def _rank3(name, t):
 
 
 def _scratch(name, workspace, like, need):
-    """(workspace, its bytes): the caller's, or one of `need` bytes"""
+    """(workspace, its address, its bytes): the caller's, or one of `need` bytes"""
     if workspace is None:
-        workspace = like.new_empty(max(need, 1), dtype=torch.uint8)
+        if need == 0:
+            return None, None, 0
+        workspace = like.new_empty(need, dtype=torch.uint8)
     elif workspace.device != like.device or not workspace.is_contiguous():
         raise InvalidArgument(INVALID_ARGUMENT, "%s: workspace must be contiguous, on the tensors' GPU" % name)
-    return workspace, workspace.numel() * workspace.element_size()
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 def qk_norm_rope(qkv, q_norm, k_norm, rope, positions, kv_heads, eps=1e-5, interleaved=False, out=None):
@@ -620,9 +622,9 @@ def qk_norm_rope_bwd(qkv, q_norm, k_norm, rope, positions, dq, dk, dv, eps=1e-5,
     """(dqkv, dq_norm, dk_norm): the gradients of qk_norm_rope; written into `grads` when given."""
     if grads is None:
         grads = torch.empty_like(qkv), torch.empty_like(q_norm), torch.empty_like(k_norm)
-    workspace, size = _scratch("qk_norm_rope_bwd", workspace, qkv, qk_norm_rope_bwd_workspace(qkv, dk))
+    workspace, at, size = _scratch("qk_norm_rope_bwd", workspace, qkv, qk_norm_rope_bwd_workspace(qkv, dk))
     _call("clk_qk_norm_rope_bwd", (qkv, q_norm, k_norm, rope, positions, dq, dk, dv) + tuple(grads), float(eps),
-          int(bool(interleaved)), ctypes.c_void_p(workspace.data_ptr()), size)
+          int(bool(interleaved)), at, size)
     return grads
 
 
@@ -674,7 +676,7 @@ def paged_attention(q, cache, page_table, lengths, scale=None, want_lse=False, o
     want_lse = want_lse or lse is not None
     if want_lse and lse is None:
         lse = q.new_empty((b, h), dtype=torch.float32)
-    workspace, size = _scratch("paged_attention", workspace, q, paged_attention_workspace(q, cache, page_table))
+    workspace, at, size = _scratch("paged_attention", workspace, q, paged_attention_workspace(q, cache, page_table))
     _call("clk_paged_attention", (q,) + bufs + (page_table, lengths, out, lse if want_lse else _one(q, torch.float32)),
-          float(d ** -0.5 if scale is None else scale), int(want_lse), ctypes.c_void_p(workspace.data_ptr()), size)
+          float(d ** -0.5 if scale is None else scale), int(want_lse), at, size)
     return out, (lse if want_lse else None)

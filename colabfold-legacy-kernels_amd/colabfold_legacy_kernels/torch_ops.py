@@ -392,13 +392,11 @@ class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, q_norm, k_norm, rope, positions, kv_heads, eps, interleaved):
         qkv = qkv.contiguous()
-        lead, (h, d) = qkv.shape[:-2], qkv.shape[-2:]
-        out = tuple(qkv.new_empty(lead + (n, d)) for n in (h - 2 * kv_heads, kv_heads, kv_heads))
-        hip.qk_norm_rope(_heads(qkv), q_norm, k_norm, rope, positions, kv_heads, eps, interleaved, tuple(map(_heads, out)))
+        out = hip.qk_norm_rope(_heads(qkv), q_norm, k_norm, rope, positions, kv_heads, eps, interleaved)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(qkv, q_norm, k_norm, rope, positions)
         ctx.rule = kv_heads, eps, interleaved
-        return out
+        return out if qkv.dim() == 3 else tuple(t.view(qkv.shape[:-2] + t.shape[1:]) for t in out)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -409,11 +407,9 @@ class _QkNormRope(torch.autograd.Function):
         lead, (h, d) = qkv.shape[:-2], qkv.shape[-2:]
         grads = [qkv.new_zeros(lead + (n, d)) if g is None else g.to(qkv.dtype).contiguous()
                  for g, n in zip(grads, (h - 2 * kv_heads, kv_heads, kv_heads))]
-        dqkv, dq_norm, dk_norm = torch.empty_like(qkv), torch.empty_like(q_norm), torch.empty_like(k_norm)
-        hip.qk_norm_rope_bwd(_heads(qkv), q_norm, k_norm, rope, positions, *map(_heads, grads), eps, interleaved,
-                             grads=(_heads(dqkv), dq_norm, dk_norm))
+        dqkv, dq_norm, dk_norm = hip.qk_norm_rope_bwd(_heads(qkv), q_norm, k_norm, rope, positions, *map(_heads, grads), eps, interleaved)
         need = ctx.needs_input_grad
-        return (dqkv if need[0] else None, dq_norm if need[1] else None, dk_norm if need[2] else None) + (None,) * 5
+        return (dqkv.view(qkv.shape) if need[0] else None, dq_norm if need[1] else None, dk_norm if need[2] else None) + (None,) * 5
 
 
 def _heads(x):
@@ -423,6 +419,8 @@ def _heads(x):
 
 def _tokens(name, what, t, lead):
     """One value a token: of the leading shape, or one that broadcasts to it, as [T]"""
+    if len(lead) == 1 and t.shape == lead:
+        return t.contiguous()
     try:
         return t.expand(lead).reshape(-1)
     except RuntimeError:
@@ -483,7 +481,7 @@ def qk_norm_rope_cache(qkv, q_norm, k_norm, rope, positions, slots, cache, eps=1
     q = hip.qk_norm_rope_cache(rows, q_norm.float().contiguous(), k_norm.float().contiguous(), rope,
                                _tokens("qk_norm_rope_cache", "positions", positions, lead),
                                _tokens("qk_norm_rope_cache", "slots", slots, lead), cache, eps, interleaved)
-    return q.reshape(lead + q.shape[1:])
+    return q if len(lead) == 1 else q.reshape(lead + q.shape[1:])
 
 
 def kv_cache_write(k, v, slots, cache):
@@ -498,6 +496,8 @@ def kv_cache_write(k, v, slots, cache):
 def kv_cache_read(cache, slots, dtype=None):
     """(k, v) [..., heads, D]: what slots [...] int32 of the cache hold, zeros for a slot that it does not have."""
     k, v = hip.kv_cache_read(cache, slots.reshape(-1), dtype)
+    if slots.dim() == 1:
+        return k, v
     return k.reshape(slots.shape + k.shape[1:]), v.reshape(slots.shape + v.shape[1:])
 
 
