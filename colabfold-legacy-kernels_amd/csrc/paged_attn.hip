@@ -35,6 +35,9 @@ constexpr int kChunk = kWaves * 16 * kBlocks;
 
 // Workgroups a CU that the kernels' registers are kept for
 constexpr int occupancy(int64_t D) { return D <= 64 ? 4 : D <= 128 ? 3 : 2; }
+// Sequences, one a lane, up to which each workgroup works out by itself which part of which item it takes
+constexpr int kPlanned = 64;
+constexpr int kPlanThreads = 256;
 constexpr int kMostSplit = 256 * 4 * 3;
 
 // Weights are taken times 2^bias, which their sum has too and which cancels: fp16 ones so that small ones keep their bits (a
@@ -62,15 +65,13 @@ struct AttnArgs {
     float* part_o;  // [2 W][16][D]
     float* part_s;  // [2 W][2][16]: running maximum, sum
     int4v* split;   // [W]: an item in parts, its first part and how many it has
-    int* meta;      // the items in parts
+    int4v* plan;    // of each workgroup: sequence, item of the sequence, part << 16 | parts, place; null: it works that out
+    int* meta;      // the items in parts; planned workgroups
 };
 
 // A wave-uniform value on the scalar unit, and a scalar load from an array that the kernel does not write: a page's number
 // by a vector load would be waited for behind all keys and values in flight.
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ int64_t uniform(int64_t v) {
-    return (int64_t)((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v));
-}
 __device__ __forceinline__ int scalar_load(const int32_t* p, int64_t i) {
     return reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p))[i];
 }
@@ -458,72 +459,164 @@ __device__ __forceinline__ int parts_in(int chunks, int c) { return chunks <= c 
 // Items in parts of about as many chunks, however the lengths differ, one a workgroup. c, the most chunks of a part, is the
 // least with which W workgroups, all at once on the chip, are enough, but at most what room = W - min(items, W / 2)
 // workgroups would need if parts were as long as that to the last (with so many items that theirs do not fit on the
-// chip at once anyway). Items of one part are finished here; parts of the others are numbered through and left for paged_attn_join_kernel.
+// chip at once anyway). Items of one part are finished at once; parts of the others are numbered through and left for
+// paged_attn_join_kernel.
 // (All chunks in W equal runs, one a workgroup, where a run could end one item and begin the next, was more even but a
 // workgroup had two short spans as often as one, each with its chain of loads: 61 sequences of up to 8192 over 8 bits
 // took 43 us.)
-template <bool BF, bool Q8, bool NT, int D>
-__global__ __launch_bounds__(kWaves* kWave, occupancy(D)) void paged_attn_split_kernel(AttnArgs a) {
-    __shared__ WaveShare<D> share;
-    const int tid = threadIdx.x, wave = uniform((int)(tid / kWave)), lane = tid % kWave;
+//
+// over(f) calls f for the caller's share of the lengths, sum adds up what the callers have.
+template <typename Over, typename Sum>
+__device__ __forceinline__ int chunks_of_parts(const AttnArgs& a, Over over, Sum sum) {
+    int64_t mine = 0;
+    over([&](int len) { mine += chunks_in(a, len); });
+    const int64_t items = (int64_t)a.B * a.heads, room = a.W - min<int64_t>(items, a.W / 2);
+    const int64_t U = (((int64_t)sum((uint32_t)(mine >> 24)) << 24) + sum((uint32_t)mine & 0xffffffu)) * a.heads;
+    const auto most = [&](int64_t groups) {
+        if (U < 1 << 30) return max(1, (int)(((uint32_t)U + (uint32_t)groups - 1) / (uint32_t)groups));
+        return (int)min<int64_t>(1 << 30, (U + groups - 1) / groups);
+    };
+    int c = most(room);
+    if (items > a.W) return c;  // which has as many parts at least
+    for (int low = most(a.W); low < c;) {  // the least c, or this one, with at most W parts
+        const int mid = low + (c - low) / 2;
+        int64_t parts = 0;
+        over([&](int len) { parts += parts_in(chunks_in(a, len), mid); });
+        if ((int64_t)sum((uint32_t)min<int64_t>(parts, 1 << 24)) * a.heads <= a.W) c = mid;  // (a lane's 2^24 are too many)
+        else low = mid + 1;
+    }
+    return c;
+}
+// A sequence's workgroups, and below them its parts (16 bits) and items in parts
+struct Count {
+    uint32_t groups, parts;
+};
+__device__ __forceinline__ Count count_of(const AttnArgs& a, int len, int c) {
+    const uint32_t k = (uint32_t)parts_in(chunks_in(a, len), c), groups = k * (uint32_t)a.heads;
+    return Count{groups, k > 1 ? groups << 16 | (uint32_t)a.heads : 0};
+}
+
+// What a workgroup does: part j of the k of an item, and the place of its results where k > 1
+struct Work {
+    int b, hr, j, k, slot;
+};
+
+// The work of paged_attn_split_kernel's workgroups where there are so many sequences that it would take each of them long
+// to go through: 256 sequences a workgroup, which counts those before by itself.
+__global__ __launch_bounds__(kPlanThreads) void paged_attn_plan_kernel(AttnArgs a) {
+    constexpr int WAVES = kPlanThreads / kWave;
+    __shared__ uint32_t red[2][WAVES];
+    const int tid = threadIdx.x, wave = uniform((int)(tid / kWave)), first = blockIdx.x * kPlanThreads;
+    int turn = 0;
+    const auto waves = [&](uint32_t v, uint32_t& below) {  // sum of v over all threads, and over the waves below
+        v = wave_sum(v);
+        if (tid % kWave == 0) red[turn][wave] = v;
+        __syncthreads();
+        uint32_t all = 0;
+        below = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            if (w == wave) below = all;
+            all += red[turn][w];
+        }
+        turn ^= 1;  // one barrier a sum: the next goes through the other half
+        return all;
+    };
+    uint32_t below;
+    const auto sum = [&](uint32_t v) { return waves(v, below); };
+    const int c = chunks_of_parts(a, [&](auto f) {
+        for (int b = tid; b < a.B; b += kPlanThreads) f(a.len[b]);
+    }, sum);
+    Count before{0, 0};
+    for (int b = tid; b < first; b += kPlanThreads) {
+        const Count n = count_of(a, a.len[b], c);
+        before.groups += n.groups;
+        before.parts += n.parts;
+    }
+    before.groups = sum(before.groups);
+    before.parts = sum(before.parts);
+    const int b = first + tid, len = b < a.B ? a.len[b] : 0;
+    const Count n = b < a.B ? count_of(a, len, c) : Count{0, 0};
+    uint32_t groups_below, parts_below;
+    const uint32_t groups = before.groups + waves(n.groups, groups_below), parts = before.parts + waves(n.parts, parts_below);
+    if (blockIdx.x == gridDim.x - 1 && tid == 0) {
+        a.meta[0] = (int)(parts & 0xffffu);
+        a.meta[1] = (int)groups;
+    }
+    const int at = (int)(before.groups + groups_below + wave_scan(n.groups) - n.groups);
+    const uint32_t p = before.parts + parts_below + wave_scan(n.parts) - n.parts;
+    if (b >= a.B) return;
+    const int k = (int)n.groups / a.heads, slot = (int)(p >> 16);
+    for (int hr = 0, i = 0; hr < a.heads; ++hr) {
+        if (k > 1) a.split[(p & 0xffffu) + hr] = int4v{b * a.heads + hr, slot + i, k, 0};
+        for (int j = 0; j < k; ++j, ++i) a.plan[at + i] = int4v{b, hr, j << 16 | k, slot + i};
+    }
+}
+
+// The workgroup's work as each works it out for itself; false: it has none
+__device__ __forceinline__ bool work_of(const AttnArgs& a, Work& work) {
+    const int tid = threadIdx.x, lane = tid % kWave;
     // each wave looks at all lengths by itself: lane's are b0 .. b1 - 1, and the first is kept
     const int per = (a.B + kWave - 1) / kWave, b0 = min(lane * per, a.B), b1 = min(b0 + per, a.B);
     const int len0 = b0 < b1 ? a.len[b0] : -1;
     const auto over = [&](auto f) {  // f of the lane's lengths, in order
         for (int b = b0; b < b1; ++b) f(b == b0 ? len0 : a.len[b]);
     };
-    int64_t mine = 0;
-    over([&](int len) { mine += chunks_in(a, len); });
-    const int64_t room = a.W - min<int64_t>((int64_t)a.B * a.heads, a.W / 2);
-    const int64_t U = (((int64_t)wave_sum((uint32_t)(mine >> 24)) << 24) + wave_sum((uint32_t)mine & 0xffffffu)) * a.heads;
-    const auto most = [&](int64_t groups) {
-        if (U < 1 << 30) return max(1, (int)(((uint32_t)U + (uint32_t)groups - 1) / (uint32_t)groups));
-        return (int)min<int64_t>(1 << 30, (U + groups - 1) / groups);
-    };
-    int c = most(room);
-    for (int low = most(a.W); low < c;) {  // the least c, or this one, with at most W parts
-        const int mid = low + (c - low) / 2;
-        int64_t parts = 0;
-        over([&](int len) { parts += parts_in(chunks_in(a, len), mid); });
-        if ((int64_t)wave_sum((uint32_t)min<int64_t>(parts, 1 << 24)) * a.heads <= a.W) c = mid;  // (a lane's 2^24 are too many)
-        else low = mid + 1;
-    }
-    // workgroups, and below them parts (16 bits) and items in parts, of the lane's sequences and of those before
-    const auto count = [&](int len, uint32_t& groups, uint32_t& parts) {
-        const int k = parts_in(chunks_in(a, len), c);
-        groups += (uint32_t)(k * a.heads);
-        if (k > 1) parts += (uint32_t)(k * a.heads) << 16 | (uint32_t)a.heads;
-    };
+    const int c = chunks_of_parts(a, over, [](uint32_t v) { return wave_sum(v); });
     uint32_t groups = 0, parts = 0;
-    over([&](int len) { count(len, groups, parts); });
+    over([&](int len) {
+        const Count n = count_of(a, len, c);
+        groups += n.groups;
+        parts += n.parts;
+    });
     const uint32_t id = blockIdx.x, groups_to = wave_scan(groups), parts_to = wave_scan(parts);
     if (id == 0 && tid == kWave - 1) a.meta[0] = (int)(parts_to & 0xffffu);
     const uint64_t has = __ballot(groups_to > id);
-    if (has == 0) return;
+    if (has == 0) return false;
     const int from = __builtin_ctzll(has);
     uint32_t before = lane_value(groups_to - groups, from), parts_before = lane_value(parts_to - parts, from);
     int b = from * per, len = (int)lane_value((uint32_t)len0, from);
-    for (;;) {
-        uint32_t g = 0, p = 0;
-        count(len, g, p);
-        if (before + g > id) break;
-        before += g;
-        parts_before += p;
+    Count n = count_of(a, len, c);
+    while (before + n.groups <= id) {
+        before += n.groups;
+        parts_before += n.parts;
         len = scalar_load(a.len, ++b);
+        n = count_of(a, len, c);
     }
-    const int chunks = chunks_in(a, len), k = parts_in(chunks, c), at = (int)(id - before);
-    const int hr = at / k, j = at - hr * k, each = (chunks - 1) / k + 1;
-    const Span sp = span_of(a, b, hr, j * each * kChunk, min(len, (j + 1) * each * kChunk));
+    const int at = (int)(id - before);
+    work.b = b;
+    work.k = parts_in(chunks_in(a, len), c);
+    work.hr = at / work.k;
+    work.j = at - work.hr * work.k;
+    work.slot = (int)(parts_before >> 16) + at;
+    if (work.k > 1 && tid == 0 && work.j == 0) a.split[(parts_before & 0xffffu) + work.hr] = int4v{b * a.heads + work.hr, work.slot, work.k, 0};
+    return true;
+}
+
+template <bool BF, bool Q8, bool NT, int D>
+__global__ __launch_bounds__(kWaves* kWave, occupancy(D)) void paged_attn_split_kernel(AttnArgs a) {
+    __shared__ WaveShare<D> share;
+    const int wave = uniform((int)(threadIdx.x / kWave));
+    Work work;
+    if (a.plan != nullptr) {
+        if ((int)blockIdx.x >= scalar_load(a.meta, 1)) return;
+        const int32_t* p = reinterpret_cast<const int32_t*>(a.plan);
+        const int64_t at = 4 * (int64_t)blockIdx.x;
+        const int jk = scalar_load(p, at + 2);
+        work = Work{scalar_load(p, at), scalar_load(p, at + 1), jk >> 16, jk & 0xffff, scalar_load(p, at + 3)};
+    } else if (!work_of(a, work)) {
+        return;
+    }
+    const int len = scalar_load(a.len, work.b), chunks = chunks_in(a, len), each = (chunks - 1) / work.k + 1;
+    const Span sp = span_of(a, work.b, work.hr, work.j * each * kChunk, min(len, (work.j + 1) * each * kChunk));
     if (chunks == 0) {
         finish_empty<BF, D>(a, sp, len > 0);
         return;
     }
     float *part_o = nullptr, *part_s = nullptr;
-    if (k > 1) {
-        const int slot = (int)(parts_before >> 16) + at;
-        part_o = a.part_o + (int64_t)slot * 16 * D;
-        part_s = a.part_s + slot * 32;
-        if (tid == 0 && j == 0) a.split[(parts_before & 0xffffu) + hr] = int4v{b * a.heads + hr, slot, k, 0};
+    if (work.k > 1) {
+        part_o = a.part_o + (int64_t)work.slot * 16 * D;
+        part_s = a.part_s + work.slot * 32;
     }
     State<D> st;
     attend<BF, Q8, NT, D>(a, sp, wave, st);
@@ -606,8 +699,8 @@ struct Plan {
     int64_t items = 0;  // 0: a shape that the entry point rejects
     int W = 0;          // of a split call, 0: a workgroup an item
     int64_t grid = 0;
-    size_t o = 0, s = 0, split = 0, meta = 0;
-    size_t bytes() const { return o + s + split + meta; }
+    size_t o = 0, s = 0, split = 0, meta = 0, plan = 0;
+    size_t bytes() const { return o + s + split + meta + plan; }
 };
 Plan plan_of(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t per, int64_t page) {
     Plan p;
@@ -617,7 +710,7 @@ Plan plan_of(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t per, int64_t
     p.items = p.grid = B * Hkv * blocks;
     if (per * page > kDirect && B > 0) {
         // One round of workgroups, but where the items nearly make one already, three, so that the long among them are cut
-        // finely enough to fill the last round: 256 ragged sequences of up to 4096 on 8 heads 155 us, 166 with one; 61 on
+        // finely enough to fill the last round: 256 ragged sequences of up to 4096 on 8 heads 157 us, 167 with two; 61 on
         // 4 heads 43 with one and 48 with three.
         p.W = 256 * occupancy(D) * (p.items > 128 * occupancy(D) ? 3 : 1);
         // With c as the kernel takes it, all chunks / c <= room = W - min(items, W / 2), and an item has under its chunks / c + 1
@@ -628,6 +721,10 @@ Plan plan_of(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t per, int64_t
         p.s = (size_t)2 * p.W * 32 * 4;
         p.split = (size_t)p.W * 16;
         p.meta = 256;
+        // Many items of many sequences are dealt out by a launch before (2.5 us and a gap): 256 sequences of up to 1024 on 8 heads
+        // 117 us, 122 without; 1024 of them 403, 692 without; 4096 ragged ones 659, 6790 without; but 50 ragged ones of up
+        // to 4096 51.5, 46.2 without, and 128 on one head 19.4, 17.1 without.
+        if (B > kPlanned && p.items > 128 * occupancy(D)) p.plan = (size_t)p.grid * 16;
     }
     return p;
 }
@@ -667,7 +764,8 @@ extern "C" int clk_paged_attention(clk_stream stream, const clk_buffer* q, const
     if (lengths->rank != 1 || lengths->dims[0] != B) return invalid("paged_attention: lengths must be [B]");
     if (!same_shape(out, q)) return invalid("paged_attention: out must be like q");
     if (want_lse && (lse->rank != 2 || lse->dims[0] != B || lse->dims[1] != Hq)) return invalid("paged_attention: lse must be [B,Hq]");
-    if (!(scale == scale) || scale - scale != 0.f) return invalid("paged_attention: scale must be finite");
+    const float scale2 = scale * kLog2e;
+    if (!(scale2 - scale2 == 0.f)) return invalid("paged_attention: scale must be finite, times log2(e) too");
     const int64_t G = Hq / c.heads, blocks = (G + 15) / 16;
     const Plan plan = plan_of(B, Hq, c.heads, c.D, page_table->dims[1], c.page);
     if (B > 0 && plan.items == 0) return invalid("paged_attention: too large");
@@ -699,13 +797,14 @@ extern "C" int clk_paged_attention(clk_stream stream, const clk_buffer* q, const
     a.by_blocks = fast_div(blocks);
     a.heads = (int)(c.heads * blocks);
     a.by_heads = fast_div(a.heads);
-    a.scale2 = scale * kLog2e;
+    a.scale2 = scale2;
     a.W = plan.W;
     char* ws = static_cast<char*>(workspace);
     a.part_o = reinterpret_cast<float*>(ws);
     a.part_s = reinterpret_cast<float*>(ws + plan.o);
     a.split = reinterpret_cast<int4v*>(ws + plan.o + plan.s);
     a.meta = reinterpret_cast<int*>(ws + plan.o + plan.s + plan.split);
+    a.plan = plan.plan ? reinterpret_cast<int4v*>(ws + plan.o + plan.s + plan.split + plan.meta) : nullptr;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     int stage = 0;
     stage_mark(s, stage);
@@ -720,6 +819,10 @@ extern "C" int clk_paged_attention(clk_stream stream, const clk_buffer* q, const
         if (plan.W == 0) {
             hipLaunchKernelGGL((paged_attn_kernel<BF, Q8, D>), dim3((unsigned)plan.grid), block, 0, s, a);
             return;
+        }
+        if (a.plan != nullptr) {
+            hipLaunchKernelGGL(paged_attn_plan_kernel, dim3((unsigned)((B + kPlanThreads - 1) / kPlanThreads)), dim3(kPlanThreads), 0, s, a);
+            stage_mark(s, ++stage);
         }
         if (past) hipLaunchKernelGGL((paged_attn_split_kernel<BF, Q8, true, D>), dim3((unsigned)plan.grid), block, 0, s, a);
         else hipLaunchKernelGGL((paged_attn_split_kernel<BF, Q8, false, D>), dim3((unsigned)plan.grid), block, 0, s, a);

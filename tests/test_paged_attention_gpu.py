@@ -134,6 +134,26 @@ def test_many_short_sequences(hip, bits):
         c.check(out, lse, 32 ** -0.5, only=list(range(0, 4100, 37)) + [4099])
 
 
+@pytest.mark.parametrize("b,longest,hq,hkv", ((256, 900, 4, 1), (257, 900, 4, 1), (513, 700, 40, 2), (1100, 1200, 3, 3), (700, 30, 2, 1)))
+def test_large_ragged_batches(hip, b, longest, hq, hkv):
+    """Batches past what a workgroup looks through by itself: a few long sequences in parts among short and empty ones, one that
+    says more tokens than its pages hold, and more items than the chip takes at once."""
+    rng = np.random.default_rng(b)
+    lengths = [int(n) for n in np.exp(rng.uniform(0, np.log(40), b))]
+    for i in range(0, b, 5):
+        lengths[i] = 0
+    for i in (1, 2, b // 2, b - 2, b - 1):
+        lengths[i] = longest
+    c = Case(lengths, hq, hkv, 32, 16, 8, "f16", seed=b)
+    table = torch.nn.functional.pad(c.table, (0, 40), value=-1)
+    c.len[3] = table.shape[1] * 16 + 1
+    out, lse = hip.paged_attention(c.q, c.cache, table, c.len, want_lse=True)
+    assert out[3].isnan().all() and lse[3].isnan().all()
+    c.check(out, lse, 32 ** -0.5, only=[i for i in range(b) if i != 3 and (i % 9 == 0 or lengths[i] == longest)])
+    again, _ = hip.paged_attention(c.q, c.cache, table, c.len)
+    assert torch.equal(again.nan_to_num(7), out.nan_to_num(7))
+
+
 @pytest.mark.parametrize("kind", TYPES)
 def test_large_and_peaked_scores(hip, kind):
     """Scores of some hundreds: one token has all the weight, and the running maximum moves often."""
