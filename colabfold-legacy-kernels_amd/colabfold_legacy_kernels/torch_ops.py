@@ -463,12 +463,19 @@ def qk_norm_rope(qkv, q_norm, k_norm, rope, positions, kv_heads, eps=1e-5, inter
 
 def cache_slots(page_table, positions, page):
     """The slots [B] or [B, S] int32 of positions [B] or [B, S] of B sequences whose pages are page_table [B, N], `page` tokens
-    a page: -1 for a negative position (a padded row), one past the table, or a page that is negative."""
-    at = positions.reshape(positions.shape[0], -1).long()
+    a page: -1 for a negative position (a padded row), one past the table, or a page that is negative or past what int32
+    slots reach."""
+    if page_table.dim() != 2 or positions.dim() not in (1, 2) or positions.shape[0] != page_table.shape[0] or page < 1:
+        raise hip.InvalidArgument(hip.INVALID_ARGUMENT, "cache_slots: expected page_table [B, N], positions [B] or [B, S] and a page "
+                                  "of 1 token at least, got %s, %s and %d" % (tuple(page_table.shape), tuple(positions.shape), page))
+    if page_table.shape[1] == 0:
+        return torch.full_like(positions, -1, dtype=torch.int32)
+    at = (positions if positions.dim() == 2 else positions[:, None]).long()
     col = at.div(page, rounding_mode="floor")
     known = (at >= 0) & (col < page_table.shape[1])
     pages = page_table.long().gather(1, torch.where(known, col, torch.zeros_like(col)))
-    slots = torch.where(known & (pages >= 0), pages * page + at % page, torch.full_like(at, -1))
+    known &= (pages >= 0) & (pages < 2 ** 31 // page)
+    slots = torch.where(known, pages * page + at % page, torch.full_like(at, -1))
     return slots.to(torch.int32).reshape(positions.shape)
 
 

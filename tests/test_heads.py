@@ -96,6 +96,20 @@ def test_cache_slots():
     assert torch_ops.cache_slots(table, torch.tensor([17, 33]), 16).tolist() == [33, 49]
 
 
+def test_cache_slots_at_the_edges():
+    pos = torch.tensor([[0, 63], [64, 127]])
+    # pages whose slots would come round to slots of other pages in int32, and the largest that do not
+    table = torch.tensor([[2 ** 26, 0], [2 ** 31 - 1, 2 ** 25 - 1]], dtype=torch.int32)
+    assert torch_ops.cache_slots(table, pos, 64).tolist() == [[-1, -1], [2 ** 31 - 64, 2 ** 31 - 1]]
+    assert torch_ops.cache_slots(table[:, :0], pos, 64).tolist() == [[-1, -1], [-1, -1]]
+    assert torch_ops.cache_slots(table[:0], pos[:0], 64).shape == (0, 2)
+    assert torch_ops.cache_slots(table[:0], pos[:0, 0], 64).shape == (0,)
+    assert torch_ops.cache_slots(table, pos[:, :0], 64).shape == (2, 0)
+    for bad in ((table, pos[:1], 64), (table[0], pos, 64), (table, pos[None], 64), (table, pos, 0), (table, torch.tensor(3), 16)):
+        with pytest.raises(H.InvalidArgument, match="cache_slots"):
+            torch_ops.cache_slots(*bad)
+
+
 def test_kv_cache():
     c = H.kv_cache(3, 2, 16, 64, device="cpu")
     assert c.k.shape == c.v.shape == (3, 2, 16, 64) and c.k.dtype == torch.int8 and c.k_scale.shape == (3, 2, 16)
@@ -279,6 +293,12 @@ def attend_args(cache=F16, b=3, n=7):
 def test_paged_attention_refusals(lib, other, message):
     a = {**attend_args(), **other}
     refused(lib, lib.clk_paged_attention(None, *refs(a.values()), 0.1, 1, 0x100000, 1 << 40), message)
+
+
+def test_paged_attention_scale_past_its_range(lib):
+    a = attend_args()
+    for scale in (3e38, -3e38):  # times log2(e) it is infinite
+        refused(lib, lib.clk_paged_attention(None, *refs(a.values()), scale, 1, 0x100000, 1 << 40), "scale must be finite")
 
 
 def test_paged_attention_scale_workspace_and_empty(lib):
