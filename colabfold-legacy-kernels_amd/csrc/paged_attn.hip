@@ -498,7 +498,7 @@ __device__ __forceinline__ Count count_of(const AttnArgs& a, int len, int c) {
 
 // What a workgroup does: part j of the k of an item, and the place of its results where k > 1
 struct Work {
-    int b, hr, j, k, slot;
+    int b, hr, j, k, slot, len;
 };
 
 // The work of paged_attn_split_kernel's workgroups where there are so many sequences that it would take each of them long
@@ -585,6 +585,7 @@ __device__ __forceinline__ bool work_of(const AttnArgs& a, Work& work) {
     }
     const int at = (int)(id - before);
     work.b = b;
+    work.len = len;
     work.k = parts_in(chunks_in(a, len), c);
     work.hr = at / work.k;
     work.j = at - work.hr * work.k;
@@ -603,11 +604,14 @@ __global__ __launch_bounds__(kWaves* kWave, occupancy(D)) void paged_attn_split_
         const int32_t* p = reinterpret_cast<const int32_t*>(a.plan);
         const int64_t at = 4 * (int64_t)blockIdx.x;
         const int jk = scalar_load(p, at + 2);
-        work = Work{scalar_load(p, at), scalar_load(p, at + 1), jk >> 16, jk & 0xffff, scalar_load(p, at + 3)};
+        work = Work{scalar_load(p, at), scalar_load(p, at + 1), jk >> 16, jk & 0xffff, scalar_load(p, at + 3), 0};
+        work.len = scalar_load(a.len, work.b);
     } else if (!work_of(a, work)) {
         return;
     }
-    const int len = scalar_load(a.len, work.b), chunks = chunks_in(a, len), each = (chunks - 1) / work.k + 1;
+    // (which the compiler does not see to be one value a wave: it would load through loops over the lanes)
+    work = Work{uniform(work.b), uniform(work.hr), uniform(work.j), uniform(work.k), uniform(work.slot), uniform(work.len)};
+    const int len = work.len, chunks = chunks_in(a, len), each = (chunks - 1) / work.k + 1;
     const Span sp = span_of(a, work.b, work.hr, work.j * each * kChunk, min(len, (work.j + 1) * each * kChunk));
     if (chunks == 0) {
         finish_empty<BF, D>(a, sp, len > 0);
@@ -710,7 +714,7 @@ Plan plan_of(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t per, int64_t
     p.items = p.grid = B * Hkv * blocks;
     if (per * page > kDirect && B > 0) {
         // One round of workgroups, but where the items nearly make one already, three, so that the long among them are cut
-        // finely enough to fill the last round: 256 ragged sequences of up to 4096 on 8 heads 157 us, 167 with two; 61 on
+        // finely enough to fill the last round: 256 ragged sequences of up to 4096 on 8 heads 151 us, a tenth more with two; 61 on
         // 4 heads 43 with one and 48 with three.
         p.W = 256 * occupancy(D) * (p.items > 128 * occupancy(D) ? 3 : 1);
         // With c as the kernel takes it, all chunks / c <= room = W - min(items, W / 2), and an item has under its chunks / c + 1
@@ -722,8 +726,8 @@ Plan plan_of(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t per, int64_t
         p.split = (size_t)p.W * 16;
         p.meta = 256;
         // Many items of many sequences are dealt out by a launch before (2.5 us and a gap): 256 sequences of up to 1024 on 8 heads
-        // 117 us, 122 without; 1024 of them 403, 692 without; 4096 ragged ones 659, 6790 without; but 50 ragged ones of up
-        // to 4096 51.5, 46.2 without, and 128 on one head 19.4, 17.1 without.
+        // 106 us, 114 without; 1024 of them 375, 472 without; 4096 ragged ones 587, 2309 without; but 50 ragged ones of up
+        // to 4096 48, 44 without, and 128 on one head 19.4, 17.1 without.
         if (B > kPlanned && p.items > 128 * occupancy(D)) p.plan = (size_t)p.grid * 16;
     }
     return p;
