@@ -10,7 +10,12 @@
 //                       token's head (each value rounded once, from fp32)
 //   kv_cache_write, kv_cache_read  keys and values into the cache as they are, and back
 //
-// All of them are bound by memory: each value is read once and written once, statistics and products are fp32.
+// All of them are bound by memory: each value is read once and written once, statistics and products are fp32. At 16384 tokens
+// of 48 + 6 + 6 heads of 128 in bf16 the forward takes 100 us (5.0 TB/s of its 503 MB, the rate of a large copy; a
+// plain copy in the same pattern 109) and the gradients 151 + 6 (5.0 TB/s of 755 MB); 32771 tokens of 8 heads of 128 take
+// 53 us into a 16-bit cache and 47 back (5.1 and 5.7 TB/s of 268 MB each); a prompt of 4099 tokens of 32 + 8 + 8 heads of
+// 128 takes 28 us into an 8-bit cache (3.3 TB/s of 92 MB: one and a half rounds of workgroups, 4.0 at 32768 tokens); one
+// token 3.7 us.
 //
 // A head is a group of LG lanes (the power of two at or past D / 8) with 8 channels each, the two halves of its pairs: a
 // lane whose channels are rotated by halves holds channels 4 j .. + 3 and R / 2 + 4 j .. + 3, so that pairs never
@@ -334,7 +339,9 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(HeadsArgs a) {
 
 // ---- backward -------------------------------------------------------------------------------
 
-constexpr int kBwdHeads = 4;  // heads a workgroup row
+// Heads a workgroup row: 151 us at the size above, 168 with two. A workgroup goes on to further tokens, so that the weights'
+// gradients have one partial row a workgroup, which are summed in a fixed order, without atomics.
+constexpr int kBwdHeads = 4;
 
 template <bool BF, int LG>
 __global__ __launch_bounds__(kThreads) void qk_norm_rope_bwd_kernel(HeadsArgs a) {
@@ -406,7 +413,7 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_bwd_kernel(HeadsArgs a)
 }
 
 // dqn and dkn (blockIdx.y): the sums of their partial rows, 64 interleaved groups of them, each in order, then the
-// groups in order: 1536 rows of 128 take four loads in a row a thread.
+// groups in order: 1536 rows of 128 take three loads of eight rows in a row a thread, 6 us.
 constexpr int kDwGroups = 64;
 __global__ __launch_bounds__(16 * kDwGroups) void qk_norm_dw_kernel(HeadsArgs a) {
     __shared__ float sums[kDwGroups][17];
@@ -437,6 +444,9 @@ __global__ __launch_bounds__(16 * kDwGroups) void qk_norm_dw_kernel(HeadsArgs a)
 
 // ---- cache in, cache out --------------------------------------------------------------------
 
+// What goes token by token into a block of the cache touches 16 bytes (keys) or 2 (values) here and there: 134 MB of keys and
+// values in 16 bits took 227 us in and out again so, and 100 now. Tokens that fill a block move together.
+//
 // Sixteen tokens of a call from 16 w on, as the cache sees them. Where a block of the cache is filled by sixteen tokens in a
 // row, whichever token it begins with, the workgroup that has its first token moves it whole, with stores (or loads) of
 // whole lines; the other tokens go one by one.
