@@ -87,6 +87,15 @@ __device__ __forceinline__ half8 cut8(half8 v, int col, int C) {
     }
     return v;
 }
+// a + b, each rounded: as a whole vector, since bf16 values past 2^121 came out times 16 where the sums were put into a half
+// vector one by one
+template <bool BF>
+__device__ __forceinline__ half8 sum8(half8 a, half8 b) {
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = act_get<BF>(a, e) + act_get<BF>(b, e);
+    return __builtin_bit_cast(half8, act_cvt8<BF>(f));
+}
 template <bool NT = false>
 __device__ __forceinline__ void store8(half_t* row, int col, int C, half8 v) {
     if (col + 8 <= C) {
@@ -187,8 +196,7 @@ __global__ __launch_bounds__(kAny) void rms_norm_any_kernel(RmsArgs a) {
             half8 v = cut8(load8(xr, c, C), c, C);
             if constexpr (RES) {
                 const half8 r = cut8(load8(rr, c, C), c, C);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = act_cvt<BF>(act_get<BF>(v, e) + act_get<BF>(r, e));
+                v = sum8<BF>(v, r);
                 store8(sr, c, C, v);
             }
             collect(c, v, 1.f);
@@ -264,8 +272,7 @@ __global__ __launch_bounds__(block_of(TPR)) void rms_norm_kernel(RmsArgs a) {
             for (int j = 0; j < NCH; ++j) {
                 v[j] = cut8(v[j], 8 * (part + TPR * j), C);
                 res[j] = cut8(res[j], 8 * (part + TPR * j), C);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[j][e] = act_cvt<BF>(act_get<BF>(v[j], e) + act_get<BF>(res[j], e));
+                v[j] = sum8<BF>(v[j], res[j]);
                 store8(a.sum + row * C, 8 * (part + TPR * j), len, v[j]);
             }
         } else {
