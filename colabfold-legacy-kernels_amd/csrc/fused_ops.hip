@@ -613,12 +613,11 @@ __global__ __launch_bounds__(kProjThreads, 4) void outproj_kernel(ProjArgs a) {
         const bool store = work == kCompute || (!RES && work == kPadding);
 #pragma unroll
         for (int i = 0; i < RBW; ++i) {
-            half8 o;
+            float o[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                o[j] = act_cvt<BF>(work == kPadding ? 0.f : acc[j >> 2][i][j & 3] + bv[j] + resf[i][j]);
+            for (int j = 0; j < 8; ++j) o[j] = work == kPadding ? 0.f : acc[j >> 2][i][j & 3] + bv[j] + resf[i][j];
             const uint32_t off = (uint32_t)((16 * (rb0 + i) + r16) * N + col) * 2u;
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), ro, store ? off : kDrop, 0, 0);
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, act_cvt8<BF>(o)), ro, store ? off : kDrop, 0, 0);
         }
     };
 

@@ -1,4 +1,4 @@
-"""bf16 results near the type's largest from the RMS norm, its gradients and the 8-bit rows: bit patterns that, read as fp16, are
+"""bf16 results near the type's largest from the RMS norm, its gradients, the 8-bit rows and the output projection: bit patterns that, read as fp16, are
 signalling NaNs (bf16 values of 2^121 to 2^125) come out as the numbers that they are."""
 import pytest
 import torch
@@ -53,3 +53,14 @@ def test_rows_back(hip, k):
     scale = 2.0 ** torch.tensor([114.0, 116.0, 118.0, 120.0])
     out = hip.dequantize_rows(q.cuda(), scale.cuda(), k, torch.bfloat16)
     assert torch.equal(out.double().cpu(), q[:, :k].double() * scale[:, None].double())
+
+
+@pytest.mark.parametrize("n", (64, 128))
+@pytest.mark.parametrize("k", (64, 128))
+def test_output_projection_keeps_its_residual(hip, k, n):
+    x = patterns(0.0)
+    x = x[x.abs().float() >= 2.0 ** -126]  # (sums of subnormal values may round to zero)
+    x = torch.nn.functional.pad(x.float(), (0, -len(x) % n), value=1.0).to(torch.bfloat16).view(-1, n).cuda()
+    o = torch.zeros(len(x), k, dtype=torch.bfloat16, device="cuda")
+    w, b = torch.ones(n, k, dtype=torch.float16, device="cuda"), torch.zeros(n, dtype=torch.float16, device="cuda")
+    assert torch.equal(hip.output_projection(o, w, b, x), x)
