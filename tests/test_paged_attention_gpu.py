@@ -309,6 +309,51 @@ def test_captured_decode_loop(hip, bits):
         assert torch.equal(eager[0], out) and torch.equal(eager[1], lse)
 
 
+def test_captured_large_batch(hip):
+    """The same for a batch whose items a launch deals out: two graphs that share a workspace, replayed one after the other, an
+    eager call with another between them."""
+    b, room = 300, 640
+    c = Case([room] * 2 + [1 + i % 40 for i in range(b - 2)], 4, 2, 32, 16, 16, "bf16")
+    table = torch.nn.functional.pad(c.table, (0, 5), value=-1)
+    ws = torch.empty(hip.paged_attention_workspace(c.q, c.cache, table), dtype=torch.uint8, device="cuda")
+    lens = [c.len.clone(), c.len.clone()]
+    outs = [torch.empty_like(c.q) for _ in lens]
+    for n, out in zip(lens, outs):
+        hip.paged_attention(c.q, c.cache, table, n, out=out, workspace=ws)
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in lens]
+    for g, n, out in zip(graphs, lens, outs):
+        with torch.cuda.graph(g):
+            hip.paged_attention(c.q, c.cache, table, n, out=out, workspace=ws)
+    for seed in range(4):
+        gen = torch.Generator().manual_seed(seed)
+        for i, n in enumerate(lens):
+            share = torch.rand(b, generator=gen) if seed else torch.zeros(b)
+            n.copy_((c.len.cpu() * share).int())
+            outs[i].fill_(7)
+        for i, g in enumerate(graphs):
+            g.replay()
+            hip.paged_attention(c.q, c.cache, table, c.len)
+        torch.cuda.synchronize()
+        for n, out in zip(lens, outs):
+            assert torch.equal(out, hip.paged_attention(c.q, c.cache, table, n)[0])
+            assert (out[n == 0] == 0).all()
+
+
+@pytest.mark.parametrize("bits", (16, 8))
+def test_pages_that_sequences_share(hip, bits):
+    """Sequences with the same first pages, one page twice in a sequence, and the same sequence in every row."""
+    c = Case([200, 90, 33], 6, 2, 64, 16, bits, "f16")
+    c.host_table[1, :3] = c.host_table[0, :3]
+    c.host_table[2, :3] = c.host_table[0, [4, 4, 0]]
+    table = torch.from_numpy(c.host_table).cuda()
+    out, lse = hip.paged_attention(c.q, c.cache, table, c.len, want_lse=True)
+    c.check(out, lse, 64 ** -0.5)
+    q, rows = c.q[:1].expand(100, 6, 64).contiguous(), table[:1].expand(100, -1).contiguous()
+    same, _ = hip.paged_attention(q, c.cache, torch.nn.functional.pad(rows, (0, 60), value=-1), c.len[:1].expand(100).contiguous())
+    assert (same == same[:1]).all()
+
+
 @pytest.mark.parametrize("bits", (16, 8))
 def test_a_serving_block(hip, bits):
     """A prompt and then tokens one by one through an attention block of 8-bit projections: norm to 8 bits, one projection for
