@@ -14,7 +14,7 @@
 // with the running maximum and sum of a softmax. Both operands come from memory to registers with nothing between.
 //
 // 256 sequences of 4096 on 8 heads of 128 in bf16 (4.2 GB) take 627 us, 6.7 TB/s, where reading alone reaches 6.9; one of 131071
-// (537 MB) 84 + 6, 6.4 TB/s; 61 ragged ones of up to 8192 on 4 heads in 8 bits (167 MB) 35 + 5, 4.7 TB/s: some 3 us
+// (537 MB) 83 + 5, 6.5 TB/s; 61 ragged ones of up to 8192 on 4 heads in 8 bits (167 MB) 35 + 5, 4.7 TB/s: some 3 us
 // before the first keys arrive and a tail of 3 to 5, as parts end unevenly; one of 77 tokens 4.1 us, a launch's time.
 #include "kv_cache.h"
 
