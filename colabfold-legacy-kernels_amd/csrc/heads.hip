@@ -14,8 +14,7 @@
 // of 48 + 6 + 6 heads of 128 in bf16 the forward takes 100 us (5.0 TB/s of its 503 MB, the rate of a large copy; a
 // plain copy in the same pattern 109) and the gradients 151 + 6 (5.0 TB/s of 755 MB); 32771 tokens of 8 heads of 128 take
 // 53 us into a 16-bit cache and 47 back (5.1 and 5.7 TB/s of 268 MB each); a prompt of 4099 tokens of 32 + 8 + 8 heads of
-// 128 takes 28 us into an 8-bit cache (3.3 TB/s of 92 MB: one and a half rounds of workgroups, 4.0 at 32768 tokens); one
-// token 3.7 us.
+// 128 takes 27 us into an 8-bit cache (3.4 TB/s of 92 MB, 4.3 at 32768 tokens); one token 3.7 us.
 //
 // A head is a group of LG lanes (the power of two at or past D / 8) with 8 channels each, the two halves of its pairs: a
 // lane whose channels are rotated by halves holds channels 4 j .. + 3 and R / 2 + 4 j .. + 3, so that pairs never
@@ -64,6 +63,7 @@ struct HeadsArgs {
     int cq, ck;          // chunks of heads: queries', keys' (values' as keys')
     int parts;           // workgroups a chunk
     int windows;         // workgroups a group of cached heads
+    int cached_heads;    // of a step: heads of a group
     FastDiv by_chunks, by_groups;
     int page, slots_end;  // the cache's page, and its tokens
     FastDiv by_page;
@@ -500,22 +500,23 @@ __device__ __forceinline__ void value_unit(int u, F f) {
 // A lane's 8 channels of a key and a value: as they come, and as the cache holds them
 struct Pair {
     raw8 key, value;
-    Angles angles;
-    bool ok;
 };
 struct Pair8 {
     uint2v key, value;
     float key_scale, value_scale;
 };
+struct Turn {  // a token's angles
+    Angles angles;
+    bool ok;
+};
 // What a token's heads of keys and values come from: the projection's row (STEP), or k and v
 template <bool STEP>
-__device__ __forceinline__ Pair fetch(const HeadsArgs& a, int64_t token, int head, int j, const Lane& lk, const Lane& lv) {
+__device__ __forceinline__ Pair fetch(const HeadsArgs& a, int64_t token, int head, const Lane& lk, const Lane& lv) {
     Pair p;
     if constexpr (STEP) {
         const half_t* row = a.x + (token * (a.Hq + 2 * a.Hkv) + a.Hq + head) * a.D;
         p.key = load_head(row, lk);
         p.value = load_head(row + (int64_t)a.Hkv * a.D, lv);
-        p.ok = load_angles(a, a.pos[token], j, lk.turned, p.angles);
     } else {
         // past the caches, which the cache is left in: 134 MB written and read again 118 us through them, 100 so
         const int64_t at = (token * a.Hkv + head) * a.D;
@@ -526,12 +527,12 @@ __device__ __forceinline__ Pair fetch(const HeadsArgs& a, int64_t token, int hea
 }
 // Norm and rotation of a step's key, and both as 8-bit rows (all lanes of the head come here)
 template <bool BF, int LG, bool Q8, bool STEP>
-__device__ __forceinline__ Pair8 held(const HeadsArgs& a, Pair& p, const float (&w)[8], const Lane& lk) {
+__device__ __forceinline__ Pair8 held(const HeadsArgs& a, Pair& p, const float (&w)[8], const Turn& turn, const Lane& lk) {
     Pair8 h{};
     float f[8];
     if constexpr (STEP || Q8) floats<BF>(p.key, f);
     if constexpr (STEP) {
-        norm_rope<BF, LG>(a, f, w, p.angles, p.ok, lk);
+        norm_rope<BF, LG>(a, f, w, turn.angles, turn.ok, lk);
         p.key = act_cvt8<BF>(f);
     }
     if constexpr (Q8) {
@@ -542,97 +543,123 @@ __device__ __forceinline__ Pair8 held(const HeadsArgs& a, Pair& p, const float (
     return h;
 }
 
-// Keys and values of the kHeadsAtOnce heads from h0 on into the cache, window by window
+// Keys and values of heads h0 .. h1 - 1, kHeadsAtOnce at a time, into the cache, window by window
 template <bool BF, int LG, bool Q8, bool STEP>
-__device__ __forceinline__ void cache_windows(const HeadsArgs& a, BlockRows<LG, Q8> (&share)[2], int64_t window, int64_t step, int h0) {
+__device__ __forceinline__ void cache_windows(const HeadsArgs& a, BlockRows<LG, Q8> (&share)[2], int64_t window, int64_t step, int h0, int h1) {
     constexpr int TOKENS = kThreads / LG, HEADS = kHeadsAtOnce<LG>, ROUNDS = kRounds<LG>, SIZE = Q8 ? 1 : 2;
-    const int j = threadIdx.x % LG, sub = threadIdx.x / LG, group = value_group(Q8, a.D), heads = min(HEADS, a.Hkv - h0);
+    const int j = threadIdx.x % LG, sub = threadIdx.x / LG, group = value_group(Q8, a.D);
     const Lane lk = lane_of(j, a.D, STEP ? a.R : 0, a.interleaved), lv = lane_of(j, a.D, 0, false);
     float w[8];
     if constexpr (STEP) load_weight(a.kn, lk, w);
     for (int64_t t0 = 16 * window; t0 < a.T; t0 += 16 * step) {
-        Pair own[ROUNDS];  // the window's own tokens, on their way before it is known which of them go one by one
-#pragma unroll
-        for (int round = 0; round < ROUNDS; ++round) {
-            const int n = sub + round * TOKENS;
-            own[round] = fetch<STEP>(a, min(t0 + (n & 15), a.T - 1), h0 + min(n >> 4, heads - 1), j, lk, lv);
-        }
-        const Window win = window_of(a, t0);
-        if (win.first >= 0) {
-            const int slot = a.slots[t0 + win.first];
-            Pair p[ROUNDS];
+        Pair p[ROUNDS];
+        Turn turn[STEP ? ROUNDS : 1];
+        const auto load = [&](int64_t from, int h) {  // sixteen tokens
 #pragma unroll
             for (int round = 0; round < ROUNDS; ++round) {
                 const int n = sub + round * TOKENS;
-                p[round] = own[round];
-                if (win.first > 0) p[round] = fetch<STEP>(a, t0 + win.first + (n & 15), h0 + min(n >> 4, heads - 1), j, lk, lv);
+                p[round] = fetch<STEP>(a, min(from + (n & 15), a.T - 1), min(h + (n >> 4), h1 - 1), lk, lv);
             }
+        };
+        const auto load_turns = [&](int64_t from) {
+            if constexpr (STEP) {
+#pragma unroll
+                for (int round = 0; round < ROUNDS; ++round) {
+                    const int n = sub + round * TOKENS;
+                    turn[round].ok = load_angles(a, a.pos[min(from + (n & 15), a.T - 1)], j, lk.turned, turn[round].angles);
+                }
+            }
+        };
+        load(t0, h0);  // on their way before it is known which of them go one by one
+        load_turns(t0);
+        const Window win = window_of(a, t0);
+        if (win.first >= 0) {
+            const int64_t from = t0 + win.first;
+            const int slot = a.slots[from];
+            if (win.first > 0) {
+                load(from, h0);
+                load_turns(from);
+            }
+            for (int h = h0;;) {
+                const int heads = min(HEADS, h1 - h);
+#pragma unroll
+                for (int round = 0; round < ROUNDS; ++round) {
+                    const int n = sub + round * TOKENS, t = n & 15, hs = n >> 4;
+                    const Pair8 q = held<BF, LG, Q8, STEP>(a, p[round], w, turn[STEP ? round : 0], lk);
+                    char* key = share[0].rows[hs][t];
+                    char* value = share[1].rows[hs][t];
+                    if (!lk.in) continue;
+                    if constexpr (Q8) {
+                        *reinterpret_cast<uint32_t*>(key + lk.c0) = q.key[0];
+                        *reinterpret_cast<uint32_t*>(key + lk.c1) = q.key[1];
+                        *reinterpret_cast<uint2v*>(value + 8 * j) = q.value;
+                        if (j == 0 && hs < heads) {
+                            const int64_t at = place_of(a, slot + t, h + hs).scale;
+                            a.ks[at] = q.key_scale;
+                            a.vs[at] = q.value_scale;
+                        }
+                    } else {
+                        store_head(reinterpret_cast<half_t*>(key), lk, p[round].key);
+                        *reinterpret_cast<raw8*>(value + 16 * j) = p[round].value;
+                    }
+                }
+                if (h + HEADS < h1) load(from, h + HEADS);
+                __syncthreads();
+                for (int n = threadIdx.x; n < a.D * SIZE * heads; n += kThreads) {  // 16 D SIZE / 16 units of 16 bytes a head
+                    const int hs = n / (a.D * SIZE), u = n - hs * a.D * SIZE;
+                    const int64_t at = place_of(a, slot, h + hs).block * SIZE + u * 16;
+                    *reinterpret_cast<raw8*>(static_cast<char*>(a.kc) + at) =
+                        *reinterpret_cast<const raw8*>(&share[0].rows[hs][u & 15][16 * (u >> 4)]);
+                    const auto& rows = share[1].rows[hs];
+                    char* to = static_cast<char*>(a.vc) + at;
+                    if constexpr (!Q8) {
+                        raw8 v;
+                        value_unit<2>(u, [&](int k, int t, int c) { v[k] = *reinterpret_cast<const uint16_t*>(&rows[t][2 * c]); });
+                        *reinterpret_cast<raw8*>(to) = v;
+                    } else {
+                        uint32_t v[4] = {};
+                        const auto byte = [&](int k, int t, int c) { v[k >> 2] |= (uint32_t)(uint8_t)rows[t][c] << 8 * (k & 3); };
+                        if (group == 4) {
+                            value_unit<4>(u, byte);
+                        } else {
+                            value_unit<2>(2 * u, byte);
+                            value_unit<2>(2 * u + 1, [&](int k, int t, int c) { byte(k + 8, t, c); });
+                        }
+                        *reinterpret_cast<uint4v*>(to) = uint4v{v[0], v[1], v[2], v[3]};
+                    }
+                }
+                __syncthreads();
+                if ((h += HEADS) >= h1) break;
+            }
+        }
+        if (win.rest == 0) continue;
+        if (win.first >= 0) {  // (again, which is rare and spares their registers above)
+            load(t0, h0);
+            load_turns(t0);
+        }
+        for (int h = h0;;) {
+            const int heads = min(HEADS, h1 - h);
 #pragma unroll
             for (int round = 0; round < ROUNDS; ++round) {
                 const int n = sub + round * TOKENS, t = n & 15, hs = n >> 4;
-                const Pair8 q = held<BF, LG, Q8, STEP>(a, p[round], w, lk);
-                char* key = share[0].rows[hs][t];
-                char* value = share[1].rows[hs][t];
-                if (!lk.in) continue;
+                const bool live = hs < heads && (win.rest >> t & 1) && lk.in;
+                const Place at = place_of(a, live ? a.slots[t0 + t] : 0, h + min(hs, heads - 1));
+                const Pair8 q = held<BF, LG, Q8, STEP>(a, p[round], w, turn[STEP ? round : 0], lk);
+                if (!live) continue;
                 if constexpr (Q8) {
-                    *reinterpret_cast<uint32_t*>(key + lk.c0) = q.key[0];
-                    *reinterpret_cast<uint32_t*>(key + lk.c1) = q.key[1];
-                    *reinterpret_cast<uint2v*>(value + 8 * j) = q.value;
-                    if (j == 0 && hs < heads) {
-                        const int64_t at = place_of(a, slot + t, h0 + hs).scale;
-                        a.ks[at] = q.key_scale;
-                        a.vs[at] = q.value_scale;
+                    cache_key8(a.kc, at, lk, q.key);
+                    cache_value8(a.vc, at, group, lv.c0, q.value);
+                    if (j == 0) {
+                        a.ks[at.scale] = q.key_scale;
+                        a.vs[at.scale] = q.value_scale;
                     }
                 } else {
-                    store_head(reinterpret_cast<half_t*>(key), lk, p[round].key);
-                    *reinterpret_cast<raw8*>(value + 16 * j) = p[round].value;
+                    cache_key16(a.kc, at, lk, p[round].key);
+                    cache_value16(a.vc, at, lv.c0, p[round].value);
                 }
             }
-            __syncthreads();
-            for (int n = threadIdx.x; n < a.D * SIZE * heads; n += kThreads) {  // 16 D SIZE / 16 units of 16 bytes a head
-                const int hs = n / (a.D * SIZE), u = n - hs * a.D * SIZE;
-                const int64_t at = place_of(a, slot, h0 + hs).block * SIZE + u * 16;
-                *reinterpret_cast<raw8*>(static_cast<char*>(a.kc) + at) =
-                    *reinterpret_cast<const raw8*>(&share[0].rows[hs][u & 15][16 * (u >> 4)]);
-                const auto& rows = share[1].rows[hs];
-                char* to = static_cast<char*>(a.vc) + at;
-                if constexpr (!Q8) {
-                    raw8 v;
-                    value_unit<2>(u, [&](int k, int t, int c) { v[k] = *reinterpret_cast<const uint16_t*>(&rows[t][2 * c]); });
-                    *reinterpret_cast<raw8*>(to) = v;
-                } else {
-                    uint32_t v[4] = {};
-                    const auto byte = [&](int k, int t, int c) { v[k >> 2] |= (uint32_t)(uint8_t)rows[t][c] << 8 * (k & 3); };
-                    if (group == 4) {
-                        value_unit<4>(u, byte);
-                    } else {
-                        value_unit<2>(2 * u, byte);
-                        value_unit<2>(2 * u + 1, [&](int k, int t, int c) { byte(k + 8, t, c); });
-                    }
-                    *reinterpret_cast<uint4v*>(to) = uint4v{v[0], v[1], v[2], v[3]};
-                }
-            }
-            __syncthreads();
-        }
-        if (win.rest == 0) continue;
-#pragma unroll
-        for (int round = 0; round < ROUNDS; ++round) {
-            const int n = sub + round * TOKENS, t = n & 15, hs = n >> 4;
-            const bool live = hs < heads && (win.rest >> t & 1) && lk.in;
-            const Place p = place_of(a, live ? a.slots[t0 + t] : 0, h0 + min(hs, heads - 1));
-            const Pair8 q = held<BF, LG, Q8, STEP>(a, own[round], w, lk);
-            if (!live) continue;
-            if constexpr (Q8) {
-                cache_key8(a.kc, p, lk, q.key);
-                cache_value8(a.vc, p, group, lv.c0, q.value);
-                if (j == 0) {
-                    a.ks[p.scale] = q.key_scale;
-                    a.vs[p.scale] = q.value_scale;
-                }
-            } else {
-                cache_key16(a.kc, p, lk, own[round].key);
-                cache_value16(a.vc, p, lv.c0, own[round].value);
-            }
+            if ((h += HEADS) >= h1) break;
+            load(t0, h);
         }
     }
 }
@@ -641,7 +668,8 @@ __device__ __forceinline__ void cache_windows(const HeadsArgs& a, BlockRows<LG, 
 template <bool BF, int LG, bool Q8>
 __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(HeadsArgs a) {
     __shared__ __attribute__((aligned(16))) BlockRows<LG, Q8> share[2];
-    cache_windows<BF, LG, Q8, false>(a, share, blockIdx.x, gridDim.x, blockIdx.y * kHeadsAtOnce<LG>);
+    const int h0 = blockIdx.y * kHeadsAtOnce<LG>;
+    cache_windows<BF, LG, Q8, false>(a, share, blockIdx.x, gridDim.x, h0, min(h0 + kHeadsAtOnce<LG>, a.Hkv));
 }
 
 // The first workgroups take windows of keys and values, which take longer, the others queries
@@ -650,8 +678,8 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_cache_kernel(HeadsArgs 
     __shared__ __attribute__((aligned(16))) BlockRows<LG, Q8> share[2];
     const int cached = a.windows * a.by_groups.d;
     if ((int)blockIdx.x < cached) {
-        const int window = fdiv(blockIdx.x, a.by_groups);
-        cache_windows<BF, LG, Q8, true>(a, share, window, a.windows, (blockIdx.x - window * a.by_groups.d) * kHeadsAtOnce<LG>);
+        const int window = fdiv(blockIdx.x, a.by_groups), h0 = (blockIdx.x - window * a.by_groups.d) * a.cached_heads;
+        cache_windows<BF, LG, Q8, true>(a, share, window, a.windows, h0, min(h0 + a.cached_heads, a.Hkv));
     } else {
         const int n = blockIdx.x - cached, block = fdiv(n, a.by_chunks);
         heads_apart<BF, LG, HPG, true>(a, block, heads_of<HPG>(a, n - block * a.by_chunks.d));
@@ -870,7 +898,14 @@ void launch_step(HeadsArgs& a, bool bf, bool q8, hipStream_t s) {
     a.cq = ceil_div(a.Hq, four ? 4 : 1);
     a.by_chunks = fast_div(a.cq);
     a.parts = token_blocks(a.T, lg, a.cq);
-    const int groups = head_groups(a.Hkv, lg);
+    // Heads that a workgroup takes one after another: more share their window's look at the slots and its angles, which are as
+    // many bytes as a key and a value, and have the next head's on their way; where that leaves enough workgroups. 4099
+    // tokens of 32 + 8 + 8 heads of 128 into 8 bits 27.1 us with four, 28.7 with one, into 16 26.5 and 29.5; 32768 tokens 170
+    // and 189; but 512 tokens 7.1 and 6.9, and eight at 4099 30.1.
+    const int once = std::max(1, kThreads / lg / 16);
+    const int64_t windows = (a.T + 15) / 16 * head_groups(a.Hkv, lg);
+    a.cached_heads = once * (windows >= 1024 ? 4 : windows >= 512 ? 2 : 1);
+    const int groups = ceil_div(a.Hkv, a.cached_heads);
     a.by_groups = fast_div(groups);
     a.windows = window_blocks(a.T, groups);
     const dim3 grid(a.parts * a.cq + a.windows * groups), block(kThreads);

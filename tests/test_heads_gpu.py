@@ -345,6 +345,20 @@ def test_norm_rope_into_the_cache(hip, t, heads, d, page, kind):
             check_written(cache, slots, page, want)
 
 
+@pytest.mark.parametrize("bits", (16, 8))
+@pytest.mark.parametrize("t,heads,d,page", ((1100, 9, 128, 32), (2100, 9, 128, 16), (1100, 17, 64, 48), (2500, 5, 256, 16), (4100, 3, 96, 64), (2100, 33, 32, 16)))
+def test_long_prompts_as_short_ones(hip, t, heads, d, page, bits):
+    """A token's rows do not depend on the call: long ones, whose workgroups take several heads, give what short ones give."""
+    x, qn, kn, rope, pos, _ = inputs(t, heads + 1, heads, d, d // 2, "bf16")
+    for slots, pages in all_slots(t, page):
+        one, many = (hip.kv_cache(pages, heads, page, d, torch.int8 if bits == 8 else torch.bfloat16) for _ in range(2))
+        q = hip.qk_norm_rope_cache(x, qn, kn, rope, pos, slots, one, EPS)
+        parts = [hip.qk_norm_rope_cache(x[i:i + 37], qn, kn, rope, pos[i:i + 37].clone(), slots[i:i + 37].clone(), many, EPS)
+                 for i in range(0, t, 37)]
+        assert torch.equal(q, torch.cat(parts))
+        assert all(torch.equal(a, b) for a, b in zip(one, many) if a is not None)
+
+
 def test_rows_that_are_not_finite(hip):
     x, qn, kn, rope, pos, _ = inputs(20, 2, 1, 64, 64, "bf16")
     x[3, 2, 5] = float("inf")
