@@ -114,7 +114,9 @@ __device__ __forceinline__ half8 join(uint2v a, uint2v b) { return __builtin_bit
 // Eight weights in two 16-bit parts each, 2^-16 (bf16) or 2^-22 of them at most away from their sum: one would make a
 // result's error half a step larger than its own rounding. The matrix cores have time for both.
 // ABOVE: the first part is a step below the weight cut off, so that the second is positive too and an infinity among
-// the values stays one (a second part of zero or below would make it NaN).
+// the values stays one (a second part of zero or below would make it NaN). The parts are then 2^-15 or 2^-21 away at
+// most. An fp16 weight under kLeastAbove has a first part of zero: attend takes infinities apart there.
+constexpr float kLeastAbove = 0x1p-23f;
 template <bool BF, bool ABOVE>
 __device__ __forceinline__ void two_parts(const float (&f)[8], half8& hi, half8& lo) {
     float rest[8];
@@ -136,6 +138,11 @@ __device__ __forceinline__ void two_parts(const float (&f)[8], half8& hi, half8&
 #pragma unroll
     for (int e = 0; e < 8; ++e) rest[e] = f[e] - act_get<BF>(hi, e);
     lo = __builtin_bit_cast(half8, act_cvt8<BF>(rest));
+}
+
+// The infinities among two fp16 values, with a zero for another value
+__device__ __forceinline__ uint32_t infinities(uint32_t w) {
+    return ((w & 0x7fffu) == 0x7c00u ? w & 0xffffu : 0u) | ((w & 0x7fff0000u) == 0x7c000000u ? w & 0xffff0000u : 0u);
 }
 
 // A tile's cached bytes as they were loaded: keys as operands, values as cells of four tokens a channel block
@@ -360,6 +367,36 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Span& sp, int wa
             }
             half8 p, plo;
             two_parts<MBF, !Q8>(pf, p, plo);
+            if constexpr (!MBF) {
+                // Where a first part is zero an infinity would become NaN: infinities are then multiplied by a weight of 1,
+                // by themselves. (Bits less one put zeros, and what no token has, on top.)
+                uint32_t least = ~0u;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) least = min(least, __builtin_bit_cast(uint32_t, pf[i]) - 1);
+                if (__any(least < __builtin_bit_cast(uint32_t, kLeastAbove) - 1)) {
+                    half8 one;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) one[i] = pf[i] == 0.f ? (half_t)0.f : (half_t)1.f;
+#pragma unroll
+                    for (int e = 0; e < DB; ++e) {
+                        uint4v inf;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            auto& v = t.v[n + w / 2][e / T::C];
+                            const int at = 2 * (e % T::C) + w % 2;
+                            inf[w] = infinities(v[at]);
+                            v[at] ^= inf[w];
+                        }
+                        st.o[e] = mfma<MBF>(__builtin_bit_cast(half8, inf), one, st.o[e]);
+                        __builtin_amdgcn_sched_barrier(0);  // (one after another, which takes no further registers)
+                    }
+                }
+                // (Without this the compiler, ROCm 7.2's, joins the operands below of registers that it has used again.)
+#pragma unroll
+                for (int b = n; b < n + 2; ++b)
+#pragma unroll
+                    for (int s = 0; s < T::NV; ++s) asm volatile("" : "+v"(t.v[b][s]));
+            }
 #pragma unroll
             for (int e = 0; e < DB; ++e) {
                 half8 op;
