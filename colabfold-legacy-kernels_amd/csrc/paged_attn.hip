@@ -46,9 +46,12 @@ constexpr int kMostSplit = 256 * 4 * 3;
 
 // Weights are taken times 2^bias, which their sum has too and which cancels: fp16 ones so that small ones keep their bits (a
 // weight of 2^-25 of the largest, of which a long sequence may have millions, would be 0), bf16 ones so that
-// sums of values near the type's largest stay in fp32's range.
+// sums of values near the type's largest stay in fp32's range: all weights of a sequence are less than 1 together. (A
+// factor for the longest would take the bits of values under 2^-100 from short ones.)
 template <bool MBF>
-constexpr float kBias = MBF ? -24.f : 15.f;
+__device__ __forceinline__ float bias_of(int len) {
+    return MBF ? -(float)(32 - __builtin_clz((uint32_t)max(len, 1))) : 15.f;
+}
 
 struct AttnArgs {
     const half_t* q;  // [B, Hq, D]
@@ -158,10 +161,10 @@ struct Tile {
 
 // One item, the query heads 16 rb .. + 15 of head of keys h of sequence b, and tokens of it
 struct Span {
-    int b, h, rb, rows, from, to;
+    int b, h, rb, rows, from, to, len;  // len: of the sequence
     int64_t qrow;
 };
-__device__ __forceinline__ Span span_of(const AttnArgs& a, int b, int hr, int from, int to) {
+__device__ __forceinline__ Span span_of(const AttnArgs& a, int b, int hr, int from, int to, int len) {
     Span s;
     s.b = b;
     s.h = fdiv(hr, a.by_blocks);
@@ -170,6 +173,7 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, int b, int hr, int fr
     s.qrow = ((int64_t)b * a.Hkv + s.h) * a.G + 16 * s.rb;
     s.from = from;
     s.to = to;
+    s.len = len;
     return s;
 }
 
@@ -264,6 +268,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Span& sp, int wa
     constexpr bool MBF = BF || Q8;   // the products' operands are bf16
     constexpr bool QLO = Q8 && !BF;  // fp16 queries in two bf16 parts, which is exact
     const int lane = threadIdx.x % kWave, i16 = lane & 15, g = lane >> 4, keys = sp.to;
+    const float bias = bias_of<MBF>(sp.len);
     const int32_t* table = a.table + (int64_t)sp.b * a.per;
 
     // the queries' operands; channels in the order of the keys'
@@ -342,7 +347,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Span& sp, int wa
             for (int e = 0; e < DB; ++e) st.o[e] *= alpha;
             st.m = m_new;
         }
-        const float base = (st.m == -__builtin_inff() ? 0.f : st.m) - kBias<MBF>;
+        const float base = (st.m == -__builtin_inff() ? 0.f : st.m) - bias;
         if (!Q8 && k0 + TILE > keys) {  // values behind the last token may be anything: zeros
 #pragma unroll
             for (int n = 0; n < NB; ++n)
@@ -458,7 +463,7 @@ __device__ __forceinline__ void join_waves(const AttnArgs& a, const Span& sp, co
             }
         } else {
             *reinterpret_cast<raw4*>(a.out + (sp.qrow + r) * D + d) = act_cvt4<BF>(o * (1.f / sum));
-            if (a.lse != nullptr && d == 0) a.lse[sp.qrow + r] = m + (__builtin_amdgcn_logf(sum) - kBias<MBF>);
+            if (a.lse != nullptr && d == 0) a.lse[sp.qrow + r] = m + (__builtin_amdgcn_logf(sum) - bias_of<MBF>(sp.len));
         }
     }
 }
@@ -480,7 +485,7 @@ __global__ __launch_bounds__(kWaves* kWave, occupancy(D)) void paged_attn_kernel
     const int b = fdiv(blockIdx.x, a.by_heads);
     const int len = scalar_load(a.len, b);
     const bool bad = (int64_t)len > (int64_t)a.per * a.page;
-    const Span sp = span_of(a, b, blockIdx.x - b * a.heads, 0, len);
+    const Span sp = span_of(a, b, blockIdx.x - b * a.heads, 0, len, len);
     if (bad || len <= 0) {
         finish_empty<BF, D>(a, sp, bad);
         return;
@@ -653,7 +658,7 @@ __global__ __launch_bounds__(kWaves* kWave, occupancy(D)) void paged_attn_split_
     // (which the compiler does not see to be one value a wave: it would load through loops over the lanes)
     work = Work{uniform(work.b), uniform(work.hr), uniform(work.j), uniform(work.k), uniform(work.slot), uniform(work.len)};
     const int len = work.len, chunks = chunks_in(a, len), each = (chunks - 1) / work.k + 1;
-    const Span sp = span_of(a, work.b, work.hr, work.j * each * kChunk, min(len, (work.j + 1) * each * kChunk));
+    const Span sp = span_of(a, work.b, work.hr, work.j * each * kChunk, min(len, (work.j + 1) * each * kChunk), len);
     if (chunks == 0) {
         finish_empty<BF, D>(a, sp, len > 0);
         return;
@@ -681,7 +686,7 @@ __global__ __launch_bounds__(WAVES* kWave) void paged_attn_join_kernel(AttnArgs 
     const int4v item = a.split[blockIdx.x];
     if ((int)blockIdx.x >= a.meta[0]) return;
     const int first = item[1], n = item[2], r = blockIdx.y, b = fdiv(item[0], a.by_heads);
-    const Span sp = span_of(a, b, item[0] - b * a.heads, 0, 0);
+    const Span sp = span_of(a, b, item[0] - b * a.heads, 0, 0, a.len[b]);
     if (r >= sp.rows) return;
     const int tid = threadIdx.x, wave = uniform((int)(tid / kWave)), lane = tid % kWave;
     const auto slot = [&](int p) { return (int64_t)first + p; };
@@ -737,7 +742,7 @@ __global__ __launch_bounds__(WAVES* kWave) void paged_attn_join_kernel(AttnArgs 
         for (int w = 0; w < WAVES; ++w) v += *reinterpret_cast<const float4v*>(&parts[w][4 * tid]);
         *reinterpret_cast<raw4*>(a.out + (sp.qrow + r) * D + 4 * tid) = act_cvt4<BF>(v * (1.f / l));
     }
-    if (a.lse != nullptr && tid == 0) a.lse[sp.qrow + r] = m + (__builtin_amdgcn_logf(l) - kBias<MBF>);
+    if (a.lse != nullptr && tid == 0) a.lse[sp.qrow + r] = m + (__builtin_amdgcn_logf(l) - bias_of<MBF>(sp.len));
 }
 
 // ---- host -----------------------------------------------------------------------------------
