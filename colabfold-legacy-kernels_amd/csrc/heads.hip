@@ -832,7 +832,10 @@ int check_heads(const char* what, const clk_buffer* qkv, int64_t hkv, const clk_
     a.R = (int)rope->dims[1];
     a.P = (int)rope->dims[0];
     a.inv_d = 1.f / (float)D;
-    a.eps = eps;
+    // The hardware's reciprocal root takes subnormal numbers for zeros. A head of fp16 has them only where all of it is zeros
+    // (their squares are past 2^-48), whose results are 0 with any eps but 0, and whose gradients, at least 2^63 2^-24 of a weight,
+    // are infinite or 0.
+    a.eps = qkv->dtype == CLK_F16 && eps > 0.f ? std::max(eps, 0x1p-126f) : eps;
     return CLK_OK;
 }
 bool is_heads(const clk_buffer* b, int64_t T, int64_t H, int64_t D) { return b->rank == 3 && dims_are(b, T, H, D); }
