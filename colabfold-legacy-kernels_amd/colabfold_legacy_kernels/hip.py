@@ -602,6 +602,8 @@ def qk_norm_rope(qkv, q_norm, k_norm, rope, positions, kv_heads, eps=1e-5, inter
             raise InvalidArgument(INVALID_ARGUMENT, "qk_norm_rope: qkv has %d heads, of which 2 * %d cannot be keys and values"
                                   % (h, kv_heads))
         out = qkv.new_empty((t, h - 2 * kv_heads, d)), qkv.new_empty((t, kv_heads, d)), qkv.new_empty((t, kv_heads, d))
+    elif _rank3("qk_norm_rope", out[1])[1] != kv_heads:
+        raise InvalidArgument(INVALID_ARGUMENT, "qk_norm_rope: out has %d key heads, not %d" % (out[1].shape[1], kv_heads))
     _call("clk_qk_norm_rope", (qkv, q_norm, k_norm, rope, positions) + tuple(out), float(eps), int(bool(interleaved)))
     return out
 
