@@ -417,15 +417,19 @@ def _heads(x):
     return x if x.dim() == 3 else x.reshape((-1,) + x.shape[-2:])
 
 
-def _tokens(name, what, t, lead):
-    """One value a token: of the leading shape, or one that broadcasts to it, as [T]"""
+def _tokens(name, what, t, lead, shared=True):
+    """One value a token: of the leading shape, or one that broadcasts to it (without `shared`: by dimensions of 1 alone, each
+    token having its own), as [T]"""
     if len(lead) == 1 and t.shape == lead:
         return t.contiguous()
     try:
-        return t.expand(lead).reshape(-1)
+        flat = t.expand(lead).reshape(-1)
     except RuntimeError:
+        flat = None
+    if flat is None or not (shared or flat.numel() == t.numel()):
         raise hip.InvalidArgument(hip.INVALID_ARGUMENT, "%s: %s must be of the tokens' shape %s, got %s"
-                                  % (name, what, tuple(lead), tuple(t.shape))) from None
+                                  % (name, what, tuple(lead), tuple(t.shape)))
+    return flat
 
 
 def _check_heads(name, x, what):
@@ -487,7 +491,7 @@ def qk_norm_rope_cache(qkv, q_norm, k_norm, rope, positions, slots, cache, eps=1
     lead = qkv.shape[:-2]
     q = hip.qk_norm_rope_cache(rows, q_norm.float().contiguous(), k_norm.float().contiguous(), rope,
                                _tokens("qk_norm_rope_cache", "positions", positions, lead),
-                               _tokens("qk_norm_rope_cache", "slots", slots, lead), cache, eps, interleaved)
+                               _tokens("qk_norm_rope_cache", "slots", slots, lead, False), cache, eps, interleaved)
     return q if len(lead) == 1 else q.reshape(lead + q.shape[1:])
 
 
@@ -497,7 +501,7 @@ def kv_cache_write(k, v, slots, cache):
         raise hip.InvalidArgument(hip.INVALID_ARGUMENT, "kv_cache_write: k and v must be alike, got %s and %s"
                                   % (tuple(k.shape), tuple(v.shape)))
     k, v, lead = _head_rows("kv_cache_write", k, "k"), _head_rows("kv_cache_write", v, "v"), k.shape[:-2]
-    hip.kv_cache_write(k, v, _tokens("kv_cache_write", "slots", slots, lead), cache)
+    hip.kv_cache_write(k, v, _tokens("kv_cache_write", "slots", slots, lead, False), cache)
 
 
 def kv_cache_read(cache, slots, dtype=None):
