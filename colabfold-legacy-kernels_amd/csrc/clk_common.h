@@ -6,6 +6,7 @@
 
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 #include "colabfold_gfx950.h"
 
@@ -48,6 +49,7 @@ constexpr int kWaitVm0 = 0x0F70;
 // converts to fp16 exactly within fp16's normal range, so MFMA operands stay fp16. Results are
 // rounded to the activation type once, on store (v_cvt_pk_bf16_f32 for bf16).
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 
 template <bool BF>
 __device__ __forceinline__ float act_get(half8 raw, int e) {
@@ -58,43 +60,37 @@ __device__ __forceinline__ float act_get(half8 raw, int e) {
     }
 }
 
-// v rounded to the activation type, as a raw 16-bit pattern
+// v rounded to the activation type, as that type (values of a vector) and as a raw 16-bit pattern (a value by itself)
+template <bool BF>
+using act_t = std::conditional_t<BF, __bf16, half_t>;
+template <bool BF>
+using act8 = std::conditional_t<BF, bf16x8, half8>;
+template <bool BF>
+using act4 = std::conditional_t<BF, bf16x4, half4>;
 template <bool BF>
 __device__ __forceinline__ half_t act_cvt(float v) {
-    if constexpr (BF) {
-        return __builtin_bit_cast(half_t, (__bf16)v);
-    } else {
-        return (half_t)v;
-    }
+    return __builtin_bit_cast(half_t, (act_t<BF>)v);
 }
+__device__ __forceinline__ half8 raw_act(half8 v) { return v; }
+__device__ __forceinline__ half8 raw_act(bf16x8 v) { return __builtin_bit_cast(half8, v); }
+__device__ __forceinline__ half4 raw_act(half4 v) { return v; }
+__device__ __forceinline__ half4 raw_act(bf16x4 v) { return __builtin_bit_cast(half4, v); }
 
 // Raw 16-bit patterns that are moved, selected or put together one by one are held as integers: a half vector made of
 // single values is packed by v_pack_b32_f16, which quiets fp16's signalling NaNs, and those are bf16 values past
-// 2^121. Results are therefore converted as whole vectors.
+// 2^121. Results are therefore vectors of their own type (act8) or converted as whole ones (act_cvt8), and raw then.
 typedef uint16_t raw8 __attribute__((ext_vector_type(8)));
 typedef uint16_t raw4 __attribute__((ext_vector_type(4)));
 template <bool BF>
 __device__ __forceinline__ raw8 act_cvt8(const float (&f)[8]) {
-    if constexpr (BF) {
-        bf16x8 v;
+    act8<BF> v;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (__bf16)f[e];
-        return __builtin_bit_cast(raw8, v);
-    } else {
-        half8 v;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (half_t)f[e];
-        return __builtin_bit_cast(raw8, v);
-    }
+    for (int e = 0; e < 8; ++e) v[e] = (act_t<BF>)f[e];
+    return __builtin_bit_cast(raw8, v);
 }
 template <bool BF>
 __device__ __forceinline__ raw4 act_cvt4(float4v f) {
-    if constexpr (BF) {
-        typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-        return __builtin_bit_cast(raw4, bf16x4{(__bf16)f[0], (__bf16)f[1], (__bf16)f[2], (__bf16)f[3]});
-    } else {
-        return __builtin_bit_cast(raw4, half4{(half_t)f[0], (half_t)f[1], (half_t)f[2], (half_t)f[3]});
-    }
+    return __builtin_bit_cast(raw4, act4<BF>{(act_t<BF>)f[0], (act_t<BF>)f[1], (act_t<BF>)f[2], (act_t<BF>)f[3]});
 }
 
 // LDS row of tile row x, for operand tiles whose A row r of block b is

@@ -301,19 +301,19 @@ __global__ __launch_bounds__(TH) void proj_kernel(ProjArgs a) {
                 const int row = m0 + 16 * rb + r16;
                 if (rb < rb0 || rb >= rb0 + rbn || row >= a.M) continue;
                 half_t* dst = a.out + (int64_t)row * a.n + col;
-                half8 o;
+                act8<BF> o;
                 if constexpr (LN) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) o[j] = act_cvt<BF>(acc[j >> 2][rb][j & 3]);
+                    for (int j = 0; j < 8; ++j) o[j] = (act_t<BF>)(acc[j >> 2][rb][j & 3]);
                 } else if (a.residual != nullptr) {
                     const half8 res = fld8(a.residual + (int64_t)row * a.n + col);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) o[j] = act_cvt<BF>(acc[j >> 2][rb][j & 3] + bv[j] + act_get<BF>(res, j));
+                    for (int j = 0; j < 8; ++j) o[j] = (act_t<BF>)(acc[j >> 2][rb][j & 3] + bv[j] + act_get<BF>(res, j));
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) o[j] = act_cvt<BF>(acc[j >> 2][rb][j & 3] + bv[j]);
+                    for (int j = 0; j < 8; ++j) o[j] = (act_t<BF>)(acc[j >> 2][rb][j & 3] + bv[j]);
                 }
-                fst8(dst, o);
+                fst8(dst, raw_act(o));
             }
         }
         if (heads_wave) {
@@ -448,22 +448,22 @@ __global__ __launch_bounds__(TH, K == 64 ? 4 : 1) void proj_fast_kernel(ProjArgs
             for (int rb = 0; rb < 4; ++rb) {
                 const int row = m0 + 16 * rb + r16;
                 if (!kFull && row >= a.M) continue;
-                half8 o;
+                act8<BF> o;
                 if constexpr (LN) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) o[j] = act_cvt<BF>(acc[j >> 2][rb][j & 3]);
+                    for (int j = 0; j < 8; ++j) o[j] = (act_t<BF>)(acc[j >> 2][rb][j & 3]);
                 } else if (a.residual != nullptr) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
-                        o[j] = act_cvt<BF>(acc[j >> 2][rb][j & 3] + bv[pp][j] + act_get<BF>(res[pp][rb], j));
+                        o[j] = (act_t<BF>)(acc[j >> 2][rb][j & 3] + bv[pp][j] + act_get<BF>(res[pp][rb], j));
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) o[j] = act_cvt<BF>(acc[j >> 2][rb][j & 3] + bv[pp][j]);
+                    for (int j = 0; j < 8; ++j) o[j] = (act_t<BF>)(acc[j >> 2][rb][j & 3] + bv[pp][j]);
                 }
                 if constexpr (K == 128) {
-                    fst8_nt(a.out + (int64_t)row * a.n + col, o);
+                    fst8_nt(a.out + (int64_t)row * a.n + col, raw_act(o));
                 } else {
-                    fst8(a.out + (int64_t)row * a.n + col, o);
+                    fst8(a.out + (int64_t)row * a.n + col, raw_act(o));
                 }
             }
         }
@@ -712,11 +712,11 @@ __global__ __launch_bounds__(kProjThreads, K == 64 ? 4 : 2) void proj_rows_kerne
                 for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                     for (int hb = 0; hb < 2; ++hb) acc[hb] = mfma16x16x32(wa[pp][hb][ks], xop[ks], acc[hb]);
-                half8 o;
+                act8<BF> o;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) o[j] = act_cvt<BF>(acc[j >> 2][j & 3]);
+                for (int j = 0; j < 8; ++j) o[j] = (act_t<BF>)(acc[j >> 2][j & 3]);
                 const int chunk = 4 * (wave + pp * TW) + g;
-                fst8(Ot + row * N + 8 * (chunk ^ (row & 15)), o);
+                fst8(Ot + row * N + 8 * (chunk ^ (row & 15)), raw_act(o));
             }
             if (heads_wave) {
                 float4v hacc = float4v{0.f, 0.f, 0.f, 0.f};
@@ -854,26 +854,26 @@ __global__ __launch_bounds__(TH) void ln_gdp_kernel(LnGdpArgs a) {
             const float bpv = (float)a.bp[col], bgv = (float)a.bg[col];
             half_t* dst = (col < ci ? a.left + (int64_t)col * a.M : a.right + (int64_t)(col - ci) * a.M) +
                           m0 + 16 * g;
-            half8 lo, hi;
+            act8<BF> lo, hi;
 #pragma unroll
             for (int rb = 0; rb < 4; ++rb)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int t = 4 * rb + i;
                     const float v = mv[t] * (ap[rb][i] + bpv) * sigmoid_fast(ag[rb][i] + bgv);
-                    if (t < 8) lo[t] = act_cvt<BF>(v); else hi[t - 8] = act_cvt<BF>(v);
+                    if (t < 8) lo[t] = (act_t<BF>)v; else hi[t - 8] = (act_t<BF>)v;
                 }
             const int rows_left = a.M - (m0 + 16 * g);
             if (lines && rows_left >= 16) {
-                fst8_nt(dst, lo);
-                fst8_nt(dst + 8, hi);
+                fst8_nt(dst, raw_act(lo));
+                fst8_nt(dst + 8, raw_act(hi));
             } else if (vec && rows_left >= 16) {
-                fst8(dst, lo);
-                fst8(dst + 8, hi);
+                fst8(dst, raw_act(lo));
+                fst8(dst + 8, raw_act(hi));
             } else {
 #pragma unroll
                 for (int t = 0; t < 16; ++t)
-                    if (t < rows_left) dst[t] = t < 8 ? lo[t] : hi[t - 8];
+                    if (t < rows_left) dst[t] = t < 8 ? raw_act(lo)[t] : raw_act(hi)[t - 8];
             }
         }
     }
@@ -1019,7 +1019,7 @@ __global__ __launch_bounds__(TH) void ln_gdp_fast_kernel(LnGdpArgs a) {
                     ag[rb] = mfma16x16x32(xop[rb][ks], wg, ag[rb]);
                 }
             }
-            half8 lo, hi;
+            act8<BF> lo, hi;
 #pragma unroll
             for (int rb = 0; rb < 4; ++rb)
 #pragma unroll
@@ -1027,11 +1027,11 @@ __global__ __launch_bounds__(TH) void ln_gdp_fast_kernel(LnGdpArgs a) {
                     const int e = 4 * rb + i;
                     const float mv = (float)(e < 8 ? mvlo[e] : mvhi[e - 8]);
                     const float v = mv * ap[rb][i] * sigmoid_fast(ag[rb][i]);
-                    if (e < 8) lo[e] = act_cvt<BF>(v); else hi[e - 8] = act_cvt<BF>(v);
+                    if (e < 8) lo[e] = (act_t<BF>)v; else hi[e - 8] = (act_t<BF>)v;
                 }
             if (zero_out) {
-                lo = fzero8();
-                hi = fzero8();
+                lo = act8<BF>{};
+                hi = act8<BF>{};
             }
             // column block cb lies wholly in left (columns < PH) or in right
             const int col = 16 * cb + r16;
@@ -1284,15 +1284,15 @@ void epilogue_kernel(EpiArgs a) {
                 for (int hb = 0; hb < 2; ++hb)
                     ag[hb] = mfma16x16x32(fld8(Wg + frag(2 * cp + hb, ks, KA, lane)), af[ks], ag[hb]);
             const int col = 32 * cp + 8 * g;
-            half8 o;
+            act8<BF> o;
             if (work == kPadding) {
-                o = fzero8();
+                o = act8<BF>{};
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const float val = ao[j >> 2][j & 3] * sigmoid_fast(ag[j >> 2][j & 3]);
                     const float res = ADD ? pin_f32(act_get<BF>(xr[cp], j)) : 0.f;
-                    o[j] = act_cvt<BF>(val + res);
+                    o[j] = (act_t<BF>)(val + res);
                 }
             }
             const uint32_t off = (uint32_t)(r16 * O + col) * 2u;
@@ -1620,13 +1620,13 @@ __global__ __launch_bounds__(WV * kWave, 2) void transition_stream_kernel(TransA
 #pragma unroll
             for (int cp = 0; cp < NCB / 2; ++cp) {
                 const uint32_t off = (uint32_t)((16 * rb + r16) * C + 32 * cp + 8 * g) * 2u;
-                half8 o;
+                act8<BF> o;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float res = !ADD ? 0.f : act_get<BF>(kNext ? xr[kNext && ADD ? rb : 0][cp] : xop[rb][cp], e);
-                    o[e] = act_cvt<BF>(ADD ? acc[2 * cp + (e >> 2)][rb][e & 3] + res : acc[2 * cp + (e >> 2)][rb][e & 3]);
+                    o[e] = (act_t<BF>)(ADD ? acc[2 * cp + (e >> 2)][rb][e & 3] + res : acc[2 * cp + (e >> 2)][rb][e & 3]);
                 }
-                if (!ADD && work == kPadding) o = fzero8();
+                if (!ADD && work == kPadding) o = act8<BF>{};
                 __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), ro, store ? off : kDrop, 0, 0);
             }
             if constexpr (ADD && !kNext) {
@@ -1801,11 +1801,11 @@ __global__ __launch_bounds__(kTransRowsThreads, 4) void transition_rows_kernel(T
 #pragma unroll
             for (int cp = 0; cp < NCB / 2; ++cp) {
                 const int col = 32 * cp + 8 * g;
-                half8 o;
+                act8<BF> o;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float res = ADD ? act_get<BF>(xr[rb][cp], e) : 0.f;
-                    o[e] = act_cvt<BF>(acc[2 * cp + (e >> 2)][rb][e & 3] + res);
+                    o[e] = (act_t<BF>)(acc[2 * cp + (e >> 2)][rb][e & 3] + res);
                 }
                 // a padding tile stores zeros (with add_input it stores nothing)
                 const u32x4 ov = !ADD && work == kPadding ? u32x4{0u, 0u, 0u, 0u} : __builtin_bit_cast(u32x4, o);

@@ -123,10 +123,10 @@ __device__ __forceinline__ void store_run(const GemmArgs& a, int m, int n, const
         }
 #pragma unroll
         for (int h = 0; h < RL / W; ++h) {
-            typename Vec16<W>::type o;
+            std::conditional_t<W == 8, act8<BF>, act4<BF>> o;
 #pragma unroll
-            for (int i = 0; i < W; ++i) o[i] = act_cvt<BF>(v[W * h + i]);
-            *reinterpret_cast<typename Vec16<W>::unaligned*>(a.out + at + W * h) = o;
+            for (int i = 0; i < W; ++i) o[i] = (act_t<BF>)v[W * h + i];
+            *reinterpret_cast<typename Vec16<W>::unaligned*>(a.out + at + W * h) = raw_act(o);
         }
     } else {
 #pragma unroll
@@ -146,13 +146,14 @@ template <bool BF, bool ADD, bool LINES>
 __device__ __forceinline__ void store_lines(const GemmArgs& a, int m0, int n, int r16, const Channels<16>& ch, const int (&sum)[16],
                                             const half8 (&res)[2]) {
     const float sx = a.qs[min(m0 + r16, a.M - 1)];
-    half8 o[2];
+    act8<BF> r[2];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         float v = scaled(sum[i], sx, ch.sw[i], ch.b[i]);
         if constexpr (ADD) v += act_get<BF>(res[i / 8], i % 8);
-        o[i / 8][i % 8] = act_cvt<BF>(v);
+        r[i / 8][i % 8] = (act_t<BF>)v;
     }
+    half8 o[2] = {raw_act(r[0]), raw_act(r[1])};
     rows_of_eight(o[0], o[1]);
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
@@ -529,15 +530,16 @@ __global__ __launch_bounds__(256) void q8_stream_kernel(GemmArgs a) {
             const int n = n0 + 32 * (h + (r16 >> 3)) + 8 * g;
 #pragma unroll
             for (int mf = 0; mf < MF; ++mf) {
-                half8 o[2];
+                act8<BF> r[2];
 #pragma unroll
                 for (int p = 0; p < 2; ++p)
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         float v = scaled(acc[2 * (h + p) + i / 4][mf][i % 4], now.qs[mf], sw[p][i], bv[p][i]);
                         if constexpr (RES) v += act_get<BF>(now.res[mf][h + p], i);
-                        o[p][i] = act_cvt<BF>(v);
+                        r[p][i] = (act_t<BF>)v;
                     }
+                half8 o[2] = {raw_act(r[0]), raw_act(r[1])};
                 rows_of_eight(o[0], o[1]);
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {

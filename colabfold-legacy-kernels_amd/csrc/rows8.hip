@@ -234,10 +234,10 @@ __global__ __launch_bounds__(kAny) void rms_norm_any_kernel(RmsArgs a) {
             for (int c = first; c < C; c += 8 * kAny) {
                 const half8 v = cut8(load8(vr, c, C), c, C);
                 const float8v w = load8f(a.w, c, C);
-                half8 o;
+                act8<BF> o;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) o[e] = act_cvt<BF>(act_get<BF>(v, e) * d * r * w[e]);
-                store8(a.out + row * a.C, c, C, o);
+                for (int e = 0; e < 8; ++e) o[e] = (act_t<BF>)(act_get<BF>(v, e) * d * r * w[e]);
+                store8(a.out + row * a.C, c, C, raw_act(o));
             }
         }
     }
@@ -324,10 +324,10 @@ __global__ __launch_bounds__(block_of(TPR)) void rms_norm_kernel(RmsArgs a) {
             if (part == 0 && in && a.stat != nullptr) a.stat[row] = r * d;
 #pragma unroll
             for (int j = 0; j < NCH; ++j) {
-                half8 o;
+                act8<BF> o;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) o[e] = act_cvt<BF>(act_get<BF>(v[j], e) * d * r * w[j][e]);
-                store8(a.out + row * C, 8 * (part + TPR * j), len, o);
+                for (int e = 0; e < 8; ++e) o[e] = (act_t<BF>)(act_get<BF>(v[j], e) * d * r * w[j][e]);
+                store8(a.out + row * C, 8 * (part + TPR * j), len, raw_act(o));
             }
         }
     }
@@ -372,14 +372,14 @@ __global__ __launch_bounds__(kAny) void rms_norm_bwd_any_kernel(RmsBwdArgs a) {
             const float8v w = load8f(a.w, c, C);
             half8 dz = {};
             if (a.dsum != nullptr) dz = cut8(load8(a.dsum + row * a.C, c, C), c, C);
-            half8 o;
+            act8<BF> o;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 float d = r * (act_get<BF>(dy, e) * w[e] - act_get<BF>(s, e) * r * dot);
                 if (a.dsum != nullptr) d += act_get<BF>(dz, e);
-                o[e] = act_cvt<BF>(d);
+                o[e] = (act_t<BF>)d;
             }
-            store8(a.ds + row * a.C, c, C, o);
+            store8(a.ds + row * a.C, c, C, raw_act(o));
         }
     }
 }
@@ -446,15 +446,15 @@ __global__ __launch_bounds__(block_of(TPR)) void rms_norm_bwd_kernel(RmsBwdArgs 
         const float dot = row_all<TPR>(t, share, turn).sum * a.inv_c;
 #pragma unroll
         for (int j = 0; j < NCH; ++j) {
-            half8 o;
+            act8<BF> o;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float xh = act_get<BF>(s[j], e) * r;
                 float d = r * (act_get<BF>(dy[j], e) * w[j][e] - xh * dot);
                 if constexpr (DSUM) d += act_get<BF>(dz[j], e);
-                o[e] = act_cvt<BF>(d);
+                o[e] = (act_t<BF>)d;
             }
-            store8(a.ds + row * C, 8 * (part + TPR * j), len, o);
+            store8(a.ds + row * C, 8 * (part + TPR * j), len, raw_act(o));
         }
     }
     if constexpr (ROWS > 1) {  // the block's row groups, in order
@@ -702,10 +702,10 @@ __global__ __launch_bounds__(256) void dequantize_kernel(DequantArgs a, int shif
             if constexpr (T == kF32) {
                 store4f<NT>(static_cast<float*>(a.out) + row * a.K + c, left, float4v{v[0], v[1], v[2], v[3]});
             } else {
-                half8 h;
+                act8<T == kBf16> h;
 #pragma unroll
-                for (int e = 0; e < E; ++e) h[e] = act_cvt<T == kBf16>(v[e]);
-                store8<NT>(static_cast<half_t*>(a.out) + row * a.K + c, 0, left, h);
+                for (int e = 0; e < E; ++e) h[e] = (act_t<T == kBf16>)v[e];
+                store8<NT>(static_cast<half_t*>(a.out) + row * a.K + c, 0, left, raw_act(h));
             }
         }
     }
