@@ -71,7 +71,7 @@ struct AttnArgs {
     int W;          // workgroups that fill the chip
     float* part_o;  // [2 W][16][D]
     float* part_s;  // [2 W][2][16]: running maximum, sum
-    int4v* split;   // [W]: an item in parts, its first part and how many it has
+    int4v* split;   // [W]: an item in parts, its first part, how many it has, the sequence's length
     int4v* plan;    // of each workgroup: sequence, item of the sequence, part << 16 | parts, place; null: it works that out
     int* meta;      // the items in parts; planned workgroups
 };
@@ -594,7 +594,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_attn_plan_kernel(AttnArgs 
     if (b >= a.B) return;
     const int k = (int)n.groups / a.heads, slot = (int)(p >> 16);
     for (int hr = 0, i = 0; hr < a.heads; ++hr) {
-        if (k > 1) a.split[(p & 0xffffu) + hr] = int4v{b * a.heads + hr, slot + i, k, 0};
+        if (k > 1) a.split[(p & 0xffffu) + hr] = int4v{b * a.heads + hr, slot + i, k, len};
         for (int j = 0; j < k; ++j, ++i) a.plan[at + i] = int4v{b, hr, j << 16 | k, slot + i};
     }
 }
@@ -636,7 +636,7 @@ __device__ __forceinline__ bool work_of(const AttnArgs& a, Work& work) {
     work.hr = at / work.k;
     work.j = at - work.hr * work.k;
     work.slot = (int)(parts_before >> 16) + at;
-    if (work.k > 1 && tid == 0 && work.j == 0) a.split[(parts_before & 0xffffu) + work.hr] = int4v{b * a.heads + work.hr, work.slot, work.k, 0};
+    if (work.k > 1 && tid == 0 && work.j == 0) a.split[(parts_before & 0xffffu) + work.hr] = int4v{b * a.heads + work.hr, work.slot, work.k, len};
     return true;
 }
 
@@ -686,7 +686,7 @@ __global__ __launch_bounds__(WAVES* kWave) void paged_attn_join_kernel(AttnArgs 
     const int4v item = a.split[blockIdx.x];
     if ((int)blockIdx.x >= a.meta[0]) return;
     const int first = item[1], n = item[2], r = blockIdx.y, b = fdiv(item[0], a.by_heads);
-    const Span sp = span_of(a, b, item[0] - b * a.heads, 0, 0, a.len[b]);
+    const Span sp = span_of(a, b, item[0] - b * a.heads, 0, 0, item[3]);
     if (r >= sp.rows) return;
     const int tid = threadIdx.x, wave = uniform((int)(tid / kWave)), lane = tid % kWave;
     const auto slot = [&](int p) { return (int64_t)first + p; };
