@@ -13,7 +13,7 @@
 // All of them are bound by memory: each value is read once and written once, statistics and products are fp32. At 16384 tokens
 // of 48 + 6 + 6 heads of 128 in bf16 the forward takes 100 us (5.0 TB/s of its 503 MB, the rate of a large copy; a
 // plain copy in the same pattern 109) and the gradients 151 + 6 (5.0 TB/s of 755 MB); 32771 tokens of 8 heads of 128 take
-// 53 us into a 16-bit cache and 47 back (5.1 and 5.7 TB/s of 268 MB each); a prompt of 4099 tokens of 32 + 8 + 8 heads of
+// 55 us into a 16-bit cache and 48 back (4.9 and 5.5 TB/s of 268 MB each); a prompt of 4099 tokens of 32 + 8 + 8 heads of
 // 128 takes 27 us into an 8-bit cache (3.4 TB/s of 92 MB, 4.3 at 32768 tokens); one token 3.7 us.
 //
 // A head is a group of LG lanes (the power of two at or past D / 8) with 8 channels each, the two halves of its pairs: a
@@ -859,8 +859,9 @@ void set_cache(HeadsArgs& a, const CacheShape& c, const clk_buffer* k, const clk
 }
 
 // Heads a workgroup: more share a token's angles and keep more loads in flight, and take longer pieces of memory in a row, where
-// there are workgroups enough without. 16384 tokens of 60 heads of 128: 100 us with eight, 110 with four, 131 with two; 4099
-// of 48 heads 27.7, 26.2 and 31.8.
+// there are workgroups enough without. 16384 tokens of 60 heads of 128: 100 us with eight, 110 with four, 131 with two; of 48
+// heads 4099 27.7, 25.7 and 31.8 (42.7 with one), 1500 12.5 with eight, 11.4 with four and 13.4 with one, 128 3.65 with one
+// and 4.1 with four. Between, four would be ahead from 256 tokens on (4.5 and 4.6; 1024 8.8 and 10.2).
 int heads_at_once(int64_t T, int heads, int lg) {
     const int64_t blocks = (T * lg + kThreads - 1) / kThreads;
     return blocks * ceil_div(heads, 8) >= 2048 ? 8 : blocks * heads >= 4096 ? 4 : 1;
@@ -903,8 +904,9 @@ void launch_step(HeadsArgs& a, bool bf, bool q8, hipStream_t s) {
     a.parts = token_blocks(a.T, lg, a.cq);
     // Heads that a workgroup takes one after another: more share their window's look at the slots and its angles, which are as
     // many bytes as a key and a value, and have the next head's on their way; where that leaves enough workgroups. 4099
-    // tokens of 32 + 8 + 8 heads of 128 into 8 bits 27.1 us with four, 28.7 with one, into 16 26.5 and 29.5; 32768 tokens 170
-    // and 189; but 512 tokens 7.1 and 6.9, and eight at 4099 30.1.
+    // tokens of 32 + 8 + 8 heads of 128 into 8 bits 27.1 us with four, 28.0 with two, 29.6 with one, into 16 26.6, 28.3 and
+    // 29.8; 32768 tokens into 8 176, 185 and 204; 1031 tokens 12.5 with four, 10.4 with two, 11.2 with one; 512 tokens 11.7,
+    // 8.5 and 7.2; and eight at 4099 30.1.
     const int once = std::max(1, kThreads / lg / 16);
     const int64_t windows = (a.T + 15) / 16 * head_groups(a.Hkv, lg);
     a.cached_heads = once * (windows >= 1024 ? 4 : windows >= 512 ? 2 : 1);

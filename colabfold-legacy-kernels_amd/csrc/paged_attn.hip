@@ -14,8 +14,9 @@
 // with the running maximum and sum of a softmax. Both operands come from memory to registers with nothing between.
 //
 // 256 sequences of 4096 on 8 heads of 128 in bf16 (4.2 GB) take 627 us, 6.7 TB/s, where reading alone reaches 6.9; one of 131071
-// (537 MB) 83 + 5, 6.5 TB/s; 61 ragged ones of up to 8192 on 4 heads in 8 bits (167 MB) 35 + 5, 4.7 TB/s: some 3 us
-// before the first keys arrive and a tail of 3 to 5, as parts end unevenly; one of 77 tokens 4.1 us, a launch's time.
+// (537 MB) 84 + 5, 6.4 TB/s; 61 ragged ones of up to 8192 on 4 heads in 8 bits (167 MB) 36 + 5, 4.7 TB/s: some 3 us
+// before the first keys arrive, and the longest parts have 1024 tokens where even shares would have 841; one of 77
+// tokens 4.2 us, a launch's time.
 #include "kv_cache.h"
 
 #include <algorithm>
@@ -30,6 +31,10 @@ typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 typedef int int4v __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
+// Tokens of room for which a workgroup takes an item whole, with nothing to plan or join: one sequence of 512 tokens on 8 heads
+// of 128 in bf16 6.4 us, 8.6 in parts; 64 of 512 26.2 and 34.4; but one of 1024 9.6 and 8.6 in parts, of 2048 18.0 and
+// 9.6; 64 of 1024 48.3 and 51.5, 256 of 512 94.5 and 91.6. The host knows the table's room, not the lengths: 77
+// tokens take 4.0 us with room for 512 and 6.3 with more, whose join has nothing to do.
 constexpr int kDirect = 512;
 
 // Blocks of 16 tokens a wave takes at a time, and the tokens of a workgroup's step. (Four blocks, where the registers hold
@@ -114,11 +119,11 @@ __device__ __forceinline__ uint2v bf16_of_bytes(uint32_t w) {
 }
 __device__ __forceinline__ half8 join(uint2v a, uint2v b) { return __builtin_bit_cast(half8, uint4v{a[0], a[1], b[0], b[1]}); }
 
-// Eight weights in two 16-bit parts each, 2^-16 (bf16) or 2^-22 of them at most away from their sum: one would make a
-// result's error half a step larger than its own rounding. The matrix cores have time for both.
+// Eight weights in two 16-bit parts each, 2^-17 of them at most away from their sum (bf16): one would make a result's error
+// half a step larger than its own rounding. The matrix cores have time for both.
 // ABOVE: the first part is a step below the weight cut off, so that the second is positive too and an infinity among
-// the values stays one (a second part of zero or below would make it NaN). The parts are then 2^-15 or 2^-21 away at
-// most. An fp16 weight under kLeastAbove has a first part of zero: attend takes infinities apart there.
+// the values stays one (a second part of zero or below would make it NaN). The parts are then 2^-15 (bf16) or 2^-21
+// away at most. An fp16 weight under kLeastAbove has a first part of zero: attend takes infinities apart there.
 constexpr float kLeastAbove = 0x1p-23f;
 template <bool BF, bool ABOVE>
 __device__ __forceinline__ void two_parts(const float (&f)[8], half8& hi, half8& lo) {
@@ -763,8 +768,8 @@ Plan plan_of(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t per, int64_t
     p.items = p.grid = B * Hkv * blocks;
     if (per * page > kDirect && B > 0) {
         // One round of workgroups, but where the items nearly make one already, three, so that the long among them are cut
-        // finely enough to fill the last round: 256 ragged sequences of up to 4096 on 8 heads 151 us, a tenth more with two; 61 on
-        // 4 heads 43 with one and 48 with three.
+        // finely enough to fill the last round: 256 ragged sequences of up to 4096 on 8 heads of 128 in bf16 232 us, 236 with two
+        // and 241 with one; but 61 of up to 8192 on 4 heads in 8 bits 43 with one, 45.5 with two and 47 with three.
         p.W = 256 * occupancy(D) * (p.items > 128 * occupancy(D) ? 3 : 1);
         // With c as the kernel takes it, all chunks / c <= room = W - min(items, W / 2), and an item has under its chunks / c + 1
         // parts: under room + items workgroups; items of two parts and more have over c chunks: under room such items
@@ -774,9 +779,9 @@ Plan plan_of(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t per, int64_t
         p.s = (size_t)2 * p.W * 32 * 4;
         p.split = (size_t)p.W * 16;
         p.meta = 256;
-        // Many items of many sequences are dealt out by a launch before (2.5 us and a gap): 256 sequences of up to 1024 on 8 heads
-        // 106 us, 114 without; 1024 of them 375, 472 without; 4096 ragged ones 587, 2309 without; but 50 ragged ones of up
-        // to 4096 48, 44 without, and 128 on one head 19.4, 17.1 without.
+        // Many items of many sequences are dealt out by a launch before (2.5 to 7 us and a gap), of 128 channels in bf16: 1024
+        // sequences of 1024 on 8 heads 661 us, 672 without; 4096 ragged ones 906, 2411 without; 256 of 1024 171 with it and
+        // without; but 50 ragged ones of up to 4096 61.8, 54.6 without, and 128 of 1024 on one head 21.3, 19.4 without.
         if (B > kPlanned && p.items > 128 * occupancy(D)) p.plan = (size_t)p.grid * 16;
     }
     return p;
@@ -863,8 +868,10 @@ extern "C" int clk_paged_attention(clk_stream stream, const clk_buffer* q, const
     stage_mark(s, stage);
     const dim3 block(kWaves * kWave);
     // Keys and values of a cache past half of the 256 MB far cache are loaded past the caches, unless more than one workgroup
-    // reads them: 61 sequences of 2600 over 8 bits (166 MB) 42.7 us, 46.9 through the caches; 256 of 4096 (4.2 GB) 691 and
-    // 752; but 61 of 650 (41 MB, of which a next call finds some) 20.4 and 19.5.
+    // reads them: 61 sequences of 2600 on 4 heads in 8 bits (164 MB) 41.1 us, 44.3 through the caches; 256 of 4096 (4.2 GB)
+    // 634 and 704; but 61 of 650 (41 MB, of which a next call finds some) 19.8 and 18.9. The host knows the cache, not how
+    // much of it the sequences hold, nor what they share: 8 of 512 in one of 670 MB 10.3 and 11.1, but 61 of 650 in one of
+    // 330 MB 19.7 and 19.0, and 64 of 1088 in bf16 that share their first 1024 28.9 and 25.2.
     const bool past = blocks == 1 && 2 * elements(k_cache) * (c.q8 ? 1 : 2) >= (int64_t)1 << 27;
     const auto kernels = [&](auto bf_, auto q8_, auto d_) {
         constexpr bool BF = decltype(bf_)::value, Q8 = decltype(q8_)::value;
@@ -880,8 +887,8 @@ extern "C" int clk_paged_attention(clk_stream stream, const clk_buffer* q, const
         if (past) hipLaunchKernelGGL((paged_attn_split_kernel<BF, Q8, true, D>), dim3((unsigned)plan.grid), block, 0, s, a);
         else hipLaunchKernelGGL((paged_attn_split_kernel<BF, Q8, false, D>), dim3((unsigned)plan.grid), block, 0, s, a);
         stage_mark(s, ++stage);
-        // Eight waves where items have sixteen parts and more: one sequence of 16384 on one head 13.6 -> 12.1 us, of 131071 on eight
-        // 92 -> 90; but 16 ragged ones of up to 4097 on one head (twelve parts) 15.0 -> 15.9.
+        // Eight waves where items have sixteen parts and more: one sequence of 16384 on one head 13.3 -> 11.8 us, of 131071 on eight
+        // 90.6 -> 89.7; but 16 ragged ones of up to 4097 on one head (twelve parts) 14.4 -> 15.3.
         const dim3 items((unsigned)std::min<int64_t>(plan.items, plan.W), (unsigned)std::min<int64_t>(G, 16));
         if (16 * plan.items <= plan.W) hipLaunchKernelGGL((paged_attn_join_kernel<BF, BF || Q8, D, 8>), items, dim3(8 * kWave), 0, s, a);
         else hipLaunchKernelGGL((paged_attn_join_kernel<BF, BF || Q8, D, 4>), items, dim3(4 * kWave), 0, s, a);
