@@ -13,7 +13,7 @@
 // All of them are bound by memory: each value is read once and written once, statistics and products are fp32. At 16384 tokens
 // of 48 + 6 + 6 heads of 128 in bf16 the forward takes 100 us (5.0 TB/s of its 503 MB, the rate of a large copy; a
 // plain copy in the same pattern 109) and the gradients 151 + 6 (5.0 TB/s of 755 MB); 32771 tokens of 8 heads of 128 take
-// 55 us into a 16-bit cache and 48 back (4.9 and 5.5 TB/s of 268 MB each); a prompt of 4099 tokens of 32 + 8 + 8 heads of
+// 55 us into a 16-bit cache and 48 back (4.9 and 5.6 TB/s of 268 MB each); a prompt of 4099 tokens of 32 + 8 + 8 heads of
 // 128 takes 27 us into an 8-bit cache (3.4 TB/s of 92 MB, 4.3 at 32768 tokens); one token 3.7 us.
 //
 // A head is a group of LG lanes (the power of two at or past D / 8) with 8 channels each, the two halves of its pairs: a

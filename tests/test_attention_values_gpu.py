@@ -18,7 +18,7 @@ def np64(t):
 
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("room", (512, 4096))
-@pytest.mark.parametrize("d", (32, 64, 96, 128, 160, 256))
+@pytest.mark.parametrize("d", (32, 64, 96, 128, 160, 192, 224, 256))
 @pytest.mark.parametrize("n", (3, 40, 500))
 def test_infinities_with_small_weights(hip, n, d, room, kind):
     """A positive weight times an infinite value is that infinity, however small the weight is against the largest (2^-90 here):
